@@ -11,8 +11,8 @@ free pages holds the rest.  One serving step is
   and give each new token its slot (page * page_size + offset in the page);
 * ``append``: copy the new tokens' K/V rows to their slots (a prompt);
 * ``attend``: one query token of each request over the request's pages;
-* ``step``: the same with the newest token's K/V row written on the way
-  (generation);
+* ``step``: the same with the newest token's K/V row written to its slot on
+  the way (generation);
 * ``release``: push the pages of finished requests back on the stack.
 
 ``run`` computes them in elementary torch operations, in 32 bits and rounded
@@ -160,6 +160,8 @@ def prepare(case, seed):
     s["scale"] = D ** -0.5
     if op == "step":
         s["new_k"], s["new_v"] = normal(B, Hkv, 1, D), normal(B, Hkv, 1, D)
+        last = lens.long() - 1
+        s["slots"] = s["block_table"].gather(1, (last // page)[:, None])[:, 0].long() * page + last % page
     return s
 
 
@@ -241,11 +243,10 @@ def run(state):
         return (out, lse) if case["lse"] else out
     if op == "step":
         if own:
-            out = paged.paged_attention(s["q"], s["k_pages"], s["v_pages"], s["block_table"], s["lengths"], scale=s["scale"], new_k=s["new_k"], new_v=s["new_v"])
+            out = paged.paged_attention(s["q"], s["k_pages"], s["v_pages"], s["block_table"], s["lengths"], scale=s["scale"], new_k=s["new_k"], new_v=s["new_v"],
+                                       slots=s["slots"])
         else:
-            last = (s["lengths"] - 1).long()
-            slots = s["block_table"].gather(1, (last // page)[:, None])[:, 0].long() * page + last % page
-            _append(s["k_pages"], s["v_pages"], s["new_k"], s["new_v"], slots)
+            _append(s["k_pages"], s["v_pages"], s["new_k"], s["new_v"], s["slots"])
             out, _ = _attend(s["q"], s["k_pages"], s["v_pages"], s["block_table"], s["lengths"], s["scale"])
         return out, s["k_pages"], s["v_pages"]
     if op == "append":
