@@ -10,6 +10,7 @@ from __future__ import annotations
 from . import _ext
 from .attention import attention
 from .cache import PreallocatedKVCache, append_kv_cache, decode_step
+from .paged import PagedKVCache, append_paged_kv, paged_attention, release_pages, reserve_pages
 
 
 def triton_available() -> bool:
@@ -33,5 +34,10 @@ __all__ = [
     "PreallocatedKVCache",
     "append_kv_cache",
     "decode_step",
+    "PagedKVCache",
+    "paged_attention",
+    "append_paged_kv",
+    "reserve_pages",
+    "release_pages",
 ]
 __version__ = "1.0.0"

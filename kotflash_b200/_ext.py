@@ -17,6 +17,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 from functools import lru_cache
 from pathlib import Path
@@ -53,6 +54,9 @@ _I = ctypes.c_int
 _F = ctypes.c_float
 _SZ = ctypes.c_size_t
 
+# A kf_tensor4* given as the bytes of the struct (see packed4)
+_T4B = ctypes.c_char_p
+
 # name -> (restype, argtypes); exactly the declarations of include/kotflash_b200.h
 SIGNATURES = {
     "kf_version": (_I, []),
@@ -68,6 +72,13 @@ SIGNATURES = {
     "kf_decode": (_I, [_T4, _T4, _T4, _T4, _T4, _I64, _T4, _VP, _I, _F, _I, _VP, _SZ, _VP]),
     "kf_merge_partials": (_I, [_VP, _VP, _I, _I64, _I64, _VP, _VP, _I, _VP]),
     "kf_decode_noalloc": (_I, [_T4, _T4, _T4, _T4, _T4, _I64, _T4, _VP, _I, _F, _I, _VP]),
+    "kf_paged_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
+    "kf_paged_decode": (_I, [_T4B, _T4B, _T4B, _VP, _I64, _I64, _VP, _T4B, _T4B, _VP, _T4B, _VP, _I, _F, _VP, _SZ,
+                             _VP]),
+    "kf_paged_append": (_I, [_T4B, _T4B, _T4B, _T4B, _VP, _I, _VP]),
+    "kf_paged_reserve": (_I, [_VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _VP,
+                              _VP]),
+    "kf_paged_release": (_I, [_VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _VP, _VP, _VP]),
     "kf_selftest_bounded_wait": (_I, [_VP, _I64, _VP]),
     "kf_selftest_exp2_poly": (_I, [_VP, _VP, _I64, _VP]),
     "kf_peer_mailbox_bytes": (_SZ, [_I, _I64, _I64]),
@@ -147,6 +158,15 @@ def t4(t: Optional[torch.Tensor]) -> Optional[KFTensor4]:
         d.size[i] = int(t.shape[i])
         d.stride[i] = int(t.stride(i))
     return d
+
+
+_PACK4 = struct.Struct("=Q8q").pack  # pointer, sizes, strides: a KFTensor4 in memory
+
+
+def packed4(t: torch.Tensor) -> bytes:
+    """The bytes of ``t4(t)``: the same descriptor about four times faster to
+    make, for calls that take microseconds."""
+    return _PACK4(t.data_ptr(), *t.shape, *t.stride())
 
 
 def ref(d: Optional[KFTensor4]):

@@ -27,7 +27,6 @@
 #include <string.h>
 
 #include <mutex>
-#include <utility>
 
 #include "kf_host.h"
 #include "kf_sm100.cuh"
@@ -1036,29 +1035,7 @@ __global__ void __launch_bounds__(kMergeThreads) merge_kernel(const MergeArgs a)
   merge_row<BF16>(a, blockIdx.x);
 }
 
-// Launch with programmatic stream serialization: the kernel may be scheduled
-// before the previous kernel in the stream finishes and orders itself with
-// griddepcontrol.wait, hiding launch latency between back-to-back kernels
-// (split -> merge, and one decode step -> the next).
-template <typename... KArgs, typename... Args>
-int launch_dependent(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
-                     const char* what, Args&&... args) {
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = grid;
-  cfg.blockDim = block;
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  if (cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) != cudaSuccess) {
-    (void)cudaGetLastError();
-    return kf::set_error(KF_ERR_CUDA, "%s: launch failed", what);
-  }
-  return kf::check_launch(what);
-}
+using kf::launch_dependent;
 
 // Keys per K/V tile of the kernel variant dispatch_split picks; split chunks
 // are multiples of it.

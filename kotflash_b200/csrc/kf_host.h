@@ -8,6 +8,8 @@
 #include <stdint.h>
 #include <stdio.h>
 
+#include <utility>
+
 #include "../../include/kotflash_b200.h"
 
 namespace kf {
@@ -54,5 +56,40 @@ class DeviceGuard {
   bool switched_ = false;
   int rc_ = 0;
 };
+
+// Launch with programmatic stream serialization: the kernel may be scheduled
+// before the previous kernel in the stream finishes and orders itself with
+// griddepcontrol.wait, hiding launch latency between back-to-back kernels
+// (split -> merge, and one decode step -> the next).  `cluster` > 1 groups
+// that many consecutive blocks (at most 8) of a one-dimensional grid.
+template <typename... KArgs, typename... Args>
+int launch_dependent_cluster(void (*kern)(KArgs...), unsigned cluster, dim3 grid, dim3 block, size_t smem,
+                             cudaStream_t st, const char* what, Args&&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = cluster;
+  attr[1].val.clusterDim.y = 1;
+  attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  if (cudaLaunchKernelEx(&cfg, kern, std::forward<Args>(args)...) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return set_error(KF_ERR_CUDA, "%s: launch failed", what);
+  }
+  return check_launch(what);
+}
+
+template <typename... KArgs, typename... Args>
+int launch_dependent(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                     const char* what, Args&&... args) {
+  return launch_dependent_cluster(kern, 1, grid, block, smem, st, what, std::forward<Args>(args)...);
+}
 
 }  // namespace kf

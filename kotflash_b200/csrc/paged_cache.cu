@@ -1,0 +1,530 @@
+// K6: the paged KV cache's own kernels: append of K/V rows to their slots,
+// and the block tables and slot maps made from request lengths.
+//
+// A pool of pages [pages, Hkv, page_size, D] holds the K (and V) rows of all
+// requests; position p of request b is row p % page_size of page
+// block_table[b][p / page_size], and its slot is page * page_size + p %
+// page_size.  The pages that no request owns are a stack, free_pages[0 ..
+// free_count).
+#include <cooperative_groups.h>
+
+#include <type_traits>
+
+#include "kf_host.h"
+#include "kf_sm100.cuh"
+
+namespace cg = cooperative_groups;
+
+namespace {
+
+// ---------------------------------------------------------------- append
+// Pure data movement: 2 x Hkv x D elements read and written per token, no
+// arithmetic, so HBM (or, for one token per request, latency) bounds it.  A
+// thread keeps one 16-byte column of a token's Hkv * D elements and walks
+// over tokens, so the division that finds (head, column) is done once; U
+// tokens are loaded before the first is stored.
+constexpr int kAppendThreads = 256;
+
+struct AppendArgs {
+  const uint16_t* src_k;
+  const uint16_t* src_v;
+  uint16_t* dst_k;
+  uint16_t* dst_v;
+  const int64_t* slots;
+  int64_t sk[4], sv[4], dk[4], dv[4];
+  int64_t num_slots;
+  uint32_t T, S;            // tokens in all, and per batch entry
+  uint32_t per_token;       // vectors of one token (Hkv * D / VEC)
+  uint32_t per_head;        // vectors of one head (D / VEC)
+  uint32_t page_size;
+  uint32_t block_tokens;    // tokens side by side in a block (0: a block walks one token's vectors)
+};
+
+template <int VEC>
+__device__ __forceinline__ void move_token(const AppendArgs& a, int64_t slot, uint32_t t, uint32_t vec, bool load,
+                                           uint4 (&val)[2]) {
+  using E = typename std::conditional<VEC == 8, uint4, uint16_t>::type;
+  const uint32_t h = vec / a.per_head, d = (vec - h * a.per_head) * VEC;
+  if (load) {
+    const uint32_t n = a.S == a.T ? 0 : t / a.S, s = t - n * a.S;
+    const E* pk = reinterpret_cast<const E*>(a.src_k + n * a.sk[0] + h * a.sk[1] + s * a.sk[2] + d * a.sk[3]);
+    const E* pv = reinterpret_cast<const E*>(a.src_v + n * a.sv[0] + h * a.sv[1] + s * a.sv[2] + d * a.sv[3]);
+    if constexpr (VEC == 8) {
+      val[0] = __ldg(pk);
+      val[1] = __ldg(pv);
+    } else {
+      val[0].x = *pk;
+      val[1].x = *pv;
+    }
+  } else {
+    // slots of a pool fit 32 bits unless it holds over 2^32 tokens
+    const bool small = a.num_slots <= 0xffffffffLL;
+    const int64_t page = small ? (int64_t)((uint32_t)slot / a.page_size) : slot / a.page_size;
+    const int64_t r = slot - page * a.page_size;
+    E* pk = reinterpret_cast<E*>(a.dst_k + page * a.dk[0] + h * a.dk[1] + r * a.dk[2] + d * a.dk[3]);
+    E* pv = reinterpret_cast<E*>(a.dst_v + page * a.dv[0] + h * a.dv[1] + r * a.dv[2] + d * a.dv[3]);
+    if constexpr (VEC == 8) {
+      *pk = val[0];
+      *pv = val[1];
+    } else {
+      *pk = (uint16_t)val[0].x;
+      *pv = (uint16_t)val[1].x;
+    }
+  }
+}
+
+template <int VEC, int U>
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs a) {
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  const uint32_t side = a.block_tokens ? a.block_tokens : 1;
+  const uint32_t local = a.block_tokens ? threadIdx.x / a.per_token : 0;
+  if (local >= side) return;
+  const uint32_t vec0 = threadIdx.x - local * (a.block_tokens ? a.per_token : 0);
+  const uint64_t step = (uint64_t)gridDim.x * side * U;
+  for (uint64_t base = (uint64_t)blockIdx.x * side * U; base < a.T; base += step) {
+    int64_t slot[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const uint64_t t = base + u * side + local;
+      slot[u] = t < a.T ? a.slots[t] : -1;
+      if (slot[u] >= a.num_slots) slot[u] = -1;  // no such slot: the token is not stored
+    }
+    for (uint32_t vec = vec0; vec < a.per_token; vec += kAppendThreads) {
+      uint4 val[U][2];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (slot[u] >= 0) move_token<VEC>(a, slot[u], (uint32_t)(base + u * side + local), vec, true, val[u]);
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (slot[u] >= 0) move_token<VEC>(a, slot[u], (uint32_t)(base + u * side + local), vec, false, val[u]);
+    }
+  }
+}
+
+bool vec_ok(const kf_tensor4* t) {
+  if (!kf::aligned16(t->ptr) || t->stride[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t->size[i] > 1 && (t->stride[i] % 8) != 0) return false;
+  return true;
+}
+
+// ---------------------------------------------------------------- tables
+// Both kernels below are prefix sums over requests followed by independent
+// writes; they move a few bytes per token and page, so latency bounds them.
+// They run as ONE cluster of up to 8 blocks: every block scans all requests
+// itself (reading 8 bytes per request is cheaper than a second launch), takes
+// its share of the writes, and the cluster barrier lets block 0 replace the
+// lengths and the stack count in place once nobody reads the old ones.
+constexpr int kTableThreads = 512;
+constexpr int kTableWarps = kTableThreads / 32;
+constexpr int kMaxCluster = 8;
+constexpr int64_t kMaxRequests = 16384;  // 9 bytes of shared memory each
+
+__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page_size) {
+  const uint32_t q = tokens / page_size;
+  return q + (tokens != q * page_size);
+}
+
+__device__ __forceinline__ int32_t saturate(int64_t x) { return x > 0x7fffffff ? 0x7fffffff : (int32_t)x; }
+
+// Inclusive sum of x over the block's threads; every thread also gets the
+// block's total.  `part` holds one value per warp and is reused by the next call.
+__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+  for (int off = 1; off < 32; off <<= 1) {
+    const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
+    if (lane >= off) x += y;
+  }
+  __syncthreads();  // the previous call's readers are done with part
+  if (lane == 31) part[warp] = x;
+  __syncthreads();
+  int64_t before = 0;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kTableWarps; ++w) {
+    const int64_t p = part[w];
+    if (w < warp) before += p;
+    total += p;
+  }
+  return x + before;
+}
+
+// Largest i in [0, n) with v[i] <= x (v is nondecreasing and v[0] <= x).
+__device__ __forceinline__ int last_at_most(const int32_t* v, int n, int64_t x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (v[mid] <= x)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  return lo;
+}
+
+struct ReserveArgs {
+  const int32_t* lengths;
+  const int32_t* added;
+  int32_t* table;
+  const int32_t* free_pages;
+  const int32_t* free_count;
+  int64_t* slots;
+  int32_t* starts;
+  int32_t* lengths_out;
+  int32_t* free_count_out;
+  int64_t table_stride;
+  int64_t T;
+  uint32_t padded;  // 0: tokens request after request; else the slots of each request
+  int B;
+  uint32_t max_pages, page_size, num_pages;
+};
+
+// need_b = ceil((len_b + new_b) / page) - ceil(len_b / page), 0 where the
+// request would outgrow its table row (or its padded slots); upto = inclusive
+// sum of need.  A request is granted when it fits and upto_b <= free_count (or it
+// needs no page); the granted requests that need pages are then a prefix, so
+// request b takes the stack entries free_count - 1 - (upto_b - need_b) - j.
+__global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const ReserveArgs a) {
+  extern __shared__ int32_t sm[];
+  int32_t* starts = sm;               // [B + 1] first token of each request
+  int32_t* first = sm + a.B + 1;      // [B] pages taken by the requests before it
+  uint8_t* refused = reinterpret_cast<uint8_t*>(first + a.B);
+  __shared__ int64_t part[kTableWarps];
+  __shared__ int taken_s;
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x;
+  const unsigned rank = blockIdx.x, blocks = gridDim.x;  // the grid is one cluster
+  if (tid == 0) taken_s = 0;
+  int32_t count = *a.free_count;
+  count = count < 0 ? 0 : (uint32_t)count > a.num_pages ? (int32_t)a.num_pages : count;
+
+  int64_t tokens = 0, pages = 0;  // of the requests of earlier rounds
+  for (int base = 0; base < a.B; base += kTableThreads) {
+    const int b = base + tid;
+    uint32_t len = 0, add = 0;
+    if (b < a.B) {
+      len = (uint32_t)max(a.lengths[b], 0);
+      add = (uint32_t)max(a.added[b], 0);
+    }
+    const uint32_t before = pages_of(len, a.page_size), after = pages_of(len + add, a.page_size);
+    const bool fits = after <= a.max_pages && len + add <= 0x7fffffffu && (a.padded == 0 || add <= a.padded);
+    const int64_t need = fits ? after - before : 0;
+    int64_t add_total, need_total;
+    const int64_t add_upto = tokens + block_scan(add, part, add_total);
+    const int64_t upto = pages + block_scan(need, part, need_total);
+    if (b < a.B) {
+      const bool granted = fits && (need == 0 || upto <= count);
+      starts[b] = saturate(a.padded ? (int64_t)b * a.padded : add_upto - add);
+      first[b] = saturate(upto - need);
+      refused[b] = !granted;
+      if (granted && need > 0) atomicMax(&taken_s, (int)upto);  // a maximum: the order does not matter
+    }
+    tokens += add_total;
+    pages += need_total;
+  }
+  if (tid == 0) starts[a.B] = saturate(a.padded ? (int64_t)a.B * a.padded : tokens);
+  __syncthreads();
+  const int taken = taken_s;
+
+  // new entries of the block table: stack entry count - 1 - p is the p-th page taken
+  for (int64_t p = (int64_t)rank * kTableThreads + tid; p < taken; p += (int64_t)blocks * kTableThreads) {
+    const int b = last_at_most(first, a.B, p);
+    const uint32_t before = pages_of((uint32_t)max(a.lengths[b], 0), a.page_size);
+    a.table[b * a.table_stride + before + (p - first[b])] = a.free_pages[count - 1 - p];
+  }
+  // slots, four consecutive tokens a thread
+  const int64_t quads = (a.T + 3) / 4;
+  for (int64_t i = (int64_t)rank * kTableThreads + tid; i < quads; i += (int64_t)blocks * kTableThreads) {
+    const int64_t t0 = i * 4;
+    int b = last_at_most(starts, a.B, t0);
+    int known_b = -1;
+    uint32_t known_page = 0;
+    int64_t slot[4], page = -1;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int64_t t = t0 + e;
+      while (b + 1 < a.B && starts[b + 1] <= t) ++b;
+      slot[e] = -1;
+      if (t >= starts[a.B] || refused[b] || (a.padded && t - starts[b] >= a.added[b])) continue;
+      const uint32_t len = (uint32_t)max(a.lengths[b], 0);
+      const uint32_t pos = len + (uint32_t)(t - starts[b]);
+      const uint32_t j = pos / a.page_size;
+      if (b != known_b || j != known_page) {  // most tokens share the page of the one before
+        const uint32_t before = pages_of(len, a.page_size);
+        page = j < before ? a.table[b * a.table_stride + j] : a.free_pages[count - 1 - (first[b] + (int64_t)(j - before))];
+        known_b = b;
+        known_page = j;
+      }
+      if (page >= 0 && page < a.num_pages) slot[e] = page * a.page_size + (pos - j * a.page_size);
+    }
+    if (t0 + 4 <= a.T) {
+      longlong2* dst = reinterpret_cast<longlong2*>(a.slots + t0);
+      dst[0] = make_longlong2(slot[0], slot[1]);
+      dst[1] = make_longlong2(slot[2], slot[3]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (t0 + e < a.T) a.slots[t0 + e] = slot[e];
+    }
+  }
+  // lengths_out and free_count_out may be lengths and free_count themselves
+  cluster.sync();
+  if (rank == 0) {
+    for (int b = tid; b < a.B; b += kTableThreads) {
+      const int32_t len = max(a.lengths[b], 0);
+      a.lengths_out[b] = refused[b] ? len : len + max(a.added[b], 0);
+    }
+    for (int b = tid; b <= a.B; b += kTableThreads) a.starts[b] = starts[b];
+    if (tid == 0) *a.free_count_out = count - taken;
+  }
+}
+
+struct ReleaseArgs {
+  const int32_t* lengths;
+  const uint8_t* finished;
+  const int32_t* table;
+  int32_t* free_pages;
+  const int32_t* free_count;
+  int32_t* lengths_out;
+  int32_t* free_count_out;
+  int64_t table_stride;
+  int B;
+  uint32_t max_pages, page_size, num_pages;
+};
+
+// One warp per request, twice: count the row's valid entries (a row may hold
+// -1 where a page was given up earlier), then, after a prefix sum over
+// requests, write them to the stack in order.  The counts reach every block
+// through distributed shared memory.
+__global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const ReleaseArgs a) {
+  extern __shared__ int32_t sm[];
+  int32_t* counts = sm;  // [B] valid pages of each request, then their exclusive sum
+  __shared__ int64_t part[kTableWarps];
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();  // every block has started: its shared memory may be written
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const unsigned rank = blockIdx.x, blocks = gridDim.x;
+  int32_t count = *a.free_count;
+  count = count < 0 ? 0 : (uint32_t)count > a.num_pages ? (int32_t)a.num_pages : count;
+
+  auto row_pages = [&](int b) -> uint32_t {
+    if (!a.finished[b]) return 0;
+    return min(pages_of((uint32_t)max(a.lengths[b], 0), a.page_size), a.max_pages);
+  };
+  for (int b = rank * kTableWarps + warp; b < a.B; b += blocks * kTableWarps) {
+    const uint32_t n = row_pages(b);
+    const int32_t* row = a.table + b * a.table_stride;
+    int c = 0;
+#pragma unroll 4
+    for (uint32_t j = lane; j < n; j += 32) c += (uint32_t)row[j] < a.num_pages;
+    c = __reduce_add_sync(0xffffffffu, c);
+    if (lane < (int)blocks) cluster.map_shared_rank(counts, lane)[b] = c;
+  }
+  cluster.sync();
+  int64_t total = 0;
+  for (int base = 0; base < a.B; base += kTableThreads) {
+    const int b = base + tid;
+    const int32_t c = b < a.B ? counts[b] : 0;
+    int64_t round;
+    const int64_t upto = total + block_scan(c, part, round);
+    if (b < a.B) counts[b] = saturate(upto - c);
+    total += round;
+  }
+  __syncthreads();
+  for (int b = rank * kTableWarps + warp; b < a.B; b += blocks * kTableWarps) {
+    const uint32_t n = row_pages(b);
+    const int32_t* row = a.table + b * a.table_stride;
+    int64_t at = (int64_t)count + counts[b];
+    for (uint32_t j0 = 0; j0 < n; j0 += 32) {
+      const int32_t page = j0 + lane < n ? row[j0 + lane] : -1;
+      const bool valid = (uint32_t)page < a.num_pages;
+      const unsigned mask = __ballot_sync(0xffffffffu, valid);
+      const int64_t to = at + __popc(mask & ((1u << lane) - 1));
+      if (valid && to < a.num_pages) a.free_pages[to] = page;  // a stack that is full keeps what it has
+      at += __popc(mask);
+    }
+  }
+  cluster.sync();
+  if (rank == 0) {
+    for (int b = tid; b < a.B; b += kTableThreads) a.lengths_out[b] = a.finished[b] ? 0 : max(a.lengths[b], 0);
+    if (tid == 0) *a.free_count_out = (int32_t)min((int64_t)a.num_pages, count + total);
+  }
+}
+
+int check_tables(const char* what, const void* lengths, const void* second, int64_t B, const void* table,
+                 int64_t max_pages, int64_t table_stride, const void* free_pages, int64_t num_pages,
+                 const void* free_count, int64_t page_size, const void* lengths_out, const void* free_count_out) {
+  using kf::set_error;
+  if (!lengths || !second || !table || !free_pages || !free_count || !lengths_out || !free_count_out)
+    return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (B <= 0 || max_pages <= 0 || num_pages <= 0)
+    return set_error(KF_ERR_INVALID, "%s: requests, table columns and pages must be non-zero", what);
+  if (page_size <= 0 || page_size > (1 << 20))
+    return set_error(KF_ERR_INVALID, "%s: page_size must be in [1, 2^20]", what);
+  if (B > 1 && table_stride < max_pages)
+    return set_error(KF_ERR_INVALID, "%s: block table rows overlap", what);
+  if (B > kMaxRequests)
+    return set_error(KF_ERR_UNSUPPORTED, "%s: at most %lld requests", what, (long long)kMaxRequests);
+  if (max_pages > 0x7fffffffLL || num_pages > 0x7fffffffLL)
+    return set_error(KF_ERR_UNSUPPORTED, "%s: too many pages", what);
+  return KF_OK;
+}
+
+template <typename... KArgs>
+int raise_smem(void (*kern)(KArgs...), size_t smem, const char* what) {
+  if (smem > 48 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return kf::set_error(KF_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory", what, smem);
+  }
+  return KF_OK;
+}
+
+unsigned cluster_for(int64_t units, int64_t per_block) {
+  int64_t n = (units + per_block - 1) / per_block;
+  if (n <= 1) return 1;
+  if (n <= 2) return 2;
+  if (n <= 4) return 4;
+  return kMaxCluster;
+}
+
+}  // namespace
+
+extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pages, const kf_tensor4* new_k,
+                               const kf_tensor4* new_v, const int64_t* slots, int dtype, void* stream) {
+  using kf::set_error;
+  if (!k_pages || !v_pages || !new_k || !new_v)
+    return set_error(KF_ERR_INVALID, "kf_paged_append: null tensor descriptor");
+  if (dtype != KF_F16 && dtype != KF_BF16)
+    return set_error(KF_ERR_INVALID, "kf_paged_append: dtype must be fp16 or bf16");
+  for (int i = 0; i < 4; ++i) {
+    if (k_pages->size[i] != v_pages->size[i])
+      return set_error(KF_ERR_INVALID, "kf_paged_append: K/V page shapes must match");
+    if (new_k->size[i] != new_v->size[i])
+      return set_error(KF_ERR_INVALID, "kf_paged_append: new K/V shapes must match");
+  }
+  const int64_t N = new_k->size[0], H = new_k->size[1], S = new_k->size[2], D = new_k->size[3];
+  if (H != k_pages->size[1] || D != k_pages->size[3])
+    return set_error(KF_ERR_INVALID, "kf_paged_append: new K/V heads and head_dim must match the pages");
+  if (N <= 0 || H <= 0 || S <= 0 || D <= 0 || k_pages->size[0] <= 0 || k_pages->size[2] <= 0)
+    return set_error(KF_ERR_INVALID, "kf_paged_append: dimensions must be non-zero");
+  if (N > 0x7fffffffLL || S > 0x7fffffffLL || N * S > 0x7fffffffLL || H > 0x7fffffffLL || D > 0x7fffffffLL ||
+      H * D > 0x7fffffffLL || k_pages->size[2] > (1 << 20))
+    return set_error(KF_ERR_UNSUPPORTED, "kf_paged_append: tensors too large");
+  if (!k_pages->ptr || !v_pages->ptr || !new_k->ptr || !new_v->ptr || !slots)
+    return set_error(KF_ERR_INVALID, "kf_paged_append: null data pointer");
+  kf::DeviceGuard guard(k_pages->ptr);
+  if (guard.status()) return guard.status();
+
+  AppendArgs a;
+  a.src_k = static_cast<const uint16_t*>(new_k->ptr);
+  a.src_v = static_cast<const uint16_t*>(new_v->ptr);
+  a.dst_k = static_cast<uint16_t*>(k_pages->ptr);
+  a.dst_v = static_cast<uint16_t*>(v_pages->ptr);
+  a.slots = slots;
+  for (int i = 0; i < 4; ++i) {
+    a.sk[i] = new_k->stride[i];
+    a.sv[i] = new_v->stride[i];
+    a.dk[i] = k_pages->stride[i];
+    a.dv[i] = v_pages->stride[i];
+  }
+  const bool vec = D % 8 == 0 && vec_ok(k_pages) && vec_ok(v_pages) && vec_ok(new_k) && vec_ok(new_v);
+  a.num_slots = k_pages->size[0] * k_pages->size[2];
+  a.T = (uint32_t)(N * S);
+  a.S = (uint32_t)S;
+  a.per_head = (uint32_t)(vec ? D / 8 : D);
+  a.per_token = (uint32_t)H * a.per_head;
+  a.page_size = (uint32_t)k_pages->size[2];
+  a.block_tokens = a.per_token <= kAppendThreads ? kAppendThreads / a.per_token : 0;
+  const int64_t side = a.block_tokens ? a.block_tokens : 1;
+  const int64_t sms = kf::sm_count_current_device();
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto go = [&](auto kern, int64_t per_block) {
+    int64_t blocks = (a.T + per_block - 1) / per_block;
+    if (blocks > sms * 64) blocks = sms * 64;
+    return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, "kf_paged_append", a);
+  };
+  if (!vec) return go(paged_append_kernel<1, 1>, side);
+  return a.T >= side * 4 * sms * 2 ? go(paged_append_kernel<8, 4>, side * 4) : go(paged_append_kernel<8, 1>, side);
+}
+
+extern "C" int kf_paged_reserve(const int32_t* lengths, const int32_t* new_lengths, int64_t B, int32_t* block_table,
+                                int64_t max_pages, int64_t table_stride, const int32_t* free_pages,
+                                int64_t num_pages, const int32_t* free_count, int64_t page_size, int64_t* slots,
+                                int64_t num_tokens, int64_t tokens_per_request, int32_t* starts,
+                                int32_t* lengths_out, int32_t* free_count_out, void* stream) {
+  using kf::set_error;
+  const char* what = "kf_paged_reserve";
+  int rc = check_tables(what, lengths, new_lengths, B, block_table, max_pages, table_stride, free_pages, num_pages,
+                        free_count, page_size, lengths_out, free_count_out);
+  if (rc != KF_OK) return rc;
+  if (num_tokens < 0 || num_tokens > 0x7fffffffLL)
+    return set_error(KF_ERR_INVALID, "%s: num_tokens must be in [0, 2^31)", what);
+  if (tokens_per_request < 0 || (tokens_per_request > 0 && tokens_per_request * B != num_tokens))
+    return set_error(KF_ERR_INVALID, "%s: num_tokens must be tokens_per_request for each request", what);
+  if (!starts || (num_tokens > 0 && !slots)) return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (num_tokens > 0 && !kf::aligned16(slots))
+    return set_error(KF_ERR_INVALID, "%s: slots must be 16-byte aligned", what);
+  kf::DeviceGuard guard(lengths);
+  if (guard.status()) return guard.status();
+  ReserveArgs a;
+  a.lengths = lengths;
+  a.added = new_lengths;
+  a.table = block_table;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.slots = slots;
+  a.starts = starts;
+  a.lengths_out = lengths_out;
+  a.free_count_out = free_count_out;
+  a.table_stride = table_stride;
+  a.T = num_tokens;
+  a.padded = (uint32_t)tokens_per_request;
+  a.B = (int)B;
+  a.max_pages = (uint32_t)max_pages;
+  a.page_size = (uint32_t)page_size;
+  a.num_pages = (uint32_t)num_pages;
+  const size_t smem = (size_t)(2 * B + 1) * 4 + (size_t)B;
+  rc = raise_smem(paged_reserve_kernel, smem, what);
+  if (rc != KF_OK) return rc;
+  const unsigned cluster = cluster_for(num_tokens, kTableThreads * 4);
+  return kf::launch_dependent_cluster(paged_reserve_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
+                                      static_cast<cudaStream_t>(stream), what, a);
+}
+
+extern "C" int kf_paged_release(const int32_t* lengths, const uint8_t* finished, int64_t B,
+                                const int32_t* block_table, int64_t max_pages, int64_t table_stride,
+                                int32_t* free_pages, int64_t num_pages, const int32_t* free_count,
+                                int64_t page_size, int32_t* lengths_out, int32_t* free_count_out, void* stream) {
+  const char* what = "kf_paged_release";
+  int rc = check_tables(what, lengths, finished, B, block_table, max_pages, table_stride, free_pages, num_pages,
+                        free_count, page_size, lengths_out, free_count_out);
+  if (rc != KF_OK) return rc;
+  kf::DeviceGuard guard(lengths);
+  if (guard.status()) return guard.status();
+  ReleaseArgs a;
+  a.lengths = lengths;
+  a.finished = finished;
+  a.table = block_table;
+  a.free_pages = free_pages;
+  a.free_count = free_count;
+  a.lengths_out = lengths_out;
+  a.free_count_out = free_count_out;
+  a.table_stride = table_stride;
+  a.B = (int)B;
+  a.max_pages = (uint32_t)max_pages;
+  a.page_size = (uint32_t)page_size;
+  a.num_pages = (uint32_t)num_pages;
+  const size_t smem = (size_t)B * 4;
+  rc = raise_smem(paged_release_kernel, smem, what);
+  if (rc != KF_OK) return rc;
+  const unsigned cluster = cluster_for(B, kTableWarps);
+  return kf::launch_dependent_cluster(paged_release_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
+                                      static_cast<cudaStream_t>(stream), what, a);
+}

@@ -1,0 +1,387 @@
+# SPDX-License-Identifier: Apache-2.0
+"""Paged KV cache: many requests of different lengths in one pool of pages.
+
+``PreallocatedKVCache`` gives every batch entry the same length and its full
+capacity from the start.  Here the K and V rows of all requests lie in pools
+``[pages, Hkv, page_size, D]``; a block table names each request's pages in
+order, and the pages that nobody owns form a stack on the GPU.  Everything a
+serving step needs is computed on the device from the device's own lengths,
+so no call synchronises and a CUDA graph of a step follows the lengths:
+
+* ``reserve_pages``: pages, table entries and slots for the tokens that each
+  request brings;
+* ``append_paged_kv``: K/V rows to their slots (prompts);
+* ``paged_attention``: one new token per request over its pages, with the
+  append of that token's own K/V row fused in on request (generation);
+* ``release_pages``: the pages of finished requests back to the stack;
+* ``PagedKVCache``: the pools, tables and stack, and these calls on them.
+
+fp16 and bf16, head dims that are multiples of 8 in [16, 128], on an sm_100
+device through ``libkotflash_b200.so``; nothing falls back to another
+implementation.  Inference only.  The reference has no paging
+(``kotflash/cache.py:91-98``).
+"""
+from __future__ import annotations
+
+import math
+from functools import lru_cache
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _ext
+
+_DTYPES = {torch.float16: _ext.KF_F16, torch.bfloat16: _ext.KF_BF16}
+
+
+def _check_device(what: str, *tensors: torch.Tensor) -> int:
+    """Index of the one sm_100 device that holds all tensors."""
+    dev = tensors[0].device
+    if dev.type != "cuda":
+        raise RuntimeError(f"{what} requires CUDA tensors on an sm_100 (B200) device")
+    for t in tensors:
+        if t.device != dev:
+            raise ValueError(f"{what}: all tensors must be on the same device")
+    if not _ext.is_sm100(dev.index):
+        raise RuntimeError(f"{what} requires an sm_100 (B200) CUDA device")
+    return dev.index
+
+
+def _check_pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, *others: torch.Tensor) -> int:
+    """Dtype code shared by the pools and the other K/V or query tensors."""
+    dtype = k_pages.dtype
+    for t in (v_pages, *others):
+        if t.dtype != dtype:
+            raise ValueError(f"{what}: dtypes must match")
+    for t in (k_pages, v_pages, *others):
+        if t.ndim != 4:
+            raise ValueError(f"{what}: expected 4-D tensors, pages in [pages, Hkv, page_size, D] layout")
+    code = _DTYPES.get(dtype)
+    if code is None:
+        raise TypeError(f"{what} supports float16 and bfloat16, got {dtype}")
+    return code
+
+
+def _check_inference(what: str, *tensors: torch.Tensor) -> None:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t.requires_grad:
+                raise RuntimeError(f"{what} is inference-only; disable gradients")
+
+
+def _check_int32(what: str, **tensors: torch.Tensor) -> None:
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: {name} must be a torch.Tensor")
+        if t.dtype != torch.int32:
+            raise TypeError(f"{what}: {name} must be int32")
+
+
+def _check_table(what: str, block_table: torch.Tensor, requests: int) -> None:
+    if block_table.ndim != 2 or block_table.shape[0] != requests:
+        raise ValueError(f"{what}: block_table must be [requests, max_pages]")
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        raise ValueError(f"{what}: block_table rows must be contiguous")
+
+
+@lru_cache(maxsize=256)
+def _workspace_bytes(hq: int, hkv: int, d: int, device_index: int) -> int:
+    return max(16, _ext.load().kf_paged_decode_workspace_bytes(hq, hkv, d, _ext.sm_count(device_index)))
+
+
+def paged_attention(
+    q: torch.Tensor,
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    block_table: torch.Tensor,
+    lengths: torch.Tensor,
+    *,
+    scale: Optional[float] = None,
+    new_k: Optional[torch.Tensor] = None,
+    new_v: Optional[torch.Tensor] = None,
+    slots: Optional[torch.Tensor] = None,
+    return_lse: bool = False,
+) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+    """Attention of one new token per request over a paged KV cache.
+
+    q is [B, Hq, 1, D]; k_pages and v_pages are [pages, Hkv, page_size, D]
+    with any strides whose rows are contiguous and 16-byte aligned;
+    block_table is int32 [B, max_pages] and lengths int32 [B].  Request b's
+    token attends to positions 0 .. lengths[b] - 1, position p being row
+    p % page_size of page block_table[b, p // page_size].  Positions whose
+    table entry is not a page of the pool (-1, say) are masked, and nothing
+    masked is read.  A request that sees nothing yields 0 (LSE -inf).
+
+    new_k and new_v [B, Hkv, 1, D] with slots (int64 [B]) append on the way:
+    where slots[b] >= 0, the slot of position lengths[b] - 1, that position's
+    row is new_k[b] / new_v[b], which is written to its page and attended to in
+    the same launch (lengths already counts it, and no other request may read
+    the slot); where slots[b] < 0 the request has no new row.  Returns [B, Hq, 1, D] in q's dtype and, with return_lse, the
+    fp32 LSE [B, Hq, 1].
+    """
+    what = "paged_attention"
+    if not (isinstance(q, torch.Tensor) and isinstance(k_pages, torch.Tensor) and isinstance(v_pages, torch.Tensor)):
+        raise TypeError("q, k_pages and v_pages must be torch.Tensor instances")
+    _check_int32(what, block_table=block_table, lengths=lengths)
+    if (new_k is None) != (new_v is None) or (new_k is None) != (slots is None):
+        raise ValueError(f"{what}: new_k, new_v and slots go together")
+    rows = () if new_k is None else (new_k, new_v)
+    if rows and not (isinstance(new_k, torch.Tensor) and isinstance(new_v, torch.Tensor)
+                     and isinstance(slots, torch.Tensor)):
+        raise TypeError("new_k, new_v and slots must be torch.Tensor instances")
+    dtype = _check_pools(what, k_pages, v_pages, q, *rows)
+    b, hq, _, d = q.shape
+    _check_table(what, block_table, b)
+    if lengths.ndim != 1 or lengths.shape[0] != b or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths must be a contiguous [requests] tensor")
+    if rows:
+        if slots.dtype != torch.int64:
+            raise TypeError(f"{what}: slots must be int64")
+        if slots.ndim != 1 or slots.shape[0] != b or not slots.is_contiguous():
+            raise ValueError(f"{what}: slots must be a contiguous [requests] tensor")
+    if scale is None:
+        scale = 1.0 / math.sqrt(d) if d else 1.0
+    else:
+        try:
+            scale = float(scale)
+        except (TypeError, ValueError) as exc:
+            raise TypeError("scale must be a finite real number or None") from exc
+        if not math.isfinite(scale):
+            raise ValueError("scale must be finite")
+    hkv = k_pages.shape[1]
+    if b == 0 or hq == 0 or hkv == 0:
+        raise ValueError(f"{what}: batch and head dimensions must be non-zero")
+    if hq % hkv:
+        raise ValueError("num_query_heads must be divisible by num_kv_heads (GQA/MQA)")
+    _check_inference(what, q, k_pages, v_pages, *rows)
+    idx = _check_device(what, q, k_pages, v_pages, block_table, lengths, *rows, *((slots,) if rows else ()))
+    lib = _ext.load()
+    dev = q.device
+    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+    lse = torch.empty((b, hq, 1), dtype=torch.float32, device=dev) if return_lse else None
+    ws_bytes = _workspace_bytes(hq, hkv, d, idx)
+    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
+    rc = lib.kf_paged_decode(
+        _ext.packed4(q), _ext.packed4(k_pages), _ext.packed4(v_pages), block_table.data_ptr(),
+        block_table.shape[1], block_table.stride(0), lengths.data_ptr(),
+        _ext.packed4(new_k) if rows else None, _ext.packed4(new_v) if rows else None,
+        slots.data_ptr() if rows else None, _ext.packed4(out), lse.data_ptr() if return_lse else None, dtype, scale,
+        workspace.data_ptr(), ws_bytes, _ext.stream_of(q),
+    )
+    _ext.check(rc, "kf_paged_decode")
+    return (out, lse) if return_lse else out
+
+
+def append_paged_kv(
+    k_pages: torch.Tensor,
+    v_pages: torch.Tensor,
+    new_k: torch.Tensor,
+    new_v: torch.Tensor,
+    slots: torch.Tensor,
+) -> None:
+    """Copy K/V rows into the pages of a pool, bit for bit.
+
+    new_k and new_v are [N, Hkv, S, D] with any strides; token t = n * S + s
+    goes to slot slots[t] (int64 [N * S]), that is row slots[t] % page_size of
+    page slots[t] // page_size.  Tokens whose slot is outside the pool (-1 for
+    those that ``reserve_pages`` refused) are skipped.
+    """
+    what = "append_paged_kv"
+    if not all(isinstance(t, torch.Tensor) for t in (k_pages, v_pages, new_k, new_v, slots)):
+        raise TypeError("pages, new K/V values and slots must be torch.Tensor instances")
+    dtype = _check_pools(what, k_pages, v_pages, new_k, new_v)
+    if slots.dtype != torch.int64:
+        raise TypeError(f"{what}: slots must be int64")
+    if slots.ndim != 1 or slots.shape[0] != new_k.shape[0] * new_k.shape[2] or not slots.is_contiguous():
+        raise ValueError(f"{what}: slots must be a contiguous [tokens] tensor, one slot for each new K/V row")
+    _check_inference(what, k_pages, v_pages, new_k, new_v)
+    _check_device(what, k_pages, v_pages, new_k, new_v, slots)
+    lib = _ext.load()
+    rc = lib.kf_paged_append(_ext.packed4(k_pages), _ext.packed4(v_pages), _ext.packed4(new_k), _ext.packed4(new_v),
+                             slots.data_ptr(), dtype, _ext.stream_of(k_pages))
+    _ext.check(rc, "kf_paged_append")
+
+
+def _check_tables(what, lengths, second, block_table, free_pages, free_count, lengths_out, free_count_out):
+    _check_int32(what, lengths=lengths, block_table=block_table, free_pages=free_pages, free_count=free_count)
+    if lengths.ndim != 1 or second.shape != lengths.shape:
+        raise ValueError(f"{what}: lengths and the per-request tensor beside it must both be [requests]")
+    _check_table(what, block_table, lengths.shape[0])
+    if free_pages.ndim != 1 or free_count.numel() != 1:
+        raise ValueError(f"{what}: free_pages must be [pages] and free_count hold one number")
+    outs = [t for t in (lengths_out, free_count_out) if t is not None]
+    for t, like, name in ((lengths_out, lengths, "lengths_out"), (free_count_out, free_count, "free_count_out")):
+        if t is not None:
+            _check_int32(what, **{name: t})
+            if t.shape != like.shape:
+                raise ValueError(f"{what}: {name} has the wrong shape")
+    if not all(t.is_contiguous() for t in (lengths, second, free_pages, free_count, *outs)):
+        raise ValueError(f"{what}: lengths, free_pages and free_count must be contiguous")
+    _check_device(what, lengths, second, block_table, free_pages, free_count, *outs)
+
+
+def reserve_pages(
+    lengths: torch.Tensor,
+    new_lengths: torch.Tensor,
+    block_table: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_count: torch.Tensor,
+    *,
+    page_size: int,
+    num_tokens: Optional[int] = None,
+    tokens_per_request: Optional[int] = None,
+    lengths_out: Optional[torch.Tensor] = None,
+    free_count_out: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """Pages, table entries and slots for the tokens that each request brings.
+
+    All tensors int32: lengths and new_lengths [B]; block_table [B, max_pages],
+    completed in place; free_pages [pages], of which the first free_count [1]
+    entries are a stack of the pages that nobody owns.  Requests are served in
+    order.  One whose pages would not fit its table row, or that the stack
+    cannot serve after those before it, is refused: its length stays, and its
+    tokens get slot -1.
+
+    Slots are packed or padded.  num_tokens is the number of packed slots to
+    write, request after request, normally the sum of new_lengths (a larger one
+    leaves -1 behind them, so that a captured step can keep one size).
+    tokens_per_request gives every request that many, with -1 behind its last
+    token: the slots of rows [B, Hkv, tokens_per_request, D].  A request that
+    brings more is refused.  Returns ``(slots, starts, lengths_out,
+    free_count_out)``: int64 slots; int32 starts [B + 1], where each request's
+    slots begin; the new lengths and count.  lengths_out=lengths and free_count_out=free_count update in place.
+    """
+    what = "reserve_pages"
+    _check_int32(what, new_lengths=new_lengths)
+    _check_tables(what, lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out)
+    lib = _ext.load()
+    dev = lengths.device
+    b = lengths.shape[0]
+    if (num_tokens is None) == (tokens_per_request is None):
+        raise ValueError(f"{what}: give num_tokens or tokens_per_request")
+    per_request = 0
+    if num_tokens is None:
+        per_request = tokens_per_request
+        if per_request <= 0:
+            raise ValueError(f"{what}: tokens_per_request must be positive")
+        num_tokens = per_request * b
+    elif num_tokens < 0:
+        raise ValueError(f"{what}: num_tokens must not be negative")
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
+    starts = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    if lengths_out is None:
+        lengths_out = torch.empty_like(lengths)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    rc = lib.kf_paged_reserve(
+        lengths.data_ptr(), new_lengths.data_ptr(), b, block_table.data_ptr(), block_table.shape[1],
+        block_table.stride(0), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size,
+        slots.data_ptr(), num_tokens, per_request, starts.data_ptr(), lengths_out.data_ptr(), free_count_out.data_ptr(),
+        _ext.stream_of(lengths),
+    )
+    _ext.check(rc, "kf_paged_reserve")
+    return slots, starts, lengths_out, free_count_out
+
+
+def release_pages(
+    lengths: torch.Tensor,
+    finished: torch.Tensor,
+    block_table: torch.Tensor,
+    free_pages: torch.Tensor,
+    free_count: torch.Tensor,
+    *,
+    page_size: int,
+    lengths_out: Optional[torch.Tensor] = None,
+    free_count_out: Optional[torch.Tensor] = None,
+) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Push the pages of finished requests (bool [B]) on the stack.
+
+    In order of requests and positions, into free_pages in place; entries that
+    are no pages of the pool are left out.  Returns ``(lengths_out,
+    free_count_out)``, the finished requests' lengths being 0; their table
+    rows keep old entries, which no length reaches any more.
+    """
+    what = "release_pages"
+    if not isinstance(finished, torch.Tensor) or finished.dtype != torch.bool:
+        raise TypeError(f"{what}: finished must be a bool tensor")
+    _check_tables(what, lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out)
+    lib = _ext.load()
+    if lengths_out is None:
+        lengths_out = torch.empty_like(lengths)
+    if free_count_out is None:
+        free_count_out = torch.empty_like(free_count)
+    rc = lib.kf_paged_release(
+        lengths.data_ptr(), finished.data_ptr(), lengths.shape[0], block_table.data_ptr(), block_table.shape[1],
+        block_table.stride(0), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size,
+        lengths_out.data_ptr(), free_count_out.data_ptr(), _ext.stream_of(lengths),
+    )
+    _ext.check(rc, "kf_paged_release")
+    return lengths_out, free_count_out
+
+
+class PagedKVCache:
+    """Pools, block table, lengths and free stack of a batch of request slots.
+
+    ``layers`` pools share one block table, so a step reserves once and then
+    appends and attends layer by layer.  Row b of the table belongs to request
+    slot b; a slot of length 0 is empty.  Not thread-safe.
+
+        cache = PagedKVCache(pages, 16, hkv, d, max_requests, max_pages, device=..., dtype=...)
+        slots, starts = cache.reserve(prompt_lengths, num_tokens=n)  # prompts
+        cache.append(k, v, slots)                                    # [1, Hkv, n, D]
+        slots, _ = cache.reserve(active, tokens_per_request=1)       # then, token by token
+        out = cache.append_and_attend(q, k, v, slots)                # [max_requests, Hq, 1, D]
+        cache.release(finished)
+    """
+
+    def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_requests: int,
+                 max_pages: int, *, layers: int = 1, device: Union[torch.device, str],
+                 dtype: torch.dtype) -> None:
+        dims = {"num_pages": num_pages, "page_size": page_size, "kv_heads": kv_heads, "head_dim": head_dim,
+                "max_requests": max_requests, "max_pages": max_pages, "layers": layers}
+        for name, value in dims.items():
+            if isinstance(value, bool) or not isinstance(value, int) or value <= 0:
+                raise ValueError(f"{name} must be a positive integer")
+        self.page_size = page_size
+        self.k = torch.empty((layers, num_pages, kv_heads, page_size, head_dim), device=device, dtype=dtype)
+        self.v = torch.empty_like(self.k)
+        self.block_table = torch.full((max_requests, max_pages), -1, device=device, dtype=torch.int32)
+        self.lengths = torch.zeros(max_requests, device=device, dtype=torch.int32)
+        # the stack gives out page 0 first
+        self.free_pages = torch.arange(num_pages - 1, -1, -1, device=device, dtype=torch.int32)
+        self.free_count = torch.full((1,), num_pages, device=device, dtype=torch.int32)
+
+    def reserve(self, new_lengths: torch.Tensor, *, num_tokens: Optional[int] = None,
+                tokens_per_request: Optional[int] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Room for new_lengths (int32 [max_requests]) more tokens; advances
+        ``lengths``.  Returns ``(slots, starts)`` of ``reserve_pages``, packed
+        or padded as there."""
+        slots, starts, _, _ = reserve_pages(
+            self.lengths, new_lengths, self.block_table, self.free_pages, self.free_count,
+            page_size=self.page_size, num_tokens=num_tokens, tokens_per_request=tokens_per_request,
+            lengths_out=self.lengths, free_count_out=self.free_count)
+        return slots, starts
+
+    def append(self, new_k: torch.Tensor, new_v: torch.Tensor, slots: torch.Tensor, *, layer: int = 0) -> None:
+        """Store K/V rows [N, Hkv, S, D] at the slots that ``reserve`` gave."""
+        append_paged_kv(self.k[layer], self.v[layer], new_k, new_v, slots)
+
+    def attend(self, q: torch.Tensor, *, layer: int = 0, scale: Optional[float] = None,
+               return_lse: bool = False):
+        """One query token per request slot [max_requests, Hq, 1, D] over its pages."""
+        return paged_attention(q, self.k[layer], self.v[layer], self.block_table, self.lengths, scale=scale,
+                               return_lse=return_lse)
+
+    def append_and_attend(self, q: torch.Tensor, new_k: torch.Tensor, new_v: torch.Tensor, slots: torch.Tensor, *,
+                          layer: int = 0, scale: Optional[float] = None, return_lse: bool = False):
+        """Store the newest K/V row [max_requests, Hkv, 1, D] of every request
+        and attend, in one pass.  slots come from ``reserve`` with
+        tokens_per_request=1; requests without one there (no new token, or
+        refused) store nothing and attend to what they have."""
+        return paged_attention(q, self.k[layer], self.v[layer], self.block_table, self.lengths, scale=scale,
+                               new_k=new_k, new_v=new_v, slots=slots, return_lse=return_lse)
+
+    def release(self, finished: torch.Tensor) -> None:
+        """Give up the pages of the request slots marked in finished (bool [max_requests])."""
+        release_pages(self.lengths, finished, self.block_table, self.free_pages, self.free_count,
+                      page_size=self.page_size, lengths_out=self.lengths, free_count_out=self.free_count)
