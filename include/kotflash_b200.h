@@ -230,8 +230,8 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * (int32 [B, max_pages]).  q and o are [B, Hq, 1, D], lengths int32 [B].
  * Request b's token sees the positions below min(lengths[b], max_pages *
  * page_size) whose table entry lies in [0, pages); every other position
- * (other entries, -1 among them, the rest of a last page) is masked and its
- * memory is not read.  A request that sees nothing gets O = 0, LSE = -inf.
+ * (other entries, -1 among them, the rest of a last page) is masked whatever
+ * its memory holds, and no page but the table's is read.  A request that sees nothing gets O = 0, LSE = -inf.
  * lse [B, Hq] fp32 (natural log, contiguous) may be NULL.  All lengths and
  * tables are read on the device when the kernel runs.
  *
@@ -242,13 +242,15 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * new row.
  *
  * 16 <= D <= 128, D % 8 == 0.  `workspace` holds
- * kf_paged_decode_workspace_bytes(...) bytes; sm_count is that of the GPU. */
+ * kf_paged_decode_workspace_bytes(...) bytes; sm_count is that of the GPU.
+ * A wait that expires sets *status (device memory, may be NULL) and shows as
+ * NaN in the outputs. */
 size_t kf_paged_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int sm_count);
 int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_tensor4* v_pages,
                     const int32_t* block_table, int64_t max_pages, int64_t table_stride,
                     const int32_t* lengths, const kf_tensor4* new_k, const kf_tensor4* new_v,
-                    const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale, void* workspace,
-                    size_t workspace_bytes, void* stream);
+                    const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale,
+                    void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
 
 /* ---- K6: the paged cache's append, tables and slots ----------------------
  * No counterpart in the reference.

@@ -74,7 +74,7 @@ SIGNATURES = {
     "kf_decode_noalloc": (_I, [_T4, _T4, _T4, _T4, _T4, _I64, _T4, _VP, _I, _F, _I, _VP]),
     "kf_paged_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "kf_paged_decode": (_I, [_T4B, _T4B, _T4B, _VP, _I64, _I64, _VP, _T4B, _T4B, _VP, _T4B, _VP, _I, _F, _VP, _SZ,
-                             _VP]),
+                             _VP, _VP]),
     "kf_paged_append": (_I, [_T4B, _T4B, _T4B, _T4B, _VP, _I, _VP]),
     "kf_paged_reserve": (_I, [_VP, _VP, _I64, _VP, _I64, _I64, _VP, _I64, _VP, _I64, _VP, _I64, _I64, _VP, _VP, _VP,
                               _VP]),

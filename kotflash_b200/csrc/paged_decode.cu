@@ -22,10 +22,11 @@
 // Inside a block four warps take different keys of each tile (or, with more
 // than 16 rows per KV head, 2 or 4 warps form a team that shares keys and
 // splits the rows).  Each team streams its own keys through its own ring of
-// shared-memory stages with 16-byte cp.async gathers: a lane resolves the
-// page of one key, the addresses go round by shuffles, so pages of any size
-// and any cache strides take one path, and teams never wait for one another
-// inside a unit.  The ring runs ahead across unit boundaries.  The products
+// shared-memory stages by TMA, so teams never wait for one another inside a
+// unit; the ring runs ahead across unit boundaries.  A tensor map over the
+// pool turns (page, head, row) into addresses, whatever the cache's strides:
+// a lane looks up the page of one key, and the lanes at the start of a box of
+// gcd(page_size, 16) rows, which never crosses a page, load it.  The products
 // are taken transposed on warp MMAs (S^T = K Q^T, O^T = V^T P^T): keys and
 // head-dim fill the m = 16 side and up to 8 query rows the n = 8 side, so
 // few rows waste little.
@@ -55,12 +56,17 @@ struct PagedArgs {
   const int32_t* lengths;
   float* part_o;           // [blocks][2][rows of a unit][D]
   float* part_lse;         // [blocks][2][rows of a unit], log2
-  int4* joins;             // [blocks]: (request, KV head and row block, last block of the unit, -) or x = -1
+  int4* joins;             // by unit if join_units, else by block: (request, KV head and row block, first
+                           // block, last block) of a unit that was cut, or x = -1
+  int32_t* status;         // set when a bounded wait expires (may be null)
   int64_t qs[2], ks[3], vs[3], nks[2], nvs[2], os[2];
   int64_t table_stride;
   int B, Hq, Hkv, G, D, row_blocks;
   uint32_t capacity;       // tokens a table row can hold
   uint32_t page_size, num_pages;
+  uint32_t page_mul, page_shift;  // x / page_size = x page_mul >> page_shift for x < 2^31
+  int box;                 // rows of a TMA box
+  bool join_units;
   float scale_log2;
 };
 
@@ -77,11 +83,13 @@ struct Cfg {
   static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
   static constexpr int PASS = 64 / NT < DP ? 64 / NT : DP;   // head-dim columns joined per pass of the epilogue
   static constexpr int OSTRIDE = PASS + 4;                   // keeps the four row pairs of a store on separate banks
-  static constexpr int SMEM = TEAMS * STAGES * STAGE + kWarps * NT * 8 * OSTRIDE * 4 + kWarps * NT * 8 * 2 * 4;
+  static constexpr int SMEM = 1024 + TEAMS * STAGES * STAGE + kWarps * NT * 8 * OSTRIDE * 4 + kWarps * NT * 8 * 2 * 4;
 };
 
-__device__ __forceinline__ uint32_t swz(int row, int chunk, int row_bytes) {
-  return (uint32_t)(row * row_bytes + ((((chunk & 7) ^ (row & 7)) | (chunk & ~7)) << 4));
+// Shared-memory offset of 16-byte chunk c of row r in a TMA tile stored as
+// 64-column panels of `rows` x 128 B with the 128-byte swizzle.
+__device__ __forceinline__ uint32_t swz(int r, int c, int rows) {
+  return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
 __device__ __forceinline__ uint32_t visible(const PagedArgs& a, int b) {
@@ -89,10 +97,11 @@ __device__ __forceinline__ uint32_t visible(const PagedArgs& a, int b) {
   return n <= 0 ? 0u : min((uint32_t)n, a.capacity);
 }
 
-// Position in the list of tiles: tile `t` of the `tiles` of unit (b, hr).
+// Position in the list of tiles: tile `t` of the `tiles` of the unit (request
+// b, KV head h, row block rb).
 template <int TILE>
 struct Cursor {
-  int b, hr;
+  int b, h, rb;
   uint32_t t, tiles, keys;
 
   __device__ __forceinline__ void set_request(const PagedArgs& a, int request) {
@@ -100,47 +109,51 @@ struct Cursor {
     keys = visible(a, b);
     tiles = (keys + TILE - 1) / TILE;
   }
-  // true when the next tile belongs to another unit
-  __device__ __forceinline__ bool next(const PagedArgs& a, int units) {
-    if (++t < tiles) return false;
+  // to the next tile of the list, which must exist
+  __device__ __forceinline__ void next(const PagedArgs& a) {
+    if (++t < tiles) return;
     t = 0;
-    if (++hr == units) {
-      hr = 0;
-      do {
-        set_request(a, b + 1);
-      } while (tiles == 0 && b + 1 < a.B);
-    }
-    return true;
+    if (++rb < a.row_blocks) return;
+    rb = 0;
+    if (++h < a.Hkv) return;
+    h = 0;
+    do {
+      set_request(a, b + 1);
+    } while (tiles == 0 && b + 1 < a.B);
   }
 };
 
+// Barrier of a team's warps that returns the AND of their `pred`, so that all
+// of them go on alike.
 template <int RG>
-__device__ __forceinline__ void team_sync(int team) {
+__device__ __forceinline__ bool team_and(int team, bool pred) {
   if constexpr (RG == 1)
-    __syncwarp();
+    return __all_sync(0xffffffffu, pred);
   else if constexpr (RG == kWarps)
-    __syncthreads();
+    return __syncthreads_and(pred);
   else
-    kf::named_bar_sync(1 + team, RG * 32);
-}
-
-__device__ __forceinline__ uint64_t shfl64(uint64_t x, int src) {
-  return __shfl_sync(0xffffffffu, (unsigned long long)x, src);
+    return kf::named_bar_and(1 + team, RG * 32, pred);
 }
 
 template <bool BF16, int NP, int NT, int RG>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(const PagedArgs a) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                    const PagedArgs a) {
   using C = Cfg<NP, NT, RG>;
   constexpr int DP = C::DP, KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
   constexpr int H = KW / 16;           // 16-key halves of a step
-  constexpr int ROW_BYTES = DP * 2;
   constexpr int CHUNKS = DP / 8;       // 16-byte chunks of a row
-  constexpr int K_BYTES = KW * ROW_BYTES;
-  extern __shared__ __align__(128) uint8_t smem[];
+  constexpr int K_BYTES = KW * DP * 2;
+  constexpr int PANEL = KW * 128;
+  constexpr uint32_t ALL = KW == 32 ? 0xffffffffu : 0xffffu;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   __shared__ int64_t warp_tiles[kWarps];
   __shared__ int first_request;
   __shared__ int64_t first_before;     // tiles of the requests before it
+  __shared__ __align__(8) uint64_t full[C::TEAMS][STAGES];
   __shared__ uint32_t seen_s[C::TEAMS][STAGES];  // visible keys of each stage
+  __shared__ int abort_any;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int team = warp / RG, rg = warp % RG;
@@ -149,14 +162,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
   float* obuf = reinterpret_cast<float*>(smem + C::TEAMS * STAGES * C::STAGE);  // [warp][NT * 8][OSTRIDE]
   float* ml = obuf + kWarps * NT * 8 * C::OSTRIDE;                              // [warp][NT * 8][2]
 
-  // columns [D, DP) of every stage stay zero: they add nothing to K Q^T
-  if (a.D < DP) {
-    const int pad = CHUNKS - a.D / 8;
-    constexpr int ALL = C::TEAMS * STAGES * 2 * KW;  // K and V rows of all rings
-    for (int i = tid; i < ALL * pad; i += kThreads) {
-      const int r = i / pad, c = a.D / 8 + i % pad;
-      *reinterpret_cast<uint4*>(smem + (r / KW) * K_BYTES + swz(r % KW, c, ROW_BYTES)) = make_uint4(0, 0, 0, 0);
-    }
+  if (tid == 0) {
+    for (int i = 0; i < C::TEAMS * STAGES; ++i) kf::mbar_init(&full[0][0] + i, 1);
+    kf::fence_barrier_init();
+    abort_any = 0;
+    kf::tma_prefetch_desc(&map_k);
+    kf::tma_prefetch_desc(&map_v);
   }
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -193,9 +204,12 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
     }
     if (a.lse)
       for (int h = tid; h < a.Hq; h += kThreads) a.lse[b * a.Hq + h] = -INFINITY;
+    if (a.join_units)
+      for (int u = tid; u < units; u += kThreads) a.joins[b * units + u].x = -1;
   }
+  const bool join_blocks = a.joins && !a.join_units;
   if (me >= shares) {
-    if (tid == 0 && a.joins) a.joins[me].x = -1;
+    if (tid == 0 && join_blocks) a.joins[me].x = -1;
     return;
   }
   const int64_t begin = me * list / shares;
@@ -221,63 +235,41 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
   work.set_request(a, first_request);
   {
     const int64_t at = begin - first_before * units;  // inside the request's tiles x units
-    work.hr = (int)(at / work.tiles);
-    work.t = (uint32_t)(at - (int64_t)work.hr * work.tiles);
+    const int hr = (int)(at / work.tiles);
+    work.t = (uint32_t)(at - (int64_t)hr * work.tiles);
+    work.h = hr / a.row_blocks;
+    work.rb = hr - work.h * a.row_blocks;
   }
   load = work;
 
-  // ---- loads: lane r (of KW) resolves key r of the team's share of the tile
-  int32_t next_page;       // of the tile the load cursor stands on, loaded one step ahead
-  uint32_t next_row;
-  bool next_in;
+  // ---- loads: lane r (of KW) looks up key r of the team's share of the tile
+  // the load cursor stands on, one step ahead of its use
+  uint32_t next_page, next_row;
   auto look_up = [&]() {
     const uint32_t key = load.t * TILE + team * KW + (KW == 32 ? lane : (lane & 15));
-    next_in = key < load.keys;
-    const uint32_t pg = next_in ? key / a.page_size : 0;
+    const uint32_t pg = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
     next_row = key - pg * a.page_size;
-    next_page = next_in ? __ldg(a.table + load.b * a.table_stride + pg) : -1;
+    next_page = key < load.keys ? (uint32_t)__ldg(a.table + load.b * a.table_stride + pg) : 0xffffffffu;
   };
   auto issue = [&](int stage) {
-    const int h = load.hr / a.row_blocks, rb = load.hr - h * a.row_blocks;
-    const bool valid = next_in && (uint32_t)next_page < a.num_pages;
-    const uint32_t seen = __ballot_sync(0xffffffffu, valid) & (KW == 32 ? 0xffffffffu : 0xffffu);
-    uint64_t row_k = 0, row_v = 0;
-    if (valid) {
-      row_k = reinterpret_cast<uint64_t>(a.k + next_page * a.ks[0] + h * a.ks[1] + next_row * a.ks[2]);
-      row_v = reinterpret_cast<uint64_t>(a.v + next_page * a.vs[0] + h * a.vs[1] + next_row * a.vs[2]);
+    const bool valid = next_page < a.num_pages;
+    const uint32_t seen = __ballot_sync(0xffffffffu, valid) & ALL;
+    const bool starts_box = valid && lane < KW && (lane & (a.box - 1)) == 0;
+    const uint32_t boxes = __ballot_sync(0xffffffffu, starts_box);
+    uint64_t* bar = &full[team][stage];
+    if (lane == 0) {
+      seen_s[team][stage] = seen;
+      kf::mbar_arrive_expect_tx(bar, (uint32_t)(__popc(boxes) * a.box) * (NP * 128 * 2));
     }
-    if (a.nk) {
-      // the newest position comes from the caller's row, and one warp stores it
-      const uint32_t r = (uint32_t)a.lengths[load.b] - 1 - (load.t * TILE + team * KW);
-      if (r < (uint32_t)KW && ((seen >> r) & 1) && a.slots[load.b] >= 0) {
-        const uint64_t src_k = reinterpret_cast<uint64_t>(a.nk + load.b * a.nks[0] + h * a.nks[1]);
-        const uint64_t src_v = reinterpret_cast<uint64_t>(a.nv + load.b * a.nvs[0] + h * a.nvs[1]);
-        const uint64_t dst_k = shfl64(row_k, r), dst_v = shfl64(row_v, r);
-        if (rb == 0 && rg == 0 && (lane & 15) < a.D / 8) {
-          const uint4* src = reinterpret_cast<const uint4*>(lane < 16 ? src_k : src_v) + (lane & 15);
-          uint4* dst = reinterpret_cast<uint4*>(lane < 16 ? dst_k : dst_v) + (lane & 15);
-          *dst = *src;
-        }
-        if ((uint32_t)(KW == 32 ? lane : (lane & 15)) == r) {
-          row_k = src_k;
-          row_v = src_v;
-        }
-      }
-    }
-    uint8_t* st = ring + stage * C::STAGE;
+    __syncwarp();
+    if (starts_box) {
+      uint8_t* st = ring + stage * C::STAGE + lane * 128;
 #pragma unroll
-    for (int i = 0; i < KW * CHUNKS / (32 * RG); ++i) {
-      const int idx = i * 32 * RG + rg * 32 + lane;
-      const int r = idx / CHUNKS, c = idx % CHUNKS;
-      const uint64_t sk = shfl64(row_k, r), sv = shfl64(row_v, r);
-      const bool ok = (seen >> r) & 1;
-      if (c * 8 < a.D) {
-        const uint32_t at = swz(r, c, ROW_BYTES);
-        kf::cp_async16(st + at, reinterpret_cast<const uint4*>(ok ? sk : (uint64_t)a.k) + (ok ? c : 0), ok);
-        kf::cp_async16(st + K_BYTES + at, reinterpret_cast<const uint4*>(ok ? sv : (uint64_t)a.v) + (ok ? c : 0), ok);
+      for (int pn = 0; pn < NP; ++pn) {
+        kf::tma_load_4d(st + pn * PANEL, &map_k, bar, pn * 64, next_row, load.h, next_page);
+        kf::tma_load_4d(st + K_BYTES + pn * PANEL, &map_v, bar, pn * 64, next_row, load.h, next_page);
       }
     }
-    if (rg == 0 && lane == 0) seen_s[team][stage] = seen;
   };
 
   // ---- state of the unit being worked on
@@ -285,11 +277,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
   float m_run[NT][2], l_run[NT][2];    // rows 2 (lane % 4) + {0, 1} of each row tile
   float ot[NT][DP / 16][4];            // O^T
   auto start_unit = [&]() {
-    const int h = work.hr / a.row_blocks, rb = work.hr - h * a.row_blocks;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      const int row = rb * C::ROWS + rg * NT * 8 + nt * 8 + (lane >> 2);
-      const uint16_t* src = a.q + work.b * a.qs[0] + (int64_t)(h * a.G + row) * a.qs[1] + 2 * (lane & 3);
+      const int row = work.rb * C::ROWS + rg * NT * 8 + nt * 8 + (lane >> 2);
+      const uint16_t* src = a.q + work.b * a.qs[0] + (int64_t)(work.h * a.G + row) * a.qs[1] + 2 * (lane & 3);
 #pragma unroll
       for (int kk = 0; kk < DP / 16; ++kk) {
 #pragma unroll
@@ -303,38 +294,76 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
     }
   };
 
-  look_up();
+  // the first warp of a team loads
+  int issued = 0;
+  if (rg == 0) {
+    look_up();
 #pragma unroll
-  for (int s = 0; s < STAGES - 1; ++s) {
-    if (s < n) {
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (s >= n) break;
       issue(s);
-      if (s + 1 < n) {
-        load.next(a, units);
+      ++issued;
+      if (issued < n) {
+        load.next(a);
         look_up();
       }
     }
-    kf::cp_async_commit();
   }
   start_unit();
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
-  if (tid == 0 && a.joins) a.joins[me].x = -1;
+  if (tid == 0 && join_blocks) a.joins[me].x = -1;
 
   int stage = 0, fill = STAGES - 1;
-  for (int i = 0; i < n; ++i) {
-    kf::cp_async_wait<STAGES - 2>();
-    team_sync<RG>(team);               // stage i has landed for the team, stage i - 1 is free
-    if (i + STAGES - 1 < n) {
+  uint32_t parity = 0;
+  bool alive = true;                   // false once a wait of this block has expired
+  int i = 0;
+  for (; i < n; ++i) {
+    // One outcome for the team: no lane reaches a collective instruction alone.
+    // The barrier also says that the team has left stage i - 1.
+    const bool landed = alive && !*(volatile int*)&abort_any && kf::mbar_wait(&full[team][stage], parity, a.status);
+    alive = team_and<RG>(team, landed);
+    if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
+    if (rg == 0 && alive && issued < n) {
       issue(fill);
-      if (i + STAGES < n) {
-        load.next(a, units);
+      ++issued;
+      if (issued < n) {
+        load.next(a);
         look_up();
       }
     }
-    kf::cp_async_commit();
 
-    const uint32_t seen = seen_s[team][stage];
+    const uint32_t seen = alive ? seen_s[team][stage] : 0u;
+    uint8_t* kt = ring + stage * C::STAGE;
+    uint8_t* vt = kt + K_BYTES;
+    const uint32_t key0 = work.t * TILE + team * KW;
+    if (seen != 0 && (seen != ALL || (a.nk && key0 + KW >= work.keys))) {
+      // The end of a request or pages without a table entry.  Rows that nobody
+      // sees hold anything: their scores are replaced below, their V rows must
+      // be zero.  A new row takes its place here and goes to its page.
+      for (int idx = rg * 32 + lane; idx < KW * CHUNKS; idx += RG * 32) {
+        const int r = idx / CHUNKS, c = idx % CHUNKS;
+        if (!((seen >> r) & 1)) *reinterpret_cast<uint4*>(vt + swz(r, c, KW)) = make_uint4(0, 0, 0, 0);
+      }
+      const uint32_t r = (uint32_t)a.lengths[work.b] - 1 - key0;
+      if (a.nk && r < (uint32_t)KW && ((seen >> r) & 1) && a.slots[work.b] >= 0) {
+        const int c = lane & 15;
+        if (rg == 0 && c < a.D / 8) {
+          const uint32_t pg = (uint32_t)(((uint64_t)(key0 + r) * a.page_mul) >> a.page_shift);
+          const int64_t page = a.table[work.b * a.table_stride + pg], row = key0 + r - pg * a.page_size;
+          const uint16_t* src = lane < 16 ? a.nk + work.b * a.nks[0] + work.h * a.nks[1]
+                                          : a.nv + work.b * a.nvs[0] + work.h * a.nvs[1];
+          uint16_t* dst = lane < 16 ? a.k + page * a.ks[0] + work.h * a.ks[1] + row * a.ks[2]
+                                    : a.v + page * a.vs[0] + work.h * a.vs[1] + row * a.vs[2];
+          const uint4 x = reinterpret_cast<const uint4*>(src)[c];
+          *reinterpret_cast<uint4*>((lane < 16 ? kt : vt) + swz(r, c, KW)) = x;
+          if (work.rb == 0) reinterpret_cast<uint4*>(dst)[c] = x;
+        }
+      }
+      kf::fence_proxy_async_smem();    // before a later load into this stage
+      team_and<RG>(team, true);
+    }
     if (seen != 0) {
-      const uint32_t sk = kf::smem_u32(ring + stage * C::STAGE), sv = sk + K_BYTES;
+      const uint32_t sk = kf::smem_u32(kt), sv = kf::smem_u32(vt);
       // S^T (keys x rows)
       float c[H][NT][4];
 #pragma unroll
@@ -346,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t ka[4];
-          kf::ldmatrix_x4(ka, sk + swz(h * 16 + (lane & 15), 2 * kk + (lane >> 4), ROW_BYTES));
+          kf::ldmatrix_x4(ka, sk + swz(h * 16 + (lane & 15), 2 * kk + (lane >> 4), KW));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(c[h][nt], ka, qb[nt][kk][0], qb[nt][kk][1]);
         }
@@ -417,7 +446,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
         for (int h = 0; h < H; ++h) {
           uint32_t va[4];
           kf::ldmatrix_x4_trans(va, sv + swz(h * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * dm + ((lane >> 3) & 1),
-                                             ROW_BYTES));
+                                             KW));
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             kf::mma_16816<BF16>(ot[nt][dm], va, pb[h][nt][0], pb[h][nt][1]);
@@ -425,7 +454,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
           }
         }
     }
-    if (++stage == STAGES) stage = 0;
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
     if (++fill == STAGES) fill = 0;
 
     const bool unit_done = work.t + 1 == work.tiles;
@@ -434,7 +466,7 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
       continue;
     }
     // ---- join the teams and write the unit's rows (or its partial)
-    const int h = work.hr / a.row_blocks, rb = work.hr - h * a.row_blocks;
+    const int h = work.h, rb = work.rb;
     const bool direct = unit_t0 == 0 && unit_done;
     const int64_t slot = me * 2 + (unit_t0 > 0 ? 0 : 1);  // 0: began in an earlier share, 1: begins here
 #pragma unroll
@@ -443,6 +475,10 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], off);
+    if (!alive) {  // a lost load shows in the result
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) l_run[nt][0] = l_run[nt][1] = m_run[nt][0] = m_run[nt][1] = NAN;
+    }
 #pragma unroll
     for (int pass = 0; pass < DP / C::PASS; ++pass) {
       __syncthreads();  // the buffer's readers of the pass (or unit) before are done
@@ -503,23 +539,33 @@ __global__ void __launch_bounds__(kThreads, kBlocksPerSm) paged_decode_kernel(co
         }
       }
     }
-    if (!direct && unit_t0 == 0 && tid == 0) {
-      // begins here and goes on: the share that holds list position p is ((p + 1) shares - 1) / list
+    if (unit_t0 == 0 && tid == 0 && (a.join_units || !direct)) {
+      // a unit that begins here and goes on ends in the share that holds list
+      // position p, its last tile: ((p + 1) shares - 1) / list
+      const int hr = h * a.row_blocks + rb;
       const int64_t last_tile = begin + i + (work.tiles - 1 - work.t);
-      a.joins[me] = make_int4(work.b, work.hr, (int)(((last_tile + 1) * shares - 1) / list), 0);
+      a.joins[a.join_units ? (int64_t)work.b * units + hr : me] =
+          direct ? make_int4(-1, 0, 0, 0)
+                 : make_int4(work.b, hr, (int)me, (int)(((last_tile + 1) * shares - 1) / list));
     }
     if (i + 1 < n) {
-      work.next(a, units);
+      work.next(a);
       start_unit();
       unit_t0 = 0;
     }
   }
+  // after a failed wait, let the loads still in flight land (bounded) before leaving
+  if (!alive && rg == 0 && lane == 0)
+    for (int s = 0; s < STAGES; ++s) {
+      const int used = issued / STAGES + (s < issued % STAGES ? 1 : 0);
+      if (used > 0) kf::mbar_wait(&full[team][s], (uint32_t)(used - 1) & 1, nullptr, 100000000ull);
+    }
 }
 
-// Joins the partials of the unit that begins in share blockIdx.x and goes on:
-// slot 1 of that share, slot 0 of the shares up to the unit's last.  One row
-// per block; groups of D / 4 lanes take every groups-th partial with a
-// running maximum, so each partial is read once and in any number.
+// Joins the partials of a unit that was cut: slot 1 of its first share, slot 0
+// of the shares up to its last.  One row per block; groups of D / 4 lanes take
+// every groups-th partial with a running maximum, so each partial is read once
+// and in any number.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBatch = 4;  // partials a group has in flight
 
@@ -532,7 +578,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   const int h = unit.y / a.row_blocks, rb = unit.y - h * a.row_blocks;
   const int r = blockIdx.y;
   if (r >= a.G - rb * rows) return;
-  const int count = unit.z - (int)blockIdx.x + 1;
+  const int count = unit.w - unit.z + 1;
   __shared__ float4 acc_s[kJoinThreads];
   __shared__ float m_s[kJoinThreads / 4], l_s[kJoinThreads / 4];
   const int lanes = a.D / 4, groups = kJoinThreads / lanes;
@@ -549,7 +595,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
         lse[x] = -INFINITY;
         o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (j < count) {
-          const int64_t row = (((int64_t)blockIdx.x + j) * 2 + (j == 0 ? 1 : 0)) * rows + r;
+          const int64_t row = (((int64_t)unit.z + j) * 2 + (j == 0 ? 1 : 0)) * rows + r;
           lse[x] = a.part_lse[row];
           o[x] = *reinterpret_cast<const float4*>(a.part_o + row * a.D + c * 4);
         }
@@ -615,7 +661,7 @@ size_t workspace_need(int blocks, int rows, int64_t D) {
 }
 
 template <bool BF16, int NP, int NT, int RG>
-int launch_variant(const PagedArgs& a, int blocks, cudaStream_t st) {
+int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
   using C = Cfg<NP, NT, RG>;
   static_assert(C::STAGES >= 3, "the ring needs three stages");
   auto kern = paged_decode_kernel<BF16, NP, NT, RG>;
@@ -623,16 +669,17 @@ int launch_variant(const PagedArgs& a, int blocks, cudaStream_t st) {
     (void)cudaGetLastError();
     return kf::set_error(KF_ERR_CUDA, "kf_paged_decode: cannot reserve %d bytes of shared memory", C::SMEM);
   }
-  return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged_decode", a);
+  return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged_decode", mk, mv, a);
 }
 
 template <bool BF16, int NP>
-int dispatch_rows(const PagedArgs& a, int rows, int blocks, cudaStream_t st) {
+int dispatch_rows(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
+                  cudaStream_t st) {
   switch (rows) {
-    case 8: return launch_variant<BF16, NP, 1, 1>(a, blocks, st);
-    case 16: return launch_variant<BF16, NP, 2, 1>(a, blocks, st);
-    case 32: return launch_variant<BF16, NP, 2, 2>(a, blocks, st);
-    default: return launch_variant<BF16, NP, 2, 4>(a, blocks, st);
+    case 8: return launch_variant<BF16, NP, 1, 1>(a, mk, mv, blocks, st);
+    case 16: return launch_variant<BF16, NP, 2, 1>(a, mk, mv, blocks, st);
+    case 32: return launch_variant<BF16, NP, 2, 2>(a, mk, mv, blocks, st);
+    default: return launch_variant<BF16, NP, 2, 4>(a, mk, mv, blocks, st);
   }
 }
 
@@ -653,8 +700,8 @@ extern "C" size_t kf_paged_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64
 extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_tensor4* v_pages,
                                const int32_t* block_table, int64_t max_pages, int64_t table_stride,
                                const int32_t* lengths, const kf_tensor4* new_k, const kf_tensor4* new_v,
-                               const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale, void* workspace,
-                               size_t workspace_bytes, void* stream) {
+                               const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale,
+                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
   using kf::set_error;
   const char* what = "kf_paged_decode";
   if (!q || !k_pages || !v_pages || !o) return set_error(KF_ERR_INVALID, "%s: null tensor descriptor", what);
@@ -728,6 +775,17 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
+  a.status = status;
+  // Division by page_size: with 2^(s-1) < page_size <= 2^s and m =
+  // ceil(2^(31+s) / page_size), m < 2^32 and m page_size exceeds 2^(31+s) by
+  // less than 2^s, so x m >> (31 + s) is exact for x < 2^31.
+  int s = 0;
+  while (((int64_t)1 << s) < page_size) ++s;
+  a.page_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + page_size - 1) / page_size);
+  a.page_shift = (uint32_t)(31 + s);
+  // boxes never cross a page nor a team's 16 or 32 keys
+  a.box = 16;
+  while (page_size % a.box) a.box /= 2;
   a.scale_log2 = scale * kLog2e;
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.
@@ -740,6 +798,7 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   a.part_o = nullptr;
   a.part_lse = nullptr;
   a.joins = nullptr;
+  a.join_units = false;
   if (most > 1) {
     const size_t need = workspace_need((int)blocks, rows, D);
     if (!workspace || workspace_bytes < need)
@@ -748,16 +807,23 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
     a.joins = reinterpret_cast<int4*>(base);
     a.part_o = reinterpret_cast<float*>(a.joins + blocks);
     a.part_lse = a.part_o + (size_t)blocks * 2 * rows * D;
+    a.join_units = units < blocks;  // whichever list is shorter
   }
+  CUtensorMap mk, mv;
+  int rc = kf::encode_tmap_4d(&mk, k_pages, 64, a.box);
+  if (rc != KF_OK) return rc;
+  rc = kf::encode_tmap_4d(&mv, v_pages, 64, a.box);
+  if (rc != KF_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   const bool bf16 = dtype == KF_BF16;
-  int rc;
   if (D <= 64)
-    rc = bf16 ? dispatch_rows<true, 1>(a, rows, (int)blocks, st) : dispatch_rows<false, 1>(a, rows, (int)blocks, st);
+    rc = bf16 ? dispatch_rows<true, 1>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 1>(a, mk, mv, rows, (int)blocks, st);
   else
-    rc = bf16 ? dispatch_rows<true, 2>(a, rows, (int)blocks, st) : dispatch_rows<false, 2>(a, rows, (int)blocks, st);
+    rc = bf16 ? dispatch_rows<true, 2>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 2>(a, mk, mv, rows, (int)blocks, st);
   if (rc != KF_OK || most == 1) return rc;
-  const dim3 grid((unsigned)blocks, (unsigned)(a.G < rows ? a.G : rows));
+  const dim3 grid((unsigned)(a.join_units ? units : blocks), (unsigned)(a.G < rows ? a.G : rows));
   return bf16 ? kf::launch_dependent(paged_join_kernel<true>, grid, dim3(kJoinThreads), 0, st, what, a, rows)
               : kf::launch_dependent(paged_join_kernel<false>, grid, dim3(kJoinThreads), 0, st, what, a, rows);
 }

@@ -109,8 +109,8 @@ def paged_attention(
     block_table is int32 [B, max_pages] and lengths int32 [B].  Request b's
     token attends to positions 0 .. lengths[b] - 1, position p being row
     p % page_size of page block_table[b, p // page_size].  Positions whose
-    table entry is not a page of the pool (-1, say) are masked, and nothing
-    masked is read.  A request that sees nothing yields 0 (LSE -inf).
+    table entry is not a page of the pool (-1, say) are masked,
+    whatever the memory there holds.  A request that sees nothing yields 0 (LSE -inf).
 
     new_k and new_v [B, Hkv, 1, D] with slots (int64 [B]) append on the way:
     where slots[b] >= 0, the slot of position lengths[b] - 1, that position's
@@ -166,7 +166,7 @@ def paged_attention(
         block_table.shape[1], block_table.stride(0), lengths.data_ptr(),
         _ext.packed4(new_k) if rows else None, _ext.packed4(new_v) if rows else None,
         slots.data_ptr() if rows else None, _ext.packed4(out), lse.data_ptr() if return_lse else None, dtype, scale,
-        workspace.data_ptr(), ws_bytes, _ext.stream_of(q),
+        workspace.data_ptr(), ws_bytes, _ext.status_word(dev).data_ptr(), _ext.stream_of(q),
     )
     _ext.check(rc, "kf_paged_decode")
     return (out, lse) if return_lse else out

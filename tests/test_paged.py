@@ -125,7 +125,7 @@ def test_c_abi_refuses_before_any_launch():
                dtype=0, ws=None, ws_bytes=0, q_strides=None, k_ptr=p):
         return lib.kf_paged_decode(_t(q, strides=q_strides), _t(k, k_ptr), _t(v or k), table, max_pages, max_pages, lens,
                                    _t(nk) if nk else None, _t(nv) if nv else None, slots, _t(o or q), None, dtype, 0.1, ws,
-                                   ws_bytes, None)
+                                   ws_bytes, None, None)
 
     for kw, code, match in [
         (dict(dtype=5), _ext.KF_ERR_INVALID, "dtype"),
