@@ -231,26 +231,42 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * Request b's token sees the positions below min(lengths[b], max_pages *
  * page_size) whose table entry lies in [0, pages); every other position
  * (other entries, -1 among them, the rest of a last page) is masked whatever
- * its memory holds, and no page but the table's is read.  A request that sees nothing gets O = 0, LSE = -inf.
- * lse [B, Hq] fp32 (natural log, contiguous) may be NULL.  All lengths and
- * tables are read on the device when the kernel runs.
+ * its memory holds, and no page but the table's is read.  A request that sees
+ * nothing gets O = 0, LSE = -inf.  lse [B, Hq] fp32 (natural log, contiguous)
+ * may be NULL.  All lengths and tables are read on the device when the kernel
+ * runs.
  *
- * new_k / new_v [B, Hkv, 1, D] with slots (int64 [B]), all or none: where
- * slots[b] >= 0 (it is then the slot of position lengths[b] - 1, which must
- * have a page), that position's row is taken from new_k / new_v, written to
- * its page and attended in the same pass; where slots[b] < 0 request b has no
- * new row.
+ * new_k / new_v [B, Hkv, 1, D] with slots (int64 [B]), all or none (ptr and
+ * slots NULL): where slots[b] >= 0 (it is then the slot of position lengths[b]
+ * - 1, which must have a page), that position's row is taken from new_k /
+ * new_v, written to its page and attended in the same pass; where slots[b] < 0
+ * request b has no new row.
  *
  * 16 <= D <= 128, D % 8 == 0.  `workspace` holds
  * kf_paged_decode_workspace_bytes(...) bytes; sm_count is that of the GPU.
  * A wait that expires sets *status (device memory, may be NULL) and shows as
- * NaN in the outputs. */
+ * NaN in the outputs.
+ *
+ * The calls of K5 and K6 take their arguments as one struct of 8-byte fields:
+ * they last microseconds, and a foreign-function call pays for every
+ * argument. */
+typedef struct kf_paged_decode_args {
+  kf_tensor4     q, k_pages, v_pages, o;
+  kf_tensor4     new_k, new_v;
+  const int64_t* slots;
+  const int32_t* block_table;
+  int64_t        max_pages, table_stride;
+  const int32_t* lengths;
+  float*         lse;
+  int64_t        dtype;
+  double         scale;
+  void*          workspace;
+  uint64_t       workspace_bytes;
+  int32_t*       status;
+  void*          stream;
+} kf_paged_decode_args;
 size_t kf_paged_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int sm_count);
-int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_tensor4* v_pages,
-                    const int32_t* block_table, int64_t max_pages, int64_t table_stride,
-                    const int32_t* lengths, const kf_tensor4* new_k, const kf_tensor4* new_v,
-                    const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale,
-                    void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+int kf_paged_decode(const kf_paged_decode_args* args);
 
 /* ---- K6: the paged cache's append, tables and slots ----------------------
  * No counterpart in the reference.
@@ -258,16 +274,26 @@ int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_ten
  * kf_paged_append copies new_k / new_v [N, Hkv, S, D], token t = n * S + s,
  * to slot slots[t] (int64 [N * S]): page slots[t] / page_size, row slots[t] %
  * page_size.  A token whose slot lies outside [0, pages * page_size) is
- * skipped.  Bit-exact; of two tokens with one slot either may stay.
+ * skipped.  Bit-exact; of two tokens with one slot either may stay. */
+typedef struct kf_paged_append_args {
+  kf_tensor4     k_pages, v_pages, new_k, new_v;
+  const int64_t* slots;
+  int64_t        dtype;
+  void*          stream;
+} kf_paged_append_args;
+int kf_paged_append(const kf_paged_append_args* args);
+
+/* The tables of B requests: lengths int32 [B] and block_table int32 [B,
+ * max_pages]; the pages that nobody owns are a stack, free_pages[0 ..
+ * *free_count), int32, of a pool of num_pages.
  *
  * kf_paged_reserve makes room for new_lengths[b] (int32, < 0 counts as 0)
- * tokens behind the lengths[b] of each of B requests.  The pages that nobody
- * owns are a stack: free_pages[0 .. *free_count), int32, of a pool of
- * num_pages.  Request b needs ceil((lengths[b] + new_lengths[b]) / page_size)
- * - ceil(lengths[b] / page_size) more pages; going through the requests in
- * order it is granted all of them, popped from the end of the stack into
- * block_table[b] in place, or, where they would not fit its max_pages or the
- * needs up to and including its own exceed the stack, refused.  Writes
+ * tokens behind the lengths[b] of each request.  Request b needs
+ * ceil((lengths[b] + new_lengths[b]) / page_size) - ceil(lengths[b] /
+ * page_size) more pages; going through the requests in order it is granted all
+ * of them, popped from the end of the stack into block_table[b] in place, or,
+ * where they would not fit its max_pages or the needs up to and including its
+ * own exceed the stack, refused.  Writes
  *   slots [num_tokens] int64 (16-byte aligned): the slots of all new tokens,
  *     request after request; -1 for those of a refused request and past the
  *     last token,
@@ -286,19 +312,32 @@ int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_ten
  *
  * lengths_out may be lengths and free_count_out may be free_count.  B <=
  * 16384; 1 <= page_size <= 2^20. */
-int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pages, const kf_tensor4* new_k,
-                    const kf_tensor4* new_v, const int64_t* slots, int dtype, void* stream);
-int kf_paged_reserve(const int32_t* lengths, const int32_t* new_lengths, int64_t B,
-                     int32_t* block_table, int64_t max_pages, int64_t table_stride,
-                     const int32_t* free_pages, int64_t num_pages, const int32_t* free_count,
-                     int64_t page_size, int64_t* slots, int64_t num_tokens,
-                     int64_t tokens_per_request, int32_t* starts, int32_t* lengths_out,
-                     int32_t* free_count_out, void* stream);
-int kf_paged_release(const int32_t* lengths, const uint8_t* finished, int64_t B,
-                     const int32_t* block_table, int64_t max_pages, int64_t table_stride,
-                     int32_t* free_pages, int64_t num_pages, const int32_t* free_count,
-                     int64_t page_size, int32_t* lengths_out, int32_t* free_count_out,
-                     void* stream);
+typedef struct kf_page_tables {
+  const int32_t* lengths;
+  int64_t        B;
+  int32_t*       block_table;    /* kf_paged_release does not write it */
+  int64_t        max_pages, table_stride;
+  int32_t*       free_pages;     /* kf_paged_reserve does not write it */
+  int64_t        num_pages;
+  const int32_t* free_count;
+  int64_t        page_size;
+  int32_t*       lengths_out;
+  int32_t*       free_count_out;
+  void*          stream;
+} kf_page_tables;
+typedef struct kf_paged_reserve_args {
+  kf_page_tables tables;
+  const int32_t* new_lengths;
+  int64_t*       slots;
+  int64_t        num_tokens, tokens_per_request;
+  int32_t*       starts;
+} kf_paged_reserve_args;
+typedef struct kf_paged_release_args {
+  kf_page_tables tables;
+  const uint8_t* finished;
+} kf_paged_release_args;
+int kf_paged_reserve(const kf_paged_reserve_args* args);
+int kf_paged_release(const kf_paged_release_args* args);
 
 /* ---- self-test of the bounded device wait -------------------------------
  * No counterpart in the reference.  Launches one kernel that waits on a

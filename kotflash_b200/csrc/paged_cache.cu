@@ -357,21 +357,19 @@ __global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const Rele
   }
 }
 
-int check_tables(const char* what, const void* lengths, const void* second, int64_t B, const void* table,
-                 int64_t max_pages, int64_t table_stride, const void* free_pages, int64_t num_pages,
-                 const void* free_count, int64_t page_size, const void* lengths_out, const void* free_count_out) {
+int check_tables(const char* what, const kf_page_tables& t) {
   using kf::set_error;
-  if (!lengths || !second || !table || !free_pages || !free_count || !lengths_out || !free_count_out)
+  if (!t.lengths || !t.block_table || !t.free_pages || !t.free_count || !t.lengths_out || !t.free_count_out)
     return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
-  if (B <= 0 || max_pages <= 0 || num_pages <= 0)
+  if (t.B <= 0 || t.max_pages <= 0 || t.num_pages <= 0)
     return set_error(KF_ERR_INVALID, "%s: requests, table columns and pages must be non-zero", what);
-  if (page_size <= 0 || page_size > (1 << 20))
+  if (t.page_size <= 0 || t.page_size > (1 << 20))
     return set_error(KF_ERR_INVALID, "%s: page_size must be in [1, 2^20]", what);
-  if (B > 1 && table_stride < max_pages)
+  if (t.B > 1 && t.table_stride < t.max_pages)
     return set_error(KF_ERR_INVALID, "%s: block table rows overlap", what);
-  if (B > kMaxRequests)
+  if (t.B > kMaxRequests)
     return set_error(KF_ERR_UNSUPPORTED, "%s: at most %lld requests", what, (long long)kMaxRequests);
-  if (max_pages > 0x7fffffffLL || num_pages > 0x7fffffffLL)
+  if (t.max_pages > 0x7fffffffLL || t.num_pages > 0x7fffffffLL)
     return set_error(KF_ERR_UNSUPPORTED, "%s: too many pages", what);
   return KF_OK;
 }
@@ -396,11 +394,11 @@ unsigned cluster_for(int64_t units, int64_t per_block) {
 
 }  // namespace
 
-extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pages, const kf_tensor4* new_k,
-                               const kf_tensor4* new_v, const int64_t* slots, int dtype, void* stream) {
+extern "C" int kf_paged_append(const kf_paged_append_args* args) {
   using kf::set_error;
-  if (!k_pages || !v_pages || !new_k || !new_v)
-    return set_error(KF_ERR_INVALID, "kf_paged_append: null tensor descriptor");
+  if (!args) return set_error(KF_ERR_INVALID, "kf_paged_append: null arguments");
+  const kf_tensor4 *k_pages = &args->k_pages, *v_pages = &args->v_pages, *new_k = &args->new_k, *new_v = &args->new_v;
+  const int64_t dtype = args->dtype;
   if (dtype != KF_F16 && dtype != KF_BF16)
     return set_error(KF_ERR_INVALID, "kf_paged_append: dtype must be fp16 or bf16");
   for (int i = 0; i < 4; ++i) {
@@ -417,7 +415,7 @@ extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pa
   if (N > 0x7fffffffLL || S > 0x7fffffffLL || N * S > 0x7fffffffLL || H > 0x7fffffffLL || D > 0x7fffffffLL ||
       H * D > 0x7fffffffLL || k_pages->size[2] > (1 << 20))
     return set_error(KF_ERR_UNSUPPORTED, "kf_paged_append: tensors too large");
-  if (!k_pages->ptr || !v_pages->ptr || !new_k->ptr || !new_v->ptr || !slots)
+  if (!k_pages->ptr || !v_pages->ptr || !new_k->ptr || !new_v->ptr || !args->slots)
     return set_error(KF_ERR_INVALID, "kf_paged_append: null data pointer");
   kf::DeviceGuard guard(k_pages->ptr);
   if (guard.status()) return guard.status();
@@ -427,7 +425,7 @@ extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pa
   a.src_v = static_cast<const uint16_t*>(new_v->ptr);
   a.dst_k = static_cast<uint16_t*>(k_pages->ptr);
   a.dst_v = static_cast<uint16_t*>(v_pages->ptr);
-  a.slots = slots;
+  a.slots = args->slots;
   for (int i = 0; i < 4; ++i) {
     a.sk[i] = new_k->stride[i];
     a.sv[i] = new_v->stride[i];
@@ -444,7 +442,7 @@ extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pa
   a.block_tokens = a.per_token <= kAppendThreads ? kAppendThreads / a.per_token : 0;
   const int64_t side = a.block_tokens ? a.block_tokens : 1;
   const int64_t sms = kf::sm_count_current_device();
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
   auto go = [&](auto kern, int64_t per_block) {
     int64_t blocks = (a.T + per_block - 1) / per_block;
     if (blocks > sms * 64) blocks = sms * 64;
@@ -454,77 +452,75 @@ extern "C" int kf_paged_append(const kf_tensor4* k_pages, const kf_tensor4* v_pa
   return a.T >= side * 4 * sms * 2 ? go(paged_append_kernel<8, 4>, side * 4) : go(paged_append_kernel<8, 1>, side);
 }
 
-extern "C" int kf_paged_reserve(const int32_t* lengths, const int32_t* new_lengths, int64_t B, int32_t* block_table,
-                                int64_t max_pages, int64_t table_stride, const int32_t* free_pages,
-                                int64_t num_pages, const int32_t* free_count, int64_t page_size, int64_t* slots,
-                                int64_t num_tokens, int64_t tokens_per_request, int32_t* starts,
-                                int32_t* lengths_out, int32_t* free_count_out, void* stream) {
+extern "C" int kf_paged_reserve(const kf_paged_reserve_args* args) {
   using kf::set_error;
   const char* what = "kf_paged_reserve";
-  int rc = check_tables(what, lengths, new_lengths, B, block_table, max_pages, table_stride, free_pages, num_pages,
-                        free_count, page_size, lengths_out, free_count_out);
+  if (!args) return set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  const kf_page_tables& t = args->tables;
+  int rc = check_tables(what, t);
   if (rc != KF_OK) return rc;
+  const int64_t num_tokens = args->num_tokens, per_request = args->tokens_per_request;
   if (num_tokens < 0 || num_tokens > 0x7fffffffLL)
     return set_error(KF_ERR_INVALID, "%s: num_tokens must be in [0, 2^31)", what);
-  if (tokens_per_request < 0 || (tokens_per_request > 0 && tokens_per_request * B != num_tokens))
+  if (per_request < 0 || (per_request > 0 && (per_request > num_tokens || per_request * t.B != num_tokens)))
     return set_error(KF_ERR_INVALID, "%s: num_tokens must be tokens_per_request for each request", what);
-  if (!starts || (num_tokens > 0 && !slots)) return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
-  if (num_tokens > 0 && !kf::aligned16(slots))
+  if (!args->new_lengths || !args->starts || (num_tokens > 0 && !args->slots))
+    return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (num_tokens > 0 && !kf::aligned16(args->slots))
     return set_error(KF_ERR_INVALID, "%s: slots must be 16-byte aligned", what);
-  kf::DeviceGuard guard(lengths);
+  kf::DeviceGuard guard(t.lengths);
   if (guard.status()) return guard.status();
   ReserveArgs a;
-  a.lengths = lengths;
-  a.added = new_lengths;
-  a.table = block_table;
-  a.free_pages = free_pages;
-  a.free_count = free_count;
-  a.slots = slots;
-  a.starts = starts;
-  a.lengths_out = lengths_out;
-  a.free_count_out = free_count_out;
-  a.table_stride = table_stride;
+  a.lengths = t.lengths;
+  a.added = args->new_lengths;
+  a.table = t.block_table;
+  a.free_pages = t.free_pages;
+  a.free_count = t.free_count;
+  a.slots = args->slots;
+  a.starts = args->starts;
+  a.lengths_out = t.lengths_out;
+  a.free_count_out = t.free_count_out;
+  a.table_stride = t.table_stride;
   a.T = num_tokens;
-  a.padded = (uint32_t)tokens_per_request;
-  a.B = (int)B;
-  a.max_pages = (uint32_t)max_pages;
-  a.page_size = (uint32_t)page_size;
-  a.num_pages = (uint32_t)num_pages;
-  const size_t smem = (size_t)(2 * B + 1) * 4 + (size_t)B;
+  a.padded = (uint32_t)per_request;
+  a.B = (int)t.B;
+  a.max_pages = (uint32_t)t.max_pages;
+  a.page_size = (uint32_t)t.page_size;
+  a.num_pages = (uint32_t)t.num_pages;
+  const size_t smem = (size_t)(2 * t.B + 1) * 4 + (size_t)t.B;
   rc = raise_smem(paged_reserve_kernel, smem, what);
   if (rc != KF_OK) return rc;
   const unsigned cluster = cluster_for(num_tokens, kTableThreads * 4);
   return kf::launch_dependent_cluster(paged_reserve_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
-                                      static_cast<cudaStream_t>(stream), what, a);
+                                      static_cast<cudaStream_t>(t.stream), what, a);
 }
 
-extern "C" int kf_paged_release(const int32_t* lengths, const uint8_t* finished, int64_t B,
-                                const int32_t* block_table, int64_t max_pages, int64_t table_stride,
-                                int32_t* free_pages, int64_t num_pages, const int32_t* free_count,
-                                int64_t page_size, int32_t* lengths_out, int32_t* free_count_out, void* stream) {
+extern "C" int kf_paged_release(const kf_paged_release_args* args) {
   const char* what = "kf_paged_release";
-  int rc = check_tables(what, lengths, finished, B, block_table, max_pages, table_stride, free_pages, num_pages,
-                        free_count, page_size, lengths_out, free_count_out);
+  if (!args) return kf::set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  const kf_page_tables& t = args->tables;
+  int rc = check_tables(what, t);
   if (rc != KF_OK) return rc;
-  kf::DeviceGuard guard(lengths);
+  if (!args->finished) return kf::set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  kf::DeviceGuard guard(t.lengths);
   if (guard.status()) return guard.status();
   ReleaseArgs a;
-  a.lengths = lengths;
-  a.finished = finished;
-  a.table = block_table;
-  a.free_pages = free_pages;
-  a.free_count = free_count;
-  a.lengths_out = lengths_out;
-  a.free_count_out = free_count_out;
-  a.table_stride = table_stride;
-  a.B = (int)B;
-  a.max_pages = (uint32_t)max_pages;
-  a.page_size = (uint32_t)page_size;
-  a.num_pages = (uint32_t)num_pages;
-  const size_t smem = (size_t)B * 4;
+  a.lengths = t.lengths;
+  a.finished = args->finished;
+  a.table = t.block_table;
+  a.free_pages = t.free_pages;
+  a.free_count = t.free_count;
+  a.lengths_out = t.lengths_out;
+  a.free_count_out = t.free_count_out;
+  a.table_stride = t.table_stride;
+  a.B = (int)t.B;
+  a.max_pages = (uint32_t)t.max_pages;
+  a.page_size = (uint32_t)t.page_size;
+  a.num_pages = (uint32_t)t.num_pages;
+  const size_t smem = (size_t)t.B * 4;
   rc = raise_smem(paged_release_kernel, smem, what);
   if (rc != KF_OK) return rc;
-  const unsigned cluster = cluster_for(B, kTableWarps);
+  const unsigned cluster = cluster_for(t.B, kTableWarps);
   return kf::launch_dependent_cluster(paged_release_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
-                                      static_cast<cudaStream_t>(stream), what, a);
+                                      static_cast<cudaStream_t>(t.stream), what, a);
 }

@@ -697,14 +697,13 @@ extern "C" size_t kf_paged_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64
   return workspace_need(sm_count * kBlocksPerSm, unit_rows(Hq / Hkv), D);
 }
 
-extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, const kf_tensor4* v_pages,
-                               const int32_t* block_table, int64_t max_pages, int64_t table_stride,
-                               const int32_t* lengths, const kf_tensor4* new_k, const kf_tensor4* new_v,
-                               const int64_t* slots, const kf_tensor4* o, float* lse, int dtype, float scale,
-                               void* workspace, size_t workspace_bytes, int32_t* status, void* stream) {
+extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   using kf::set_error;
   const char* what = "kf_paged_decode";
-  if (!q || !k_pages || !v_pages || !o) return set_error(KF_ERR_INVALID, "%s: null tensor descriptor", what);
+  if (!args) return set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  const kf_tensor4 *q = &args->q, *k_pages = &args->k_pages, *v_pages = &args->v_pages, *o = &args->o;
+  const kf_tensor4 *new_k = &args->new_k, *new_v = &args->new_v;
+  const int64_t dtype = args->dtype, max_pages = args->max_pages;
   if (dtype != KF_F16 && dtype != KF_BF16) return set_error(KF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
   const int64_t B = q->size[0], Hq = q->size[1], D = q->size[3];
   const int64_t pages = k_pages->size[0], Hkv = k_pages->size[1], page_size = k_pages->size[2];
@@ -725,11 +724,12 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
     return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
   if (!rows16(q, 2) || !rows16(k_pages, 3) || !rows16(v_pages, 3) || !rows16(o, 2))
     return set_error(KF_ERR_INVALID, "%s: tensors need a contiguous last dim and 16-byte aligned rows", what);
-  if (!q->ptr || !k_pages->ptr || !v_pages->ptr || !o->ptr || !block_table || !lengths)
+  if (!q->ptr || !k_pages->ptr || !v_pages->ptr || !o->ptr || !args->block_table || !args->lengths)
     return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
-  const bool fused = new_k != nullptr || new_v != nullptr;
+  const bool fused = new_k->ptr || new_v->ptr || args->slots;
   if (fused) {
-    if (!new_k || !new_v) return set_error(KF_ERR_INVALID, "%s: new_k and new_v go together", what);
+    if (!new_k->ptr || !new_v->ptr || !args->slots)
+      return set_error(KF_ERR_INVALID, "%s: new_k, new_v and slots go together", what);
     for (int i = 0; i < 4; ++i)
       if (new_v->size[i] != new_k->size[i])
         return set_error(KF_ERR_INVALID, "%s: new K and V shapes must match", what);
@@ -737,7 +737,6 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
       return set_error(KF_ERR_INVALID, "%s: new K/V must be [B, Hkv, 1, D]", what);
     if (!rows16(new_k, 2) || !rows16(new_v, 2))
       return set_error(KF_ERR_INVALID, "%s: new K/V rows must be 16-byte aligned", what);
-    if (!new_k->ptr || !new_v->ptr || !slots) return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
   }
   kf::DeviceGuard guard(q->ptr);
   if (guard.status()) return guard.status();
@@ -749,11 +748,11 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   a.v = static_cast<uint16_t*>(v_pages->ptr);
   a.nk = fused ? static_cast<const uint16_t*>(new_k->ptr) : nullptr;
   a.nv = fused ? static_cast<const uint16_t*>(new_v->ptr) : nullptr;
-  a.slots = slots;
+  a.slots = args->slots;
   a.o = static_cast<uint16_t*>(o->ptr);
-  a.lse = lse;
-  a.table = block_table;
-  a.lengths = lengths;
+  a.lse = args->lse;
+  a.table = args->block_table;
+  a.lengths = args->lengths;
   for (int i = 0; i < 2; ++i) {
     a.qs[i] = q->stride[i];
     a.os[i] = o->stride[i];
@@ -764,7 +763,7 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
     a.ks[i] = k_pages->stride[i];
     a.vs[i] = v_pages->stride[i];
   }
-  a.table_stride = table_stride;
+  a.table_stride = args->table_stride;
   a.B = (int)B;
   a.Hq = (int)Hq;
   a.Hkv = (int)Hkv;
@@ -775,7 +774,7 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
-  a.status = status;
+  a.status = args->status;
   // Division by page_size: with 2^(s-1) < page_size <= 2^s and m =
   // ceil(2^(31+s) / page_size), m < 2^32 and m page_size exceeds 2^(31+s) by
   // less than 2^s, so x m >> (31 + s) is exact for x < 2^31.
@@ -786,7 +785,7 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   // boxes never cross a page nor a team's 16 or 32 keys
   a.box = 16;
   while (page_size % a.box) a.box /= 2;
-  a.scale_log2 = scale * kLog2e;
+  a.scale_log2 = (float)args->scale * kLog2e;
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.
   // A unit of one tile is never cut, so nothing is left to join.
@@ -801,9 +800,9 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   a.join_units = false;
   if (most > 1) {
     const size_t need = workspace_need((int)blocks, rows, D);
-    if (!workspace || workspace_bytes < need)
+    if (!args->workspace || args->workspace_bytes < need)
       return set_error(KF_ERR_WORKSPACE, "%s: workspace needs %zu bytes", what, need);
-    uintptr_t base = (reinterpret_cast<uintptr_t>(workspace) + 255) & ~uintptr_t(255);
+    uintptr_t base = (reinterpret_cast<uintptr_t>(args->workspace) + 255) & ~uintptr_t(255);
     a.joins = reinterpret_cast<int4*>(base);
     a.part_o = reinterpret_cast<float*>(a.joins + blocks);
     a.part_lse = a.part_o + (size_t)blocks * 2 * rows * D;
@@ -814,7 +813,7 @@ extern "C" int kf_paged_decode(const kf_tensor4* q, const kf_tensor4* k_pages, c
   if (rc != KF_OK) return rc;
   rc = kf::encode_tmap_4d(&mv, v_pages, 64, a.box);
   if (rc != KF_OK) return rc;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
   const bool bf16 = dtype == KF_BF16;
   if (D <= 64)
     rc = bf16 ? dispatch_rows<true, 1>(a, mk, mv, rows, (int)blocks, st)

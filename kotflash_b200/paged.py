@@ -32,10 +32,16 @@ import torch
 from . import _ext
 
 _DTYPES = {torch.float16: _ext.KF_F16, torch.bfloat16: _ext.KF_BF16}
+_INT32, _INT64, _BOOL = torch.int32, torch.int64, torch.bool
+_NO_ROWS = (0,) * 18  # two empty kf_tensor4
 
 
-def _check_device(what: str, *tensors: torch.Tensor) -> int:
-    """Index of the one sm_100 device that holds all tensors."""
+# Each entry point below tests everything in one expression, which is what a
+# valid call pays for (a few us of a call that lasts about ten); only when it
+# is false do these functions find out what to say.
+
+def _check_device(what: str, *tensors: torch.Tensor) -> None:
+    """All tensors on one sm_100 device."""
     dev = tensors[0].device
     if dev.type != "cuda":
         raise RuntimeError(f"{what} requires CUDA tensors on an sm_100 (B200) device")
@@ -44,29 +50,25 @@ def _check_device(what: str, *tensors: torch.Tensor) -> int:
             raise ValueError(f"{what}: all tensors must be on the same device")
     if not _ext.is_sm100(dev.index):
         raise RuntimeError(f"{what} requires an sm_100 (B200) CUDA device")
-    return dev.index
 
 
-def _check_pools(what: str, k_pages: torch.Tensor, v_pages: torch.Tensor, *others: torch.Tensor) -> int:
-    """Dtype code shared by the pools and the other K/V or query tensors."""
-    dtype = k_pages.dtype
-    for t in (v_pages, *others):
-        if t.dtype != dtype:
+def _check_pools(what: str, *tensors: torch.Tensor) -> None:
+    """Pools and the K/V or query tensors beside them."""
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{what}: K/V pages, K/V rows and queries must be torch.Tensor instances")
+    for t in tensors:
+        if t.dtype != tensors[0].dtype:
             raise ValueError(f"{what}: dtypes must match")
-    for t in (k_pages, v_pages, *others):
         if t.ndim != 4:
             raise ValueError(f"{what}: expected 4-D tensors, pages in [pages, Hkv, page_size, D] layout")
-    code = _DTYPES.get(dtype)
-    if code is None:
-        raise TypeError(f"{what} supports float16 and bfloat16, got {dtype}")
-    return code
+    if tensors[0].dtype not in _DTYPES:
+        raise TypeError(f"{what} supports float16 and bfloat16, got {tensors[0].dtype}")
 
 
 def _check_inference(what: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t.requires_grad:
-                raise RuntimeError(f"{what} is inference-only; disable gradients")
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} is inference-only; disable gradients")
 
 
 def _check_int32(what: str, **tensors: torch.Tensor) -> None:
@@ -77,6 +79,15 @@ def _check_int32(what: str, **tensors: torch.Tensor) -> None:
             raise TypeError(f"{what}: {name} must be int32")
 
 
+def _check_slots(what: str, slots: torch.Tensor, count: int, meaning: str) -> None:
+    if not isinstance(slots, torch.Tensor):
+        raise TypeError(f"{what}: slots must be a torch.Tensor")
+    if slots.dtype != torch.int64:
+        raise TypeError(f"{what}: slots must be int64")
+    if slots.ndim != 1 or slots.shape[0] != count or not slots.is_contiguous():
+        raise ValueError(f"{what}: slots must be contiguous, {meaning}")
+
+
 def _check_table(what: str, block_table: torch.Tensor, requests: int) -> None:
     if block_table.ndim != 2 or block_table.shape[0] != requests:
         raise ValueError(f"{what}: block_table must be [requests, max_pages]")
@@ -84,9 +95,32 @@ def _check_table(what: str, block_table: torch.Tensor, requests: int) -> None:
         raise ValueError(f"{what}: block_table rows must be contiguous")
 
 
+def _check_attention(q, k_pages, v_pages, block_table, lengths, new_k, new_v, slots) -> None:
+    what = "paged_attention"
+    if (new_k is None) != (new_v is None) or (new_k is None) != (slots is None):
+        raise ValueError(f"{what}: new_k, new_v and slots go together")
+    rows = () if new_k is None else (new_k, new_v)
+    _check_pools(what, q, k_pages, v_pages, *rows)
+    _check_int32(what, block_table=block_table, lengths=lengths)
+    b, hq = q.shape[:2]
+    hkv = k_pages.shape[1]
+    _check_table(what, block_table, b)
+    if lengths.ndim != 1 or lengths.shape[0] != b or not lengths.is_contiguous():
+        raise ValueError(f"{what}: lengths must be a contiguous [requests] tensor")
+    if rows:
+        _check_slots(what, slots, b, "one for each request")
+    if b == 0 or hq == 0 or hkv == 0:
+        raise ValueError(f"{what}: batch and head dimensions must be non-zero")
+    if hq % hkv:
+        raise ValueError("num_query_heads must be divisible by num_kv_heads (GQA/MQA)")
+    _check_inference(what, q, k_pages, v_pages, *rows)
+    _check_device(what, q, k_pages, v_pages, block_table, lengths, *rows, *((slots,) if rows else ()))
+
+
 @lru_cache(maxsize=256)
-def _workspace_bytes(hq: int, hkv: int, d: int, device_index: int) -> int:
-    return max(16, _ext.load().kf_paged_decode_workspace_bytes(hq, hkv, d, _ext.sm_count(device_index)))
+def _workspace_elements(hq: int, hkv: int, d: int, device_index: int) -> int:
+    """Workspace of kf_paged_decode in 16-bit elements."""
+    return _ext.load().kf_paged_decode_workspace_bytes(hq, hkv, d, _ext.sm_count(device_index)) // 2 + 8
 
 
 def paged_attention(
@@ -119,56 +153,62 @@ def paged_attention(
     the slot); where slots[b] < 0 the request has no new row.  Returns [B, Hq, 1, D] in q's dtype and, with return_lse, the
     fp32 LSE [B, Hq, 1].
     """
-    what = "paged_attention"
-    if not (isinstance(q, torch.Tensor) and isinstance(k_pages, torch.Tensor) and isinstance(v_pages, torch.Tensor)):
-        raise TypeError("q, k_pages and v_pages must be torch.Tensor instances")
-    _check_int32(what, block_table=block_table, lengths=lengths)
-    if (new_k is None) != (new_v is None) or (new_k is None) != (slots is None):
-        raise ValueError(f"{what}: new_k, new_v and slots go together")
-    rows = () if new_k is None else (new_k, new_v)
-    if rows and not (isinstance(new_k, torch.Tensor) and isinstance(new_v, torch.Tensor)
-                     and isinstance(slots, torch.Tensor)):
-        raise TypeError("new_k, new_v and slots must be torch.Tensor instances")
-    dtype = _check_pools(what, k_pages, v_pages, q, *rows)
-    b, hq, _, d = q.shape
-    _check_table(what, block_table, b)
-    if lengths.ndim != 1 or lengths.shape[0] != b or not lengths.is_contiguous():
-        raise ValueError(f"{what}: lengths must be a contiguous [requests] tensor")
-    if rows:
-        if slots.dtype != torch.int64:
-            raise TypeError(f"{what}: slots must be int64")
-        if slots.ndim != 1 or slots.shape[0] != b or not slots.is_contiguous():
-            raise ValueError(f"{what}: slots must be a contiguous [requests] tensor")
-    if scale is None:
-        scale = 1.0 / math.sqrt(d) if d else 1.0
-    else:
+    if scale is not None:
         try:
             scale = float(scale)
         except (TypeError, ValueError) as exc:
             raise TypeError("scale must be a finite real number or None") from exc
         if not math.isfinite(scale):
             raise ValueError("scale must be finite")
-    hkv = k_pages.shape[1]
-    if b == 0 or hq == 0 or hkv == 0:
-        raise ValueError(f"{what}: batch and head dimensions must be non-zero")
-    if hq % hkv:
-        raise ValueError("num_query_heads must be divisible by num_kv_heads (GQA/MQA)")
-    _check_inference(what, q, k_pages, v_pages, *rows)
-    idx = _check_device(what, q, k_pages, v_pages, block_table, lengths, *rows, *((slots,) if rows else ()))
+    try:
+        index = q.get_device()
+        b, hq, _, d = qs = q.shape
+        ks = k_pages.shape
+        dtype = q.dtype
+        good = (
+            index >= 0 and _ext.is_sm100(index) and k_pages.dtype is dtype and v_pages.dtype is dtype
+            and dtype in _DTYPES and len(ks) == 4 and v_pages.ndim == 4
+            and block_table.dtype is _INT32 and lengths.dtype is _INT32 and lengths.shape == qs[:1]
+            and lengths.is_contiguous() and block_table.ndim == 2 and block_table.shape[0] == b
+            and block_table.stride(1) == 1 and b > 0 and hq > 0 and ks[1] > 0 and hq % ks[1] == 0
+            and k_pages.get_device() == index and v_pages.get_device() == index
+            and block_table.get_device() == index and lengths.get_device() == index
+            and not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))
+            and (new_k is None and new_v is None and slots is None
+                 or new_k.dtype is dtype and new_v.dtype is dtype and slots.dtype is _INT64
+                 and new_k.ndim == 4 and new_v.ndim == 4 and slots.shape == qs[:1] and slots.is_contiguous()
+                 and new_k.get_device() == index and new_v.get_device() == index and slots.get_device() == index
+                 and not (torch.is_grad_enabled() and (new_k.requires_grad or new_v.requires_grad)))
+        )
+    except (AttributeError, TypeError, ValueError, RuntimeError):
+        good = False
+    if not good:
+        _check_attention(q, k_pages, v_pages, block_table, lengths, new_k, new_v, slots)
+        index = q.get_device()
+        b, hq, _, d = qs = q.shape
+        ks = k_pages.shape
+        dtype = q.dtype
+    if scale is None:
+        scale = 1.0 / math.sqrt(d) if d else 1.0
     lib = _ext.load()
-    dev = q.device
-    out = torch.empty(q.shape, dtype=q.dtype, device=dev)
-    lse = torch.empty((b, hq, 1), dtype=torch.float32, device=dev) if return_lse else None
-    ws_bytes = _workspace_bytes(hq, hkv, d, idx)
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=dev)
-    rc = lib.kf_paged_decode(
-        _ext.packed4(q), _ext.packed4(k_pages), _ext.packed4(v_pages), block_table.data_ptr(),
-        block_table.shape[1], block_table.stride(0), lengths.data_ptr(),
-        _ext.packed4(new_k) if rows else None, _ext.packed4(new_v) if rows else None,
-        slots.data_ptr() if rows else None, _ext.packed4(out), lse.data_ptr() if return_lse else None, dtype, scale,
-        workspace.data_ptr(), ws_bytes, _ext.status_word(dev).data_ptr(), _ext.stream_of(q),
-    )
-    _ext.check(rc, "kf_paged_decode")
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((b, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
+    elements = _workspace_elements(hq, ks[1], d, index)
+    workspace = q.new_empty(elements)
+    if new_k is None:
+        rows, slots_ptr = _NO_ROWS, 0
+    else:
+        rows = (new_k.data_ptr(), *new_k.shape, *new_k.stride(), new_v.data_ptr(), *new_v.shape, *new_v.stride())
+        slots_ptr = slots.data_ptr()
+    rc = lib.kf_paged_decode(_ext.pack_paged_decode(
+        q.data_ptr(), *qs, *q.stride(), k_pages.data_ptr(), *ks, *k_pages.stride(),
+        v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(), out.data_ptr(), *qs, *out.stride(), *rows,
+        slots_ptr, block_table.data_ptr(), block_table.shape[1], block_table.stride(0), lengths.data_ptr(),
+        lse.data_ptr() if return_lse else 0, _DTYPES[dtype], scale, workspace.data_ptr(), elements * 2,
+        _ext.status_word(q.device).data_ptr(), _ext.raw_stream(index),
+    ))
+    if rc:
+        _ext.check(rc, "kf_paged_decode")
     return (out, lse) if return_lse else out
 
 
@@ -186,20 +226,53 @@ def append_paged_kv(
     page slots[t] // page_size.  Tokens whose slot is outside the pool (-1 for
     those that ``reserve_pages`` refused) are skipped.
     """
-    what = "append_paged_kv"
-    if not all(isinstance(t, torch.Tensor) for t in (k_pages, v_pages, new_k, new_v, slots)):
-        raise TypeError("pages, new K/V values and slots must be torch.Tensor instances")
-    dtype = _check_pools(what, k_pages, v_pages, new_k, new_v)
-    if slots.dtype != torch.int64:
-        raise TypeError(f"{what}: slots must be int64")
-    if slots.ndim != 1 or slots.shape[0] != new_k.shape[0] * new_k.shape[2] or not slots.is_contiguous():
-        raise ValueError(f"{what}: slots must be a contiguous [tokens] tensor, one slot for each new K/V row")
-    _check_inference(what, k_pages, v_pages, new_k, new_v)
-    _check_device(what, k_pages, v_pages, new_k, new_v, slots)
-    lib = _ext.load()
-    rc = lib.kf_paged_append(_ext.packed4(k_pages), _ext.packed4(v_pages), _ext.packed4(new_k), _ext.packed4(new_v),
-                             slots.data_ptr(), dtype, _ext.stream_of(k_pages))
-    _ext.check(rc, "kf_paged_append")
+    try:
+        index = k_pages.get_device()
+        dtype = k_pages.dtype
+        ns = new_k.shape
+        good = (
+            index >= 0 and _ext.is_sm100(index) and dtype in _DTYPES and v_pages.dtype is dtype
+            and new_k.dtype is dtype and new_v.dtype is dtype and slots.dtype is _INT64 and k_pages.ndim == 4
+            and v_pages.ndim == 4 and len(ns) == 4 and new_v.ndim == 4 and slots.shape == (ns[0] * ns[2],)
+            and slots.is_contiguous() and v_pages.get_device() == index and new_k.get_device() == index
+            and new_v.get_device() == index and slots.get_device() == index
+            and not (torch.is_grad_enabled() and (k_pages.requires_grad or v_pages.requires_grad
+                                                  or new_k.requires_grad or new_v.requires_grad))
+        )
+    except (AttributeError, TypeError, RuntimeError):
+        good = False
+    if not good:
+        what = "append_paged_kv"
+        _check_pools(what, k_pages, v_pages, new_k, new_v)
+        _check_slots(what, slots, new_k.shape[0] * new_k.shape[2], "one slot for each new K/V row")
+        _check_inference(what, k_pages, v_pages, new_k, new_v)
+        _check_device(what, k_pages, v_pages, new_k, new_v, slots)
+        index, dtype, ns = k_pages.get_device(), k_pages.dtype, new_k.shape
+    rc = _ext.load().kf_paged_append(_ext.pack_paged_append(
+        k_pages.data_ptr(), *k_pages.shape, *k_pages.stride(), v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(),
+        new_k.data_ptr(), *ns, *new_k.stride(), new_v.data_ptr(), *new_v.shape, *new_v.stride(),
+        slots.data_ptr(), _DTYPES[dtype], _ext.raw_stream(index),
+    ))
+    if rc:
+        _ext.check(rc, "kf_paged_append")
+
+
+def _tables_good(lengths, second, block_table, free_pages, free_count, lengths_out, free_count_out) -> bool:
+    try:
+        index = lengths.get_device()
+        shape = lengths.shape
+        return (
+            index >= 0 and _ext.is_sm100(index) and lengths.dtype is _INT32 and block_table.dtype is _INT32
+            and free_pages.dtype is _INT32 and free_count.dtype is _INT32 and len(shape) == 1
+            and second.shape == shape and block_table.ndim == 2 and block_table.shape[0] == shape[0]
+            and block_table.stride(1) == 1 and free_pages.ndim == 1 and free_count.numel() == 1
+            and lengths.is_contiguous() and second.is_contiguous() and free_pages.is_contiguous()
+            and second.get_device() == index and block_table.get_device() == index
+            and free_pages.get_device() == index and free_count.get_device() == index
+            and (lengths_out is None or lengths_out is lengths) and (free_count_out is None or free_count_out is free_count)
+        )
+    except (AttributeError, TypeError, RuntimeError):
+        return False
 
 
 def _check_tables(what, lengths, second, block_table, free_pages, free_count, lengths_out, free_count_out):
@@ -253,9 +326,8 @@ def reserve_pages(
     """
     what = "reserve_pages"
     _check_int32(what, new_lengths=new_lengths)
-    _check_tables(what, lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out)
-    lib = _ext.load()
-    dev = lengths.device
+    if not _tables_good(lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out):
+        _check_tables(what, lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out)
     b = lengths.shape[0]
     if (num_tokens is None) == (tokens_per_request is None):
         raise ValueError(f"{what}: give num_tokens or tokens_per_request")
@@ -267,19 +339,20 @@ def reserve_pages(
         num_tokens = per_request * b
     elif num_tokens < 0:
         raise ValueError(f"{what}: num_tokens must not be negative")
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=dev)
-    starts = torch.empty(b + 1, dtype=torch.int32, device=dev)
+    slots = torch.empty(num_tokens, dtype=torch.int64, device=lengths.device)
+    starts = lengths.new_empty(b + 1)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
     if free_count_out is None:
         free_count_out = torch.empty_like(free_count)
-    rc = lib.kf_paged_reserve(
-        lengths.data_ptr(), new_lengths.data_ptr(), b, block_table.data_ptr(), block_table.shape[1],
-        block_table.stride(0), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size,
-        slots.data_ptr(), num_tokens, per_request, starts.data_ptr(), lengths_out.data_ptr(), free_count_out.data_ptr(),
-        _ext.stream_of(lengths),
-    )
-    _ext.check(rc, "kf_paged_reserve")
+    rc = _ext.load().kf_paged_reserve(_ext.pack_paged_reserve(
+        lengths.data_ptr(), b, block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
+        free_count_out.data_ptr(), _ext.raw_stream(lengths.get_device()), new_lengths.data_ptr(), slots.data_ptr(),
+        num_tokens, per_request, starts.data_ptr(),
+    ))
+    if rc:
+        _ext.check(rc, "kf_paged_reserve")
     return slots, starts, lengths_out, free_count_out
 
 
@@ -302,20 +375,21 @@ def release_pages(
     rows keep old entries, which no length reaches any more.
     """
     what = "release_pages"
-    if not isinstance(finished, torch.Tensor) or finished.dtype != torch.bool:
+    if not isinstance(finished, torch.Tensor) or finished.dtype is not _BOOL:
         raise TypeError(f"{what}: finished must be a bool tensor")
-    _check_tables(what, lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out)
-    lib = _ext.load()
+    if not _tables_good(lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out):
+        _check_tables(what, lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
     if free_count_out is None:
         free_count_out = torch.empty_like(free_count)
-    rc = lib.kf_paged_release(
-        lengths.data_ptr(), finished.data_ptr(), lengths.shape[0], block_table.data_ptr(), block_table.shape[1],
-        block_table.stride(0), free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size,
-        lengths_out.data_ptr(), free_count_out.data_ptr(), _ext.stream_of(lengths),
-    )
-    _ext.check(rc, "kf_paged_release")
+    rc = _ext.load().kf_paged_release(_ext.pack_paged_release(
+        lengths.data_ptr(), lengths.shape[0], block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
+        free_count_out.data_ptr(), _ext.raw_stream(lengths.get_device()), finished.data_ptr(),
+    ))
+    if rc:
+        _ext.check(rc, "kf_paged_release")
     return lengths_out, free_count_out
 
 

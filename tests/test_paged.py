@@ -2,6 +2,9 @@
 """Paged KV cache on the CPU: refusals of the Python layer and of the C ABI
 (before any launch), and the arithmetic of the decode kernel's work split."""
 import random
+import shutil
+import subprocess
+from pathlib import Path
 
 import pytest
 import torch
@@ -104,28 +107,37 @@ def test_cache_constructor():
 
 
 def _t(shape, ptr=0x1000, strides=None):
-    d = _ext.KFTensor4()
-    d.ptr = ptr
-    strides = strides or [shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1]
-    for i in range(4):
-        d.size[i], d.stride[i] = shape[i], strides[i]
-    return bytes(d)
+    if shape is None:
+        return (0,) * 9
+    return (ptr, *shape, *(strides or [shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1]))
 
 
-def test_packed_descriptor_is_the_struct():
-    x = torch.zeros(3, 5, 7, 16)[:, 1:, ::2]
-    assert _ext.packed4(x) == bytes(_ext.t4(x))
+def test_structs_have_the_headers_sizes(tmp_path):
+    """The packed layouts against sizeof of the C structs and the offset of their last fields."""
+    if shutil.which("gcc") is None:
+        pytest.skip("needs gcc")
+    root = Path(__file__).resolve().parents[1]
+    names = [("decode", "stream"), ("append", "stream"), ("reserve", "starts"), ("release", "finished")]
+    (tmp_path / "s.c").write_text("#include <stdio.h>\n#include <stddef.h>\n#include \"kotflash_b200.h\"\nint main(void) {"
+                                  + "".join(f'printf("%zu %zu\\n", sizeof(kf_paged_{n}_args), offsetof(kf_paged_{n}_args, {last}));'
+                                            for n, last in names) + "return 0; }")
+    subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", str(root / "include"), str(tmp_path / "s.c"), "-o",
+                    str(tmp_path / "s")], check=True, capture_output=True, text=True)
+    lines = subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()
+    for i, (n, _) in enumerate(names):
+        size = getattr(_ext, f"pack_paged_{n}").__self__.size
+        assert int(lines[2 * i]) == size and int(lines[2 * i + 1]) == size - 8
 
 
 def test_c_abi_refuses_before_any_launch():
     lib = _ext.load()
     p = 0x1000
 
-    def decode(q=(3, 4, 1, 64), k=(5, 2, 16, 64), v=None, o=None, table=p, max_pages=2, lens=p, nk=None, nv=None, slots=None,
-               dtype=0, ws=None, ws_bytes=0, q_strides=None, k_ptr=p):
-        return lib.kf_paged_decode(_t(q, strides=q_strides), _t(k, k_ptr), _t(v or k), table, max_pages, max_pages, lens,
-                                   _t(nk) if nk else None, _t(nv) if nv else None, slots, _t(o or q), None, dtype, 0.1, ws,
-                                   ws_bytes, None, None)
+    def decode(q=(3, 4, 1, 64), k=(5, 2, 16, 64), v=None, o=None, table=p, max_pages=2, lens=p, nk=None, nv=None, slots=0,
+               dtype=0, ws=0, ws_bytes=0, q_strides=None, k_ptr=p):
+        return lib.kf_paged_decode(_ext.pack_paged_decode(
+            *_t(q, strides=q_strides), *_t(k, k_ptr), *_t(v or k), *_t(o or q), *_t(nk), *_t(nv), slots, table, max_pages,
+            max_pages, lens, 0, dtype, 0.1, ws, ws_bytes, 0, 0))
 
     for kw, code, match in [
         (dict(dtype=5), _ext.KF_ERR_INVALID, "dtype"),
@@ -141,36 +153,42 @@ def test_c_abi_refuses_before_any_launch():
         (dict(k=(5, 2, 1 << 21, 64)), _ext.KF_ERR_UNSUPPORTED, "too large"),
         (dict(q_strides=[256, 68, 68, 1]), _ext.KF_ERR_INVALID, "16-byte"),
         (dict(k_ptr=0x1008), _ext.KF_ERR_INVALID, "16-byte"),
-        (dict(table=None), _ext.KF_ERR_INVALID, "null data"),
+        (dict(table=0), _ext.KF_ERR_INVALID, "null data"),
         (dict(nk=(3, 2, 1, 64)), _ext.KF_ERR_INVALID, "go together"),
+        (dict(nk=(3, 2, 1, 64), nv=(3, 2, 1, 64)), _ext.KF_ERR_INVALID, "go together"),
         (dict(nk=(3, 2, 2, 64), nv=(3, 2, 2, 64), slots=p), _ext.KF_ERR_INVALID, "new K/V must be"),
-        (dict(nk=(3, 2, 1, 64), nv=(3, 2, 1, 64)), _ext.KF_ERR_INVALID, "null data"),
+        (dict(nk=(3, 2, 1, 64), nv=(3, 2, 1, 72), slots=p), _ext.KF_ERR_INVALID, "new K and V shapes"),
         (dict(max_pages=100), _ext.KF_ERR_WORKSPACE, "workspace needs"),
     ]:
         assert decode(**kw) == code, kw
         assert match in _ext.last_error(), (kw, _ext.last_error())
+    assert lib.kf_paged_decode(None) == _ext.KF_ERR_INVALID
 
     def append(k=(5, 2, 16, 64), nk=(1, 2, 3, 64), nv=None, slots=p, dtype=1):
-        return lib.kf_paged_append(_t(k), _t(k), _t(nk), _t(nv or nk), slots, dtype, None)
+        return lib.kf_paged_append(_ext.pack_paged_append(*_t(k), *_t(k), *_t(nk), *_t(nv or nk), slots, dtype, 0))
 
-    for kw, match in [(dict(nk=(1, 3, 3, 64)), "heads"), (dict(nv=(1, 2, 4, 64)), "new K/V shapes"), (dict(slots=None), "null"),
+    for kw, match in [(dict(nk=(1, 3, 3, 64)), "heads"), (dict(nv=(1, 2, 4, 64)), "new K/V shapes"), (dict(slots=0), "null"),
                       (dict(dtype=9), "dtype"), (dict(nk=(1, 2, 0, 64)), "non-zero")]:
         assert append(**kw) == _ext.KF_ERR_INVALID, kw
         assert match in _ext.last_error()
 
-    def reserve(B=3, max_pages=4, stride=4, pages=9, page=16, slots=p, n=8, per=0, starts=p, lens=p):
-        return lib.kf_paged_reserve(lens, p, B, p, max_pages, stride, p, pages, p, page, slots, n, per, starts, p, p, None)
+    def tables(B=3, max_pages=4, stride=4, pages=9, page=16, lens=p, out=p):
+        return (lens, B, p, max_pages, stride, p, pages, p, page, out, p, 0)
 
-    def release(B=3, max_pages=4, stride=4, pages=9, page=16, out=p):
-        return lib.kf_paged_release(p, p, B, p, max_pages, stride, p, pages, p, page, out, p, None)
+    def reserve(slots=p, n=8, per=0, starts=p, **kw):
+        return lib.kf_paged_reserve(_ext.pack_paged_reserve(*tables(**kw), p, slots, n, per, starts))
+
+    def release(finished=p, **kw):
+        return lib.kf_paged_release(_ext.pack_paged_release(*tables(**kw), finished))
 
     for call, kw, code, match in [
         (reserve, dict(B=0), _ext.KF_ERR_INVALID, "non-zero"), (reserve, dict(page=0), _ext.KF_ERR_INVALID, "page_size"),
         (reserve, dict(stride=3), _ext.KF_ERR_INVALID, "overlap"), (reserve, dict(B=20000), _ext.KF_ERR_UNSUPPORTED, "requests"),
         (reserve, dict(n=-1), _ext.KF_ERR_INVALID, "num_tokens"), (reserve, dict(per=2), _ext.KF_ERR_INVALID, "tokens_per_request"),
-        (reserve, dict(slots=None), _ext.KF_ERR_INVALID, "null"), (reserve, dict(slots=0x1008), _ext.KF_ERR_INVALID, "16-byte"),
-        (reserve, dict(starts=None), _ext.KF_ERR_INVALID, "null"), (reserve, dict(lens=None), _ext.KF_ERR_INVALID, "null"),
-        (release, dict(pages=0), _ext.KF_ERR_INVALID, "non-zero"), (release, dict(out=None), _ext.KF_ERR_INVALID, "null"),
+        (reserve, dict(slots=0), _ext.KF_ERR_INVALID, "null"), (reserve, dict(slots=0x1008), _ext.KF_ERR_INVALID, "16-byte"),
+        (reserve, dict(starts=0), _ext.KF_ERR_INVALID, "null"), (reserve, dict(lens=0), _ext.KF_ERR_INVALID, "null"),
+        (release, dict(pages=0), _ext.KF_ERR_INVALID, "non-zero"), (release, dict(out=0), _ext.KF_ERR_INVALID, "null"),
+        (release, dict(finished=0), _ext.KF_ERR_INVALID, "null"),
         (release, dict(pages=2**31), _ext.KF_ERR_UNSUPPORTED, "too many pages"),
     ]:
         assert call(**kw) == code, kw
