@@ -35,6 +35,17 @@ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 
 
 int sm_count_current_device();
 
+// Multiplier and shift of the division by d in [1, 2^31): x / d = x * mul >>
+// shift in 64 bits for every x < 2^31.  With 2^(s-1) < d <= 2^s and mul =
+// ceil(2^(31+s) / d): mul < 2^32, and mul * d exceeds 2^(31+s) by less than
+// 2^s, so the error of x * mul / 2^(31+s) stays below 1 / d.
+inline void division(int64_t d, uint32_t* mul, uint32_t* shift) {
+  int s = 0;
+  while (((int64_t)1 << s) < d) ++s;
+  *mul = (uint32_t)((((uint64_t)1 << (31 + s)) + d - 1) / d);
+  *shift = (uint32_t)(31 + s);
+}
+
 // Makes the GPU that owns `ptr` the current device for the guard's lifetime
 // and restores the caller's device afterwards, so an entry point launches,
 // encodes tensor maps and reads device properties on the tensor's own GPU

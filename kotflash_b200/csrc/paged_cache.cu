@@ -119,36 +119,57 @@ bool vec_ok(const kf_tensor4* t) {
 constexpr int kTableThreads = 512;
 constexpr int kTableWarps = kTableThreads / 32;
 constexpr int kMaxCluster = 8;
-constexpr int64_t kMaxRequests = 16384;  // 9 bytes of shared memory each
+constexpr int64_t kMaxRequests = 16384;  // 12 bytes of shared memory each
 
-__device__ __forceinline__ uint32_t pages_of(uint32_t tokens, uint32_t page_size) {
-  const uint32_t q = tokens / page_size;
-  return q + (tokens != q * page_size);
-}
+// x / page_size for x < 2^31
+struct PageDiv {
+  uint32_t size, mul, shift;
+  __device__ __forceinline__ uint32_t operator()(uint32_t x) const { return (uint32_t)(((uint64_t)x * mul) >> shift); }
+  __device__ __forceinline__ uint32_t pages(uint32_t tokens) const {  // rounded up
+    const uint32_t q = (*this)(tokens);
+    return q + (q * size != tokens);
+  }
+};
 
 __device__ __forceinline__ int32_t saturate(int64_t x) { return x > 0x7fffffff ? 0x7fffffff : (int32_t)x; }
 
-// Inclusive sum of x over the block's threads; every thread also gets the
-// block's total.  `part` holds one value per warp and is reused by the next call.
-__device__ __forceinline__ int64_t block_scan(int64_t x, int64_t* part, int64_t& total) {
+// Inclusive sums of x and y over the block's threads; every thread also gets
+// the block's totals.  `part` is reused by the next call.
+__device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*part)[2], int64_t& x_total,
+                                           int64_t& y_total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, x, off);
-    if (lane >= off) x += y;
+    const int64_t u = __shfl_up_sync(0xffffffffu, (long long)x, off), v = __shfl_up_sync(0xffffffffu, (long long)y, off);
+    if (lane >= off) {
+      x += u;
+      y += v;
+    }
   }
   __syncthreads();  // the previous call's readers are done with part
-  if (lane == 31) part[warp] = x;
-  __syncthreads();
-  int64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int w = 0; w < kTableWarps; ++w) {
-    const int64_t p = part[w];
-    if (w < warp) before += p;
-    total += p;
+  if (lane == 31) {
+    part[warp][0] = x;
+    part[warp][1] = y;
   }
-  return x + before;
+  __syncthreads();
+  // every warp sums the warps' totals itself: lane w holds warp w's
+  int64_t u = lane < kTableWarps ? part[lane][0] : 0, v = lane < kTableWarps ? part[lane][1] : 0;
+#pragma unroll
+  for (int off = 1; off < kTableWarps; off <<= 1) {
+    const int64_t p = __shfl_up_sync(0xffffffffu, (long long)u, off), q = __shfl_up_sync(0xffffffffu, (long long)v, off);
+    if (lane >= off) {
+      u += p;
+      v += q;
+    }
+  }
+  x_total = __shfl_sync(0xffffffffu, (long long)u, kTableWarps - 1);
+  y_total = __shfl_sync(0xffffffffu, (long long)v, kTableWarps - 1);
+  const int64_t x_before = __shfl_sync(0xffffffffu, (long long)u, warp > 0 ? warp - 1 : 0);
+  const int64_t y_before = __shfl_sync(0xffffffffu, (long long)v, warp > 0 ? warp - 1 : 0);
+  if (warp > 0) {
+    x += x_before;
+    y += y_before;
+  }
 }
 
 // Largest i in [0, n) with v[i] <= x (v is nondecreasing and v[0] <= x).
@@ -176,22 +197,23 @@ struct ReserveArgs {
   int32_t* free_count_out;
   int64_t table_stride;
   int64_t T;
+  PageDiv div;
   uint32_t padded;  // 0: tokens request after request; else the slots of each request
   int B;
-  uint32_t max_pages, page_size, num_pages;
+  uint32_t max_pages, num_pages;
 };
 
 // need_b = ceil((len_b + new_b) / page) - ceil(len_b / page), 0 where the
 // request would outgrow its table row (or its padded slots); upto = inclusive
-// sum of need.  A request is granted when it fits and upto_b <= free_count (or it
-// needs no page); the granted requests that need pages are then a prefix, so
-// request b takes the stack entries free_count - 1 - (upto_b - need_b) - j.
+// sum of need.  A request is granted when it fits and upto_b <= free_count (or
+// it needs no page); the granted requests that need pages are then a prefix,
+// so request b takes the stack entries free_count - 1 - (upto_b - need_b) - j.
 __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* starts = sm;               // [B + 1] first token of each request
   int32_t* first = sm + a.B + 1;      // [B] pages taken by the requests before it
-  uint8_t* refused = reinterpret_cast<uint8_t*>(first + a.B);
-  __shared__ int64_t part[kTableWarps];
+  int32_t* held = first + a.B;        // [B] its length so far, or -1 where it is refused
+  __shared__ int64_t part[kTableWarps][2];
   __shared__ int taken_s;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -210,17 +232,19 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
       len = (uint32_t)max(a.lengths[b], 0);
       add = (uint32_t)max(a.added[b], 0);
     }
-    const uint32_t before = pages_of(len, a.page_size), after = pages_of(len + add, a.page_size);
-    const bool fits = after <= a.max_pages && len + add <= 0x7fffffffu && (a.padded == 0 || add <= a.padded);
+    const uint32_t end = len + add;  // below 2^32
+    const uint32_t before = a.div.pages(len), after = end <= 0x7fffffffu ? a.div.pages(end) : 0xffffffffu;
+    const bool fits = after <= a.max_pages && (a.padded == 0 || add <= a.padded);
     const int64_t need = fits ? after - before : 0;
-    int64_t add_total, need_total;
-    const int64_t add_upto = tokens + block_scan(add, part, add_total);
-    const int64_t upto = pages + block_scan(need, part, need_total);
+    int64_t add_upto = add, upto = need, add_total, need_total;
+    block_scan(add_upto, upto, part, add_total, need_total);
+    add_upto += tokens;
+    upto += pages;
     if (b < a.B) {
       const bool granted = fits && (need == 0 || upto <= count);
       starts[b] = saturate(a.padded ? (int64_t)b * a.padded : add_upto - add);
       first[b] = saturate(upto - need);
-      refused[b] = !granted;
+      held[b] = granted ? (int32_t)len : -1;
       if (granted && need > 0) atomicMax(&taken_s, (int)upto);  // a maximum: the order does not matter
     }
     tokens += add_total;
@@ -230,38 +254,51 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
   __syncthreads();
   const int taken = taken_s;
 
-  // new entries of the block table: stack entry count - 1 - p is the p-th page taken
-  for (int64_t p = (int64_t)rank * kTableThreads + tid; p < taken; p += (int64_t)blocks * kTableThreads) {
-    const int b = last_at_most(first, a.B, p);
-    const uint32_t before = pages_of((uint32_t)max(a.lengths[b], 0), a.page_size);
-    a.table[b * a.table_stride + before + (p - first[b])] = a.free_pages[count - 1 - p];
-  }
-  // slots, four consecutive tokens a thread
-  const int64_t quads = (a.T + 3) / 4;
-  for (int64_t i = (int64_t)rank * kTableThreads + tid; i < quads; i += (int64_t)blocks * kTableThreads) {
-    const int64_t t0 = i * 4;
+  // page j of request b, a new one or one that it holds
+  auto page_at = [&](int b, uint32_t before, uint32_t j) -> int64_t {
+    const int32_t p = j < before ? a.table[b * a.table_stride + j]
+                                 : a.free_pages[count - 1 - (first[b] + (int32_t)(j - before))];
+    return (uint32_t)p < a.num_pages ? (int64_t)p * a.div.size : -1;
+  };
+  // Slots.  A thread takes `run` consecutive tokens: one, so that a step of
+  // single tokens is one pass of independent lookups, or four where there are
+  // more tokens than threads; along a run it moves from row to row and looks
+  // a page up only where one begins.
+  const int64_t threads = (int64_t)blocks * kTableThreads;
+  const int run = a.T > threads ? 4 : 1;
+  for (int64_t t0 = ((int64_t)rank * kTableThreads + tid) * run; t0 < a.T; t0 += threads * run) {
+    int64_t slot[4];
     int b = last_at_most(starts, a.B, t0);
-    int known_b = -1;
-    uint32_t known_page = 0;
-    int64_t slot[4], page = -1;
+    int64_t base = -1;
+    int32_t next = starts[b], stop = 0;  // the run's request ends before token `next`, its new tokens before `stop`
+    uint32_t before = 0, j = 0, r = 0;
+    bool inside = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      const int64_t t = t0 + e;
-      while (b + 1 < a.B && starts[b + 1] <= t) ++b;
       slot[e] = -1;
-      if (t >= starts[a.B] || refused[b] || (a.padded && t - starts[b] >= a.added[b])) continue;
-      const uint32_t len = (uint32_t)max(a.lengths[b], 0);
-      const uint32_t pos = len + (uint32_t)(t - starts[b]);
-      const uint32_t j = pos / a.page_size;
-      if (b != known_b || j != known_page) {  // most tokens share the page of the one before
-        const uint32_t before = pages_of(len, a.page_size);
-        page = j < before ? a.table[b * a.table_stride + j] : a.free_pages[count - 1 - (first[b] + (int64_t)(j - before))];
-        known_b = b;
-        known_page = j;
+      if (e >= run) continue;
+      const int64_t t = t0 + e;
+      if (!inside || t >= next) {  // the first token of the run, or of another request
+        while (b + 1 < a.B && starts[b + 1] <= t) ++b;
+        next = b + 1 < a.B ? starts[b + 1] : 0x7fffffff;
+        stop = held[b] < 0 ? 0 : a.padded ? starts[b] + max(a.added[b], 0) : starts[b + 1];
+        inside = true;
+        if (t < stop) {
+          const uint32_t pos = (uint32_t)held[b] + (uint32_t)(t - starts[b]);
+          before = a.div.pages((uint32_t)held[b]);
+          j = a.div(pos);
+          r = pos - j * a.div.size;
+          base = page_at(b, before, j);
+        }
+      } else if (t < stop && ++r == a.div.size) {
+        r = 0;
+        base = page_at(b, before, ++j);
       }
-      if (page >= 0 && page < a.num_pages) slot[e] = page * a.page_size + (pos - j * a.page_size);
+      if (t < stop && base >= 0) slot[e] = base + r;
     }
-    if (t0 + 4 <= a.T) {
+    if (run == 1) {
+      a.slots[t0] = slot[0];
+    } else if (t0 + 4 <= a.T) {
       longlong2* dst = reinterpret_cast<longlong2*>(a.slots + t0);
       dst[0] = make_longlong2(slot[0], slot[1]);
       dst[1] = make_longlong2(slot[2], slot[3]);
@@ -271,12 +308,19 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
         if (t0 + e < a.T) a.slots[t0 + e] = slot[e];
     }
   }
+  // New entries of the block table: stack entry count - 1 - p is the p-th page
+  // taken.  From the far end of the threads, which a short list of tokens
+  // leaves free.
+  for (int64_t p = threads - 1 - ((int64_t)rank * kTableThreads + tid); p < taken; p += threads) {
+    const int b = last_at_most(first, a.B, p);
+    a.table[b * a.table_stride + a.div.pages((uint32_t)held[b]) + (p - first[b])] = a.free_pages[count - 1 - p];
+  }
   // lengths_out and free_count_out may be lengths and free_count themselves
   cluster.sync();
   if (rank == 0) {
     for (int b = tid; b < a.B; b += kTableThreads) {
-      const int32_t len = max(a.lengths[b], 0);
-      a.lengths_out[b] = refused[b] ? len : len + max(a.added[b], 0);
+      const int32_t len = held[b];
+      a.lengths_out[b] = len < 0 ? max(a.lengths[b], 0) : len + max(a.added[b], 0);
     }
     for (int b = tid; b <= a.B; b += kTableThreads) a.starts[b] = starts[b];
     if (tid == 0) *a.free_count_out = count - taken;
@@ -292,62 +336,96 @@ struct ReleaseArgs {
   int32_t* lengths_out;
   int32_t* free_count_out;
   int64_t table_stride;
+  PageDiv div;
   int B;
-  uint32_t max_pages, page_size, num_pages;
+  uint32_t max_pages, num_pages;
 };
 
-// One warp per request, twice: count the row's valid entries (a row may hold
-// -1 where a page was given up earlier), then, after a prefix sum over
-// requests, write them to the stack in order.  The counts reach every block
-// through distributed shared memory.
+// One warp per request: count the row's valid entries (a row may hold -1 where
+// a page was given up earlier), then, after a prefix sum over requests, write
+// them to the stack in order.  The counts reach every block through
+// distributed shared memory.  The first kKept * 32 entries of a warp's first
+// request stay in registers from the count to the write.
+constexpr int kKept = 16;
+
 __global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const ReleaseArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* counts = sm;  // [B] valid pages of each request, then their exclusive sum
-  __shared__ int64_t part[kTableWarps];
+  __shared__ int64_t part[kTableWarps][2];
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.barrier_arrive();  // this block has started: its shared memory may be written
   kf::griddep_wait();
   kf::griddep_launch_dependents();
-  cg::cluster_group cluster = cg::this_cluster();
-  cluster.sync();  // every block has started: its shared memory may be written
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const unsigned rank = blockIdx.x, blocks = gridDim.x;
   int32_t count = *a.free_count;
   count = count < 0 ? 0 : (uint32_t)count > a.num_pages ? (int32_t)a.num_pages : count;
 
   auto row_pages = [&](int b) -> uint32_t {
-    if (!a.finished[b]) return 0;
-    return min(pages_of((uint32_t)max(a.lengths[b], 0), a.page_size), a.max_pages);
+    const int32_t len = a.lengths[b];
+    return a.finished[b] ? min(a.div.pages((uint32_t)max(len, 0)), a.max_pages) : 0;
   };
-  for (int b = rank * kTableWarps + warp; b < a.B; b += blocks * kTableWarps) {
+  const int b0 = (int)rank * kTableWarps + warp;  // this warp's first request
+  uint32_t kept[kKept];
+  bool waited = false;
+  for (int b = b0; b < a.B; b += blocks * kTableWarps) {
     const uint32_t n = row_pages(b);
     const int32_t* row = a.table + b * a.table_stride;
     int c = 0;
-#pragma unroll 4
-    for (uint32_t j = lane; j < n; j += 32) c += (uint32_t)row[j] < a.num_pages;
+    uint32_t j = lane;
+    if (b == b0) {
+#pragma unroll
+      for (int k = 0; k < kKept; ++k) kept[k] = j + k * 32 < n ? (uint32_t)row[j + k * 32] : 0xffffffffu;
+#pragma unroll
+      for (int k = 0; k < kKept; ++k) c += kept[k] < a.num_pages;
+      j += kKept * 32;
+    }
+#pragma unroll 8
+    for (; j < n; j += 32) c += (uint32_t)row[j] < a.num_pages;
     c = __reduce_add_sync(0xffffffffu, c);
+    if (!waited) cluster.barrier_wait();
+    waited = true;
     if (lane < (int)blocks) cluster.map_shared_rank(counts, lane)[b] = c;
   }
+  if (!waited) cluster.barrier_wait();
   cluster.sync();
   int64_t total = 0;
   for (int base = 0; base < a.B; base += kTableThreads) {
     const int b = base + tid;
     const int32_t c = b < a.B ? counts[b] : 0;
-    int64_t round;
-    const int64_t upto = total + block_scan(c, part, round);
-    if (b < a.B) counts[b] = saturate(upto - c);
+    int64_t upto = c, none = 0, round, unused;
+    block_scan(upto, none, part, round, unused);
+    if (b < a.B) counts[b] = saturate(total + upto - c);
     total += round;
   }
   __syncthreads();
-  for (int b = rank * kTableWarps + warp; b < a.B; b += blocks * kTableWarps) {
+  for (int b = b0; b < a.B; b += blocks * kTableWarps) {
     const uint32_t n = row_pages(b);
     const int32_t* row = a.table + b * a.table_stride;
     int64_t at = (int64_t)count + counts[b];
-    for (uint32_t j0 = 0; j0 < n; j0 += 32) {
-      const int32_t page = j0 + lane < n ? row[j0 + lane] : -1;
-      const bool valid = (uint32_t)page < a.num_pages;
+    auto push = [&](uint32_t page) {
+      const bool valid = page < a.num_pages;
       const unsigned mask = __ballot_sync(0xffffffffu, valid);
       const int64_t to = at + __popc(mask & ((1u << lane) - 1));
-      if (valid && to < a.num_pages) a.free_pages[to] = page;  // a stack that is full keeps what it has
+      if (valid && to < a.num_pages) a.free_pages[to] = (int32_t)page;  // a stack that is full keeps what it has
       at += __popc(mask);
+    };
+    uint32_t j0 = 0;
+    if (b == b0) {
+#pragma unroll
+      for (int k = 0; k < kKept; ++k)
+        if (k * 32 < n) push(kept[k]);
+      j0 = kKept * 32;
+    }
+    for (; j0 < n; j0 += 128) {
+      uint32_t page[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t j = j0 + k * 32 + lane;
+        page[k] = j < n ? (uint32_t)row[j] : 0xffffffffu;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k) push(page[k]);
     }
   }
   cluster.sync();
@@ -382,6 +460,13 @@ int raise_smem(void (*kern)(KArgs...), size_t smem, const char* what) {
     return kf::set_error(KF_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory", what, smem);
   }
   return KF_OK;
+}
+
+PageDiv page_div(int64_t page_size) {
+  PageDiv d;
+  d.size = (uint32_t)page_size;
+  kf::division(page_size, &d.mul, &d.shift);
+  return d;
 }
 
 unsigned cluster_for(int64_t units, int64_t per_block) {
@@ -485,9 +570,9 @@ extern "C" int kf_paged_reserve(const kf_paged_reserve_args* args) {
   a.padded = (uint32_t)per_request;
   a.B = (int)t.B;
   a.max_pages = (uint32_t)t.max_pages;
-  a.page_size = (uint32_t)t.page_size;
+  a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
-  const size_t smem = (size_t)(2 * t.B + 1) * 4 + (size_t)t.B;
+  const size_t smem = (size_t)(3 * t.B + 1) * 4;
   rc = raise_smem(paged_reserve_kernel, smem, what);
   if (rc != KF_OK) return rc;
   const unsigned cluster = cluster_for(num_tokens, kTableThreads * 4);
@@ -515,7 +600,7 @@ extern "C" int kf_paged_release(const kf_paged_release_args* args) {
   a.table_stride = t.table_stride;
   a.B = (int)t.B;
   a.max_pages = (uint32_t)t.max_pages;
-  a.page_size = (uint32_t)t.page_size;
+  a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
   const size_t smem = (size_t)t.B * 4;
   rc = raise_smem(paged_release_kernel, smem, what);

@@ -775,13 +775,7 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
-  // Division by page_size: with 2^(s-1) < page_size <= 2^s and m =
-  // ceil(2^(31+s) / page_size), m < 2^32 and m page_size exceeds 2^(31+s) by
-  // less than 2^s, so x m >> (31 + s) is exact for x < 2^31.
-  int s = 0;
-  while (((int64_t)1 << s) < page_size) ++s;
-  a.page_mul = (uint32_t)((((uint64_t)1 << (31 + s)) + page_size - 1) / page_size);
-  a.page_shift = (uint32_t)(31 + s);
+  kf::division(page_size, &a.page_mul, &a.page_shift);
   // boxes never cross a page nor a team's 16 or 32 keys
   a.box = 16;
   while (page_size % a.box) a.box /= 2;
