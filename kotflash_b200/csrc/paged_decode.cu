@@ -148,9 +148,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   constexpr uint32_t ALL = KW == 32 ? 0xffffffffu : 0xffffu;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  __shared__ int64_t warp_tiles[kWarps];
+  __shared__ uint32_t warp_tiles[kWarps];
   __shared__ int first_request;
-  __shared__ int64_t first_before;     // tiles of the requests before it
+  __shared__ uint32_t first_before;    // tiles of the requests before it
   __shared__ __align__(8) uint64_t full[C::TEAMS][STAGES];
   __shared__ uint32_t seen_s[C::TEAMS][STAGES];  // visible keys of each stage
   __shared__ int abort_any;
@@ -172,87 +172,93 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
-  // ---- this block's share of the list of tiles
+  // ---- this block's share of the list of tiles (fewer than 2^31, see the host's check)
   const int per = (a.B + kThreads - 1) / kThreads;  // requests per thread, contiguous
   const int b_lo = min(tid * per, a.B), b_hi = min(b_lo + per, a.B);
-  int64_t mine = 0;
+  uint32_t mine = 0;
   for (int b = b_lo; b < b_hi; ++b) mine += (visible(a, b) + TILE - 1) / TILE;
-  int64_t upto = mine;
+  uint32_t upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
-    const int64_t y = __shfl_up_sync(0xffffffffu, (long long)upto, off);
+    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, off);
     if (lane >= off) upto += y;
   }
   if (lane == 31) warp_tiles[warp] = upto;
   __syncthreads();
-  int64_t total = 0;
+  uint32_t total = 0;
 #pragma unroll
   for (int w = 0; w < kWarps; ++w) {
     if (w < warp) upto += warp_tiles[w];
     total += warp_tiles[w];
   }
-  const int64_t list = total * units;
-  const int64_t shares = min((int64_t)gridDim.x, list);
-  const int64_t me = blockIdx.x;
+  const uint32_t list = total * units;
+  const uint32_t shares = min(gridDim.x, list), me = blockIdx.x;
 
   // requests without a visible position are nobody's unit
-  for (int64_t b = me; b < a.B; b += gridDim.x) {
-    if (visible(a, (int)b) != 0) continue;
-    for (int i = tid; i < a.Hq * (a.D / 8); i += kThreads) {
-      const int h = i / (a.D / 8), c = i % (a.D / 8);
-      *reinterpret_cast<uint4*>(a.o + b * a.os[0] + h * a.os[1] + c * 8) = make_uint4(0, 0, 0, 0);
+  auto clear_empty = [&]() {
+    for (int b = (int)me; b < a.B; b += gridDim.x) {
+      if (visible(a, b) != 0) continue;
+      for (int i = tid; i < a.Hq * (a.D / 8); i += kThreads) {
+        const int h = i / (a.D / 8), c = i % (a.D / 8);
+        *reinterpret_cast<uint4*>(a.o + b * a.os[0] + h * a.os[1] + c * 8) = make_uint4(0, 0, 0, 0);
+      }
+      if (a.lse)
+        for (int h = tid; h < a.Hq; h += kThreads) a.lse[(int64_t)b * a.Hq + h] = -INFINITY;
+      if (a.join_units)
+        for (int u = tid; u < units; u += kThreads) a.joins[b * units + u].x = -1;
     }
-    if (a.lse)
-      for (int h = tid; h < a.Hq; h += kThreads) a.lse[b * a.Hq + h] = -INFINITY;
-    if (a.join_units)
-      for (int u = tid; u < units; u += kThreads) a.joins[b * units + u].x = -1;
-  }
+  };
   const bool join_blocks = a.joins && !a.join_units;
   if (me >= shares) {
     if (tid == 0 && join_blocks) a.joins[me].x = -1;
+    clear_empty();
     return;
   }
-  const int64_t begin = me * list / shares;
-  const int n = (int)((me + 1) * list / shares - begin);
-  {
-    const int64_t before = (upto - mine) * units;
-    if (begin >= before && begin < upto * units) {  // exactly one thread
-      int64_t sum = upto - mine;
-      int b = b_lo;
-      while (true) {
-        const int64_t tiles = (visible(a, b) + TILE - 1) / TILE;
-        if (begin < (sum + tiles) * units) break;
-        sum += tiles;
-        ++b;
-      }
-      first_request = b;
-      first_before = sum;
+  // shares differ by one tile at most, the longer ones first
+  const uint32_t even = list / shares, longer = list - even * shares;
+  const uint32_t begin = me * even + min(me, longer);
+  const int n = (int)(even + (me < longer ? 1 : 0));
+  if (begin >= (upto - mine) * units && begin < upto * units) {  // exactly one thread
+    uint32_t sum = upto - mine;
+    int b = b_lo;
+    while (true) {
+      const uint32_t tiles = (visible(a, b) + TILE - 1) / TILE;
+      if (begin < (sum + tiles) * units) break;
+      sum += tiles;
+      ++b;
     }
+    first_request = b;
+    first_before = sum;
   }
   __syncthreads();
 
   Cursor<TILE> load, work;
   work.set_request(a, first_request);
   {
-    const int64_t at = begin - first_before * units;  // inside the request's tiles x units
+    const uint32_t at = begin - first_before * units;  // inside the request's tiles x units
     const int hr = (int)(at / work.tiles);
-    work.t = (uint32_t)(at - (int64_t)hr * work.tiles);
+    work.t = at - hr * work.tiles;
     work.h = hr / a.row_blocks;
     work.rb = hr - work.h * a.row_blocks;
   }
   load = work;
 
-  // ---- loads: lane r (of KW) looks up key r of the team's share of the tile
-  // the load cursor stands on, one step ahead of its use
-  uint32_t next_page, next_row;
+  // ---- loads: lane r (of KW) looks up key r of the team's share of a tile
+  struct Place {
+    uint32_t page, row;
+    int h;
+  };
   auto look_up = [&]() {
     const uint32_t key = load.t * TILE + team * KW + (KW == 32 ? lane : (lane & 15));
     const uint32_t pg = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
-    next_row = key - pg * a.page_size;
-    next_page = key < load.keys ? (uint32_t)__ldg(a.table + load.b * a.table_stride + pg) : 0xffffffffu;
+    Place p;
+    p.row = key - pg * a.page_size;
+    p.page = key < load.keys ? (uint32_t)__ldg(a.table + load.b * a.table_stride + pg) : 0xffffffffu;
+    p.h = load.h;
+    return p;
   };
-  auto issue = [&](int stage) {
-    const bool valid = next_page < a.num_pages;
+  auto issue = [&](int stage, const Place& p) {
+    const bool valid = p.page < a.num_pages;
     const uint32_t seen = __ballot_sync(0xffffffffu, valid) & ALL;
     const bool starts_box = valid && lane < KW && (lane & (a.box - 1)) == 0;
     const uint32_t boxes = __ballot_sync(0xffffffffu, starts_box);
@@ -266,8 +272,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       uint8_t* st = ring + stage * C::STAGE + lane * 128;
 #pragma unroll
       for (int pn = 0; pn < NP; ++pn) {
-        kf::tma_load_4d(st + pn * PANEL, &map_k, bar, pn * 64, next_row, load.h, next_page);
-        kf::tma_load_4d(st + K_BYTES + pn * PANEL, &map_v, bar, pn * 64, next_row, load.h, next_page);
+        kf::tma_load_4d(st + pn * PANEL, &map_k, bar, pn * 64, p.row, p.h, p.page);
+        kf::tma_load_4d(st + K_BYTES + pn * PANEL, &map_v, bar, pn * 64, p.row, p.h, p.page);
       }
     }
   };
@@ -294,24 +300,32 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
   };
 
-  // the first warp of a team loads
+  // The first warp of a team loads.  To begin with it looks up the pages of the
+  // whole ring at once, then always one step ahead of their use.
   int issued = 0;
+  Place ahead;
   if (rg == 0) {
-    look_up();
+    Place first[STAGES - 1];
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      if (s >= n) break;
-      issue(s);
-      ++issued;
-      if (issued < n) {
-        load.next(a);
-        look_up();
+      if (s < n) {
+        if (s > 0) load.next(a);
+        first[s] = look_up();
       }
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < n) issue(s, first[s]);
+    issued = min(n, STAGES - 1);
+    if (issued < n) {
+      load.next(a);
+      ahead = look_up();
     }
   }
   start_unit();
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
+  clear_empty();
 
   int stage = 0, fill = STAGES - 1;
   uint32_t parity = 0;
@@ -324,11 +338,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     alive = team_and<RG>(team, landed);
     if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
     if (rg == 0 && alive && issued < n) {
-      issue(fill);
+      issue(fill, ahead);
       ++issued;
       if (issued < n) {
         load.next(a);
-        look_up();
+        ahead = look_up();
       }
     }
 
@@ -364,21 +378,39 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     if (seen != 0) {
       const uint32_t sk = kf::smem_u32(kt), sv = kf::smem_u32(vt);
-      // S^T (keys x rows)
-      float c[H][NT][4];
+      // S^T (keys x rows).  Operands are loaded four at a time ahead of their
+      // products, and a lone chain of products is cut in two: with two warps
+      // per scheduler the latency of a step is what short shares wait for.
+      constexpr int CHAINS = H * NT == 1 ? 2 : 1;
+      float cc[CHAINS][H][NT][4];
 #pragma unroll
-      for (int h = 0; h < H; ++h)
+      for (int x = 0; x < CHAINS; ++x)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) c[h][nt][0] = c[h][nt][1] = c[h][nt][2] = c[h][nt][3] = 0.f;
+        for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk)
+          for (int nt = 0; nt < NT; ++nt) cc[x][h][nt][0] = cc[x][h][nt][1] = cc[x][h][nt][2] = cc[x][h][nt][3] = 0.f;
+      constexpr int KG = H == 1 ? 4 : 2;
 #pragma unroll
-        for (int h = 0; h < H; ++h) {
-          uint32_t ka[4];
-          kf::ldmatrix_x4(ka, sk + swz(h * 16 + (lane & 15), 2 * kk + (lane >> 4), KW));
+      for (int k0 = 0; k0 < DP / 16; k0 += KG) {
+        uint32_t ka[KG][H][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(c[h][nt], ka, qb[nt][kk][0], qb[nt][kk][1]);
-        }
+        for (int x = 0; x < KG; ++x)
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+            kf::ldmatrix_x4(ka[x][h], sk + swz(h * 16 + (lane & 15), 2 * (k0 + x) + (lane >> 4), KW));
+#pragma unroll
+        for (int x = 0; x < KG; ++x)
+#pragma unroll
+          for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              kf::mma_16816<BF16>(cc[x % CHAINS][h][nt], ka[x][h], qb[nt][k0 + x][0], qb[nt][k0 + x][1]);
+      }
+      float (&c)[H][NT][4] = cc[0];
+      if constexpr (CHAINS == 2) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[0][0][e] += cc[1][0][0][e];
+      }
       uint32_t pb[H][NT][2], pl[H][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -439,19 +471,26 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           }
         }
       }
-      // O^T (head dim x rows) += V^T P^T
+      // O^T (head dim x rows) += V^T P^T, the two parts of P apart from one
+      // another so that no product waits for the one before it
+      constexpr int VG = NT == 1 ? 4 : 2;
 #pragma unroll
-      for (int dm = 0; dm < DP / 16; ++dm)
+      for (int d0 = 0; d0 < DP / 16; d0 += VG)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          uint32_t va[4];
-          kf::ldmatrix_x4_trans(va, sv + swz(h * 16 + (lane & 7) + ((lane >> 4) << 3), 2 * dm + ((lane >> 3) & 1),
-                                             KW));
+          uint32_t va[VG][4];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            kf::mma_16816<BF16>(ot[nt][dm], va, pb[h][nt][0], pb[h][nt][1]);
-            kf::mma_16816<BF16>(ot[nt][dm], va, pl[h][nt][0], pl[h][nt][1]);
-          }
+          for (int x = 0; x < VG; ++x)
+            kf::ldmatrix_x4_trans(va[x], sv + swz(h * 16 + (lane & 7) + ((lane >> 4) << 3),
+                                                  2 * (d0 + x) + ((lane >> 3) & 1), KW));
+#pragma unroll
+          for (int x = 0; x < VG; ++x)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pb[h][nt][0], pb[h][nt][1]);
+#pragma unroll
+          for (int x = 0; x < VG; ++x)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pl[h][nt][0], pl[h][nt][1]);
         }
     }
     if (++stage == STAGES) {
@@ -468,7 +507,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     // ---- join the teams and write the unit's rows (or its partial)
     const int h = work.h, rb = work.rb;
     const bool direct = unit_t0 == 0 && unit_done;
-    const int64_t slot = me * 2 + (unit_t0 > 0 ? 0 : 1);  // 0: began in an earlier share, 1: begins here
+    const int64_t slot = (int64_t)me * 2 + (unit_t0 > 0 ? 0 : 1);  // 0: began in an earlier share, 1: begins here
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -540,13 +579,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
     }
     if (unit_t0 == 0 && tid == 0 && (a.join_units || !direct)) {
-      // a unit that begins here and goes on ends in the share that holds list
-      // position p, its last tile: ((p + 1) shares - 1) / list
+      // a unit that begins here and goes on ends in the share of its last tile
       const int hr = h * a.row_blocks + rb;
-      const int64_t last_tile = begin + i + (work.tiles - 1 - work.t);
-      a.joins[a.join_units ? (int64_t)work.b * units + hr : me] =
+      const uint32_t last = begin + i + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
+      const uint32_t end = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
+      a.joins[a.join_units ? (int64_t)work.b * units + hr : (int64_t)me] =
           direct ? make_int4(-1, 0, 0, 0)
-                 : make_int4(work.b, hr, (int)me, (int)(((last_tile + 1) * shares - 1) / list));
+                 : make_int4(work.b, hr, (int)me, (int)end);
     }
     if (i + 1 < n) {
       work.next(a);
@@ -786,7 +825,7 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   const int64_t tile = tile_keys(D, rows), most = (a.capacity + tile - 1) / tile;
   const int64_t units = B * Hkv * a.row_blocks;
   int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
-  if (units * most > (int64_t)1 << 38) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
+  if (units * most > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
   if (units * most < blocks) blocks = units * most;
   a.part_o = nullptr;
   a.part_lse = nullptr;

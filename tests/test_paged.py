@@ -210,10 +210,13 @@ def _walk(lens, units, tile, grid):
     shares = min(grid, listed)
     flat = [(b, h, x) for b in range(len(lens)) for h in range(units) for x in range(tiles[b])]
     done, parts, joins = set(), {}, {}
+    even, longer = (listed // shares, listed % shares) if shares else (0, 0)
+    covered = 0
     for me in range(shares):
-        begin = me * listed // shares
-        n = (me + 1) * listed // shares - begin
-        assert n > 0
+        begin = me * even + min(me, longer)
+        n = even + (1 if me < longer else 0)
+        assert n > 0 and begin == covered
+        covered += n
         unit_t0 = flat[begin][2]
         for i in range(n):
             b, h, x = flat[begin + i]
@@ -229,8 +232,11 @@ def _walk(lens, units, tile, grid):
                 parts[slot] = (b, h, unit_t0, x)
                 if unit_t0 == 0:
                     last = begin + i + (tiles[b] - 1 - x)
-                    joins[me] = (b, h, ((last + 1) * shares - 1) // listed)
+                    in_longer = longer * (even + 1)
+                    end = last // (even + 1) if last < in_longer else longer + (last - in_longer) // even
+                    joins[me] = (b, h, end)
             unit_t0 = 0
+    assert covered == listed
     for me, (b, h, end) in joins.items():
         assert (b, h) not in done
         done.add((b, h))
