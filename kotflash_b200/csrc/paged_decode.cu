@@ -62,6 +62,7 @@ struct PagedArgs {
   int64_t qs[2], ks[3], vs[3], nks[2], nvs[2], os[2];
   int64_t table_stride;
   int B, Hq, Hkv, G, D, row_blocks;
+  int64_t max_pages;
   uint32_t capacity;       // tokens a table row can hold
   uint32_t page_size, num_pages;
   uint32_t page_mul, page_shift;  // x / page_size = x page_mul >> page_shift for x < 2^31
@@ -123,6 +124,10 @@ struct Cursor {
   }
 };
 
+__device__ __forceinline__ void prefetch_l2(const void* p) {
+  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
+}
+
 // Barrier of a team's warps that returns the AND of their `pred`, so that all
 // of them go on alike.
 template <int RG>
@@ -168,6 +173,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     abort_any = 0;
     kf::tma_prefetch_desc(&map_k);
     kf::tma_prefetch_desc(&map_v);
+  }
+  // The chain lengths -> table -> K/V starts cold: bring the lengths and, over
+  // all blocks, the first part of the table to L2 while the previous kernel
+  // still runs (hints only: L2 stays coherent with what that kernel writes).
+  {
+    const int64_t line = (int64_t)blockIdx.x * kThreads + tid;  // of 32 entries
+    if (line * 32 < a.B) prefetch_l2(a.lengths + line * 32);
+    const int64_t lines_per_row = (a.max_pages + 31) / 32;
+    if (line < a.B * lines_per_row) {
+      const int64_t b = line / lines_per_row;
+      prefetch_l2(a.table + b * a.table_stride + (line - b * lines_per_row) * 32);
+    }
   }
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -514,13 +531,20 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int off = 4; off < 32; off <<= 1) l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], off);
+    // one team: each warp has its rows to itself
+    auto unit_sync = [&]() {
+      if constexpr (C::TEAMS == 1)
+        __syncwarp();
+      else
+        __syncthreads();
+    };
     if (!alive) {  // a lost load shows in the result
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) l_run[nt][0] = l_run[nt][1] = m_run[nt][0] = m_run[nt][1] = NAN;
     }
 #pragma unroll
     for (int pass = 0; pass < DP / C::PASS; ++pass) {
-      __syncthreads();  // the buffer's readers of the pass (or unit) before are done
+      unit_sync();  // the buffer's readers of the pass (or unit) before are done
       if (pass == 0 && lane < 4) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -542,9 +566,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             row[x * 16 + (lane >> 2) + 8] = ot[nt][dm][2 + j];
           }
         }
-      __syncthreads();
+      unit_sync();
       const int valid_rows = min(C::ROWS, a.G - rb * C::ROWS);
-      for (int idx = tid; idx < valid_rows * (C::PASS / 4); idx += kThreads) {
+      const int from = C::TEAMS == 1 ? rg * NT * 8 * (C::PASS / 4) + lane : tid;
+      const int to = C::TEAMS == 1 ? min(valid_rows, (rg + 1) * NT * 8) : valid_rows;
+      for (int idx = from; idx < to * (C::PASS / 4); idx += C::TEAMS == 1 ? 32 : kThreads) {
         const int r = idx / (C::PASS / 4), col = (idx % (C::PASS / 4)) * 4;
         const int d = pass * C::PASS + col;
         if (d >= a.D) continue;
@@ -602,35 +628,36 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 }
 
 // Joins the partials of a unit that was cut: slot 1 of its first share, slot 0
-// of the shares up to its last.  One row per block; groups of D / 4 lanes take
-// every groups-th partial with a running maximum, so each partial is read once
-// and in any number.
+// of the shares up to its last.  A group of D / 4 lanes takes one row, alone
+// or, where a unit has many partials, with `split` - 1 others that take every
+// split-th partial; each partial is read once, with a running maximum, and the
+// groups' results meet in shared memory.
 constexpr int kJoinThreads = 256;
 constexpr int kJoinBatch = 4;  // partials a group has in flight
 
 template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int rows) {
+__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int rows, int split) {
   kf::griddep_wait();
   kf::griddep_launch_dependents();
   const int4 unit = a.joins[blockIdx.x];
   if (unit.x < 0) return;
   const int h = unit.y / a.row_blocks, rb = unit.y - h * a.row_blocks;
-  const int r = blockIdx.y;
-  if (r >= a.G - rb * rows) return;
   const int count = unit.w - unit.z + 1;
   __shared__ float4 acc_s[kJoinThreads];
   __shared__ float m_s[kJoinThreads / 4], l_s[kJoinThreads / 4];
-  const int lanes = a.D / 4, groups = kJoinThreads / lanes;
+  const int lanes = a.D / 4, per_block = kJoinThreads / lanes / split;  // rows of a block
   const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
-  if (g < groups) {
-    float m = -INFINITY, l = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int j0 = g; j0 < count; j0 += groups * kJoinBatch) {
+  const int part = g % split, r = blockIdx.y * per_block + g / split;
+  const bool mine = g < per_block * split && r < min(rows, a.G - rb * rows);
+  float m = -INFINITY, l = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (mine) {
+    for (int j0 = part; j0 < count; j0 += split * kJoinBatch) {
       float lse[kJoinBatch];
       float4 o[kJoinBatch];
 #pragma unroll
       for (int x = 0; x < kJoinBatch; ++x) {
-        const int j = j0 + x * groups;
+        const int j = j0 + x * split;
         lse[x] = -INFINITY;
         o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
         if (j < count) {
@@ -660,33 +687,42 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
       }
       m = top;
     }
+  }
+  if (split > 1) {
     acc_s[threadIdx.x] = acc;
-    if (c == 0) {
+    if (mine && c == 0) {
       m_s[g] = m;
       l_s[g] = l;
     }
+    __syncthreads();
+    if (mine && part == 0) {
+      float top = m;
+      for (int i = 1; i < split; ++i) top = fmaxf(top, m_s[g + i]);
+      const float mu = top == -INFINITY ? 0.f : top;
+      const float old = kf::ex2(m - mu);
+      l *= old;
+      acc.x *= old;
+      acc.y *= old;
+      acc.z *= old;
+      acc.w *= old;
+      for (int i = 1; i < split; ++i) {
+        const float w = kf::ex2(m_s[g + i] - mu);
+        const float4 x = acc_s[threadIdx.x + i * lanes];
+        l += w * l_s[g + i];
+        acc.x += w * x.x;
+        acc.y += w * x.y;
+        acc.z += w * x.z;
+        acc.w += w * x.w;
+      }
+      m = top;
+    }
   }
-  __syncthreads();
-  if (g != 0) return;
-  float M = -INFINITY;
-  for (int i = 0; i < groups; ++i) M = fmaxf(M, m_s[i]);
-  const float mu = M == -INFINITY ? 0.f : M;
-  float L = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = 0; i < groups; ++i) {
-    const float w = kf::ex2(m_s[i] - mu);
-    const float4 x = acc_s[i * lanes + c];
-    L += w * l_s[i];
-    acc.x += w * x.x;
-    acc.y += w * x.y;
-    acc.z += w * x.z;
-    acc.w += w * x.w;
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
+  if (!mine || part != 0) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
   const int head = h * a.G + rb * rows + r;
   *reinterpret_cast<uint2*>(a.o + unit.x * a.os[0] + head * a.os[1] + c * 4) =
       make_uint2(kf::pack2<BF16>(acc.x * inv, acc.y * inv), kf::pack2<BF16>(acc.z * inv, acc.w * inv));
-  if (a.lse && c == 0) a.lse[(int64_t)unit.x * a.Hq + head] = L == 0.f ? -INFINITY : (M + log2f(L)) * kLn2;
+  if (a.lse && c == 0) a.lse[(int64_t)unit.x * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
 
 // Query rows of a unit for G rows per KV head, and the variant that has them.
@@ -811,6 +847,7 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.row_blocks = (a.G + rows - 1) / rows;
   const int64_t capacity = max_pages * page_size;
   a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
+  a.max_pages = max_pages;
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
@@ -855,7 +892,14 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
     rc = bf16 ? dispatch_rows<true, 2>(a, mk, mv, rows, (int)blocks, st)
               : dispatch_rows<false, 2>(a, mk, mv, rows, (int)blocks, st);
   if (rc != KF_OK || most == 1) return rc;
-  const dim3 grid((unsigned)(a.join_units ? units : blocks), (unsigned)(a.G < rows ? a.G : rows));
-  return bf16 ? kf::launch_dependent(paged_join_kernel<true>, grid, dim3(kJoinThreads), 0, st, what, a, rows)
-              : kf::launch_dependent(paged_join_kernel<false>, grid, dim3(kJoinThreads), 0, st, what, a, rows);
+  // Groups that share a row: as many as leave each about one batch of the
+  // partials that a unit has on average (2 where units outnumber the blocks).
+  const int groups = kJoinThreads / (int)(D / 4);
+  const int64_t partials = a.join_units ? blocks / units + 1 : 2;
+  int split = 1;
+  while (split * kJoinBatch < partials && split * 2 <= groups) split *= 2;
+  const int per_block = groups / split, row_count = a.G < rows ? a.G : rows;
+  const dim3 grid((unsigned)(a.join_units ? units : blocks), (unsigned)((row_count + per_block - 1) / per_block));
+  return bf16 ? kf::launch_dependent(paged_join_kernel<true>, grid, dim3(kJoinThreads), 0, st, what, a, rows, split)
+              : kf::launch_dependent(paged_join_kernel<false>, grid, dim3(kJoinThreads), 0, st, what, a, rows, split);
 }
