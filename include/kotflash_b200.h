@@ -227,7 +227,8 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * [pages, Hkv, page_size, D] (any strides with a contiguous last dim and
  * 16-byte aligned rows; K and V may differ in strides).  Position p of request
  * b is row p % page_size of page block_table[b * table_stride + p / page_size]
- * (int32 [B, max_pages]).  q and o are [B, Hq, 1, D], lengths int32 [B].
+ * (int32 [B, max_pages]).  q and o are [B, Hq, 1, D], o contiguous; lengths
+ * int32 [B].
  * Request b's token sees the positions below min(lengths[b], max_pages *
  * page_size) whose table entry lies in [0, pages); every other position
  * (other entries, -1 among them, the rest of a last page) is masked whatever
@@ -251,12 +252,13 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * they last microseconds, and a foreign-function call pays for every
  * argument. */
 typedef struct kf_paged_decode_args {
-  kf_tensor4     q, k_pages, v_pages, o;
+  kf_tensor4     q, k_pages, v_pages;
   kf_tensor4     new_k, new_v;
   const int64_t* slots;
   const int32_t* block_table;
   int64_t        max_pages, table_stride;
   const int32_t* lengths;
+  void*          o;
   float*         lse;
   int64_t        dtype;
   double         scale;

@@ -168,7 +168,9 @@ def t4(t: Optional[torch.Tensor]) -> Optional[KFTensor4]:
 # takes microseconds cannot afford to fill ctypes structures field by field
 # (a KFTensor4 takes 3 us to make and to pass, its part of a pack 0.6 us).
 _PT4 = "Q8q"  # a kf_tensor4: pointer, sizes, strides
-pack_paged_decode = struct.Struct("=" + _PT4 * 6 + "QQqqQQqdQQQQ").pack
+_DECODE = "QqqQQQqdQQQQ"  # from block_table on
+pack_paged_decode = struct.Struct("=" + _PT4 * 3 + "152x" + _DECODE).pack  # without new rows: their fields are zero
+pack_paged_step = struct.Struct("=" + _PT4 * 5 + "Q" + _DECODE).pack
 pack_paged_append = struct.Struct("=" + _PT4 * 4 + "QqQ").pack
 _TABLES = "QqQqqQqQqQQQ"  # a kf_page_tables
 pack_paged_reserve = struct.Struct("=" + _TABLES + "QQqqQ").pack

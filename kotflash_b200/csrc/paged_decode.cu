@@ -30,6 +30,7 @@
 // are taken transposed on warp MMAs (S^T = K Q^T, O^T = V^T P^T): keys and
 // head-dim fill the m = 16 side and up to 8 query rows the n = 8 side, so
 // few rows waste little.
+#include <float.h>
 #include <math.h>
 
 #include "kf_host.h"
@@ -50,7 +51,7 @@ struct PagedArgs {
   const uint16_t* nk;      // null: no fused append
   const uint16_t* nv;
   const int64_t* slots;    // of the new rows; < 0: this request has none
-  uint16_t* o;
+  uint16_t* o;             // [B][Hq][D]
   float* lse;              // may be null
   const int32_t* table;
   const int32_t* lengths;
@@ -59,30 +60,32 @@ struct PagedArgs {
   int4* joins;             // by unit if join_units, else by block: (request, KV head and row block, first
                            // block, last block) of a unit that was cut, or x = -1
   int32_t* status;         // set when a bounded wait expires (may be null)
-  int64_t qs[2], ks[3], vs[3], nks[2], nvs[2], os[2];
+  int64_t qs[2], ks[3], vs[3], nks[2], nvs[2];
   int64_t table_stride;
   int B, Hq, Hkv, G, D, row_blocks;
-  int64_t max_pages;
+  uint32_t max_pages;
   uint32_t capacity;       // tokens a table row can hold
   uint32_t page_size, num_pages;
   uint32_t page_mul, page_shift;  // x / page_size = x page_mul >> page_shift for x < 2^31
   int box;                 // rows of a TMA box
   bool join_units;
-  float scale_log2;
+  float scale_log2;        // |scale| log2(e), at least the smallest normal number
+  uint32_t q_sign;         // flips the signs of two elements of Q where scale is negative
 };
 
-// Variants: NP = 64-column panels of the padded head dim; NT = 8-row tiles of
+// Variants: KD = 16-column steps of the padded head dim; NT = 8-row tiles of
 // query rows per warp; RG = warps of a team (row groups).
-template <int NP, int NT, int RG>
+template <int KD, int NT, int RG>
 struct Cfg {
-  static constexpr int DP = NP * 64;
-  static constexpr int KW = (NP == 2 && RG == 1) ? 16 : 32;  // keys a team takes of a tile
+  static constexpr int DP = KD * 16;
+  static constexpr int NP = (KD + 3) / 4;                    // 64-column panels of a K or V tile
+  static constexpr int KW = (KD > 4 && RG == 1) ? 16 : 32;  // keys a team takes of a tile
   static constexpr int TEAMS = kWarps / RG;
   static constexpr int TILE = TEAMS * KW;                    // keys of a tile
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
-  static constexpr int STAGE = KW * DP * 2 * 2;              // bytes: K rows, then V rows
+  static constexpr int STAGE = KW * NP * 128 * 2;            // bytes: K rows, then V rows
   static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
-  static constexpr int PASS = 64 / NT < DP ? 64 / NT : DP;   // head-dim columns joined per pass of the epilogue
+  static constexpr int PASS = DP % 64 == 0 ? 64 / NT : 32;   // head-dim columns joined per pass of the epilogue
   static constexpr int OSTRIDE = PASS + 4;                   // keeps the four row pairs of a store on separate banks
   static constexpr int SMEM = 1024 + TEAMS * STAGES * STAGE + kWarps * NT * 8 * OSTRIDE * 4 + kWarps * NT * 8 * 2 * 4;
 };
@@ -140,16 +143,16 @@ __device__ __forceinline__ bool team_and(int team, bool pred) {
     return kf::named_bar_and(1 + team, RG * 32, pred);
 }
 
-template <bool BF16, int NP, int NT, int RG>
+template <bool BF16, int KD, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const PagedArgs a) {
-  using C = Cfg<NP, NT, RG>;
-  constexpr int DP = C::DP, KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
+  using C = Cfg<KD, NT, RG>;
+  constexpr int NP = C::NP, KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
   constexpr int H = KW / 16;           // 16-key halves of a step
-  constexpr int CHUNKS = DP / 8;       // 16-byte chunks of a row
-  constexpr int K_BYTES = KW * DP * 2;
+  constexpr int CHUNKS = NP * 8;       // 16-byte chunks of a row
   constexpr int PANEL = KW * 128;
+  constexpr int K_BYTES = NP * PANEL;
   constexpr uint32_t ALL = KW == 32 ? 0xffffffffu : 0xffffu;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -178,13 +181,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // all blocks, the first part of the table to L2 while the previous kernel
   // still runs (hints only: L2 stays coherent with what that kernel writes).
   {
-    const int64_t line = (int64_t)blockIdx.x * kThreads + tid;  // of 32 entries
-    if (line * 32 < a.B) prefetch_l2(a.lengths + line * 32);
-    const int64_t lines_per_row = (a.max_pages + 31) / 32;
-    if (line < a.B * lines_per_row) {
-      const int64_t b = line / lines_per_row;
-      prefetch_l2(a.table + b * a.table_stride + (line - b * lines_per_row) * 32);
-    }
+    const uint32_t line = blockIdx.x * kThreads + tid;  // of 32 entries
+    if (line * 32 < (uint32_t)a.B) prefetch_l2(a.lengths + line * 32);
+    const uint32_t lines_per_row = (a.max_pages + 31) / 32, b = line / lines_per_row;
+    if (b < (uint32_t)a.B) prefetch_l2(a.table + b * a.table_stride + (line - b * lines_per_row) * 32);
+    const uint32_t request = line / a.Hq;
+    if (request < (uint32_t)a.B)
+      kf::prefetch_l2_bulk(a.q + request * a.qs[0] + (line - request * a.Hq) * a.qs[1], a.D * 2);
   }
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -217,7 +220,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       if (visible(a, b) != 0) continue;
       for (int i = tid; i < a.Hq * (a.D / 8); i += kThreads) {
         const int h = i / (a.D / 8), c = i % (a.D / 8);
-        *reinterpret_cast<uint4*>(a.o + b * a.os[0] + h * a.os[1] + c * 8) = make_uint4(0, 0, 0, 0);
+        *reinterpret_cast<uint4*>(a.o + ((int64_t)b * a.Hq + h) * a.D + c * 8) = make_uint4(0, 0, 0, 0);
       }
       if (a.lse)
         for (int h = tid; h < a.Hq; h += kThreads) a.lse[(int64_t)b * a.Hq + h] = -INFINITY;
@@ -296,16 +299,26 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   };
 
   // ---- state of the unit being worked on
-  uint32_t qb[NT][DP / 16][2];         // Q^T as B fragments
-  float m_run[NT][2], l_run[NT][2];    // rows 2 (lane % 4) + {0, 1} of each row tile
-  float ot[NT][DP / 16][4];            // O^T
+  uint32_t qb[NT][KD][2];              // Q^T as B fragments
+  // rows 2 (lane % 4) + {0, 1} of each row tile: the reference of the weights
+  // 2^(x - m), their sum, and m again as it enters the exponent (0 for -inf)
+  float m_run[NT][2], l_run[NT][2], mu[NT][2];
+  float ot[NT][KD][4];                 // O^T
+  // offsets of a lane's ldmatrix rows in a K or V panel, by 16-column step mod 4
+  uint32_t k_off[4], v_off[4];
+#pragma unroll
+  for (int x = 0; x < 4; ++x) {
+    k_off[x] = swz(lane & 15, 2 * x + (lane >> 4), KW);
+    v_off[x] = swz((lane & 7) + ((lane >> 4) << 3), 2 * x + ((lane >> 3) & 1), KW);
+  }
+  // (the loads of Q; sign_unit() follows where they are first needed)
   auto start_unit = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = work.rb * C::ROWS + rg * NT * 8 + nt * 8 + (lane >> 2);
       const uint16_t* src = a.q + work.b * a.qs[0] + (int64_t)(work.h * a.G + row) * a.qs[1] + 2 * (lane & 3);
 #pragma unroll
-      for (int kk = 0; kk < DP / 16; ++kk) {
+      for (int kk = 0; kk < KD; ++kk) {
 #pragma unroll
         for (int e = 0; e < 2; ++e)
           qb[nt][kk][e] = (row < a.G && kk * 16 + e * 8 < a.D)
@@ -313,10 +326,21 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         ot[nt][kk][0] = ot[nt][kk][1] = ot[nt][kk][2] = ot[nt][kk][3] = 0.f;
       }
       m_run[nt][0] = m_run[nt][1] = -INFINITY;
-      l_run[nt][0] = l_run[nt][1] = 0.f;
+      l_run[nt][0] = l_run[nt][1] = mu[nt][0] = mu[nt][1] = 0.f;
     }
   };
+  auto sign_unit = [&]() {
+    if (a.q_sign == 0) return;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int kk = 0; kk < KD; ++kk) {
+        qb[nt][kk][0] ^= a.q_sign;
+        qb[nt][kk][1] ^= a.q_sign;
+      }
+  };
 
+  start_unit();  // ahead of the K/V loads, behind which its own would queue
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
@@ -339,10 +363,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       ahead = look_up();
     }
   }
-  start_unit();
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
   clear_empty();
+  sign_unit();
 
   int stage = 0, fill = STAGES - 1;
   uint32_t parity = 0;
@@ -351,9 +375,13 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   for (; i < n; ++i) {
     // One outcome for the team: no lane reaches a collective instruction alone.
     // The barrier also says that the team has left stage i - 1.
-    const bool landed = alive && !*(volatile int*)&abort_any && kf::mbar_wait(&full[team][stage], parity, a.status);
-    alive = team_and<RG>(team, landed);
+    uint32_t seen = RG == 1 ? seen_s[team][stage] : 0u;  // (this warp's own word: read before the wait)
+    bool landed = kf::mbar_try_wait(&full[team][stage], parity);
+    if (!landed) landed = alive && !*(volatile int*)&abort_any && kf::mbar_wait(&full[team][stage], parity, a.status);
+    alive = team_and<RG>(team, alive && landed);
     if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
+    if (RG > 1) seen = seen_s[team][stage];
+    if (!alive) seen = 0;
     if (rg == 0 && alive && issued < n) {
       issue(fill, ahead);
       ++issued;
@@ -363,7 +391,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
     }
 
-    const uint32_t seen = alive ? seen_s[team][stage] : 0u;
     uint8_t* kt = ring + stage * C::STAGE;
     uint8_t* vt = kt + K_BYTES;
     const uint32_t key0 = work.t * TILE + team * KW;
@@ -408,15 +435,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int nt = 0; nt < NT; ++nt) cc[x][h][nt][0] = cc[x][h][nt][1] = cc[x][h][nt][2] = cc[x][h][nt][3] = 0.f;
       constexpr int KG = H == 1 ? 4 : 2;
 #pragma unroll
-      for (int k0 = 0; k0 < DP / 16; k0 += KG) {
+      for (int k0 = 0; k0 < KD; k0 += KG) {
         uint32_t ka[KG][H][4];
 #pragma unroll
-        for (int x = 0; x < KG; ++x)
+        for (int x = 0; x < KG && k0 + x < KD; ++x)
 #pragma unroll
           for (int h = 0; h < H; ++h)
-            kf::ldmatrix_x4(ka[x][h], sk + swz(h * 16 + (lane & 15), 2 * (k0 + x) + (lane >> 4), KW));
+            kf::ldmatrix_x4(ka[x][h], sk + k_off[(k0 + x) & 3] + ((k0 + x) >> 2) * PANEL + h * 2048);
 #pragma unroll
-        for (int x = 0; x < KG; ++x)
+        for (int x = 0; x < KG && k0 + x < KD; ++x)
 #pragma unroll
           for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -428,41 +455,61 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 #pragma unroll
         for (int e = 0; e < 4; ++e) c[0][0][e] += cc[1][0][0][e];
       }
-      uint32_t pb[H][NT][2], pl[H][NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        // rows 2 (lane % 4) + {0, 1}; keys 16 h + lane / 4 (c0, c1) and + 8 (c2, c3)
-        float mx[2] = {-INFINITY, -INFINITY};
+      // rows 2 (lane % 4) + {0, 1}; keys 16 h + lane / 4 (c0, c1) and + 8 (c2, c3)
+      if (seen != ALL) {
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           const uint32_t bits = seen >> (h * 16 + (lane >> 2));
 #pragma unroll
-          for (int e = 0; e < 4; ++e)
-            c[h][nt][e] = (bits & (e < 2 ? 1u : 256u)) ? c[h][nt][e] * a.scale_log2 : -INFINITY;
-          mx[0] = kf::fmax3(mx[0], c[h][nt][0], c[h][nt][2]);
-          mx[1] = kf::fmax3(mx[1], c[h][nt][1], c[h][nt][3]);
-        }
+          for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          mx[0] = fmaxf(mx[0], __shfl_xor_sync(0xffffffffu, mx[0], off));
-          mx[1] = fmaxf(mx[1], __shfl_xor_sync(0xffffffffu, mx[1], off));
+            for (int e = 0; e < 4; ++e) c[h][nt][e] = (bits & (e < 2 ? 1u : 256u)) ? c[h][nt][e] : -INFINITY;
         }
-        float alpha[2], mu[2];
+      }
+      // The reference m of a row follows its maximum only when a score passes
+      // it by 2^8: weights up to 256 lose nothing in fp32 sums and 16-bit
+      // parts, and most steps need no exchange between lanes (a step took 2240
+      // cycles with one, of which the shuffles and the rescale a quarter).
+      bool raise = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          const float m_new = fmaxf(m_run[nt][j], mx[j]);
-          mu[j] = m_new == -INFINITY ? 0.f : m_new;
-          alpha[j] = kf::ex2(m_run[nt][j] - mu[j]);
-          m_run[nt][j] = m_new;
+          float top = fmaxf(c[0][nt][j], c[0][nt][2 + j]);
+          if constexpr (H == 2) top = kf::fmax3(top, c[H - 1][nt][j], c[H - 1][nt][2 + j]);
+          raise |= top * a.scale_log2 > m_run[nt][j] + 8.f;
         }
-        float ls[2] = {0.f, 0.f};
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float top = fmaxf(c[0][nt][j], c[0][nt][2 + j]);
+            if constexpr (H == 2) top = kf::fmax3(top, c[H - 1][nt][j], c[H - 1][nt][2 + j]);
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+            const float m_new = fmaxf(m_run[nt][j], top * a.scale_log2);
+            mu[nt][j] = m_new == -INFINITY ? 0.f : m_new;
+            const float old = kf::ex2(m_run[nt][j] - mu[nt][j]);
+            m_run[nt][j] = m_new;
+            l_run[nt][j] *= old;
+#pragma unroll
+            for (int dm = 0; dm < KD; ++dm) {
+              ot[nt][dm][j] *= old;
+              ot[nt][dm][2 + j] *= old;
+            }
+          }
+      }
+      uint32_t pb[H][NT][2], pl[H][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
-          float p[4], r[4];
+          float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            p[e] = kf::ex2(c[h][nt][e] - mu[e & 1]);
-            ls[e & 1] += p[e];
+            p[e] = kf::ex2(fmaf(c[h][nt][e], a.scale_log2, -mu[nt][e & 1]));
+            l_run[nt][e & 1] += p[e];
           }
           // P as a 16-bit value plus the 16-bit rest: two products keep the
           // weights at about fp32 accuracy, as a plain fp32 softmax has them
@@ -470,42 +517,27 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int x = 0; x < 2; ++x) {
             const uint32_t hi = kf::pack2<BF16>(p[2 * x], p[2 * x + 1]);
             const float2 back = kf::unpack2<BF16>(hi);
-            r[2 * x] = p[2 * x] - back.x;
-            r[2 * x + 1] = p[2 * x + 1] - back.y;
             pb[h][nt][x] = kf::movmatrix_trans(hi);
-            pl[h][nt][x] = kf::movmatrix_trans(kf::pack2<BF16>(r[2 * x], r[2 * x + 1]));
+            pl[h][nt][x] = kf::movmatrix_trans(kf::pack2<BF16>(p[2 * x] - back.x, p[2 * x + 1] - back.y));
           }
         }
-        l_run[nt][0] = l_run[nt][0] * alpha[0] + ls[0];
-        l_run[nt][1] = l_run[nt][1] * alpha[1] + ls[1];
-        if (__any_sync(0xffffffffu, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-          for (int dm = 0; dm < DP / 16; ++dm) {
-            ot[nt][dm][0] *= alpha[0];
-            ot[nt][dm][1] *= alpha[1];
-            ot[nt][dm][2] *= alpha[0];
-            ot[nt][dm][3] *= alpha[1];
-          }
-        }
-      }
       // O^T (head dim x rows) += V^T P^T, the two parts of P apart from one
       // another so that no product waits for the one before it
       constexpr int VG = NT == 1 ? 4 : 2;
 #pragma unroll
-      for (int d0 = 0; d0 < DP / 16; d0 += VG)
+      for (int d0 = 0; d0 < KD; d0 += VG)
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t va[VG][4];
 #pragma unroll
-          for (int x = 0; x < VG; ++x)
-            kf::ldmatrix_x4_trans(va[x], sv + swz(h * 16 + (lane & 7) + ((lane >> 4) << 3),
-                                                  2 * (d0 + x) + ((lane >> 3) & 1), KW));
+          for (int x = 0; x < VG && d0 + x < KD; ++x)
+            kf::ldmatrix_x4_trans(va[x], sv + v_off[(d0 + x) & 3] + ((d0 + x) >> 2) * PANEL + h * 2048);
 #pragma unroll
-          for (int x = 0; x < VG; ++x)
+          for (int x = 0; x < VG && d0 + x < KD; ++x)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pb[h][nt][0], pb[h][nt][1]);
 #pragma unroll
-          for (int x = 0; x < VG; ++x)
+          for (int x = 0; x < VG && d0 + x < KD; ++x)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pl[h][nt][0], pl[h][nt][1]);
         }
@@ -543,7 +575,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       for (int nt = 0; nt < NT; ++nt) l_run[nt][0] = l_run[nt][1] = m_run[nt][0] = m_run[nt][1] = NAN;
     }
 #pragma unroll
-    for (int pass = 0; pass < DP / C::PASS; ++pass) {
+    for (int pass = 0; pass < C::DP / C::PASS; ++pass) {
       unit_sync();  // the buffer's readers of the pass (or unit) before are done
       if (pass == 0 && lane < 4) {
 #pragma unroll
@@ -594,7 +626,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float lse2 = L == 0.f ? -INFINITY : M + log2f(L);
         const int head = h * a.G + rb * C::ROWS + r;
         if (direct) {
-          *reinterpret_cast<uint2*>(a.o + work.b * a.os[0] + head * a.os[1] + d) =
+          *reinterpret_cast<uint2*>(a.o + ((int64_t)work.b * a.Hq + head) * a.D + d) =
               make_uint2(kf::pack2<BF16>(acc[0] * inv, acc[1] * inv), kf::pack2<BF16>(acc[2] * inv, acc[3] * inv));
           if (a.lse && d == 0) a.lse[(int64_t)work.b * a.Hq + head] = lse2 * kLn2;
         } else {
@@ -616,6 +648,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (i + 1 < n) {
       work.next(a);
       start_unit();
+      sign_unit();
       unit_t0 = 0;
     }
   }
@@ -720,7 +753,7 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
   if (!mine || part != 0) return;
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int head = h * a.G + rb * rows + r;
-  *reinterpret_cast<uint2*>(a.o + unit.x * a.os[0] + head * a.os[1] + c * 4) =
+  *reinterpret_cast<uint2*>(a.o + ((int64_t)unit.x * a.Hq + head) * a.D + c * 4) =
       make_uint2(kf::pack2<BF16>(acc.x * inv, acc.y * inv), kf::pack2<BF16>(acc.z * inv, acc.w * inv));
   if (a.lse && c == 0) a.lse[(int64_t)unit.x * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
 }
@@ -735,11 +768,11 @@ size_t workspace_need(int blocks, int rows, int64_t D) {
   return 256 + (size_t)blocks * (16 + (size_t)2 * rows * 4 + (size_t)2 * rows * D * 4);
 }
 
-template <bool BF16, int NP, int NT, int RG>
+template <bool BF16, int KD, int NT, int RG>
 int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
-  using C = Cfg<NP, NT, RG>;
+  using C = Cfg<KD, NT, RG>;
   static_assert(C::STAGES >= 3, "the ring needs three stages");
-  auto kern = paged_decode_kernel<BF16, NP, NT, RG>;
+  auto kern = paged_decode_kernel<BF16, KD, NT, RG>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
     (void)cudaGetLastError();
     return kf::set_error(KF_ERR_CUDA, "kf_paged_decode: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -747,14 +780,14 @@ int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap&
   return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged_decode", mk, mv, a);
 }
 
-template <bool BF16, int NP>
+template <bool BF16, int KD>
 int dispatch_rows(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
                   cudaStream_t st) {
   switch (rows) {
-    case 8: return launch_variant<BF16, NP, 1, 1>(a, mk, mv, blocks, st);
-    case 16: return launch_variant<BF16, NP, 2, 1>(a, mk, mv, blocks, st);
-    case 32: return launch_variant<BF16, NP, 2, 2>(a, mk, mv, blocks, st);
-    default: return launch_variant<BF16, NP, 2, 4>(a, mk, mv, blocks, st);
+    case 8: return launch_variant<BF16, KD, 1, 1>(a, mk, mv, blocks, st);
+    case 16: return launch_variant<BF16, KD, 2, 1>(a, mk, mv, blocks, st);
+    case 32: return launch_variant<BF16, KD, 2, 2>(a, mk, mv, blocks, st);
+    default: return launch_variant<BF16, KD, 2, 4>(a, mk, mv, blocks, st);
   }
 }
 
@@ -776,17 +809,15 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   using kf::set_error;
   const char* what = "kf_paged_decode";
   if (!args) return set_error(KF_ERR_INVALID, "%s: null arguments", what);
-  const kf_tensor4 *q = &args->q, *k_pages = &args->k_pages, *v_pages = &args->v_pages, *o = &args->o;
+  const kf_tensor4 *q = &args->q, *k_pages = &args->k_pages, *v_pages = &args->v_pages;
   const kf_tensor4 *new_k = &args->new_k, *new_v = &args->new_v;
   const int64_t dtype = args->dtype, max_pages = args->max_pages;
   if (dtype != KF_F16 && dtype != KF_BF16) return set_error(KF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
   const int64_t B = q->size[0], Hq = q->size[1], D = q->size[3];
   const int64_t pages = k_pages->size[0], Hkv = k_pages->size[1], page_size = k_pages->size[2];
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < 4; ++i)
     if (k_pages->size[i] != v_pages->size[i])
       return set_error(KF_ERR_INVALID, "%s: K/V page shapes must match", what);
-    if (o->size[i] != q->size[i]) return set_error(KF_ERR_INVALID, "%s: O must have Q's shape", what);
-  }
   if (B <= 0 || Hq <= 0 || Hkv <= 0 || pages <= 0 || page_size <= 0 || max_pages <= 0)
     return set_error(KF_ERR_INVALID, "%s: dimensions must be non-zero", what);
   if (q->size[2] != 1) return set_error(KF_ERR_INVALID, "%s: Q must hold one token per request", what);
@@ -797,9 +828,10 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
     return set_error(KF_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [16, 128]", what);
   if (page_size > (1 << 20) || pages > 0x7fffffffLL || max_pages > 0x7fffffffLL || B > (1 << 20) || Hq > (1 << 16))
     return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
-  if (!rows16(q, 2) || !rows16(k_pages, 3) || !rows16(v_pages, 3) || !rows16(o, 2))
+  if (!rows16(q, 2) || !rows16(k_pages, 3) || !rows16(v_pages, 3) ||
+      !kf::aligned16(args->o))
     return set_error(KF_ERR_INVALID, "%s: tensors need a contiguous last dim and 16-byte aligned rows", what);
-  if (!q->ptr || !k_pages->ptr || !v_pages->ptr || !o->ptr || !args->block_table || !args->lengths)
+  if (!q->ptr || !k_pages->ptr || !v_pages->ptr || !args->o || !args->block_table || !args->lengths)
     return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
   const bool fused = new_k->ptr || new_v->ptr || args->slots;
   if (fused) {
@@ -824,13 +856,12 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.nk = fused ? static_cast<const uint16_t*>(new_k->ptr) : nullptr;
   a.nv = fused ? static_cast<const uint16_t*>(new_v->ptr) : nullptr;
   a.slots = args->slots;
-  a.o = static_cast<uint16_t*>(o->ptr);
+  a.o = static_cast<uint16_t*>(args->o);
   a.lse = args->lse;
   a.table = args->block_table;
   a.lengths = args->lengths;
   for (int i = 0; i < 2; ++i) {
     a.qs[i] = q->stride[i];
-    a.os[i] = o->stride[i];
     a.nks[i] = fused ? new_k->stride[i] : 0;
     a.nvs[i] = fused ? new_v->stride[i] : 0;
   }
@@ -847,7 +878,7 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.row_blocks = (a.G + rows - 1) / rows;
   const int64_t capacity = max_pages * page_size;
   a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
-  a.max_pages = max_pages;
+  a.max_pages = (uint32_t)max_pages;
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
@@ -855,7 +886,11 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   // boxes never cross a page nor a team's 16 or 32 keys
   a.box = 16;
   while (page_size % a.box) a.box /= 2;
-  a.scale_log2 = (float)args->scale * kLog2e;
+  // A negative scale is taken as -q and a positive one, so that the largest
+  // product is the largest score; 0 as a scale that no product survives, so
+  // that a masked -inf stays -inf.
+  a.scale_log2 = fmaxf(fabsf((float)args->scale) * kLog2e, FLT_MIN);
+  a.q_sign = args->scale < 0 ? 0x80008000u : 0u;
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.
   // A unit of one tile is never cut, so nothing is left to join.
@@ -886,11 +921,14 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   cudaStream_t st = static_cast<cudaStream_t>(args->stream);
   const bool bf16 = dtype == KF_BF16;
   if (D <= 64)
-    rc = bf16 ? dispatch_rows<true, 1>(a, mk, mv, rows, (int)blocks, st)
-              : dispatch_rows<false, 1>(a, mk, mv, rows, (int)blocks, st);
+    rc = bf16 ? dispatch_rows<true, 4>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 4>(a, mk, mv, rows, (int)blocks, st);
+  else if (D <= 96)
+    rc = bf16 ? dispatch_rows<true, 6>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 6>(a, mk, mv, rows, (int)blocks, st);
   else
-    rc = bf16 ? dispatch_rows<true, 2>(a, mk, mv, rows, (int)blocks, st)
-              : dispatch_rows<false, 2>(a, mk, mv, rows, (int)blocks, st);
+    rc = bf16 ? dispatch_rows<true, 8>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 8>(a, mk, mv, rows, (int)blocks, st);
   if (rc != KF_OK || most == 1) return rc;
   // Groups that share a row: as many as leave each about one batch of the
   // partials that a unit has on average (2 where units outnumber the blocks).

@@ -33,7 +33,10 @@ from . import _ext
 
 _DTYPES = {torch.float16: _ext.KF_F16, torch.bfloat16: _ext.KF_BF16}
 _INT32, _INT64, _BOOL = torch.int32, torch.int64, torch.bool
-_NO_ROWS = (0,) * 18  # two empty kf_tensor4
+_CONTIGUOUS = torch.contiguous_format
+_pack_decode, _pack_step, _pack_append = _ext.pack_paged_decode, _ext.pack_paged_step, _ext.pack_paged_append
+_pack_reserve, _pack_release = _ext.pack_paged_reserve, _ext.pack_paged_release
+_raw_stream, _is_sm100 = _ext.raw_stream, _ext.is_sm100
 
 
 # Each entry point below tests everything in one expression, which is what a
@@ -117,6 +120,12 @@ def _check_attention(q, k_pages, v_pages, block_table, lengths, new_k, new_v, sl
     _check_device(what, q, k_pages, v_pages, block_table, lengths, *rows, *((slots,) if rows else ()))
 
 
+@lru_cache(maxsize=16)
+def _status_ptr(index: int) -> int:
+    """Address of the device's status word, which lives as long as the process."""
+    return _ext.status_word(torch.device("cuda", index)).data_ptr()
+
+
 @lru_cache(maxsize=256)
 def _workspace_elements(hq: int, hkv: int, d: int, device_index: int) -> int:
     """Workspace of kf_paged_decode in 16-bit elements."""
@@ -162,51 +171,61 @@ def paged_attention(
             raise ValueError("scale must be finite")
     try:
         index = q.get_device()
-        b, hq, _, d = qs = q.shape
-        ks = k_pages.shape
         dtype = q.dtype
+        b, hq, _, d = qs = q.shape
+        _, hkv, _, _ = ks = k_pages.shape
+        requests, max_pages = block_table.shape
+        row_stride, column_stride = block_table.stride()
+        grad = torch.is_grad_enabled()
         good = (
-            index >= 0 and _ext.is_sm100(index) and k_pages.dtype is dtype and v_pages.dtype is dtype
-            and dtype in _DTYPES and len(ks) == 4 and v_pages.ndim == 4
-            and block_table.dtype is _INT32 and lengths.dtype is _INT32 and lengths.shape == qs[:1]
-            and lengths.is_contiguous() and block_table.ndim == 2 and block_table.shape[0] == b
-            and block_table.stride(1) == 1 and b > 0 and hq > 0 and ks[1] > 0 and hq % ks[1] == 0
-            and k_pages.get_device() == index and v_pages.get_device() == index
-            and block_table.get_device() == index and lengths.get_device() == index
-            and not (torch.is_grad_enabled() and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))
-            and (new_k is None and new_v is None and slots is None
-                 or new_k.dtype is dtype and new_v.dtype is dtype and slots.dtype is _INT64
-                 and new_k.ndim == 4 and new_v.ndim == 4 and slots.shape == qs[:1] and slots.is_contiguous()
-                 and new_k.get_device() == index and new_v.get_device() == index and slots.get_device() == index
-                 and not (torch.is_grad_enabled() and (new_k.requires_grad or new_v.requires_grad)))
+            index >= 0 and k_pages.get_device() == index and v_pages.get_device() == index
+            and block_table.get_device() == index and lengths.get_device() == index and _is_sm100(index)
+            and k_pages.dtype is dtype and v_pages.dtype is dtype and v_pages.dim() == 4
+            and block_table.dtype is _INT32 and lengths.dtype is _INT32 and lengths.dim() == 1
+            and lengths.numel() == b and requests == b and column_stride == 1 and lengths.is_contiguous()
+            and b > 0 and hq > 0 and hkv > 0 and hq % hkv == 0
+            and not (grad and (q.requires_grad or k_pages.requires_grad or v_pages.requires_grad))
         )
+        if new_k is not None or new_v is not None or slots is not None:
+            good = good and (
+                new_k.get_device() == index and new_v.get_device() == index and slots.get_device() == index
+                and new_k.dtype is dtype and new_v.dtype is dtype and new_k.dim() == 4 and new_v.dim() == 4
+                and slots.dtype is _INT64 and slots.dim() == 1 and slots.numel() == b and slots.is_contiguous()
+                and not (grad and (new_k.requires_grad or new_v.requires_grad)))
+        code = _DTYPES.get(dtype, -1)
     except (AttributeError, TypeError, ValueError, RuntimeError):
         good = False
-    if not good:
+    if not good or code < 0:
         _check_attention(q, k_pages, v_pages, block_table, lengths, new_k, new_v, slots)
-        index = q.get_device()
-        b, hq, _, d = qs = q.shape
-        ks = k_pages.shape
-        dtype = q.dtype
+        # a table of one column may have any stride
+        index, dtype, qs, ks = q.get_device(), q.dtype, q.shape, k_pages.shape
+        b, hq, _, d = qs
+        hkv, max_pages, row_stride, code = ks[1], block_table.shape[1], block_table.stride(0), _DTYPES[dtype]
     if scale is None:
         scale = 1.0 / math.sqrt(d) if d else 1.0
     lib = _ext.load()
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((b, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
-    elements = _workspace_elements(hq, ks[1], d, index)
+    out = torch.empty_like(q, memory_format=_CONTIGUOUS)
+    elements = _workspace_elements(hq, hkv, d, index)
     workspace = q.new_empty(elements)
-    if new_k is None:
-        rows, slots_ptr = _NO_ROWS, 0
+    if return_lse:
+        lse = q.new_empty((b, hq, 1), dtype=torch.float32)
+        lse_ptr = lse.data_ptr()
     else:
-        rows = (new_k.data_ptr(), *new_k.shape, *new_k.stride(), new_v.data_ptr(), *new_v.shape, *new_v.stride())
-        slots_ptr = slots.data_ptr()
-    rc = lib.kf_paged_decode(_ext.pack_paged_decode(
-        q.data_ptr(), *qs, *q.stride(), k_pages.data_ptr(), *ks, *k_pages.stride(),
-        v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(), out.data_ptr(), *qs, *out.stride(), *rows,
-        slots_ptr, block_table.data_ptr(), block_table.shape[1], block_table.stride(0), lengths.data_ptr(),
-        lse.data_ptr() if return_lse else 0, _DTYPES[dtype], scale, workspace.data_ptr(), elements * 2,
-        _ext.status_word(q.device).data_ptr(), _ext.raw_stream(index),
-    ))
+        lse_ptr = 0
+    if new_k is None:
+        args = _pack_decode(
+            q.data_ptr(), *qs, *q.stride(), k_pages.data_ptr(), *ks, *k_pages.stride(),
+            v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(), block_table.data_ptr(), max_pages, row_stride,
+            lengths.data_ptr(), out.data_ptr(), lse_ptr, code, scale, workspace.data_ptr(), elements * 2,
+            _status_ptr(index), _raw_stream(index))
+    else:
+        args = _pack_step(
+            q.data_ptr(), *qs, *q.stride(), k_pages.data_ptr(), *ks, *k_pages.stride(),
+            v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(), new_k.data_ptr(), *new_k.shape, *new_k.stride(),
+            new_v.data_ptr(), *new_v.shape, *new_v.stride(), slots.data_ptr(), block_table.data_ptr(), max_pages,
+            row_stride, lengths.data_ptr(), out.data_ptr(), lse_ptr, code, scale, workspace.data_ptr(), elements * 2,
+            _status_ptr(index), _raw_stream(index))
+    rc = lib.kf_paged_decode(args)
     if rc:
         _ext.check(rc, "kf_paged_decode")
     return (out, lse) if return_lse else out
@@ -231,7 +250,7 @@ def append_paged_kv(
         dtype = k_pages.dtype
         ns = new_k.shape
         good = (
-            index >= 0 and _ext.is_sm100(index) and dtype in _DTYPES and v_pages.dtype is dtype
+            index >= 0 and _is_sm100(index) and dtype in _DTYPES and v_pages.dtype is dtype
             and new_k.dtype is dtype and new_v.dtype is dtype and slots.dtype is _INT64 and k_pages.ndim == 4
             and v_pages.ndim == 4 and len(ns) == 4 and new_v.ndim == 4 and slots.shape == (ns[0] * ns[2],)
             and slots.is_contiguous() and v_pages.get_device() == index and new_k.get_device() == index
@@ -248,10 +267,10 @@ def append_paged_kv(
         _check_inference(what, k_pages, v_pages, new_k, new_v)
         _check_device(what, k_pages, v_pages, new_k, new_v, slots)
         index, dtype, ns = k_pages.get_device(), k_pages.dtype, new_k.shape
-    rc = _ext.load().kf_paged_append(_ext.pack_paged_append(
+    rc = _ext.load().kf_paged_append(_pack_append(
         k_pages.data_ptr(), *k_pages.shape, *k_pages.stride(), v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(),
         new_k.data_ptr(), *ns, *new_k.stride(), new_v.data_ptr(), *new_v.shape, *new_v.stride(),
-        slots.data_ptr(), _DTYPES[dtype], _ext.raw_stream(index),
+        slots.data_ptr(), _DTYPES[dtype], _raw_stream(index),
     ))
     if rc:
         _ext.check(rc, "kf_paged_append")
@@ -262,7 +281,7 @@ def _tables_good(lengths, second, block_table, free_pages, free_count, lengths_o
         index = lengths.get_device()
         shape = lengths.shape
         return (
-            index >= 0 and _ext.is_sm100(index) and lengths.dtype is _INT32 and block_table.dtype is _INT32
+            index >= 0 and _is_sm100(index) and lengths.dtype is _INT32 and block_table.dtype is _INT32
             and free_pages.dtype is _INT32 and free_count.dtype is _INT32 and len(shape) == 1
             and second.shape == shape and block_table.ndim == 2 and block_table.shape[0] == shape[0]
             and block_table.stride(1) == 1 and free_pages.ndim == 1 and free_count.numel() == 1
@@ -345,10 +364,10 @@ def reserve_pages(
         lengths_out = torch.empty_like(lengths)
     if free_count_out is None:
         free_count_out = torch.empty_like(free_count)
-    rc = _ext.load().kf_paged_reserve(_ext.pack_paged_reserve(
+    rc = _ext.load().kf_paged_reserve(_pack_reserve(
         lengths.data_ptr(), b, block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
-        free_count_out.data_ptr(), _ext.raw_stream(lengths.get_device()), new_lengths.data_ptr(), slots.data_ptr(),
+        free_count_out.data_ptr(), _raw_stream(lengths.get_device()), new_lengths.data_ptr(), slots.data_ptr(),
         num_tokens, per_request, starts.data_ptr(),
     ))
     if rc:
@@ -383,10 +402,10 @@ def release_pages(
         lengths_out = torch.empty_like(lengths)
     if free_count_out is None:
         free_count_out = torch.empty_like(free_count)
-    rc = _ext.load().kf_paged_release(_ext.pack_paged_release(
+    rc = _ext.load().kf_paged_release(_pack_release(
         lengths.data_ptr(), lengths.shape[0], block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
         free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
-        free_count_out.data_ptr(), _ext.raw_stream(lengths.get_device()), finished.data_ptr(),
+        free_count_out.data_ptr(), _raw_stream(lengths.get_device()), finished.data_ptr(),
     ))
     if rc:
         _ext.check(rc, "kf_paged_release")

@@ -124,6 +124,7 @@ def test_structs_have_the_headers_sizes(tmp_path):
     subprocess.run(["gcc", "-std=c99", "-Wall", "-Werror", "-I", str(root / "include"), str(tmp_path / "s.c"), "-o",
                     str(tmp_path / "s")], check=True, capture_output=True, text=True)
     lines = subprocess.run([str(tmp_path / "s")], check=True, capture_output=True, text=True).stdout.split()
+    assert _ext.pack_paged_step.__self__.size == _ext.pack_paged_decode.__self__.size
     for i, (n, _) in enumerate(names):
         size = getattr(_ext, f"pack_paged_{n}").__self__.size
         assert int(lines[2 * i]) == size and int(lines[2 * i + 1]) == size - 8
@@ -133,16 +134,18 @@ def test_c_abi_refuses_before_any_launch():
     lib = _ext.load()
     p = 0x1000
 
-    def decode(q=(3, 4, 1, 64), k=(5, 2, 16, 64), v=None, o=None, table=p, max_pages=2, lens=p, nk=None, nv=None, slots=0,
+    def decode(q=(3, 4, 1, 64), k=(5, 2, 16, 64), v=None, o=p, table=p, max_pages=2, lens=p, nk=None, nv=None, slots=0,
                dtype=0, ws=0, ws_bytes=0, q_strides=None, k_ptr=p):
-        return lib.kf_paged_decode(_ext.pack_paged_decode(
-            *_t(q, strides=q_strides), *_t(k, k_ptr), *_t(v or k), *_t(o or q), *_t(nk), *_t(nv), slots, table, max_pages,
-            max_pages, lens, 0, dtype, 0.1, ws, ws_bytes, 0, 0))
+        rows = (*_t(nk), *_t(nv), slots)
+        pack, rows = (_ext.pack_paged_step, rows) if any(rows) else (_ext.pack_paged_decode, ())
+        return lib.kf_paged_decode(pack(*_t(q, strides=q_strides), *_t(k, k_ptr), *_t(v or k), *rows, table, max_pages,
+                                        max_pages, lens, o, 0, dtype, 0.1, ws, ws_bytes, 0, 0))
 
     for kw, code, match in [
         (dict(dtype=5), _ext.KF_ERR_INVALID, "dtype"),
         (dict(v=(5, 2, 16, 72)), _ext.KF_ERR_INVALID, "K/V page shapes"),
-        (dict(o=(3, 4, 1, 72)), _ext.KF_ERR_INVALID, "O must have"),
+        (dict(o=0), _ext.KF_ERR_INVALID, "null data"),
+        (dict(o=0x1008), _ext.KF_ERR_INVALID, "16-byte"),
         (dict(q=(3, 4, 2, 64)), _ext.KF_ERR_INVALID, "one token"),
         (dict(q=(3, 5, 1, 64)), _ext.KF_ERR_INVALID, "divisible"),
         (dict(q=(3, 4, 1, 72)), _ext.KF_ERR_INVALID, "head dimensions"),
