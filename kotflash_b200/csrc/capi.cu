@@ -80,6 +80,36 @@ int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box
   return KF_OK;
 }
 
+int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows, int panels, bool swizzle) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  if (t->stride[3] != 1) return set_error(KF_ERR_INVALID, "TMA view needs a contiguous last dim");
+  if (!aligned16(t->ptr)) return set_error(KF_ERR_INVALID, "TMA base pointer not 16-byte aligned");
+  cuuint64_t dims[5] = {(cuuint64_t)(panels > 1 ? cols : t->size[3]), (cuuint64_t)t->size[2], (cuuint64_t)panels,
+                        (cuuint64_t)t->size[1], (cuuint64_t)t->size[0]};
+  cuuint64_t strides[4] = {(cuuint64_t)t->stride[2] * 2, (cuuint64_t)cols * 2, (cuuint64_t)t->stride[1] * 2,
+                           (cuuint64_t)t->stride[0] * 2};
+  for (int i = 0; i < 4; ++i) {
+    if (strides[i] % 16 == 0 && strides[i] != 0) continue;
+    // a size-1 dimension may carry any stride; give it a legal one
+    if (dims[i + 1] != 1)
+      return set_error(KF_ERR_INVALID, "TMA stride %llu bytes is not a positive multiple of 16",
+                       (unsigned long long)strides[i]);
+    strides[i] = 128;
+  }
+  cuuint32_t box[5] = {(cuuint32_t)cols, (cuuint32_t)rows, (cuuint32_t)panels, 1, 1};
+  const CUtensorMapSwizzle mode = !swizzle      ? CU_TENSOR_MAP_SWIZZLE_NONE
+                                  : cols == 64 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                  : cols == 32 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                               : CU_TENSOR_MAP_SWIZZLE_32B;
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, t->ptr, dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, mode,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
+  return KF_OK;
+}
+
 int encode_tmap_2d_f32(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int box_cols,
                        int box_rows) {
   EncodeTiledFn fn = get_encode_fn();

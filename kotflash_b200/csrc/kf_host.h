@@ -25,6 +25,15 @@ int check_launch(const char* what);
 // as zero.  Returns KF_OK or an error code with the message recorded.
 int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box_rows);
 
+// Encode a 5-D tiled TMA descriptor over a 16-bit pool of pages [n0 pages, n1
+// heads, n2 rows, n3 columns] whose innermost dimension is contiguous, with
+// coordinates (column, row, panel, head, page).  panels == 1: columns are n3,
+// the box is (cols, rows).  panels > 1: n3 = panels * cols, columns run within
+// a panel and the box holds its rows of all panels, panel after panel.
+// Swizzle over the panel's 32, 64 or 128 bytes, or none; out-of-range elements
+// read as zero.
+int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows, int panels, bool swizzle);
+
 // Encode a 2-D tiled TMA descriptor over a row-major fp32 matrix
 // [rows][cols] (cols contiguous) with a (box_cols x box_rows) box and 128-byte
 // swizzle (box_cols * 4 must be <= 128).

@@ -67,33 +67,48 @@ struct PagedArgs {
   uint32_t capacity;       // tokens a table row can hold
   uint32_t page_size, num_pages;
   uint32_t page_mul, page_shift;  // x / page_size = x page_mul >> page_shift for x < 2^31
-  int box;                 // rows of a TMA box
+  int box, box_ops;        // rows of a TMA box, and loads that bring its columns
+  int box_bytes;           // of K and V together
+  int width;               // 16-byte chunks of a panel's rows (8, 4 or 2), or 0: dense rows (see tile_offset)
+  int block_bytes, row_bytes;  // from 16 rows of a tile to the next, and between rows as boxes of fewer start
+  bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
   bool join_units;
   float scale_log2;        // |scale| log2(e), at least the smallest normal number
   uint32_t q_sign;         // flips the signs of two elements of Q where scale is negative
 };
 
-// Variants: KD = 16-column steps of the padded head dim; NT = 8-row tiles of
-// query rows per warp; RG = warps of a team (row groups).
+// Variants: KD = 16-column steps of the padded head dim (4, 6 or 8); FULL: D is
+// KD * 16; NT = 8-row tiles of query rows per warp; RG = warps of a team (row
+// groups).
 template <int KD, int NT, int RG>
 struct Cfg {
   static constexpr int DP = KD * 16;
-  static constexpr int NP = (KD + 3) / 4;                    // 64-column panels of a K or V tile
-  static constexpr int KW = (KD > 4 && RG == 1) ? 16 : 32;  // keys a team takes of a tile
+  static constexpr int KW = (KD > 6 && RG == 1) ? 16 : 32;  // keys a team takes of a tile
   static constexpr int TEAMS = kWarps / RG;
   static constexpr int TILE = TEAMS * KW;                    // keys of a tile
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
-  static constexpr int STAGE = KW * NP * 128 * 2;            // bytes: K rows, then V rows
+  static constexpr int STAGE = KW * DP * 2 * 2;              // bytes: K rows, then V rows
   static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
   static constexpr int PASS = DP % 64 == 0 ? 64 / NT : 32;   // head-dim columns joined per pass of the epilogue
   static constexpr int OSTRIDE = PASS + 4;                   // keeps the four row pairs of a store on separate banks
   static constexpr int SMEM = 1024 + TEAMS * STAGES * STAGE + kWarps * NT * 8 * OSTRIDE * 4 + kWarps * NT * 8 * 2 * 4;
 };
 
-// Shared-memory offset of 16-byte chunk c of row r in a TMA tile stored as
-// 64-column panels of `rows` x 128 B with the 128-byte swizzle.
-__device__ __forceinline__ uint32_t swz(int r, int c, int rows) {
-  return (uint32_t)((c >> 3) * rows * 128 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+// Offset of 16-byte chunk c of row r in a K or V tile as TMA writes it: blocks
+// of 16 rows, in a block the panels of `width` chunks one after another, in a
+// panel row after row with the chunks swizzled, so that the 8 rows an ldmatrix
+// reads lie on different banks.  Panels are as wide as divides D (64, 32 or 16
+// columns), since a panel wider than what is left of a row fetches the columns
+// beyond it as well (D = 72 in 64-column panels: 638 MB through L2 for 302 MB).
+// An odd number of chunks per row (72, 104) needs neither panels nor a
+// swizzle: width 0, rows one after another.  Boxes of fewer than 16 rows
+// (page sizes that 16 does not divide) bring one panel at a time, so they
+// keep 64-column panels; dense rows can still be boxes of 8.
+__device__ __forceinline__ uint32_t tile_at(int r, int c, int width, int block_bytes) {
+  if (width == 0) return (uint32_t)((r >> 4) * block_bytes + (r & 15) * (block_bytes >> 4) + c * 16);
+  const int log = width == 8 ? 3 : width == 4 ? 2 : 1, x = r >> (3 - log);
+  return (uint32_t)((r >> 4) * block_bytes + (c >> log) * 256 * width + (r & 15) * 16 * width +
+                    (((c ^ x) & (width - 1)) << 4));
 }
 
 __device__ __forceinline__ uint32_t visible(const PagedArgs& a, int b) {
@@ -143,16 +158,14 @@ __device__ __forceinline__ bool team_and(int team, bool pred) {
     return kf::named_bar_and(1 + team, RG * 32, pred);
 }
 
-template <bool BF16, int KD, int NT, int RG>
+template <bool BF16, int KD, bool FULL, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const PagedArgs a) {
   using C = Cfg<KD, NT, RG>;
-  constexpr int NP = C::NP, KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
+  constexpr int KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
   constexpr int H = KW / 16;           // 16-key halves of a step
-  constexpr int CHUNKS = NP * 8;       // 16-byte chunks of a row
-  constexpr int PANEL = KW * 128;
-  constexpr int K_BYTES = NP * PANEL;
+  constexpr int K_BYTES = KW * C::DP * 2;
   constexpr uint32_t ALL = KW == 32 ? 0xffffffffu : 0xffffu;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -264,6 +277,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   load = work;
 
   // ---- loads: lane r (of KW) looks up key r of the team's share of a tile
+  const int block_bytes = FULL ? KD * 512 : a.block_bytes;
+  auto tile_offset = [&](int r, int c) { return tile_at(r, c, FULL ? 8 : a.width, block_bytes); };
   struct Place {
     uint32_t page, row;
     int h;
@@ -285,15 +300,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     uint64_t* bar = &full[team][stage];
     if (lane == 0) {
       seen_s[team][stage] = seen;
-      kf::mbar_arrive_expect_tx(bar, (uint32_t)(__popc(boxes) * a.box) * (NP * 128 * 2));
+      kf::mbar_arrive_expect_tx(bar, (uint32_t)(__popc(boxes) * a.box_bytes));
     }
     __syncwarp();
     if (starts_box) {
-      uint8_t* st = ring + stage * C::STAGE + lane * 128;
-#pragma unroll
-      for (int pn = 0; pn < NP; ++pn) {
-        kf::tma_load_4d(st + pn * PANEL, &map_k, bar, pn * 64, p.row, p.h, p.page);
-        kf::tma_load_4d(st + K_BYTES + pn * PANEL, &map_v, bar, pn * 64, p.row, p.h, p.page);
+      uint8_t* st = ring + stage * C::STAGE + (lane >> 4) * block_bytes + (lane & 15) * a.row_bytes;
+      kf::tma_load_5d(st, &map_k, bar, 0, p.row, 0, p.h, p.page);
+      kf::tma_load_5d(st + K_BYTES, &map_v, bar, 0, p.row, 0, p.h, p.page);
+      if (KD == 8 && a.box_ops == 2) {  // the second 64-column panel
+        kf::tma_load_5d(st + 2048, &map_k, bar, 64, p.row, 0, p.h, p.page);
+        kf::tma_load_5d(st + K_BYTES + 2048, &map_v, bar, 64, p.row, 0, p.h, p.page);
       }
     }
   };
@@ -304,13 +320,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // 2^(x - m), their sum, and m again as it enters the exponent (0 for -inf)
   float m_run[NT][2], l_run[NT][2], mu[NT][2];
   float ot[NT][KD][4];                 // O^T
-  // offsets of a lane's ldmatrix rows in a K or V panel, by 16-column step mod 4
-  uint32_t k_off[4], v_off[4];
+  // offsets of a lane's ldmatrix rows in a K or V tile, by 16-column step (mod
+  // 4 in panels); in a dense tile a step's missing second half repeats its first
+  constexpr int OFFSETS = FULL ? 4 : KD;
+  uint32_t k_off[OFFSETS], v_off[OFFSETS];
 #pragma unroll
-  for (int x = 0; x < 4; ++x) {
-    k_off[x] = swz(lane & 15, 2 * x + (lane >> 4), KW);
-    v_off[x] = swz((lane & 7) + ((lane >> 4) << 3), 2 * x + ((lane >> 3) & 1), KW);
+  for (int x = 0; x < OFFSETS; ++x) {
+    const int last = FULL ? KD * 2 - 1 : a.D / 8 - 1;
+    k_off[x] = tile_offset(lane & 15, min(2 * x + (lane >> 4), last));
+    v_off[x] = tile_offset((lane & 7) + ((lane >> 4) << 3), min(2 * x + ((lane >> 3) & 1), last));
   }
+  auto at = [&](const uint32_t (&off)[OFFSETS], int step, int h) -> uint32_t {
+    if constexpr (FULL)
+      return off[step & 3] + (step >> 2) * 2048 + h * (KD * 512);
+    else
+      return off[step] + h * block_bytes;
+  };
   // (the loads of Q; sign_unit() follows where they are first needed)
   auto start_unit = [&]() {
 #pragma unroll
@@ -341,6 +366,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   };
 
   start_unit();  // ahead of the K/V loads, behind which its own would queue
+  // Tiles loaded ahead of the one in use
+  // (short units drain the ring at each end and want all of it; for the rest a
+  // third, 64 KB per SM, is what HBM needs, and more only queues: blocks then
+  // get unequal shares of the bandwidth and end far apart.  D = 128, 8192 keys:
+  // 174 -> 165 us; 400 keys: 77.5 us deep, 79.4 shallow)
+  const int depth = a.shallow && total >= 16u * a.B ? STAGES / 3 : STAGES - 1;
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
@@ -349,15 +380,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     Place first[STAGES - 1];
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      if (s < n) {
+      if (s < min(n, depth)) {
         if (s > 0) load.next(a);
         first[s] = look_up();
       }
     }
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s)
-      if (s < n) issue(s, first[s]);
-    issued = min(n, STAGES - 1);
+      if (s < min(n, depth)) issue(s, first[s]);
+    issued = min(n, depth);
     if (issued < n) {
       load.next(a);
       ahead = look_up();
@@ -368,7 +399,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   clear_empty();
   sign_unit();
 
-  int stage = 0, fill = STAGES - 1;
+  int stage = 0, fill = depth;
   uint32_t parity = 0;
   bool alive = true;                   // false once a wait of this block has expired
   int i = 0;
@@ -398,9 +429,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       // The end of a request or pages without a table entry.  Rows that nobody
       // sees hold anything: their scores are replaced below, their V rows must
       // be zero.  A new row takes its place here and goes to its page.
-      for (int idx = rg * 32 + lane; idx < KW * CHUNKS; idx += RG * 32) {
-        const int r = idx / CHUNKS, c = idx % CHUNKS;
-        if (!((seen >> r) & 1)) *reinterpret_cast<uint4*>(vt + swz(r, c, KW)) = make_uint4(0, 0, 0, 0);
+      for (int idx = rg * 32 + lane; idx < KW * 16; idx += RG * 32) {
+        const int r = idx / 16, c = idx % 16;
+        if (c < a.D / 8 && !((seen >> r) & 1)) *reinterpret_cast<uint4*>(vt + tile_offset(r, c)) = make_uint4(0, 0, 0, 0);
       }
       const uint32_t r = (uint32_t)a.lengths[work.b] - 1 - key0;
       if (a.nk && r < (uint32_t)KW && ((seen >> r) & 1) && a.slots[work.b] >= 0) {
@@ -413,7 +444,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           uint16_t* dst = lane < 16 ? a.k + page * a.ks[0] + work.h * a.ks[1] + row * a.ks[2]
                                     : a.v + page * a.vs[0] + work.h * a.vs[1] + row * a.vs[2];
           const uint4 x = reinterpret_cast<const uint4*>(src)[c];
-          *reinterpret_cast<uint4*>((lane < 16 ? kt : vt) + swz(r, c, KW)) = x;
+          *reinterpret_cast<uint4*>((lane < 16 ? kt : vt) + tile_offset(r, c)) = x;
           if (work.rb == 0) reinterpret_cast<uint4*>(dst)[c] = x;
         }
       }
@@ -441,14 +472,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int x = 0; x < KG && k0 + x < KD; ++x)
 #pragma unroll
           for (int h = 0; h < H; ++h)
-            kf::ldmatrix_x4(ka[x][h], sk + k_off[(k0 + x) & 3] + ((k0 + x) >> 2) * PANEL + h * 2048);
+            if (FULL || (k0 + x) * 16 < a.D) kf::ldmatrix_x4(ka[x][h], sk + at(k_off, k0 + x, h));
 #pragma unroll
-        for (int x = 0; x < KG && k0 + x < KD; ++x)
+        for (int x = 0; x < KG && k0 + x < KD; ++x) {
+          if (FULL || (k0 + x) * 16 + 8 < a.D) {
 #pragma unroll
-          for (int h = 0; h < H; ++h)
+            for (int h = 0; h < H; ++h)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-              kf::mma_16816<BF16>(cc[x % CHAINS][h][nt], ka[x][h], qb[nt][k0 + x][0], qb[nt][k0 + x][1]);
+              for (int nt = 0; nt < NT; ++nt)
+                kf::mma_16816<BF16>(cc[x % CHAINS][h][nt], ka[x][h], qb[nt][k0 + x][0], qb[nt][k0 + x][1]);
+          } else if ((k0 + x) * 16 < a.D) {
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt)
+                kf::mma_1688<BF16>(cc[x % CHAINS][h][nt], ka[x][h][0], ka[x][h][1], qb[nt][k0 + x][0]);
+          }
+        }
       }
       float (&c)[H][NT][4] = cc[0];
       if constexpr (CHAINS == 2) {
@@ -531,15 +571,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           uint32_t va[VG][4];
 #pragma unroll
           for (int x = 0; x < VG && d0 + x < KD; ++x)
-            kf::ldmatrix_x4_trans(va[x], sv + v_off[(d0 + x) & 3] + ((d0 + x) >> 2) * PANEL + h * 2048);
+            if (FULL || (d0 + x) * 16 < a.D) kf::ldmatrix_x4_trans(va[x], sv + at(v_off, d0 + x, h));
 #pragma unroll
           for (int x = 0; x < VG && d0 + x < KD; ++x)
+            if (FULL || (d0 + x) * 16 < a.D) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pb[h][nt][0], pb[h][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pb[h][nt][0], pb[h][nt][1]);
+            }
 #pragma unroll
           for (int x = 0; x < VG && d0 + x < KD; ++x)
+            if (FULL || (d0 + x) * 16 < a.D) {
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pl[h][nt][0], pl[h][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pl[h][nt][0], pl[h][nt][1]);
+            }
         }
     }
     if (++stage == STAGES) {
@@ -762,17 +806,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
 int unit_rows(int64_t G) { return G <= 8 ? 8 : G <= 16 ? 16 : G <= 32 ? 32 : 64; }
 
 // Keys per tile of the variant (Cfg::TILE).
-int tile_keys(int64_t D, int rows) { return rows <= 16 ? (D <= 64 ? 128 : 64) : rows == 32 ? 64 : 32; }
+int tile_keys(int64_t D, bool wide, int rows) {
+  return rows <= 16 ? (D <= 64 || (D <= 96 && !wide) ? 128 : 64) : rows == 32 ? 64 : 32;
+}
 
 size_t workspace_need(int blocks, int rows, int64_t D) {
   return 256 + (size_t)blocks * (16 + (size_t)2 * rows * 4 + (size_t)2 * rows * D * 4);
 }
 
-template <bool BF16, int KD, int NT, int RG>
+template <bool BF16, int KD, bool FULL, int NT, int RG>
 int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
   using C = Cfg<KD, NT, RG>;
-  static_assert(C::STAGES >= 3, "the ring needs three stages");
-  auto kern = paged_decode_kernel<BF16, KD, NT, RG>;
+  static_assert(C::STAGES >= 2, "the ring needs two stages");
+  auto kern = paged_decode_kernel<BF16, KD, FULL, NT, RG>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
     (void)cudaGetLastError();
     return kf::set_error(KF_ERR_CUDA, "kf_paged_decode: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -780,14 +826,14 @@ int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap&
   return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged_decode", mk, mv, a);
 }
 
-template <bool BF16, int KD>
+template <bool BF16, int KD, bool FULL>
 int dispatch_rows(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
                   cudaStream_t st) {
   switch (rows) {
-    case 8: return launch_variant<BF16, KD, 1, 1>(a, mk, mv, blocks, st);
-    case 16: return launch_variant<BF16, KD, 2, 1>(a, mk, mv, blocks, st);
-    case 32: return launch_variant<BF16, KD, 2, 2>(a, mk, mv, blocks, st);
-    default: return launch_variant<BF16, KD, 2, 4>(a, mk, mv, blocks, st);
+    case 8: return launch_variant<BF16, KD, FULL, 1, 1>(a, mk, mv, blocks, st);
+    case 16: return launch_variant<BF16, KD, FULL, 2, 1>(a, mk, mv, blocks, st);
+    case 32: return launch_variant<BF16, KD, FULL, 2, 2>(a, mk, mv, blocks, st);
+    default: return launch_variant<BF16, KD, FULL, 2, 4>(a, mk, mv, blocks, st);
   }
 }
 
@@ -883,9 +929,26 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
   kf::division(page_size, &a.page_mul, &a.page_shift);
-  // boxes never cross a page nor a team's 16 or 32 keys
-  a.box = 16;
+  // Boxes of 16 rows (32 where one panel or no swizzle holds a row) never cross
+  // a page nor a team's keys; smaller ones where 16 does not divide the pages.
+  const bool full = D == 64 || D == 128, odd = D % 16 != 0;
+  a.box = D == 64 || odd ? (D <= 96 || rows > 16 ? 32 : 16) : 16;
   while (page_size % a.box) a.box /= 2;
+  if (full || a.box < (odd ? 8 : 16)) {
+    a.width = 8;
+  } else {
+    a.width = odd ? 0 : D % 32 == 0 ? 4 : 2;
+  }
+  const bool wide = a.width == 8;
+  const int cols = wide ? 64 : a.width ? a.width * 8 : (int)D;
+  // boxes of 16 rows bring all panels at once
+  const int panels = wide ? (D == 128 && a.box == 16 ? 2 : 1) : (int)D / cols;
+  a.box_ops = wide && D > 64 && panels == 1 ? 2 : 1;
+  a.block_bytes = wide ? (D <= 64 ? 2048 : 4096) : (int)D * 32;
+  a.row_bytes = wide ? 128 : (int)D * 2;
+  a.box_bytes = a.box * (a.block_bytes / 16) * 2;
+  a.shallow = full;
+
   // A negative scale is taken as -q and a positive one, so that the largest
   // product is the largest score; 0 as a scale that no product survives, so
   // that a masked -inf stays -inf.
@@ -894,7 +957,7 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.
   // A unit of one tile is never cut, so nothing is left to join.
-  const int64_t tile = tile_keys(D, rows), most = (a.capacity + tile - 1) / tile;
+  const int64_t tile = tile_keys(D, wide, rows), most = (a.capacity + tile - 1) / tile;
   const int64_t units = B * Hkv * a.row_blocks;
   int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
   if (units * most > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
@@ -914,21 +977,27 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
     a.join_units = units < blocks;  // whichever list is shorter
   }
   CUtensorMap mk, mv;
-  int rc = kf::encode_tmap_4d(&mk, k_pages, 64, a.box);
+  int rc = kf::encode_tmap_pages(&mk, k_pages, cols, a.box, panels, a.width != 0);
   if (rc != KF_OK) return rc;
-  rc = kf::encode_tmap_4d(&mv, v_pages, 64, a.box);
+  rc = kf::encode_tmap_pages(&mv, v_pages, cols, a.box, panels, a.width != 0);
   if (rc != KF_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(args->stream);
   const bool bf16 = dtype == KF_BF16;
-  if (D <= 64)
-    rc = bf16 ? dispatch_rows<true, 4>(a, mk, mv, rows, (int)blocks, st)
-              : dispatch_rows<false, 4>(a, mk, mv, rows, (int)blocks, st);
-  else if (D <= 96)
-    rc = bf16 ? dispatch_rows<true, 6>(a, mk, mv, rows, (int)blocks, st)
-              : dispatch_rows<false, 6>(a, mk, mv, rows, (int)blocks, st);
+  if (D == 64)
+    rc = bf16 ? dispatch_rows<true, 4, true>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 4, true>(a, mk, mv, rows, (int)blocks, st);
+  else if (D == 128)
+    rc = bf16 ? dispatch_rows<true, 8, true>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 8, true>(a, mk, mv, rows, (int)blocks, st);
+  else if (D < 64)
+    rc = bf16 ? dispatch_rows<true, 4, false>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 4, false>(a, mk, mv, rows, (int)blocks, st);
+  else if (D <= 96 && !wide)
+    rc = bf16 ? dispatch_rows<true, 6, false>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 6, false>(a, mk, mv, rows, (int)blocks, st);
   else
-    rc = bf16 ? dispatch_rows<true, 8>(a, mk, mv, rows, (int)blocks, st)
-              : dispatch_rows<false, 8>(a, mk, mv, rows, (int)blocks, st);
+    rc = bf16 ? dispatch_rows<true, 8, false>(a, mk, mv, rows, (int)blocks, st)
+              : dispatch_rows<false, 8, false>(a, mk, mv, rows, (int)blocks, st);
   if (rc != KF_OK || most == 1) return rc;
   // Groups that share a row: as many as leave each about one batch of the
   // partials that a unit has on average (2 where units outnumber the blocks).

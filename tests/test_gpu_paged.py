@@ -100,6 +100,19 @@ def test_ragged_batches_against_the_oracle(hq, hkv, d, dtype, page):
     assert torch.equal(out, again)  # the same sums in the same order, with and without the LSE
 
 
+@pytest.mark.parametrize("d", range(16, 129, 8))
+@pytest.mark.parametrize("page", [4, 8, 16, 32])
+def test_every_head_dim_and_tile_layout(d, page):
+    """Every way a tile lies in shared memory: panels of 64, 32 and 16 columns,
+    dense rows, boxes of 4 to 32 rows, both team shapes."""
+    lens = [33, 1, 150, 260]
+    for hq, dtype in ((6, torch.bfloat16), (40, torch.float16)):
+        k, v, table, lengths = _pool(lens, page, 2, d, dtype, 200 + d + page)
+        q = _rand((len(lens), hq, 1, d), dtype, 201, 1.5)
+        out, lse = paged_attention(q, k, v, table, lengths, return_lse=True)
+        _check(out, lse, q, k, v, table, lengths, d ** -0.5, f"layout {d},{page},{hq}")
+
+
 @pytest.mark.parametrize("hq,hkv,d,dtype,page,lens", [
     (8, 2, 64, torch.float16, 64, [30000, 12345]),         # few requests: many partials to join
     (4, 1, 128, torch.bfloat16, 16, [20011]),
