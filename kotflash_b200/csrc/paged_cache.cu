@@ -19,8 +19,9 @@ namespace {
 
 // ---------------------------------------------------------------- append
 // Pure data movement: 2 x Hkv x D elements read and written per token, no
-// arithmetic, so HBM (or, for one token per request, latency) bounds it.  A
-// thread keeps one 16-byte column of a token's Hkv * D elements and walks
+// arithmetic, so HBM (or, for one token per request, latency) bounds it: 16384
+// tokens of 8 x 128 take 22.7 us, 90% of the measured copy rate.  A thread
+// keeps one 16-byte column of a token's Hkv * D elements and walks
 // over tokens, so the division that finds (head, column) is done once; U
 // tokens are loaded before the first is stored.
 constexpr int kAppendThreads = 256;
@@ -116,8 +117,11 @@ bool vec_ok(const kf_tensor4* t) {
 // itself (reading 8 bytes per request is cheaper than a second launch), takes
 // its share of the writes, and the cluster barrier lets block 0 replace the
 // lengths and the stack count in place once nobody reads the old ones.
-constexpr int kTableThreads = 512;
-constexpr int kTableWarps = kTableThreads / 32;
+// Blocks of kSmall threads, whose barriers and scans are quicker, for what one
+// such block passes over once or a few times (256 single tokens: 3.5 us with
+// 512 threads, 3.6 with 256, 4.3 with 1024), else of kLarge (122377 prompt
+// tokens: 14.4 us with 512 threads, 12.0 with 1024).
+constexpr int kSmall = 512, kLarge = 1024;
 constexpr int kMaxCluster = 8;
 constexpr int64_t kMaxRequests = 16384;  // 12 bytes of shared memory each
 
@@ -135,8 +139,10 @@ __device__ __forceinline__ int32_t saturate(int64_t x) { return x > 0x7fffffff ?
 
 // Inclusive sums of x and y over the block's threads; every thread also gets
 // the block's totals.  `part` is reused by the next call.
+template <int THREADS>
 __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*part)[2], int64_t& x_total,
                                            int64_t& y_total) {
+  constexpr int WARPS = THREADS / 32;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -153,17 +159,17 @@ __device__ __forceinline__ void block_scan(int64_t& x, int64_t& y, int64_t (*par
   }
   __syncthreads();
   // every warp sums the warps' totals itself: lane w holds warp w's
-  int64_t u = lane < kTableWarps ? part[lane][0] : 0, v = lane < kTableWarps ? part[lane][1] : 0;
+  int64_t u = lane < WARPS ? part[lane][0] : 0, v = lane < WARPS ? part[lane][1] : 0;
 #pragma unroll
-  for (int off = 1; off < kTableWarps; off <<= 1) {
+  for (int off = 1; off < WARPS; off <<= 1) {
     const int64_t p = __shfl_up_sync(0xffffffffu, (long long)u, off), q = __shfl_up_sync(0xffffffffu, (long long)v, off);
     if (lane >= off) {
       u += p;
       v += q;
     }
   }
-  x_total = __shfl_sync(0xffffffffu, (long long)u, kTableWarps - 1);
-  y_total = __shfl_sync(0xffffffffu, (long long)v, kTableWarps - 1);
+  x_total = __shfl_sync(0xffffffffu, (long long)u, WARPS - 1);
+  y_total = __shfl_sync(0xffffffffu, (long long)v, WARPS - 1);
   const int64_t x_before = __shfl_sync(0xffffffffu, (long long)u, warp > 0 ? warp - 1 : 0);
   const int64_t y_before = __shfl_sync(0xffffffffu, (long long)v, warp > 0 ? warp - 1 : 0);
   if (warp > 0) {
@@ -208,12 +214,13 @@ struct ReserveArgs {
 // sum of need.  A request is granted when it fits and upto_b <= free_count (or
 // it needs no page); the granted requests that need pages are then a prefix,
 // so request b takes the stack entries free_count - 1 - (upto_b - need_b) - j.
-__global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const ReserveArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* starts = sm;               // [B + 1] first token of each request
   int32_t* first = sm + a.B + 1;      // [B] pages taken by the requests before it
   int32_t* held = first + a.B;        // [B] its length so far, or -1 where it is refused
-  __shared__ int64_t part[kTableWarps][2];
+  __shared__ int64_t part[THREADS / 32][2];
   __shared__ int taken_s;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
   count = count < 0 ? 0 : (uint32_t)count > a.num_pages ? (int32_t)a.num_pages : count;
 
   int64_t tokens = 0, pages = 0;  // of the requests of earlier rounds
-  for (int base = 0; base < a.B; base += kTableThreads) {
+  for (int base = 0; base < a.B; base += THREADS) {
     const int b = base + tid;
     uint32_t len = 0, add = 0;
     if (b < a.B) {
@@ -237,7 +244,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
     const bool fits = after <= a.max_pages && (a.padded == 0 || add <= a.padded);
     const int64_t need = fits ? after - before : 0;
     int64_t add_upto = add, upto = need, add_total, need_total;
-    block_scan(add_upto, upto, part, add_total, need_total);
+    block_scan<THREADS>(add_upto, upto, part, add_total, need_total);
     add_upto += tokens;
     upto += pages;
     if (b < a.B) {
@@ -264,9 +271,9 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
   // single tokens is one pass of independent lookups, or four where there are
   // more tokens than threads; along a run it moves from row to row and looks
   // a page up only where one begins.
-  const int64_t threads = (int64_t)blocks * kTableThreads;
+  const int64_t threads = (int64_t)blocks * THREADS;
   const int run = a.T > threads ? 4 : 1;
-  for (int64_t t0 = ((int64_t)rank * kTableThreads + tid) * run; t0 < a.T; t0 += threads * run) {
+  for (int64_t t0 = ((int64_t)rank * THREADS + tid) * run; t0 < a.T; t0 += threads * run) {
     int64_t slot[4];
     int b = last_at_most(starts, a.B, t0);
     int64_t base = -1;
@@ -311,18 +318,18 @@ __global__ void __launch_bounds__(kTableThreads) paged_reserve_kernel(const Rese
   // New entries of the block table: stack entry count - 1 - p is the p-th page
   // taken.  From the far end of the threads, which a short list of tokens
   // leaves free.
-  for (int64_t p = threads - 1 - ((int64_t)rank * kTableThreads + tid); p < taken; p += threads) {
+  for (int64_t p = threads - 1 - ((int64_t)rank * THREADS + tid); p < taken; p += threads) {
     const int b = last_at_most(first, a.B, p);
     a.table[b * a.table_stride + a.div.pages((uint32_t)held[b]) + (p - first[b])] = a.free_pages[count - 1 - p];
   }
   // lengths_out and free_count_out may be lengths and free_count themselves
   cluster.sync();
   if (rank == 0) {
-    for (int b = tid; b < a.B; b += kTableThreads) {
+    for (int b = tid; b < a.B; b += THREADS) {
       const int32_t len = held[b];
       a.lengths_out[b] = len < 0 ? max(a.lengths[b], 0) : len + max(a.added[b], 0);
     }
-    for (int b = tid; b <= a.B; b += kTableThreads) a.starts[b] = starts[b];
+    for (int b = tid; b <= a.B; b += THREADS) a.starts[b] = starts[b];
     if (tid == 0) *a.free_count_out = count - taken;
   }
 }
@@ -348,10 +355,11 @@ struct ReleaseArgs {
 // request stay in registers from the count to the write.
 constexpr int kKept = 16;
 
-__global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const ReleaseArgs a) {
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) paged_release_kernel(const ReleaseArgs a) {
   extern __shared__ int32_t sm[];
   int32_t* counts = sm;  // [B] valid pages of each request, then their exclusive sum
-  __shared__ int64_t part[kTableWarps][2];
+  __shared__ int64_t part[THREADS / 32][2];
   cg::cluster_group cluster = cg::this_cluster();
   cluster.barrier_arrive();  // this block has started: its shared memory may be written
   kf::griddep_wait();
@@ -365,10 +373,10 @@ __global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const Rele
     const int32_t len = a.lengths[b];
     return a.finished[b] ? min(a.div.pages((uint32_t)max(len, 0)), a.max_pages) : 0;
   };
-  const int b0 = (int)rank * kTableWarps + warp;  // this warp's first request
+  const int b0 = (int)rank * (THREADS / 32) + warp;  // this warp's first request
   uint32_t kept[kKept];
   bool waited = false;
-  for (int b = b0; b < a.B; b += blocks * kTableWarps) {
+  for (int b = b0; b < a.B; b += blocks * (THREADS / 32)) {
     const uint32_t n = row_pages(b);
     const int32_t* row = a.table + b * a.table_stride;
     int c = 0;
@@ -390,16 +398,16 @@ __global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const Rele
   if (!waited) cluster.barrier_wait();
   cluster.sync();
   int64_t total = 0;
-  for (int base = 0; base < a.B; base += kTableThreads) {
+  for (int base = 0; base < a.B; base += THREADS) {
     const int b = base + tid;
     const int32_t c = b < a.B ? counts[b] : 0;
     int64_t upto = c, none = 0, round, unused;
-    block_scan(upto, none, part, round, unused);
+    block_scan<THREADS>(upto, none, part, round, unused);
     if (b < a.B) counts[b] = saturate(total + upto - c);
     total += round;
   }
   __syncthreads();
-  for (int b = b0; b < a.B; b += blocks * kTableWarps) {
+  for (int b = b0; b < a.B; b += blocks * (THREADS / 32)) {
     const uint32_t n = row_pages(b);
     const int32_t* row = a.table + b * a.table_stride;
     int64_t at = (int64_t)count + counts[b];
@@ -430,7 +438,7 @@ __global__ void __launch_bounds__(kTableThreads) paged_release_kernel(const Rele
   }
   cluster.sync();
   if (rank == 0) {
-    for (int b = tid; b < a.B; b += kTableThreads) a.lengths_out[b] = a.finished[b] ? 0 : max(a.lengths[b], 0);
+    for (int b = tid; b < a.B; b += THREADS) a.lengths_out[b] = a.finished[b] ? 0 : max(a.lengths[b], 0);
     if (tid == 0) *a.free_count_out = (int32_t)min((int64_t)a.num_pages, count + total);
   }
 }
@@ -534,7 +542,10 @@ extern "C" int kf_paged_append(const kf_paged_append_args* args) {
     return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kAppendThreads), 0, st, "kf_paged_append", a);
   };
   if (!vec) return go(paged_append_kernel<1, 1>, side);
-  return a.T >= side * 4 * sms * 2 ? go(paged_append_kernel<8, 4>, side * 4) : go(paged_append_kernel<8, 1>, side);
+  // Four tokens a thread in flight once that still leaves three blocks per SM
+  // (4096 tokens of 8 x 128: 7.1 us with one, 6.5 with four; 20000 of 1 x 128:
+  // 4.2 with one, 5.4 with four).
+  return a.T >= side * 4 * sms * 3 ? go(paged_append_kernel<8, 4>, side * 4) : go(paged_append_kernel<8, 1>, side);
 }
 
 extern "C" int kf_paged_reserve(const kf_paged_reserve_args* args) {
@@ -573,10 +584,12 @@ extern "C" int kf_paged_reserve(const kf_paged_reserve_args* args) {
   a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
   const size_t smem = (size_t)(3 * t.B + 1) * 4;
-  rc = raise_smem(paged_reserve_kernel, smem, what);
+  const bool large = t.B > kSmall || num_tokens > 4 * kSmall;
+  const unsigned cluster = large ? cluster_for(num_tokens, kLarge * 4) : 1;
+  auto kern = large ? paged_reserve_kernel<kLarge> : paged_reserve_kernel<kSmall>;
+  rc = raise_smem(kern, smem, what);
   if (rc != KF_OK) return rc;
-  const unsigned cluster = cluster_for(num_tokens, kTableThreads * 4);
-  return kf::launch_dependent_cluster(paged_reserve_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
+  return kf::launch_dependent_cluster(kern, cluster, dim3(cluster), dim3(large ? kLarge : kSmall), smem,
                                       static_cast<cudaStream_t>(t.stream), what, a);
 }
 
@@ -603,9 +616,11 @@ extern "C" int kf_paged_release(const kf_paged_release_args* args) {
   a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
   const size_t smem = (size_t)t.B * 4;
-  rc = raise_smem(paged_release_kernel, smem, what);
+  const bool large = t.B > kSmall / 32;  // a warp per request
+  const unsigned cluster = large ? cluster_for(t.B, kLarge / 32) : 1;
+  auto kern = large ? paged_release_kernel<kLarge> : paged_release_kernel<kSmall>;
+  rc = raise_smem(kern, smem, what);
   if (rc != KF_OK) return rc;
-  const unsigned cluster = cluster_for(t.B, kTableWarps);
-  return kf::launch_dependent_cluster(paged_release_kernel, cluster, dim3(cluster), dim3(kTableThreads), smem,
+  return kf::launch_dependent_cluster(kern, cluster, dim3(cluster), dim3(large ? kLarge : kSmall), smem,
                                       static_cast<cudaStream_t>(t.stream), what, a);
 }

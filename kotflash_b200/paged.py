@@ -25,6 +25,7 @@ from __future__ import annotations
 
 import math
 from functools import lru_cache
+from operator import index as _whole
 from typing import Optional, Tuple, Union
 
 import torch
@@ -276,19 +277,19 @@ def append_paged_kv(
         _ext.check(rc, "kf_paged_append")
 
 
-def _tables_good(lengths, second, block_table, free_pages, free_count, lengths_out, free_count_out) -> bool:
+def _tables_good(index, lengths, second, block_table, free_pages, free_count, lengths_out, free_count_out) -> bool:
     try:
-        index = lengths.get_device()
         shape = lengths.shape
         return (
-            index >= 0 and _is_sm100(index) and lengths.dtype is _INT32 and block_table.dtype is _INT32
-            and free_pages.dtype is _INT32 and free_count.dtype is _INT32 and len(shape) == 1
-            and second.shape == shape and block_table.ndim == 2 and block_table.shape[0] == shape[0]
-            and block_table.stride(1) == 1 and free_pages.ndim == 1 and free_count.numel() == 1
-            and lengths.is_contiguous() and second.is_contiguous() and free_pages.is_contiguous()
-            and second.get_device() == index and block_table.get_device() == index
-            and free_pages.get_device() == index and free_count.get_device() == index
-            and (lengths_out is None or lengths_out is lengths) and (free_count_out is None or free_count_out is free_count)
+            index >= 0 and second.get_device() == index and block_table.get_device() == index
+            and free_pages.get_device() == index and free_count.get_device() == index and _is_sm100(index)
+            and lengths.dtype is _INT32 and block_table.dtype is _INT32 and free_pages.dtype is _INT32
+            and free_count.dtype is _INT32 and lengths.dim() == 1 and second.shape == shape
+            and block_table.dim() == 2 and block_table.shape[0] == shape[0] and block_table.stride(1) == 1
+            and free_pages.dim() == 1 and free_count.numel() == 1 and lengths.is_contiguous()
+            and second.is_contiguous() and free_pages.is_contiguous()
+            and (lengths_out is None or lengths_out is lengths)
+            and (free_count_out is None or free_count_out is free_count)
         )
     except (AttributeError, TypeError, RuntimeError):
         return False
@@ -344,21 +345,23 @@ def reserve_pages(
     slots begin; the new lengths and count.  lengths_out=lengths and free_count_out=free_count update in place.
     """
     what = "reserve_pages"
-    _check_int32(what, new_lengths=new_lengths)
-    if not _tables_good(lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out):
+    index = lengths.get_device() if isinstance(lengths, torch.Tensor) else -1
+    if not _tables_good(index, lengths, new_lengths, block_table, free_pages, free_count, lengths_out,
+                        free_count_out) or new_lengths.dtype is not _INT32:
+        _check_int32(what, new_lengths=new_lengths)
         _check_tables(what, lengths, new_lengths, block_table, free_pages, free_count, lengths_out, free_count_out)
     b = lengths.shape[0]
     if (num_tokens is None) == (tokens_per_request is None):
         raise ValueError(f"{what}: give num_tokens or tokens_per_request")
     per_request = 0
     if num_tokens is None:
-        per_request = tokens_per_request
+        per_request = _whole(tokens_per_request)
         if per_request <= 0:
             raise ValueError(f"{what}: tokens_per_request must be positive")
         num_tokens = per_request * b
-    elif num_tokens < 0:
+    elif _whole(num_tokens) < 0:
         raise ValueError(f"{what}: num_tokens must not be negative")
-    slots = torch.empty(num_tokens, dtype=torch.int64, device=lengths.device)
+    slots = lengths.new_empty(num_tokens, dtype=_INT64)
     starts = lengths.new_empty(b + 1)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
@@ -366,8 +369,8 @@ def reserve_pages(
         free_count_out = torch.empty_like(free_count)
     rc = _ext.load().kf_paged_reserve(_pack_reserve(
         lengths.data_ptr(), b, block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
-        free_count_out.data_ptr(), _raw_stream(lengths.get_device()), new_lengths.data_ptr(), slots.data_ptr(),
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), _whole(page_size), lengths_out.data_ptr(),
+        free_count_out.data_ptr(), _raw_stream(index), new_lengths.data_ptr(), slots.data_ptr(),
         num_tokens, per_request, starts.data_ptr(),
     ))
     if rc:
@@ -396,7 +399,8 @@ def release_pages(
     what = "release_pages"
     if not isinstance(finished, torch.Tensor) or finished.dtype is not _BOOL:
         raise TypeError(f"{what}: finished must be a bool tensor")
-    if not _tables_good(lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out):
+    index = lengths.get_device() if isinstance(lengths, torch.Tensor) else -1
+    if not _tables_good(index, lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out):
         _check_tables(what, lengths, finished, block_table, free_pages, free_count, lengths_out, free_count_out)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)
@@ -404,8 +408,8 @@ def release_pages(
         free_count_out = torch.empty_like(free_count)
     rc = _ext.load().kf_paged_release(_pack_release(
         lengths.data_ptr(), lengths.shape[0], block_table.data_ptr(), block_table.shape[1], block_table.stride(0),
-        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), page_size, lengths_out.data_ptr(),
-        free_count_out.data_ptr(), _raw_stream(lengths.get_device()), finished.data_ptr(),
+        free_pages.data_ptr(), free_pages.shape[0], free_count.data_ptr(), _whole(page_size), lengths_out.data_ptr(),
+        free_count_out.data_ptr(), _raw_stream(index), finished.data_ptr(),
     ))
     if rc:
         _ext.check(rc, "kf_paged_release")
