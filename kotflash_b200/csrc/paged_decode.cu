@@ -336,36 +336,39 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     else
       return off[step] + h * block_bytes;
   };
-  // (the loads of Q; sign_unit() follows where they are first needed)
-  auto start_unit = [&]() {
+  // The loads of the unit's Q, issued where they are written: early, since they
+  // queue behind the K/V loads in flight.  start_unit() follows where the unit
+  // begins.
+  auto load_q = [&]() {
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
       const int row = work.rb * C::ROWS + rg * NT * 8 + nt * 8 + (lane >> 2);
       const uint16_t* src = a.q + work.b * a.qs[0] + (int64_t)(work.h * a.G + row) * a.qs[1] + 2 * (lane & 3);
 #pragma unroll
-      for (int kk = 0; kk < KD; ++kk) {
+      for (int kk = 0; kk < KD; ++kk)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
-          qb[nt][kk][e] = (row < a.G && kk * 16 + e * 8 < a.D)
-                              ? __ldg(reinterpret_cast<const uint32_t*>(src + kk * 16 + e * 8)) : 0u;
+        for (int e = 0; e < 2; ++e) {
+          qb[nt][kk][e] = 0u;
+          if (row < a.G && kk * 16 + e * 8 < a.D)
+            asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(qb[nt][kk][e]) : "l"(src + kk * 16 + e * 8));
+        }
+    }
+  };
+  auto start_unit = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int kk = 0; kk < KD; ++kk) {
+        qb[nt][kk][0] ^= a.q_sign;
+        qb[nt][kk][1] ^= a.q_sign;
         ot[nt][kk][0] = ot[nt][kk][1] = ot[nt][kk][2] = ot[nt][kk][3] = 0.f;
       }
       m_run[nt][0] = m_run[nt][1] = -INFINITY;
       l_run[nt][0] = l_run[nt][1] = mu[nt][0] = mu[nt][1] = 0.f;
     }
   };
-  auto sign_unit = [&]() {
-    if (a.q_sign == 0) return;
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int kk = 0; kk < KD; ++kk) {
-        qb[nt][kk][0] ^= a.q_sign;
-        qb[nt][kk][1] ^= a.q_sign;
-      }
-  };
 
-  start_unit();  // ahead of the K/V loads, behind which its own would queue
+  load_q();
   // Tiles loaded ahead of the one in use
   // (short units drain the ring at each end and want all of it; for the rest a
   // third, 64 KB per SM, is what HBM needs, and more only queues: blocks then
@@ -397,7 +400,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
   clear_empty();
-  sign_unit();
+  start_unit();
 
   int stage = 0, fill = depth;
   uint32_t parity = 0;
@@ -598,7 +601,19 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       continue;
     }
     // ---- join the teams and write the unit's rows (or its partial)
-    const int h = work.h, rb = work.rb;
+    const int b = work.b, h = work.h, rb = work.rb;
+    if (unit_t0 == 0 && tid == 0 && (a.join_units || !unit_done)) {
+      // a unit that begins here and goes on ends in the share of its last tile
+      const int hr = h * a.row_blocks + rb;
+      const uint32_t last = begin + i + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
+      const uint32_t end = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
+      a.joins[a.join_units ? (int64_t)b * units + hr : (int64_t)me] =
+          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)end);
+    }
+    if (i + 1 < n) {
+      work.next(a);
+      load_q();  // of the next unit: it arrives during what follows
+    }
     const bool direct = unit_t0 == 0 && unit_done;
     const int64_t slot = (int64_t)me * 2 + (unit_t0 > 0 ? 0 : 1);  // 0: began in an earlier share, 1: begins here
 #pragma unroll
@@ -670,9 +685,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         const float lse2 = L == 0.f ? -INFINITY : M + log2f(L);
         const int head = h * a.G + rb * C::ROWS + r;
         if (direct) {
-          *reinterpret_cast<uint2*>(a.o + ((int64_t)work.b * a.Hq + head) * a.D + d) =
+          *reinterpret_cast<uint2*>(a.o + ((int64_t)b * a.Hq + head) * a.D + d) =
               make_uint2(kf::pack2<BF16>(acc[0] * inv, acc[1] * inv), kf::pack2<BF16>(acc[2] * inv, acc[3] * inv));
-          if (a.lse && d == 0) a.lse[(int64_t)work.b * a.Hq + head] = lse2 * kLn2;
+          if (a.lse && d == 0) a.lse[(int64_t)b * a.Hq + head] = lse2 * kLn2;
         } else {
           *reinterpret_cast<float4*>(a.part_o + (slot * C::ROWS + r) * a.D + d) =
               make_float4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
@@ -680,19 +695,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
       }
     }
-    if (unit_t0 == 0 && tid == 0 && (a.join_units || !direct)) {
-      // a unit that begins here and goes on ends in the share of its last tile
-      const int hr = h * a.row_blocks + rb;
-      const uint32_t last = begin + i + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
-      const uint32_t end = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
-      a.joins[a.join_units ? (int64_t)work.b * units + hr : (int64_t)me] =
-          direct ? make_int4(-1, 0, 0, 0)
-                 : make_int4(work.b, hr, (int)me, (int)end);
-    }
     if (i + 1 < n) {
-      work.next(a);
       start_unit();
-      sign_unit();
       unit_t0 = 0;
     }
   }
