@@ -10,8 +10,8 @@
 // 16 bits), so HBM bounds it up to a few dozen rows per KV head.
 //
 // Work split.  A unit is (request, KV head, block of query rows); its keys
-// are cut into tiles.  All tiles of the call, unit after unit, form one list
-// that is dealt out in equal contiguous shares to a grid that fills the GPU
+// are cut into tiles.  All tiles of the call, unit after unit with a position
+// for the unit's end, form one list that is dealt out in equal contiguous shares to a grid that fills the GPU
 // once.  Each block finds its share from the lengths by a prefix sum, so
 // ragged batches are balanced without the host knowing a length (no
 // synchronisation, and a captured graph follows the lengths).  A unit that
@@ -116,21 +116,28 @@ __device__ __forceinline__ uint32_t visible(const PagedArgs& a, int b) {
   return n <= 0 ? 0u : min((uint32_t)n, a.capacity);
 }
 
-// Position in the list of tiles: tile `t` of the `tiles` of the unit (request
-// b, KV head h, row block rb).
+// A tile and its position in the list: tile `t` of the `tiles` of the unit
+// (request b, KV head h, row block rb).  A unit takes tiles + 1 positions: its
+// end (joining the teams, writing, the next unit's Q) costs about what a tile
+// does, 1.0 us where a tile takes 1.4, so a position counts as much.
 template <int TILE>
 struct Cursor {
   int b, h, rb;
-  uint32_t t, tiles, keys;
+  uint32_t t, tiles, keys, pos;
 
   __device__ __forceinline__ void set_request(const PagedArgs& a, int request) {
     b = request;
     keys = visible(a, b);
     tiles = (keys + TILE - 1) / TILE;
   }
-  // to the next tile of the list, which must exist
+  __device__ __forceinline__ bool unit_ends() const { return t + 1 == tiles; }
+  // whether another tile follows before position `end`
+  __device__ __forceinline__ bool more(uint32_t end) const { return pos + (unit_ends() ? 2 : 1) < end; }
+  // to that tile
   __device__ __forceinline__ void next(const PagedArgs& a) {
+    ++pos;
     if (++t < tiles) return;
+    ++pos;
     t = 0;
     if (++rb < a.row_blocks) return;
     rb = 0;
@@ -205,11 +212,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
-  // ---- this block's share of the list of tiles (fewer than 2^31, see the host's check)
+  // ---- this block's share of the list (of fewer than 2^31 positions, see the host's check)
   const int per = (a.B + kThreads - 1) / kThreads;  // requests per thread, contiguous
   const int b_lo = min(tid * per, a.B), b_hi = min(b_lo + per, a.B);
   uint32_t mine = 0;
-  for (int b = b_lo; b < b_hi; ++b) mine += (visible(a, b) + TILE - 1) / TILE;
+  auto positions = [&](int b) {        // of one unit of request b
+    const uint32_t keys = visible(a, b);
+    return keys == 0 ? 0u : (keys + TILE - 1) / TILE + 1;
+  };
+  for (int b = b_lo; b < b_hi; ++b) mine += positions(b);
   uint32_t upto = mine;
 #pragma unroll
   for (int off = 1; off < 32; off <<= 1) {
@@ -247,17 +258,17 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     clear_empty();
     return;
   }
-  // shares differ by one tile at most, the longer ones first
+  // shares differ by one position at most, the longer ones first
   const uint32_t even = list / shares, longer = list - even * shares;
   const uint32_t begin = me * even + min(me, longer);
-  const int n = (int)(even + (me < longer ? 1 : 0));
+  const uint32_t end = begin + even + (me < longer ? 1 : 0);
   if (begin >= (upto - mine) * units && begin < upto * units) {  // exactly one thread
     uint32_t sum = upto - mine;
     int b = b_lo;
     while (true) {
-      const uint32_t tiles = (visible(a, b) + TILE - 1) / TILE;
-      if (begin < (sum + tiles) * units) break;
-      sum += tiles;
+      const uint32_t here = positions(b);
+      if (begin < (sum + here) * units) break;
+      sum += here;
       ++b;
     }
     first_request = b;
@@ -268,11 +279,26 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   Cursor<TILE> load, work;
   work.set_request(a, first_request);
   {
-    const uint32_t at = begin - first_before * units;  // inside the request's tiles x units
-    const int hr = (int)(at / work.tiles);
-    work.t = at - hr * work.tiles;
+    const uint32_t at = begin - first_before * units;  // inside the request's units
+    const int hr = (int)(at / (work.tiles + 1));
+    work.t = at - hr * (work.tiles + 1);
     work.h = hr / a.row_blocks;
     work.rb = hr - work.h * a.row_blocks;
+    work.pos = begin;
+  }
+  bool some = true;                    // whether this share has a tile at all
+  if (work.t == work.tiles) {          // it begins with a unit's end: the first tile is the next unit's
+    some = begin + 1 < end;
+    if (some) {
+      --work.t;
+      --work.pos;
+      work.next(a);
+    }
+  }
+  if (!some) {
+    if (tid == 0 && join_blocks) a.joins[me].x = -1;
+    clear_empty();
+    return;
   }
   load = work;
 
@@ -378,24 +404,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
+  bool more = rg == 0;                 // whether the load cursor stands on a tile that is not loaded yet
   Place ahead;
   if (rg == 0) {
     Place first[STAGES - 1];
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
-      if (s < min(n, depth)) {
-        if (s > 0) load.next(a);
+      if (more && s < depth) {
         first[s] = look_up();
+        issued = s + 1;
+        more = load.more(end);
+        if (more) load.next(a);
       }
     }
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s)
-      if (s < min(n, depth)) issue(s, first[s]);
-    issued = min(n, depth);
-    if (issued < n) {
-      load.next(a);
-      ahead = look_up();
-    }
+      if (s < issued) issue(s, first[s]);
+    if (more) ahead = look_up();
   }
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
@@ -405,8 +430,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   int stage = 0, fill = depth;
   uint32_t parity = 0;
   bool alive = true;                   // false once a wait of this block has expired
-  int i = 0;
-  for (; i < n; ++i) {
+  for (bool going = true; going;) {
     // One outcome for the team: no lane reaches a collective instruction alone.
     // The barrier also says that the team has left stage i - 1.
     uint32_t seen = RG == 1 ? seen_s[team][stage] : 0u;  // (this warp's own word: read before the wait)
@@ -416,10 +440,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
     if (RG > 1) seen = seen_s[team][stage];
     if (!alive) seen = 0;
-    if (rg == 0 && alive && issued < n) {
+    if (rg == 0 && alive && more) {
       issue(fill, ahead);
       ++issued;
-      if (issued < n) {
+      more = load.more(end);
+      if (more) {
         load.next(a);
         ahead = look_up();
       }
@@ -452,6 +477,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
       }
       kf::fence_proxy_async_smem();    // before a later load into this stage
+      __syncwarp();                    // (the vote of a team of one warp orders no memory)
       team_and<RG>(team, true);
     }
     if (seen != 0) {
@@ -595,9 +621,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
     if (++fill == STAGES) fill = 0;
 
-    const bool unit_done = work.t + 1 == work.tiles;
-    if (!unit_done && i + 1 < n) {
+    const bool unit_done = work.unit_ends();
+    going = work.more(end);
+    if (!unit_done && going) {
       ++work.t;
+      ++work.pos;
       continue;
     }
     // ---- join the teams and write the unit's rows (or its partial)
@@ -605,12 +633,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (unit_t0 == 0 && tid == 0 && (a.join_units || !unit_done)) {
       // a unit that begins here and goes on ends in the share of its last tile
       const int hr = h * a.row_blocks + rb;
-      const uint32_t last = begin + i + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
-      const uint32_t end = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
+      const uint32_t last = work.pos + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
+      const uint32_t share = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
       a.joins[a.join_units ? (int64_t)b * units + hr : (int64_t)me] =
-          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)end);
+          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)share);
     }
-    if (i + 1 < n) {
+    if (going) {
       work.next(a);
       load_q();  // of the next unit: it arrives during what follows
     }
@@ -695,7 +723,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         }
       }
     }
-    if (i + 1 < n) {
+    if (going) {
       start_unit();
       unit_t0 = 0;
     }
@@ -964,8 +992,9 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   const int64_t tile = tile_keys(D, wide, rows), most = (a.capacity + tile - 1) / tile;
   const int64_t units = B * Hkv * a.row_blocks;
   int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
-  if (units * most > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
-  if (units * most < blocks) blocks = units * most;
+  if (units * (most + 1) > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
+  if (most == 1 && units < blocks) blocks = units;
+  if (units * (most + 1) < blocks) blocks = units * (most + 1);
   a.part_o = nullptr;
   a.part_lse = nullptr;
   a.joins = nullptr;

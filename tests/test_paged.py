@@ -206,45 +206,54 @@ def test_workspace_grows_with_the_row_tiles():
 
 
 def _walk(lens, units, tile, grid):
-    """The kernel's walk over its list of tiles: every unit is finished once,
-    whole or from partials that cover its tiles in order and use each slot once."""
+    """The kernel's walk over its list, in which a unit has a position for each
+    tile and one for its end: every unit is finished once, whole or from
+    partials that cover its tiles in order and use each slot once."""
     tiles = [(max(0, n) + tile - 1) // tile for n in lens]
-    listed = sum(tiles) * units
-    shares = min(grid, listed)
-    flat = [(b, h, x) for b in range(len(lens)) for h in range(units) for x in range(tiles[b])]
-    done, parts, joins = set(), {}, {}
-    even, longer = (listed // shares, listed % shares) if shares else (0, 0)
+    flat = [(b, h, x) for b in range(len(lens)) if tiles[b] for h in range(units) for x in range(tiles[b] + 1)]
+    shares = min(grid, len(flat))
+    done, parts, joins, tiles_done = set(), {}, {}, set()
+    even, longer = (len(flat) // shares, len(flat) % shares) if shares else (0, 0)
     covered = 0
     for me in range(shares):
         begin = me * even + min(me, longer)
-        n = even + (1 if me < longer else 0)
-        assert n > 0 and begin == covered
-        covered += n
-        unit_t0 = flat[begin][2]
-        for i in range(n):
-            b, h, x = flat[begin + i]
-            unit_done = x + 1 == tiles[b]
-            if not unit_done and i + 1 < n:
+        end = begin + even + (1 if me < longer else 0)
+        assert end > begin == covered
+        covered = end
+        pos = begin
+        if flat[pos][2] == tiles[flat[pos][0]]:  # a unit's end comes first
+            if begin + 1 >= end:
                 continue
-            if unit_t0 == 0 and unit_done:
-                assert (b, h) not in done
-                done.add((b, h))
-            else:
-                slot = (me, 0 if unit_t0 > 0 else 1)
-                assert slot not in parts
-                parts[slot] = (b, h, unit_t0, x)
-                if unit_t0 == 0:
-                    last = begin + i + (tiles[b] - 1 - x)
-                    in_longer = longer * (even + 1)
-                    end = last // (even + 1) if last < in_longer else longer + (last - in_longer) // even
-                    joins[me] = (b, h, end)
-            unit_t0 = 0
-    assert covered == listed
-    for me, (b, h, end) in joins.items():
+            pos += 1
+        unit_t0 = flat[pos][2]
+        going = True
+        while going:
+            b, h, x = flat[pos]
+            assert x < tiles[b] and pos < end and (b, h, x) not in tiles_done
+            tiles_done.add((b, h, x))
+            unit_done = x + 1 == tiles[b]
+            following = pos + (2 if unit_done else 1)
+            going = following < end
+            if unit_done or not going:
+                if unit_t0 == 0 and unit_done:
+                    assert (b, h) not in done
+                    done.add((b, h))
+                else:
+                    slot = (me, 0 if unit_t0 > 0 else 1)
+                    assert slot not in parts
+                    parts[slot] = (b, h, unit_t0, x)
+                    if unit_t0 == 0:
+                        last = pos + (tiles[b] - 1 - x)
+                        in_longer = longer * (even + 1)
+                        joins[me] = (b, h, last // (even + 1) if last < in_longer else longer + (last - in_longer) // even)
+                unit_t0 = 0
+            pos = following
+    assert covered == len(flat) and len(tiles_done) == units * sum(tiles)
+    for me, (b, h, last_share) in joins.items():
         assert (b, h) not in done
         done.add((b, h))
         at = 0
-        for j in range(end - me + 1):
+        for j in range(last_share - me + 1):
             pb, ph, first, last = parts.pop((me + j, 1 if j == 0 else 0))
             assert (pb, ph, first) == (b, h, at)
             at = last + 1
@@ -254,8 +263,8 @@ def _walk(lens, units, tile, grid):
 
 def test_work_split_covers_every_unit_once():
     r = random.Random(0)
-    for _ in range(400):
-        lens = [r.choice([0, 1, r.randint(0, 3000)]) for _ in range(r.randint(1, 12))]
+    for _ in range(600):
+        lens = [r.choice([0, 1, r.randint(0, 100), r.randint(0, 3000)]) for _ in range(r.randint(1, 12))]
         _walk(lens, r.randint(1, 6), r.choice([32, 64, 128]), r.randint(1, 60))
 
 
