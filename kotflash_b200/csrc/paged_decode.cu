@@ -227,6 +227,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (request < (uint32_t)a.B)
       kf::prefetch_l2_bulk(a.q + request * a.qs[0] + (line - request * a.Hq) * a.qs[1], a.D * 2);
   }
+  // where things lie in a tile
+  const int block_bytes = FULL ? KD * 512 : a.block_bytes;
+  auto tile_offset = [&](int r, int c) { return tile_at(r, c, FULL ? 8 : a.width, block_bytes); };
+  // what a lane clears of an unseen row: the row's pitch, and this lane's chunk (swizzle aside) or -1
+  const int row_pitch = FULL ? 128 : a.width ? a.width * 16 : block_bytes >> 4;
+  const int zero_chunk = (lane & 15) < (block_bytes >> 8) ? (int)tile_offset(0, lane & 15) : -1;
+  // offsets of a lane's ldmatrix rows in a K or V tile, by 16-column step (mod
+  // 4 in panels); in a dense tile a step's missing second half repeats its first
+  constexpr int OFFSETS = FULL ? 4 : KD;
+  uint32_t k_off[OFFSETS], v_off[OFFSETS];
+#pragma unroll
+  for (int x = 0; x < OFFSETS; ++x) {
+    const int last = FULL ? KD * 2 - 1 : a.D / 8 - 1;
+    k_off[x] = tile_offset(lane & 15, min(2 * x + (lane >> 4), last));
+    v_off[x] = tile_offset((lane & 7) + ((lane >> 4) << 3), min(2 * x + ((lane >> 3) & 1), last));
+  }
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
@@ -321,11 +337,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   load = work;
 
   // ---- loads: lane r (of KW) looks up key r of the team's share of a tile
-  const int block_bytes = FULL ? KD * 512 : a.block_bytes;
-  auto tile_offset = [&](int r, int c) { return tile_at(r, c, FULL ? 8 : a.width, block_bytes); };
-  // what a lane clears of an unseen row: the row's pitch, and this lane's chunk (swizzle aside) or -1
-  const int row_pitch = FULL ? 128 : a.width ? a.width * 16 : block_bytes >> 4;
-  const int zero_chunk = (lane & 15) < (block_bytes >> 8) ? (int)tile_offset(0, lane & 15) : -1;
   struct Place {
     uint32_t page, row;
     int h;
@@ -367,16 +378,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // 2^(x - m), their sum, and m again as it enters the exponent (0 for -inf)
   float m_run[NT][2], l_run[NT][2], mu[NT][2];
   float ot[NT][KD][4];                 // O^T
-  // offsets of a lane's ldmatrix rows in a K or V tile, by 16-column step (mod
-  // 4 in panels); in a dense tile a step's missing second half repeats its first
-  constexpr int OFFSETS = FULL ? 4 : KD;
-  uint32_t k_off[OFFSETS], v_off[OFFSETS];
-#pragma unroll
-  for (int x = 0; x < OFFSETS; ++x) {
-    const int last = FULL ? KD * 2 - 1 : a.D / 8 - 1;
-    k_off[x] = tile_offset(lane & 15, min(2 * x + (lane >> 4), last));
-    v_off[x] = tile_offset((lane & 7) + ((lane >> 4) << 3), min(2 * x + ((lane >> 3) & 1), last));
-  }
   auto at = [&](const uint32_t (&off)[OFFSETS], int step, int h) -> uint32_t {
     if constexpr (FULL)
       return off[step & 3] + (step >> 2) * 2048 + h * (KD * 512);

@@ -235,6 +235,43 @@ def test_offsets_past_32_bits():
     _check(out, lse, q, k, v, table, lengths, d ** -0.5, "far pages")
 
 
+@pytest.mark.parametrize("seed", range(40))
+def test_random_cases(seed):
+    """Seeded draws over heads, head dims, pages, lengths, layouts, masked table
+    entries and the fused append, which must equal appending first."""
+    import random
+
+    r = random.Random(seed)
+    hkv = r.choice([1, 2, 3, 5, 8])
+    hq = hkv * r.choice([1, 2, 3, 4, 7, 8, 9, 16, 17, 33, 65][: 11 if hkv < 3 else 6])
+    d = 8 * r.randint(2, 16)
+    page = r.choice([1, 2, 3, 8, 12, 16, 16, 32, 40, 64, 128])
+    dtype = r.choice([torch.float16, torch.bfloat16])
+    top = r.choice([3, 40, 200, 1500])
+    lens = [r.choice([0, 1, top, r.randint(0, top), r.randint(0, top)]) for _ in range(r.choice([1, 2, 7, 40, 130]))]
+    if not any(lens):
+        lens[0] = top
+    k, v, table, lengths = _pool(lens, page, hkv, d, dtype, 1000 + seed)
+    if r.random() < 0.5:  # tokens outside heads
+        k = k.transpose(1, 2).contiguous().transpose(1, 2)
+    for b, n in enumerate(lens):  # some pages in the middle are given up
+        held = -(-n // page)
+        if held > 1 and r.random() < 0.3:
+            table[b, r.randrange(held - 1)] = r.choice([-1, k.shape[0], -2**31])
+    q = _rand((len(lens), hq, 1, d), dtype, 2000 + seed, r.choice([0.5, 2.0]))
+    scale = r.choice([None, None, 0.3, -0.1])
+    out, lse = paged_attention(q, k, v, table, lengths, scale=scale, return_lse=True)
+    _check(out, lse, q, k, v, table, lengths, d ** -0.5 if scale is None else scale, f"seed {seed}")
+    nk, nv = _rand((len(lens), hkv, 1, d), dtype, 3000 + seed), _rand((len(lens), hkv, 1, d), dtype, 4000 + seed)
+    slots = torch.tensor([int(table[b, (n - 1) // page]) * page + (n - 1) % page if n and r.random() < 0.8 else -1
+                          for b, n in enumerate(lens)], device="cuda")
+    k2, v2 = k.clone(), v.clone()
+    got = paged_attention(q, k2, v2, table, lengths, scale=scale, new_k=nk, new_v=nv, slots=slots)
+    append_paged_kv(k, v, nk, nv, slots)
+    assert torch.equal(got, paged_attention(q, k, v, table, lengths, scale=scale))
+    assert torch.equal(k.view(torch.int16), k2.view(torch.int16)) and torch.equal(v.view(torch.int16), v2.view(torch.int16))
+
+
 # ---------------------------------------------------------------- fused append
 
 @pytest.mark.parametrize("hq,hkv,d,dtype,page", [
