@@ -11,8 +11,8 @@
 //
 // Work split.  A unit is (request, KV head, block of query rows); its keys
 // are cut into tiles.  All tiles of the call, unit after unit with a position
-// for the unit's end, form one list that is dealt out in equal contiguous shares to a grid that fills the GPU
-// once.  Each block finds its share from the lengths by a prefix sum, so
+// for the unit's end, form one list that is dealt out in equal contiguous
+// shares to a grid that fills the GPU once.  Each block finds its share from the lengths by a prefix sum, so
 // ragged batches are balanced without the host knowing a length (no
 // synchronisation, and a captured graph follows the lengths).  A unit that
 // lies inside one share is finished there; one cut by a share's end leaves
@@ -417,12 +417,12 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   };
 
   load_q();
-  // Tiles loaded ahead of the one in use
-  // (short units drain the ring at each end and want all of it; for the rest a
-  // third, 64 KB per SM, is what HBM needs, and more only queues: blocks then
-  // get unequal shares of the bandwidth and end far apart.  D = 128, 8192 keys:
-  // 174 -> 165 us; 400 keys: 77.5 us deep, 79.4 shallow)
-  const int depth = a.shallow && total >= 16u * a.B ? STAGES / 3 : STAGES - 1;
+  // Tiles loaded ahead of the one in use.  Short units drain the ring at each
+  // end and want all of it; for the rest a third, 64 KB per SM, is what HBM
+  // needs, and more only queues: blocks then get unequal shares of the
+  // bandwidth and end far apart (D = 128, 8192 keys: 174 us deep, 165 shallow;
+  // 800 keys: 73.2 and 72.4; 400 keys: 73.8 and 75.0).
+  const int depth = a.shallow && total >= 10u * a.B ? STAGES / 3 : STAGES - 1;
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
@@ -565,8 +565,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       // The reference m of a row follows its maximum only when a score passes
       // it by 2^8: weights up to 256 lose nothing in fp32 sums and 16-bit
-      // parts, and most steps need no exchange between lanes (a step took 2240
-      // cycles with one, of which the shuffles and the rescale a quarter).
+      // parts, and most steps need no exchange between lanes (the softmax of a
+      // step: 295 -> 194 cycles of 1770 with one row tile, 558 -> 257 of
+      // 2280 with two).
       bool raise = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -816,7 +817,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
 // split-th partial; each partial is read once, with a running maximum, and the
 // groups' results meet in shared memory.
 constexpr int kJoinThreads = 256;
-constexpr int kJoinBatch = 4;  // partials a group has in flight
+constexpr int kJoinBatch = 8;  // partials a group has in flight (4: 0.3 to 0.5 us more on calls of 12 to 50 us)
 
 template <bool BF16>
 __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int rows, int split) {
