@@ -191,6 +191,14 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   constexpr int H = KW / 16;           // 16-key halves of a step
   constexpr int K_BYTES = KW * C::DP * 2;
   constexpr uint32_t ALL = KW == 32 ? 0xffffffffu : 0xffffu;
+  // The reference m of a row's weights 2^(x - m) lies BELOW under a maximum of
+  // the row and is raised once a score passes it by LIMIT.  bf16 holds small
+  // weights as well as large ones.  fp16's two parts end at 2^-24 whatever the
+  // weight, so weights use the top of its range: 2^11 at the maximum, 2^15 at
+  // most, and the parts end 2^-35 below the row's largest weight or lower.
+  // (With the maximum as the reference 32768 keys 2^25 below one that leads
+  // were lost from O and counted in the sum: 8e-4 of O.)
+  constexpr float BELOW = BF16 ? 0.f : 11.f, LIMIT = BF16 ? 8.f : 15.f;
   extern __shared__ uint8_t smem_raw[];
   // (an offset, not a rounded address: the compiler keeps seeing shared memory)
   uint8_t* smem = smem_raw + (-kf::smem_u32(smem_raw) & 1023u);
@@ -563,11 +571,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             for (int e = 0; e < 4; ++e) c[h][nt][e] = (bits & (e < 2 ? 1u : 256u)) ? c[h][nt][e] : -INFINITY;
         }
       }
-      // The reference m of a row follows its maximum only when a score passes
-      // it by 2^8: weights up to 256 lose nothing in fp32 sums and 16-bit
-      // parts, and most steps need no exchange between lanes (the softmax of a
+      // The reference of a row follows its maximum only when a score passes it
+      // by LIMIT: most steps need no exchange between lanes (the softmax of a
       // step: 295 -> 194 cycles of 1770 with one row tile, 558 -> 257 of
-      // 2280 with two).
+      // 2280 with two).  The test computes what the exponent will be, so no
+      // weight exceeds 2^LIMIT however large the scores.
       bool raise = false;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -575,7 +583,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int j = 0; j < 2; ++j) {
           float top = fmaxf(c[0][nt][j], c[0][nt][2 + j]);
           if constexpr (H == 2) top = kf::fmax3(top, c[H - 1][nt][j], c[H - 1][nt][2 + j]);
-          raise |= top * a.scale_log2 > m_run[nt][j] + 8.f;
+          raise |= fmaf(top, a.scale_log2, -m_run[nt][j]) > LIMIT;
         }
       if (__any_sync(0xffffffffu, raise)) {
 #pragma unroll
@@ -586,7 +594,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             if constexpr (H == 2) top = kf::fmax3(top, c[H - 1][nt][j], c[H - 1][nt][2 + j]);
 #pragma unroll
             for (int off = 4; off < 32; off <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-            const float m_new = fmaxf(m_run[nt][j], top * a.scale_log2);
+            const float m_new = fmaxf(m_run[nt][j], fmaf(top, a.scale_log2, -BELOW));
             mu[nt][j] = m_new == -INFINITY ? 0.f : m_new;
             const float old = kf::ex2(m_run[nt][j] - mu[nt][j]);
             m_run[nt][j] = m_new;
@@ -609,8 +617,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             p[e] = kf::ex2(fmaf(c[h][nt][e], a.scale_log2, -mu[nt][e & 1]));
             l_run[nt][e & 1] += p[e];
           }
-          // P as a 16-bit value plus the 16-bit rest: two products keep the
-          // weights at about fp32 accuracy, as a plain fp32 softmax has them
+          // P as a 16-bit value plus the 16-bit rest: two products hold a
+          // weight to 2^-16 of itself (bf16), or to 2^-21 of itself and 2^-36
+          // of the row's largest (fp16)
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
             const uint32_t hi = kf::pack2<BF16>(p[2 * x], p[2 * x + 1]);
