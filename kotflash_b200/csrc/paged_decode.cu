@@ -608,14 +608,15 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
       }
       uint32_t pb[H][NT][2], pl[H][NT][2];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[2] = {0.f, 0.f};  // of the step: fewer roundings against a large l
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           float p[4];
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             p[e] = kf::ex2(fmaf(c[h][nt][e], a.scale_log2, -mu[nt][e & 1]));
-            l_run[nt][e & 1] += p[e];
+            sum[e & 1] += p[e];
           }
           // P as a 16-bit value plus the 16-bit rest: two products hold a
           // weight to 2^-16 of itself (bf16), or to 2^-21 of itself and 2^-36
@@ -628,11 +629,23 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             pl[h][nt][x] = kf::movmatrix_trans(kf::pack2<BF16>(p[2 * x] - back.x, p[2 * x + 1] - back.y));
           }
         }
+        l_run[nt][0] += sum[0];
+        l_run[nt][1] += sum[1];
+      }
       // O^T (head dim x rows) += V^T P^T, the two parts of P apart from one
-      // another so that no product waits for the one before it
+      // another so that no product waits for the one before it.  The products
+      // of a step are summed from zero and then added: an MMA cuts each of its
+      // products off where its accumulator's digits end, which lost 4e-3 of O
+      // on 131072 keys beside one that leads by 2^23.5.  (It costs nothing up to
+      // 8 rows per KV head, 56.2 -> 58.8 us at 32: 32 requests of 16384 keys.)
       constexpr int VG = NT == 1 ? 4 : 2;
 #pragma unroll
-      for (int d0 = 0; d0 < KD; d0 += VG)
+      for (int d0 = 0; d0 < KD; d0 += VG) {
+        float step[VG][NT][4];
+#pragma unroll
+        for (int x = 0; x < VG; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) step[x][nt][0] = step[x][nt][1] = step[x][nt][2] = step[x][nt][3] = 0.f;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t va[VG][4];
@@ -643,15 +656,22 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
           for (int x = 0; x < VG && d0 + x < KD; ++x)
             if (FULL || (d0 + x) * 16 < a.D) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pb[h][nt][0], pb[h][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(step[x][nt], va[x], pb[h][nt][0], pb[h][nt][1]);
             }
 #pragma unroll
           for (int x = 0; x < VG && d0 + x < KD; ++x)
             if (FULL || (d0 + x) * 16 < a.D) {
 #pragma unroll
-              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(ot[nt][d0 + x], va[x], pl[h][nt][0], pl[h][nt][1]);
+              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<BF16>(step[x][nt], va[x], pl[h][nt][0], pl[h][nt][1]);
             }
         }
+#pragma unroll
+        for (int x = 0; x < VG && d0 + x < KD; ++x)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) ot[nt][d0 + x][e] += step[x][nt][e];
+      }
     }
     if (++stage == STAGES) {
       stage = 0;

@@ -47,3 +47,24 @@ def test_the_rest_of_a_row_that_one_key_dominates(dtype, hq, lead, place):
         want = lead * math.log(2) + math.log1p(others)
         err = (lse.double() - want).abs().max().item()
         assert err <= hold + want * 2.0 ** -22, f"LSE off by {err:.3e}"
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq", [1, 40])
+@pytest.mark.parametrize("lead", [20.0, 22.5, 23.5, 24.25, 25.25, 26.0])
+def test_many_small_weights_beside_a_large_sum(dtype, hq, lead):
+    """131072 keys beside one that leads by 2^lead, all values 1: O = 1.
+
+    Bounds: as above, with the large sum from the first tile on."""
+    n, d, page, b = 131072, 64, 64, 300
+    k = torch.zeros(n // page, 1, page, d, device="cuda", dtype=dtype)
+    k[0, 0, 5, 0] = lead
+    q = torch.zeros(b, hq, 1, d, device="cuda", dtype=dtype)
+    q[..., 0] = 1
+    table = torch.arange(n // page, dtype=torch.int32, device="cuda").expand(b, -1).contiguous()
+    lengths = torch.full((b,), n, dtype=torch.int32, device="cuda")
+    out, lse = paged_attention(q, k, torch.ones_like(k), table, lengths, scale=math.log(2), return_lse=True)
+    hold = 2.0 ** -16 + 2.0 ** -19 + (n / 16 + 64) * 2.0 ** -23
+    assert (out.double() - 1).abs().max().item() <= UNIT[dtype] + hold
+    want = lead * math.log(2) + math.log1p((n - 1) * 2.0 ** -lead)
+    assert (lse.double() - want).abs().max().item() <= hold + want * 2.0 ** -22
