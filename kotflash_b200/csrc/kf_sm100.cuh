@@ -506,6 +506,19 @@ KF_DEVI void mma_1688(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t b0) {
   }
 }
 
+// The largest 16-bit values below two positive fp32 (lo = a).
+template <bool BF16>
+KF_DEVI uint32_t pack2_below(float a, float b) {
+  const uint32_t x = __float_as_uint(a) - 1, y = __float_as_uint(b) - 1;
+  if constexpr (BF16) {
+    return __byte_perm(x, y, 0x7632);  // the upper halves: truncated
+  } else {
+    uint32_t r;
+    asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(__uint_as_float(y)), "f"(__uint_as_float(x)));
+    return r;
+  }
+}
+
 // Pack two fp32 into one 32-bit register of two 16-bit values (lo = a).
 template <bool BF16>
 KF_DEVI uint32_t pack2(float a, float b) {

@@ -195,10 +195,11 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // the row and is raised once a score passes it by LIMIT.  bf16 holds small
   // weights as well as large ones.  fp16's two parts end at 2^-24 whatever the
   // weight, so weights use the top of its range: 2^11 at the maximum, 2^15 at
-  // most, and the parts end 2^-35 below the row's largest weight or lower.
+  // most, and the parts end at 2^-35 of the row's largest weight or lower.
   // (With the maximum as the reference 32768 keys 2^25 below one that leads
   // were lost from O and counted in the sum: 8e-4 of O.)
   constexpr float BELOW = BF16 ? 0.f : 11.f, LIMIT = BF16 ? 8.f : 15.f;
+  constexpr float LEAST = BF16 ? FLT_MIN : 1.f / (1 << 24);  // of a part of a weight
   extern __shared__ uint8_t smem_raw[];
   // (an offset, not a rounded address: the compiler keeps seeing shared memory)
   uint8_t* smem = smem_raw + (-kf::smem_u32(smem_raw) & 1023u);
@@ -618,15 +619,18 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
             p[e] = kf::ex2(fmaf(c[h][nt][e], a.scale_log2, -mu[nt][e & 1]));
             sum[e & 1] += p[e];
           }
-          // P as a 16-bit value plus the 16-bit rest: two products hold a
-          // weight to 2^-16 of itself (bf16), or to 2^-21 of itself and 2^-36
-          // of the row's largest (fp16)
+          // P as the next smaller 16-bit value plus the 16-bit rest: two
+          // products hold a weight to 2^-16 of itself (bf16), or to 2^-21 of
+          // itself and 2^-34 of the row's largest (fp16).  Both parts are
+          // positive whatever the weight, so that an infinity in V stays one
+          // (0 times it would be NaN); the V of masked keys is 0.
 #pragma unroll
           for (int x = 0; x < 2; ++x) {
-            const uint32_t hi = kf::pack2<BF16>(p[2 * x], p[2 * x + 1]);
+            const float w0 = fmaxf(p[2 * x], 2 * LEAST), w1 = fmaxf(p[2 * x + 1], 2 * LEAST);
+            const uint32_t hi = kf::pack2_below<BF16>(w0, w1);
             const float2 back = kf::unpack2<BF16>(hi);
             pb[h][nt][x] = kf::movmatrix_trans(hi);
-            pl[h][nt][x] = kf::movmatrix_trans(kf::pack2<BF16>(p[2 * x] - back.x, p[2 * x + 1] - back.y));
+            pl[h][nt][x] = kf::movmatrix_trans(kf::pack2<BF16>(fmaxf(w0 - back.x, LEAST), fmaxf(w1 - back.y, LEAST)));
           }
         }
         l_run[nt][0] += sum[0];

@@ -6,10 +6,15 @@ import pytest
 import torch
 
 from kotflash_b200 import paged_attention
+from oracle import paged_oracle as oracle
 
 pytestmark = pytest.mark.gpu
 
 UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
+
+
+def _i32(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
 
 
 # ---------------------------------------------------------------- one dominant key
@@ -68,3 +73,61 @@ def test_many_small_weights_beside_a_large_sum(dtype, hq, lead):
     assert (out.double() - 1).abs().max().item() <= UNIT[dtype] + hold
     want = lead * math.log(2) + math.log1p((n - 1) * 2.0 ** -lead)
     assert (lse.double() - want).abs().max().item() <= hold + want * 2.0 ** -22
+
+
+# ---------------------------------------------------------------- infinities
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("hq,hkv,d,page", [(4, 2, 64, 16), (16, 1, 128, 16), (24, 1, 72, 24), (40, 1, 104, 8), (3, 3, 16, 5)])
+def test_infinite_values_stay_infinite(dtype, hq, hkv, d, page):
+    """O = sum w v with w > 0: +inf or -inf where a column sees one, NaN where
+    it sees both or a NaN; every other column as without them."""
+    lens = [100, 1, 33, 700, 9000, 60]
+    g = torch.Generator(device="cuda").manual_seed(hq + d)
+    held = [-(-n // page) for n in lens]
+    cols = max(held)
+    table = torch.full((len(lens), cols), -1, dtype=torch.int32)
+    at = 0
+    for b, h in enumerate(held):
+        table[b, :h] = torch.arange(at, at + h)
+        at += h
+    shape = (at, hkv, page, d)
+    k = torch.randn(shape, device="cuda", generator=g).to(dtype)
+    v = torch.randn(shape, device="cuda", generator=g).to(dtype)
+    q = (torch.randn(len(lens), hq, 1, d, device="cuda", generator=g) * 1.5).to(dtype)
+    for b, n in enumerate(lens):                       # position, head, column, value
+        for i in range(6 if n > 40 else 1):
+            p = (i * 37 + b) % n
+            v[int(table[b, p // page]), i % hkv, p % page, (5 * i + b) % d] = (math.inf, -math.inf, math.inf)[i % 3]
+        if n > 40:                                     # a column with both, and one with a NaN
+            for p, x in ((3, math.inf), (n - 2, -math.inf)):
+                v[int(table[b, p // page]), 0, p % page, d - 1] = x
+            v[int(table[b, 7 // page]), 0, 7 % page, d - 2] = math.nan
+    table, lengths, scale = table.cuda(), _i32(lens), d ** -0.5
+    out, lse = paged_attention(q, k, v, table, lengths, return_lse=True)
+    want, want_lse, _ = oracle.attention(q, k, v, table, lengths, scale)
+    finite = torch.isfinite(want)
+    assert (~finite).any() and torch.isinf(want).any() and torch.isnan(want).any()
+    got = out.double().cpu()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)], want[torch.isinf(want)])
+    tame = torch.where(torch.isfinite(v), v, torch.zeros_like(v))
+    same, _, sizes = oracle.attention(q, k, tame, table, lengths, scale)
+    for b, (prod, vmax, n) in enumerate(sizes):        # as for finite values: see the checks of ragged batches
+        dx = prod * (d + 2) * 2.0 ** -23 + 2.0 ** -22
+        bound = UNIT[dtype] * same[b].abs() + vmax * (2.0 ** -16 + 2 * dx + (n / 16 + 64) * 2.0 ** -23) + 2.0 ** -24
+        off = torch.where(finite[b], (got[b] - same[b]).abs() - bound, -1.0)
+        assert (off <= 0).all()
+    assert torch.isfinite(lse).all()
+
+
+def test_an_infinite_value_behind_a_small_weight():
+    """fp16 holds a weight of 2^-40 of the largest as no number; its V still decides the sign of an infinity."""
+    k = torch.zeros(4, 1, 16, 64, device="cuda", dtype=torch.float16)
+    v = torch.ones_like(k)
+    k[0, 0, 0, 0], v[3, 0, 2, 7], v[1, 0, 3, 9] = 40.0, math.inf, -math.inf
+    q = torch.zeros(1, 1, 1, 64, device="cuda", dtype=torch.float16)
+    q[..., 0] = 1
+    out = paged_attention(q, k, v, _i32([[0, 1, 2, 3]]), _i32([64]), scale=math.log(2))[0, 0, 0]
+    assert out[7] == math.inf and out[9] == -math.inf
+    assert (out[[c for c in range(64) if c not in (7, 9)]] == 1).all()
