@@ -460,12 +460,19 @@ int check_tables(const char* what, const kf_page_tables& t) {
   return KF_OK;
 }
 
+// Dynamic shared memory of the two kernels.
+constexpr size_t reserve_smem(int64_t B) { return (size_t)(3 * B + 1) * 4; }
+constexpr size_t release_smem(int64_t B) { return (size_t)B * 4; }
+
+// Without this a block gets 48 KB, its static arrays (up to 528 bytes)
+// included.  The limit is raised to the kernel's largest size, `most`, never to
+// that of one call: calls of other threads may lie between this and the launch.
 template <typename... KArgs>
-int raise_smem(void (*kern)(KArgs...), size_t smem, const char* what) {
-  if (smem > 48 * 1024 &&
-      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) {
+int raise_smem(void (*kern)(KArgs...), size_t smem, size_t most, const char* what) {
+  if (smem > 47 * 1024 &&
+      cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most) != cudaSuccess) {
     (void)cudaGetLastError();
-    return kf::set_error(KF_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory", what, smem);
+    return kf::set_error(KF_ERR_CUDA, "%s: cannot reserve %zu bytes of shared memory", what, most);
   }
   return KF_OK;
 }
@@ -583,11 +590,11 @@ extern "C" int kf_paged_reserve(const kf_paged_reserve_args* args) {
   a.max_pages = (uint32_t)t.max_pages;
   a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
-  const size_t smem = (size_t)(3 * t.B + 1) * 4;
+  const size_t smem = reserve_smem(t.B);
   const bool large = t.B > kSmall || num_tokens > 4 * kSmall;
   const unsigned cluster = large ? cluster_for(num_tokens, kLarge * 4) : 1;
   auto kern = large ? paged_reserve_kernel<kLarge> : paged_reserve_kernel<kSmall>;
-  rc = raise_smem(kern, smem, what);
+  rc = raise_smem(kern, smem, reserve_smem(kMaxRequests), what);
   if (rc != KF_OK) return rc;
   return kf::launch_dependent_cluster(kern, cluster, dim3(cluster), dim3(large ? kLarge : kSmall), smem,
                                       static_cast<cudaStream_t>(t.stream), what, a);
@@ -615,11 +622,11 @@ extern "C" int kf_paged_release(const kf_paged_release_args* args) {
   a.max_pages = (uint32_t)t.max_pages;
   a.div = page_div(t.page_size);
   a.num_pages = (uint32_t)t.num_pages;
-  const size_t smem = (size_t)t.B * 4;
+  const size_t smem = release_smem(t.B);
   const bool large = t.B > kSmall / 32;  // a warp per request
   const unsigned cluster = large ? cluster_for(t.B, kLarge / 32) : 1;
   auto kern = large ? paged_release_kernel<kLarge> : paged_release_kernel<kSmall>;
-  rc = raise_smem(kern, smem, what);
+  rc = raise_smem(kern, smem, release_smem(kMaxRequests), what);
   if (rc != KF_OK) return rc;
   return kf::launch_dependent_cluster(kern, cluster, dim3(cluster), dim3(large ? kLarge : kSmall), smem,
                                       static_cast<cudaStream_t>(t.stream), what, a);

@@ -1,6 +1,9 @@
 # SPDX-License-Identifier: Apache-2.0
 """The paged KV cache at its edges (GPU)."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -10,6 +13,7 @@ from oracle import paged_oracle as oracle
 
 pytestmark = pytest.mark.gpu
 
+ROOT = Path(__file__).resolve().parents[1]
 UNIT = {torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}
 
 
@@ -131,3 +135,33 @@ def test_an_infinite_value_behind_a_small_weight():
     out = paged_attention(q, k, v, _i32([[0, 1, 2, 3]]), _i32([64]), scale=math.log(2))[0, 0, 0]
     assert out[7] == math.inf and out[9] == -math.inf
     assert (out[[c for c in range(64) if c not in (7, 9)]] == 1).all()
+
+
+# ---------------------------------------------------------------- sizes of the tables
+
+def _fresh(code, *args):
+    """Runs code in a process of its own, where nothing of the package has been called yet."""
+    done = subprocess.run([sys.executable, "-c", code, *map(str, args)], cwd=ROOT, capture_output=True, text=True, timeout=600)
+    assert done.returncode == 0, done.stdout + done.stderr
+
+
+def test_table_sizes_around_the_shared_memory_limit():
+    """Batches whose tables of 12 (reserve) or 4 (release) bytes per request lie
+    around 48 KB, from the smallest up, and the largest."""
+    _fresh("""
+import torch
+from kotflash_b200 import release_pages, reserve_pages
+i32 = dict(dtype=torch.int32, device="cuda")
+for b in (4051, 4052, 4095, 4096, 16384):
+    table = torch.full((b, 1), -1, **i32)
+    slots, starts, lengths, count = reserve_pages(torch.zeros(b, **i32), torch.ones(b, **i32), table, torch.arange(b, **i32),
+                                                  torch.full((1,), b, **i32), page_size=16, num_tokens=b)
+    pages = torch.arange(b - 1, -1, -1, device="cuda")
+    assert torch.equal(slots, pages * 16) and torch.equal(table[:, 0], pages.int()), b
+    assert torch.equal(starts, torch.arange(b + 1, **i32)) and (lengths == 1).all() and count.item() == 0, b
+for b in (12160, 12161, 12288, 12289, 16384):
+    free = torch.full((b,), -1, **i32)
+    lengths, count = release_pages(torch.ones(b, **i32), torch.ones(b, dtype=torch.bool, device="cuda"),
+                                   torch.arange(b, **i32)[:, None], free, torch.zeros(1, **i32), page_size=16)
+    assert torch.equal(free, torch.arange(b, **i32)) and (lengths == 0).all() and count.item() == b, b
+""")
