@@ -294,8 +294,9 @@ int kf_paged_append(const kf_paged_append_args* args);
  * ceil((lengths[b] + new_lengths[b]) / page_size) - ceil(lengths[b] /
  * page_size) more pages; going through the requests in order it is granted all
  * of them, popped from the end of the stack into block_table[b] in place, or,
- * where they would not fit its max_pages or the needs up to and including its
- * own exceed the stack, refused.  Writes
+ * where they would not fit its max_pages, the needs up to and including its
+ * own exceed the stack or its packed tokens end past num_tokens, refused.
+ * Writes
  *   slots [num_tokens] int64 (16-byte aligned): the slots of all new tokens,
  *     request after request; -1 for those of a refused request and past the
  *     last token,

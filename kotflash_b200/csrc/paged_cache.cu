@@ -211,9 +211,11 @@ struct ReserveArgs {
 
 // need_b = ceil((len_b + new_b) / page) - ceil(len_b / page), 0 where the
 // request would outgrow its table row (or its padded slots); upto = inclusive
-// sum of need.  A request is granted when it fits and upto_b <= free_count (or
-// it needs no page); the granted requests that need pages are then a prefix,
-// so request b takes the stack entries free_count - 1 - (upto_b - need_b) - j.
+// sum of need.  A request is granted when it fits, upto_b <= free_count (or
+// it needs no page) and its packed slots end within num_tokens (or it has no
+// token); the granted requests that need pages are then a prefix, since both
+// sums only grow, so request b takes the stack entries free_count - 1 -
+// (upto_b - need_b) - j.
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(const ReserveArgs a) {
   extern __shared__ int32_t sm[];
@@ -248,7 +250,8 @@ __global__ void __launch_bounds__(THREADS) paged_reserve_kernel(const ReserveArg
     add_upto += tokens;
     upto += pages;
     if (b < a.B) {
-      const bool granted = fits && (need == 0 || upto <= count);
+      const bool slotted = a.padded != 0 || add == 0 || add_upto <= a.T;
+      const bool granted = fits && slotted && (need == 0 || upto <= count);
       starts[b] = saturate(a.padded ? (int64_t)b * a.padded : add_upto - add);
       first[b] = saturate(upto - need);
       held[b] = granted ? (int32_t)len : -1;

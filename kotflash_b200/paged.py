@@ -344,7 +344,8 @@ def reserve_pages(
 
     Slots are packed or padded.  num_tokens is the number of packed slots to
     write, request after request, normally the sum of new_lengths (a larger one
-    leaves -1 behind them, so that a captured step can keep one size).
+    leaves -1 behind them, so that a captured step can keep one size; with a
+    smaller one the requests whose tokens end past it are refused).
     tokens_per_request gives every request that many, with -1 behind its last
     token: the slots of rows [B, Hkv, tokens_per_request, D].  A request that
     brings more is refused.  Returns ``(slots, starts, lengths_out,

@@ -66,7 +66,8 @@ def reserve(lengths, added, table, free_pages, free_count, page_size, num_tokens
         fits = after <= len(table[b]) and n + m < 2**31 and (per_request is None or m <= per_request)
         if fits:
             claimed += need
-        granted = fits and (need == 0 or claimed <= count)
+        slotted = per_request is not None or m == 0 or len(slots) + m <= num_tokens
+        granted = fits and slotted and (need == 0 or claimed <= count)
         if granted:
             for j in range(need):
                 table[b][before + j] = free_pages[count - 1 - taken - j]

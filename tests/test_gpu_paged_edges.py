@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from kotflash_b200 import paged_attention
+from kotflash_b200 import paged_attention, reserve_pages
 from oracle import paged_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -165,3 +165,23 @@ for b in (12160, 12161, 12288, 12289, 16384):
                                    torch.arange(b, **i32)[:, None], free, torch.zeros(1, **i32), page_size=16)
     assert torch.equal(free, torch.arange(b, **i32)) and (lengths == 0).all() and count.item() == b, b
 """)
+
+
+def test_reserve_gives_no_token_without_a_slot():
+    """Packed slots that end before a request's tokens do: the request is refused, and so are those after it."""
+    def reserve(added, num_tokens):
+        b = len(added)
+        table = torch.full((b, 4), -1, dtype=torch.int32, device="cuda")
+        free = torch.arange(10, dtype=torch.int32, device="cuda")
+        slots, starts, lengths, count = reserve_pages(_i32([0] * b), _i32(added), table, free, _i32([10]), page_size=4,
+                                                      num_tokens=num_tokens)
+        return slots.tolist(), starts.tolist(), lengths.tolist(), count.item(), table.tolist()
+
+    slots, starts, lengths, count, table = reserve([3, 5, 0, 2, 0], 9)
+    assert slots == [36, 37, 38, 32, 33, 34, 35, 28, -1] and starts == [0, 3, 8, 8, 10, 10]
+    assert lengths == [3, 5, 0, 0, 0] and count == 7
+    assert table == [[9, -1, -1, -1], [8, 7, -1, -1]] + [[-1] * 4] * 3
+    assert reserve([3, 5, 0, 2, 0], 8)[2] == [3, 5, 0, 0, 0]
+    assert reserve([3, 5, 0, 2, 0], 7)[2] == [3, 0, 0, 0, 0]
+    assert reserve([3, 5, 0, 2, 0], 10)[2] == [3, 5, 0, 2, 0]
+    assert reserve([3, 1], 0) == ([], [0, 3, 4], [0, 0], 10, [[-1] * 4] * 2)
