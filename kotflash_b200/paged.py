@@ -251,7 +251,7 @@ def append_paged_kv(
     new_k and new_v are [N, Hkv, S, D] with any strides; token t = n * S + s
     goes to slot slots[t] (int64 [N * S]), that is row slots[t] % page_size of
     page slots[t] // page_size.  Tokens whose slot is outside the pool (-1 for
-    those that ``reserve_pages`` refused) are skipped.
+    those that ``reserve_pages`` refused) are skipped; N or S may be 0.
     """
     try:
         index = k_pages.get_device()
@@ -275,6 +275,14 @@ def append_paged_kv(
         _check_inference(what, k_pages, v_pages, new_k, new_v)
         _check_device(what, k_pages, v_pages, new_k, new_v, slots)
         index, dtype, ns = k_pages.get_device(), k_pages.dtype, new_k.shape
+    if ns[0] == 0 or ns[2] == 0:  # a step that admits no prompt
+        if k_pages.shape != v_pages.shape:
+            raise ValueError("append_paged_kv: K/V page shapes must match")
+        if new_v.shape != ns:
+            raise ValueError("append_paged_kv: new K/V shapes must match")
+        if ns[1] != k_pages.shape[1] or ns[3] != k_pages.shape[3]:
+            raise ValueError("append_paged_kv: new K/V heads and head_dim must match the pages")
+        return
     rc = _ext.load().kf_paged_append(_pack_append(
         k_pages.data_ptr(), *k_pages.shape, *k_pages.stride(), v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(),
         new_k.data_ptr(), *ns, *new_k.stride(), new_v.data_ptr(), *new_v.shape, *new_v.stride(),

@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from kotflash_b200 import paged_attention, reserve_pages
+from kotflash_b200 import PagedKVCache, append_paged_kv, paged_attention, reserve_pages
 from oracle import paged_oracle as oracle
 
 pytestmark = pytest.mark.gpu
@@ -185,3 +185,22 @@ def test_reserve_gives_no_token_without_a_slot():
     assert reserve([3, 5, 0, 2, 0], 7)[2] == [3, 0, 0, 0, 0]
     assert reserve([3, 5, 0, 2, 0], 10)[2] == [3, 5, 0, 2, 0]
     assert reserve([3, 1], 0) == ([], [0, 3, 4], [0, 0], 10, [[-1] * 4] * 2)
+
+
+# ---------------------------------------------------------------- nothing to store
+
+def test_appending_no_tokens():
+    """A step that admits no prompt: no slots, no rows, nothing stored."""
+    cache = PagedKVCache(6, 16, 2, 64, 3, 2, device="cuda", dtype=torch.float16)
+    cache.k.zero_()
+    cache.v.zero_()
+    slots, starts = cache.reserve(_i32([0, 0, 0]), num_tokens=0)
+    assert slots.shape == (0,) and starts.tolist() == [0, 0, 0, 0]
+    rows = torch.ones(1, 2, 0, 64, device="cuda", dtype=torch.float16)
+    cache.append(rows, rows, slots)
+    none = torch.ones(0, 2, 5, 64, device="cuda", dtype=torch.float16)
+    append_paged_kv(cache.k[0], cache.v[0], none, none, slots)
+    assert not cache.k.any() and not cache.v.any()
+    for k, v, match in ((rows[:, :1], rows[:, :1], "heads"), (rows[..., :32], rows[..., :32], "head"), (rows, none, "shapes")):
+        with pytest.raises(ValueError, match=match):
+            cache.append(k, v, slots)

@@ -1,0 +1,19 @@
+# SPDX-License-Identifier: Apache-2.0
+"""Paged KV cache on the CPU: refusals at its edges, before any launch."""
+import pytest
+import torch
+
+from kotflash_b200 import append_paged_kv
+
+
+def test_appending_no_tokens_is_checked_like_any_append():
+    pool, slots = torch.zeros(5, 2, 16, 64, dtype=torch.float16), torch.zeros(0, dtype=torch.int64)
+    rows = torch.zeros(1, 2, 0, 64, dtype=torch.float16)
+    for args, error, match in [
+        ((pool, pool, rows, rows, slots.int()), TypeError, "int64"),
+        ((pool, pool, rows, rows, torch.zeros(1, dtype=torch.int64)), ValueError, "one slot for each"),
+        ((pool, pool, rows, rows.bfloat16(), slots), ValueError, "dtypes"),
+        ((pool, pool, rows, rows, slots), RuntimeError, "sm_100"),
+    ]:
+        with pytest.raises(error, match=match):
+            append_paged_kv(*args)
