@@ -51,8 +51,11 @@ __device__ __forceinline__ void move_token(const AppendArgs& a, int64_t slot, ui
     const E* pk = reinterpret_cast<const E*>(a.src_k + n * a.sk[0] + h * a.sk[1] + s * a.sk[2] + d * a.sk[3]);
     const E* pv = reinterpret_cast<const E*>(a.src_v + n * a.sv[0] + h * a.sv[1] + s * a.sv[2] + d * a.sv[3]);
     if constexpr (VEC == 8) {
-      val[0] = __ldg(pk);
-      val[1] = __ldg(pv);
+      // through L2: the predecessor may have written these while this kernel was
+      // alive, so not non-coherently (16384 tokens: 22.9 us as with non-coherent
+      // loads, 24.3 with loads that look in L1 first)
+      val[0] = __ldcg(pk);
+      val[1] = __ldcg(pv);
     } else {
       val[0].x = *pk;
       val[1].x = *pv;

@@ -252,6 +252,8 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     k_off[x] = tile_offset(lane & 15, min(2 * x + (lane >> 4), last));
     v_off[x] = tile_offset((lane & 7) + ((lane >> 4) << 3), min(2 * x + ((lane >> 3) & 1), last));
   }
+  // (The kernel may have been alive while its predecessor wrote the lengths,
+  // tables, Q or slots, so none of them is read through the non-coherent path.)
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
@@ -355,7 +357,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     const uint32_t pg = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
     Place p;
     p.row = key - pg * a.page_size;
-    p.page = key < load.keys ? (uint32_t)__ldg(a.table + load.b * a.table_stride + pg) : 0xffffffffu;
+    p.page = key < load.keys ? (uint32_t)a.table[load.b * a.table_stride + pg] : 0xffffffffu;
     p.h = load.h;
     return p;
   };
@@ -407,7 +409,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
         for (int e = 0; e < 2; ++e) {
           qb[nt][kk][e] = 0u;
           if (row < a.G && kk * 16 + e * 8 < a.D)
-            asm volatile("ld.global.nc.b32 %0, [%1];" : "=r"(qb[nt][kk][e]) : "l"(src + kk * 16 + e * 8));
+            asm volatile("ld.global.b32 %0, [%1];" : "=r"(qb[nt][kk][e]) : "l"(src + kk * 16 + e * 8));
         }
     }
   };

@@ -1,5 +1,8 @@
 # SPDX-License-Identifier: Apache-2.0
-"""Paged KV cache on the CPU: refusals at its edges, before any launch."""
+"""Paged KV cache on the CPU: refusals at its edges, before any launch, and what its sources must not hold."""
+import re
+from pathlib import Path
+
 import pytest
 import torch
 
@@ -17,3 +20,15 @@ def test_appending_no_tokens_is_checked_like_any_append():
     ]:
         with pytest.raises(error, match=match):
             append_paged_kv(*args)
+
+
+def test_dependent_launches_read_no_memory_non_coherently():
+    """A kernel launched as a programmatic dependent lives while its predecessor
+    writes; the non-coherent load path is for memory that nobody writes while
+    the kernel lives."""
+    csrc = Path(__file__).resolve().parents[1] / "kotflash_b200" / "csrc"
+    sources = [p for p in csrc.glob("*.cu") if "launch_dependent" in p.read_text()]
+    assert {p.name for p in sources} >= {"decode.cu", "paged_cache.cu", "paged_decode.cu"}
+    for path in sources:
+        found = re.findall(r"__ldg\b|ld\.global\.nc|__restrict__", path.read_text())
+        assert not found, (path.name, found)
