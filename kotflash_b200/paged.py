@@ -127,13 +127,6 @@ def _status_ptr(index: int) -> int:
     return _ext.status_word(torch.device("cuda", index)).data_ptr()
 
 
-@lru_cache(maxsize=16)
-def _like_int64(index: int) -> torch.Tensor:
-    """An empty int64 tensor of the device: its new_empty(n) takes 0.6 us less
-    than one with a dtype."""
-    return torch.empty(0, dtype=torch.int64, device=torch.device("cuda", index))
-
-
 @lru_cache(maxsize=256)
 def _workspace_elements(hq: int, hkv: int, d: int, device_index: int) -> int:
     """Workspace of kf_paged_decode in 16-bit elements."""
@@ -377,7 +370,7 @@ def reserve_pages(
         num_tokens = per_request * b
     elif _whole(num_tokens) < 0:
         raise ValueError(f"{what}: num_tokens must not be negative")
-    slots = _like_int64(index).new_empty(num_tokens)
+    slots = lengths.new_empty(num_tokens, dtype=_INT64)
     starts = lengths.new_empty(b + 1)
     if lengths_out is None:
         lengths_out = torch.empty_like(lengths)

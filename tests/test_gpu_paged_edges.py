@@ -204,3 +204,26 @@ def test_appending_no_tokens():
     for k, v, match in ((rows[:, :1], rows[:, :1], "heads"), (rows[..., :32], rows[..., :32], "head"), (rows, none, "shapes")):
         with pytest.raises(ValueError, match=match):
             cache.append(k, v, slots)
+
+
+# ---------------------------------------------------------------- the first call of a process
+
+def test_first_reserve_under_a_tracing_mode():
+    """A call on tensors without memory fails; the process's later calls do not."""
+    _fresh("""
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+from kotflash_b200 import reserve_pages
+i32 = dict(dtype=torch.int32, device="cuda")
+def reserve():
+    return reserve_pages(torch.zeros(2, **i32), torch.ones(2, **i32), torch.full((2, 4), -1, **i32), torch.arange(9, **i32),
+                         torch.full((1,), 9, **i32), page_size=16, num_tokens=2)
+try:
+    with FakeTensorMode():
+        reserve()
+except Exception as exc:
+    print(type(exc), exc)
+else:
+    raise SystemExit("a call without memory went through")
+assert reserve()[0].tolist() == [128, 112]
+""")

@@ -6,7 +6,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from kotflash_b200 import append_paged_kv
+from kotflash_b200 import _ext, append_paged_kv, paged, reserve_pages
 
 
 def test_appending_no_tokens_is_checked_like_any_append():
@@ -32,3 +32,28 @@ def test_dependent_launches_read_no_memory_non_coherently():
     for path in sources:
         found = re.findall(r"__ldg\b|ld\.global\.nc|__restrict__", path.read_text())
         assert not found, (path.name, found)
+
+
+@pytest.mark.filterwarnings("ignore:Accessing the data pointer")
+def test_nothing_of_a_tracing_mode_stays(monkeypatch):
+    """reserve_pages on tensors without memory (an export, a shape pass) leaves no
+    tensor of that mode in the module for later calls."""
+    from torch._subclasses.fake_tensor import FakeTensor, FakeTensorMode
+
+    calls = []
+
+    class Library:
+        def __getattr__(self, name):
+            return lambda args: calls.append(name) or 0
+
+    monkeypatch.setattr(_ext, "load", Library)
+    monkeypatch.setattr(paged, "_is_sm100", lambda index: True)
+    monkeypatch.setattr(paged, "_raw_stream", lambda index: 0)
+    for mode in (FakeTensorMode(), FakeTensorMode()):
+        with mode:
+            i32 = dict(dtype=torch.int32, device="cuda")
+            lengths = torch.empty(3, **i32)
+            slots, _, _, _ = reserve_pages(lengths, torch.empty(3, **i32), torch.empty(3, 4, **i32), torch.empty(9, **i32),
+                                           torch.empty(1, **i32), page_size=16, num_tokens=6)
+            assert isinstance(slots, FakeTensor) and slots.fake_mode is mode and slots.dtype is torch.int64
+    assert calls == ["kf_paged_reserve"] * 2
