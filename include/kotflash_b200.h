@@ -342,6 +342,13 @@ typedef struct kf_paged_release_args {
 int kf_paged_reserve(const kf_paged_reserve_args* args);
 int kf_paged_release(const kf_paged_release_args* args);
 
+/* ---- the process's status word -------------------------------------------
+ * No counterpart in the reference.  *word is the address of an int32 of
+ * `device`'s memory for the `status` arguments above: 0 until an expired wait
+ * sets it, there as long as the process.  May be called while a stream
+ * captures; nothing is recorded. */
+int kf_device_status(int device, int32_t** word);
+
 /* ---- self-test of the bounded device wait -------------------------------
  * No counterpart in the reference.  Launches one kernel that waits on a
  * barrier nothing completes; after `budget_us` microseconds the wait gives

@@ -77,6 +77,7 @@ SIGNATURES = {
     "kf_paged_append": (_I, [_BYTES]),
     "kf_paged_reserve": (_I, [_BYTES]),
     "kf_paged_release": (_I, [_BYTES]),
+    "kf_device_status": (_I, [_I, ctypes.POINTER(_VP)]),
     "kf_selftest_bounded_wait": (_I, [_VP, _I64, _VP]),
     "kf_selftest_exp2_poly": (_I, [_VP, _VP, _I64, _VP]),
     "kf_peer_mailbox_bytes": (_SZ, [_I, _I64, _I64]),
@@ -191,17 +192,27 @@ raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
-_status_words = {}
+@lru_cache(maxsize=16)
+def status_ptr(device_index: int) -> int:
+    """Address of the device's int32 word that kernels set when a bounded wait
+    expires.  The library's own memory, so that it is the same whatever mode
+    (inference, tracing, graph capture) the first call runs in."""
+    word = _VP()
+    check(load().kf_device_status(device_index, ctypes.byref(word)), "kf_device_status")
+    return word.value
+
+
+class _StatusWord:
+    def __init__(self, index: int) -> None:
+        self.__cuda_array_interface__ = {"shape": (1,), "typestr": "<i4", "data": (status_ptr(index), False),
+                                         "strides": None, "version": 3}
 
 
 def status_word(device: torch.device) -> torch.Tensor:
-    """Per-device int32 word that kernels set when a bounded wait expires."""
+    """The device's status word as a tensor."""
     idx = device.index if device.index is not None else torch.cuda.current_device()
-    w = _status_words.get(idx)
-    if w is None:
-        w = torch.zeros(1, dtype=torch.int32, device=torch.device("cuda", idx))
-        _status_words[idx] = w
-    return w
+    with torch.inference_mode(False):
+        return torch.as_tensor(_StatusWord(idx), device=torch.device("cuda", idx))
 
 
 def read_device_status(device: torch.device) -> int:

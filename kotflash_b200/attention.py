@@ -241,7 +241,7 @@ def attention_forward(q, k, v, *, causal: bool, scale: float):
     rc = lib.kf_attn_fwd(
         _ext.ref(_ext.t4(qp)), _ext.ref(_ext.t4(kp)), _ext.ref(_ext.t4(vp)),
         _ext.ref(_ext.t4(out)), lse.data_ptr(), _ext.dtype_code(q.dtype), float(scale),
-        int(bool(causal)), _ext.status_word(q.device).data_ptr(), _ext.stream_of(q),
+        int(bool(causal)), _ext.status_ptr(q.device.index), _ext.stream_of(q),
     )
     _ext.check(rc, "kf_attn_fwd")
     if d_pad != d:
@@ -274,7 +274,7 @@ def attention_backward(q, k, v, out, lse, grad_out, *, causal: bool, scale: floa
         _ext.ref(_ext.t4(dq)), _ext.ref(_ext.t4(dk)), _ext.ref(_ext.t4(dv)),
         _ext.dtype_code(q.dtype), float(scale), int(bool(causal)),
         workspace.data_ptr(), int(workspace.numel()),
-        _ext.status_word(q.device).data_ptr(), _ext.stream_of(q),
+        _ext.status_ptr(q.device.index), _ext.stream_of(q),
     )
     _ext.check(rc, "kf_attn_bwd")
     if d_pad != d:

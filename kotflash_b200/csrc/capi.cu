@@ -174,6 +174,33 @@ extern "C" int kf_version(void) { return 10000; }  // 1.0.0
 
 extern "C" const char* kf_last_error(void) { return kf::g_last_error.c_str(); }
 
+// Zero when the module is loaded, so that nothing ever has to clear it in
+// stream order: a clear that a capture recorded would be repeated by every
+// replay and hide an expired wait.
+static __device__ int32_t g_device_status;
+
+extern "C" int kf_device_status(int device, int32_t** word) {
+  if (!word || device < 0) return kf::set_error(KF_ERR_INVALID, "kf_device_status: need a device and an address");
+  // the lookup loads the module on first use, which a capturing thread may do in relaxed mode only
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  int cur = -1;
+  void* p = nullptr;
+  cudaError_t e = cudaThreadExchangeStreamCaptureMode(&mode);
+  if (e == cudaSuccess) {
+    e = cudaGetDevice(&cur);
+    if (e == cudaSuccess && cur != device) e = cudaSetDevice(device);
+    if (e == cudaSuccess) e = cudaGetSymbolAddress(&p, g_device_status);
+    if (cur >= 0 && cur != device) (void)cudaSetDevice(cur);
+    (void)cudaThreadExchangeStreamCaptureMode(&mode);
+  }
+  if (e != cudaSuccess) {
+    (void)cudaGetLastError();
+    return kf::set_error(KF_ERR_CUDA, "kf_device_status: %s", cudaGetErrorString(e));
+  }
+  *word = static_cast<int32_t*>(p);
+  return KF_OK;
+}
+
 // Self-test of the bounded device wait: one thread waits on an mbarrier that
 // nothing arrives on, gives up after `budget_ns`, and records the timeout in
 // the status word, exactly as the attention kernels do when a peer stalls.

@@ -37,7 +37,7 @@ _INT32, _INT64, _BOOL = torch.int32, torch.int64, torch.bool
 _CONTIGUOUS = torch.contiguous_format
 _pack_decode, _pack_step, _pack_append = _ext.pack_paged_decode, _ext.pack_paged_step, _ext.pack_paged_append
 _pack_reserve, _pack_release = _ext.pack_paged_reserve, _ext.pack_paged_release
-_raw_stream, _is_sm100 = _ext.raw_stream, _ext.is_sm100
+_raw_stream, _is_sm100, _status_ptr = _ext.raw_stream, _ext.is_sm100, _ext.status_ptr
 
 
 # Each entry point below tests everything in one expression, which is what a
@@ -119,12 +119,6 @@ def _check_attention(q, k_pages, v_pages, block_table, lengths, new_k, new_v, sl
         raise ValueError("num_query_heads must be divisible by num_kv_heads (GQA/MQA)")
     _check_inference(what, q, k_pages, v_pages, *rows)
     _check_device(what, q, k_pages, v_pages, block_table, lengths, *rows, *((slots,) if rows else ()))
-
-
-@lru_cache(maxsize=16)
-def _status_ptr(index: int) -> int:
-    """Address of the device's status word, which lives as long as the process."""
-    return _ext.status_word(torch.device("cuda", index)).data_ptr()
 
 
 @lru_cache(maxsize=256)

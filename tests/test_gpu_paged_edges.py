@@ -227,3 +227,63 @@ else:
     raise SystemExit("a call without memory went through")
 assert reserve()[0].tolist() == [128, 112]
 """)
+
+
+_FIRST = """
+import torch
+from kotflash_b200 import _ext, paged_attention
+dev = torch.device("cuda", 0)
+def attend():
+    f16, i32 = dict(dtype=torch.float16, device="cuda"), dict(dtype=torch.int32, device="cuda")
+    return paged_attention(torch.zeros(1, 2, 1, 64, **f16), torch.zeros(4, 2, 16, 64, **f16), torch.zeros(4, 2, 16, 64, **f16),
+                           torch.zeros(1, 4, **i32), torch.full((1,), 40, **i32))
+"""
+
+
+def test_first_call_in_inference_mode():
+    _fresh(_FIRST + """
+with torch.inference_mode():
+    attend()
+_ext.clear_device_status(dev)
+assert _ext.read_device_status(dev) == 0
+""")
+
+
+def test_first_call_inside_a_graph_capture():
+    """The status word is not cleared by the graph's replays."""
+    _fresh(_FIRST + """
+f16, i32 = dict(dtype=torch.float16, device="cuda"), dict(dtype=torch.int32, device="cuda")
+q, k = torch.zeros(1, 2, 1, 64, **f16), torch.zeros(4, 2, 16, 64, **f16)
+table, lengths = torch.zeros(1, 4, **i32), torch.full((1,), 40, **i32)
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    out = paged_attention(q, k, k, table, lengths)
+word = _ext.status_word(dev)
+assert word.item() == 0 and _ext.read_device_status(dev) == 0
+word.fill_(1)
+graph.replay()
+torch.cuda.synchronize()
+assert _ext.read_device_status(dev) == 1
+_ext.clear_device_status(dev)
+assert _ext.read_device_status(dev) == 0 and (out == 0).all()
+del graph
+""")
+
+
+def test_first_attention_under_a_tracing_mode():
+    """A call on tensors without memory fails; the status word of later calls is there."""
+    _fresh(_FIRST + """
+from torch._subclasses.fake_tensor import FakeTensorMode
+try:
+    with FakeTensorMode():
+        attend()
+except Exception as exc:
+    print(type(exc), exc)
+else:
+    raise SystemExit("a call without memory went through")
+assert (attend() == 0).all()
+_ext.status_word(dev).fill_(1)
+assert _ext.read_device_status(dev) == 1
+_ext.clear_device_status(dev)
+assert _ext.read_device_status(dev) == 0
+""")
