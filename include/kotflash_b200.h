@@ -243,8 +243,8 @@ int kf_decode_peer_merge(void* mailbox, int64_t rows, int64_t D, int dtype, int 
  * new_v, written to its page and attended in the same pass; where slots[b] < 0
  * request b has no new row.
  *
- * 16 <= D <= 128, D % 8 == 0.  `workspace` holds
- * kf_paged_decode_workspace_bytes(...) bytes; sm_count is that of the GPU.
+ * 16 <= D <= 128, D % 8 == 0; scale log2(e) is finite as a float.  `workspace`
+ * holds kf_paged_decode_workspace_bytes(...) bytes; sm_count is that of the GPU.
  * A wait that expires sets *status (device memory, may be NULL) and shows as
  * NaN in the outputs.
  *

@@ -1021,6 +1021,8 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
     return set_error(KF_ERR_INVALID, "%s: tensors need a contiguous last dim and 16-byte aligned rows", what);
   if (!q->ptr || !k_pages->ptr || !v_pages->ptr || !args->o || !args->block_table || !args->lengths)
     return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (!isfinite((float)args->scale * kLog2e))
+    return set_error(KF_ERR_INVALID, "%s: scale must be finite in single precision", what);
   const bool fused = new_k->ptr || new_v->ptr || args->slots;
   if (fused) {
     if (!new_k->ptr || !new_v->ptr || !args->slots)

@@ -1,5 +1,6 @@
 # SPDX-License-Identifier: Apache-2.0
 """Paged KV cache on the CPU: refusals at its edges, before any launch, and what its sources must not hold."""
+import math
 import re
 from pathlib import Path
 
@@ -57,3 +58,13 @@ def test_nothing_of_a_tracing_mode_stays(monkeypatch):
                                            torch.empty(1, **i32), page_size=16, num_tokens=6)
             assert isinstance(slots, FakeTensor) and slots.fake_mode is mode and slots.dtype is torch.int64
     assert calls == ["kf_paged_reserve"] * 2
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39, -3e38])
+def test_c_abi_refuses_a_scale_that_single_precision_does_not_hold(scale):
+    def t4(*shape):
+        return (0x1000, *shape, shape[1] * shape[2] * shape[3], shape[2] * shape[3], shape[3], 1)
+
+    args = _ext.pack_paged_decode(*t4(3, 4, 1, 64), *t4(5, 2, 16, 64), *t4(5, 2, 16, 64), 0x1000, 2, 2, 0x1000, 0x1000, 0, 0,
+                                  scale, 0, 0, 0, 0)
+    assert _ext.load().kf_paged_decode(args) == _ext.KF_ERR_INVALID and "scale" in _ext.last_error()
