@@ -73,7 +73,7 @@ struct PagedArgs {
   int block_bytes, row_bytes;  // from 16 rows of a tile to the next, and between rows as boxes of fewer start
   bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
   bool join_units;
-  float scale_log2;        // |scale| log2(e), at least the smallest normal number
+  float scale_log2;        // |scale| log2(e), at least the smallest number
   uint32_t q_sign;         // flips the signs of two elements of Q where scale is negative
 };
 
@@ -1094,9 +1094,9 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.shallow = full;
 
   // A negative scale is taken as -q and a positive one, so that the largest
-  // product is the largest score; 0 as a scale that no product survives, so
-  // that a masked -inf stays -inf.
-  a.scale_log2 = fmaxf(fabsf((float)args->scale) * kLog2e, FLT_MIN);
+  // product is the largest score; 0 as a scale that no product survives (the
+  // largest number times this is 5e-7), so that a masked -inf stays -inf.
+  a.scale_log2 = fmaxf(fabsf((float)args->scale) * kLog2e, FLT_TRUE_MIN);
   a.q_sign = args->scale < 0 ? 0x80008000u : 0u;
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.

@@ -137,6 +137,18 @@ def test_an_infinite_value_behind_a_small_weight():
     assert (out[[c for c in range(64) if c not in (7, 9)]] == 1).all()
 
 
+def test_a_scale_of_zero_leaves_no_score():
+    """Products of 1e38 included: all weights are equal."""
+    k = torch.full((4, 1, 16, 64), 0.0, device="cuda", dtype=torch.bfloat16)
+    k[:, :, ::2, 0], k[:, :, 1::2, 0] = 1e19, -1e19
+    v = torch.arange(64, device="cuda", dtype=torch.bfloat16)[:, None].expand(64, 64).reshape(4, 1, 16, 64).contiguous()
+    q = torch.zeros(1, 1, 1, 64, device="cuda", dtype=torch.bfloat16)
+    q[..., 0] = 1e19
+    for scale in (0.0, -0.0, 1e-60):
+        out, lse = paged_attention(q, k, v, _i32([[0, 1, 2, 3]]), _i32([64]), scale=scale, return_lse=True)
+        assert (out == 31.5).all() and abs(lse.item() - math.log(64)) < 4e-6
+
+
 # ---------------------------------------------------------------- sizes of the tables
 
 def _fresh(code, *args):
