@@ -89,6 +89,7 @@ struct Cfg {
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
   static constexpr int STAGE = KW * DP * 2 * 2;              // bytes: K rows, then V rows
   static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
+  static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;  // stages loaded ahead for long units, at least one
   static constexpr int HANDED = KD * 4 * 32;                 // floats of a warp's O^T of one row tile
   static constexpr int SMEM = 1024 + TEAMS * STAGES * STAGE + (TEAMS > 1 ? 2 * HANDED + kWarps * NT * 16 : 0) * 4;
 };
@@ -431,9 +432,10 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // Tiles loaded ahead of the one in use.  Short units drain the ring at each
   // end and want all of it; for the rest a third, 64 KB per SM, is what HBM
   // needs, and more only queues: blocks then get unequal shares of the
-  // bandwidth and end far apart (D = 128, 8192 keys: 174 us deep, 165 shallow;
-  // 800 keys: 73.2 and 72.4; 400 keys: 73.8 and 75.0).
-  const int depth = a.shallow && total >= 10u * a.B ? STAGES / 3 : STAGES - 1;
+  // bandwidth and end far apart.  Whole ring against a third, D = 128: 8192
+  // keys 171.5 and 165.6 us, 600 to 1000 keys 72.8 and 72.9, 200 to 600 keys
+  // 72.3 and 74.5, so long starts at 10 tiles; D = 64, 8192 keys: 91.9 and 87.4.
+  const int depth = a.shallow && total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
@@ -947,9 +949,19 @@ __global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArg
 // Query rows of a unit for G rows per KV head, and the variant that has them.
 int unit_rows(int64_t G) { return G <= 8 ? 8 : G <= 16 ? 16 : G <= 32 ? 32 : 64; }
 
-// Keys per tile of the variant (Cfg::TILE).
-int tile_keys(int64_t D, bool wide, int rows) {
-  return rows <= 16 ? (D <= 64 || (D <= 96 && !wide) ? 128 : 64) : rows == 32 ? 64 : 32;
+// KD of the variant for a head dim.
+int head_steps(int64_t D, bool wide) { return D <= 64 ? 4 : D <= 96 && !wide ? 6 : 8; }
+
+// Keys per tile of the variant.
+template <int KD>
+int tile_keys_of(int rows) {
+  return rows == 8    ? Cfg<KD, 1, 1>::TILE
+         : rows == 16 ? Cfg<KD, 2, 1>::TILE
+         : rows == 32 ? Cfg<KD, 2, 2>::TILE
+                      : Cfg<KD, 2, 4>::TILE;
+}
+int tile_keys(int steps, int rows) {
+  return steps == 4 ? tile_keys_of<4>(rows) : steps == 6 ? tile_keys_of<6>(rows) : tile_keys_of<8>(rows);
 }
 
 size_t workspace_need(int blocks, int rows, int64_t D) {
@@ -971,6 +983,9 @@ int launch_variant(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap&
 template <bool BF16, int KD, bool FULL>
 int dispatch_rows(const PagedArgs& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
                   cudaStream_t st) {
+  static_assert(Cfg<KD, 1, 1>::ROWS == 8 && Cfg<KD, 2, 1>::ROWS == 16 && Cfg<KD, 2, 2>::ROWS == 32 &&
+                    Cfg<KD, 2, 4>::ROWS == 64,
+                "the cases are unit_rows()'s");
   switch (rows) {
     case 8: return launch_variant<BF16, KD, FULL, 1, 1>(a, mk, mv, blocks, st);
     case 16: return launch_variant<BF16, KD, FULL, 2, 1>(a, mk, mv, blocks, st);
@@ -1091,6 +1106,11 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.block_bytes = wide ? (D <= 64 ? 2048 : 4096) : (int)D * 32;
   a.row_bytes = wide ? 128 : (int)D * 2;
   a.box_bytes = a.box * (a.block_bytes / 16) * 2;
+  // The other head dims keep the ring full: up to 48 they wait for
+  // instructions, not for HBM (32 requests of 8192 keys, D = 16: 65.7 us with
+  // the whole ring, 65.9 with a third, D = 40: 69.5 and 70.7), 72 to 96 have
+  // two stages, of which one is ahead either way, and 104 shows nothing (141 to
+  // 153 us with either).
   a.shallow = full;
 
   // A negative scale is taken as -q and a positive one, so that the largest
@@ -1101,7 +1121,8 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
 
   // One wave of blocks, or fewer when the tables cannot hold that many tiles.
   // A unit of one tile is never cut, so nothing is left to join.
-  const int64_t tile = tile_keys(D, wide, rows), most = (a.capacity + tile - 1) / tile;
+  const int steps = head_steps(D, wide);
+  const int64_t tile = tile_keys(steps, rows), most = (a.capacity + tile - 1) / tile;
   const int64_t units = B * Hkv * a.row_blocks;
   int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
   if (units * (most + 1) > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
@@ -1134,10 +1155,10 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   else if (D == 128)
     rc = bf16 ? dispatch_rows<true, 8, true>(a, mk, mv, rows, (int)blocks, st)
               : dispatch_rows<false, 8, true>(a, mk, mv, rows, (int)blocks, st);
-  else if (D < 64)
+  else if (steps == 4)
     rc = bf16 ? dispatch_rows<true, 4, false>(a, mk, mv, rows, (int)blocks, st)
               : dispatch_rows<false, 4, false>(a, mk, mv, rows, (int)blocks, st);
-  else if (D <= 96 && !wide)
+  else if (steps == 6)
     rc = bf16 ? dispatch_rows<true, 6, false>(a, mk, mv, rows, (int)blocks, st)
               : dispatch_rows<false, 6, false>(a, mk, mv, rows, (int)blocks, st);
   else
