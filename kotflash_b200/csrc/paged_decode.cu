@@ -1106,11 +1106,10 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.block_bytes = wide ? (D <= 64 ? 2048 : 4096) : (int)D * 32;
   a.row_bytes = wide ? 128 : (int)D * 2;
   a.box_bytes = a.box * (a.block_bytes / 16) * 2;
-  // The other head dims keep the ring full: up to 48 they wait for
-  // instructions, not for HBM (32 requests of 8192 keys, D = 16: 65.7 us with
-  // the whole ring, 65.9 with a third, D = 40: 69.5 and 70.7), 72 to 96 have
-  // two stages, of which one is ahead either way, and 104 shows nothing (141 to
-  // 153 us with either).
+  // The other head dims keep the ring full: below 64 HBM is not the only bound
+  // (32 requests of 8192 keys, D = 16: 65.7 us with the whole ring, 65.9 with a
+  // third, D = 40: 69.5 and 70.7), 72 to 96 have two stages, of which one is
+  // ahead either way, and 104 shows nothing (141 to 153 us with either).
   a.shallow = full;
 
   // A negative scale is taken as -q and a positive one, so that the largest
