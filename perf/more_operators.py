@@ -313,7 +313,7 @@ def run(state):
     if op.startswith("rotate"):
         neighbours = case["pairs"] == "neighbours"
         if own:
-            out = rotary.rotary(s["q"], s["k"], s["positions"], s["frequencies"], interleaved=neighbours, magnitude=s["magnitude"])
+            out = rotary.apply_rotary(s["q"], s["k"], s["positions"], s["frequencies"], interleaved=neighbours, magnitude=s["magnitude"])
             if op == "rotate":
                 return out
             return (*out, *torch.autograd.grad(out, (s["q"], s["k"]), (s["dq"], s["dk"])))
