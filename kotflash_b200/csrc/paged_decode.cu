@@ -33,46 +33,23 @@
 #include <float.h>
 #include <math.h>
 
-#include "kf_host.h"
-#include "kf_sm100.cuh"
+#include "paged_split.cuh"
 
 namespace {
 
-constexpr int kWarps = 4;
-constexpr int kThreads = kWarps * 32;
-constexpr int kBlocksPerSm = 2;
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
-
-struct PagedArgs {
+struct PagedArgs : PagedWork {
   const uint16_t* q;
   uint16_t* k;             // written only by the fused append
   uint16_t* v;
   const uint16_t* nk;      // null: no fused append
   const uint16_t* nv;
   const int64_t* slots;    // of the new rows; < 0: this request has none
-  uint16_t* o;             // [B][Hq][D]
-  float* lse;              // may be null
-  const int32_t* table;
-  const int32_t* lengths;
-  float* part_o;           // [blocks][2][rows of a unit][D]
-  float* part_lse;         // [blocks][2][rows of a unit], log2
-  int4* joins;             // by unit if join_units, else by block: (request, KV head and row block, first
-                           // block, last block) of a unit that was cut, or x = -1
-  int32_t* status;         // set when a bounded wait expires (may be null)
   int64_t qs[2], ks[3], vs[3], nks[2], nvs[2];
-  int64_t table_stride;
-  int B, Hq, Hkv, G, D, row_blocks;
-  uint32_t max_pages;
-  uint32_t capacity;       // tokens a table row can hold
-  uint32_t page_size, num_pages;
-  uint32_t page_mul, page_shift;  // x / page_size = x page_mul >> page_shift for x < 2^31
   int box, box_ops;        // rows of a TMA box, and loads that bring its columns
   int box_bytes;           // of K and V together
   int width;               // 16-byte chunks of a panel's rows (8, 4 or 2), or 0: dense rows (see tile_offset)
   int block_bytes, row_bytes;  // from 16 rows of a tile to the next, and between rows as boxes of fewer start
   bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
-  bool join_units;
   float scale_log2;        // |scale| log2(e), at least the smallest number
   uint32_t q_sign;         // flips the signs of two elements of Q where scale is negative
 };
@@ -111,78 +88,6 @@ __device__ __forceinline__ uint32_t tile_at(int r, int c, int width, int block_b
                     (((c ^ x) & (width - 1)) << 4));
 }
 
-__device__ __forceinline__ uint32_t visible(const PagedArgs& a, int b) {
-  const int32_t n = a.lengths[b];
-  return n <= 0 ? 0u : min((uint32_t)n, a.capacity);
-}
-
-// A tile and its position in the list: tile `t` of the `tiles` of the unit
-// (request b, KV head h, row block rb).  A unit takes tiles + 1 positions: its
-// end (joining the teams, writing, the next unit's Q) costs about what a tile
-// does, 1.0 us where a tile takes 1.4, so a position counts as much.
-template <int TILE>
-struct Cursor {
-  int b, h, rb;
-  uint32_t t, tiles, keys, pos;
-  bool whole;  // the table holds all of the request's positions
-
-  __device__ __forceinline__ void set_request(const PagedArgs& a, int request) {
-    b = request;
-    const int32_t length = a.lengths[b];
-    whole = length <= 0 || (uint32_t)length <= a.capacity;
-    keys = length <= 0 ? 0u : min((uint32_t)length, a.capacity);
-    tiles = (keys + TILE - 1) / TILE;
-  }
-  __device__ __forceinline__ bool unit_ends() const { return t + 1 == tiles; }
-  // whether another tile follows before position `end`
-  __device__ __forceinline__ bool more(uint32_t end) const { return pos + (unit_ends() ? 2 : 1) < end; }
-  // to that tile
-  __device__ __forceinline__ void next(const PagedArgs& a) {
-    ++pos;
-    if (++t < tiles) return;
-    ++pos;
-    t = 0;
-    if (++rb < a.row_blocks) return;
-    rb = 0;
-    if (++h < a.Hkv) return;
-    h = 0;
-    do {
-      set_request(a, b + 1);
-    } while (tiles == 0 && b + 1 < a.B);
-  }
-};
-
-// 16 bytes of zeros to shared memory where `pred` (without a branch).
-__device__ __forceinline__ void clear16(uint32_t at, bool pred) {
-  asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %1, 0;\n\t@p st.shared.v4.b32 [%0], {%2, %2, %2, %2};\n\t}" ::"r"(at),
-               "r"((uint32_t)pred), "r"(0)
-               : "memory");
-}
-
-// 1 / x to one unit in the last place (x is a sum of weights, 1 or more
-// wherever a row sees anything finite).
-__device__ __forceinline__ float reciprocal(float x) {
-  float y;
-  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-
-__device__ __forceinline__ void prefetch_l2(const void* p) {
-  asm volatile("prefetch.global.L2 [%0];" ::"l"(p));
-}
-
-// Barrier of a team's warps that returns the AND of their `pred`, so that all
-// of them go on alike.
-template <int RG>
-__device__ __forceinline__ bool team_and(int team, bool pred) {
-  if constexpr (RG == 1)
-    return __all_sync(0xffffffffu, pred);
-  else if constexpr (RG == kWarps)
-    return __syncthreads_and(pred);
-  else
-    return kf::named_bar_and(1 + team, RG * 32, pred);
-}
-
 template <bool BF16, int KD, bool FULL, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
@@ -204,9 +109,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   extern __shared__ uint8_t smem_raw[];
   // (an offset, not a rounded address: the compiler keeps seeing shared memory)
   uint8_t* smem = smem_raw + (-kf::smem_u32(smem_raw) & 1023u);
-  __shared__ uint32_t warp_tiles[kWarps];
-  __shared__ int first_request;
-  __shared__ uint32_t first_before;    // tiles of the requests before it
+  __shared__ ShareScratch scratch;
   __shared__ __align__(8) uint64_t full[C::TEAMS][STAGES];
   __shared__ uint32_t seen_s[C::TEAMS][STAGES];  // visible keys of each stage
   __shared__ int abort_any;
@@ -258,94 +161,16 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
-  // ---- this block's share of the list (of fewer than 2^31 positions, see the host's check)
-  const int per = (a.B + kThreads - 1) / kThreads;  // requests per thread, contiguous
-  const int b_lo = min(tid * per, a.B), b_hi = min(b_lo + per, a.B);
-  uint32_t mine = 0;
-  auto positions = [&](int b) {        // of one unit of request b
-    const uint32_t keys = visible(a, b);
-    return keys == 0 ? 0u : (keys + TILE - 1) / TILE + 1;
-  };
-  for (int b = b_lo; b < b_hi; ++b) mine += positions(b);
-  uint32_t upto = mine;
-#pragma unroll
-  for (int off = 1; off < 32; off <<= 1) {
-    const uint32_t y = __shfl_up_sync(0xffffffffu, upto, off);
-    if (lane >= off) upto += y;
-  }
-  if (lane == 31) warp_tiles[warp] = upto;
-  __syncthreads();
-  uint32_t total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) upto += warp_tiles[w];
-    total += warp_tiles[w];
-  }
-  const uint32_t list = total * units;
-  const uint32_t shares = min(gridDim.x, list), me = blockIdx.x;
-
-  // requests without a visible position are nobody's unit
-  auto clear_empty = [&]() {
-    for (int b = (int)me; b < a.B; b += gridDim.x) {
-      if (visible(a, b) != 0) continue;
-      for (int i = tid; i < a.Hq * (a.D / 8); i += kThreads) {
-        const int h = i / (a.D / 8), c = i % (a.D / 8);
-        *reinterpret_cast<uint4*>(a.o + ((int64_t)b * a.Hq + h) * a.D + c * 8) = make_uint4(0, 0, 0, 0);
-      }
-      if (a.lse)
-        for (int h = tid; h < a.Hq; h += kThreads) a.lse[(int64_t)b * a.Hq + h] = -INFINITY;
-      if (a.join_units)
-        for (int u = tid; u < units; u += kThreads) a.joins[b * units + u].x = -1;
-    }
-  };
+  const uint32_t me = blockIdx.x;
   const bool join_blocks = a.joins && !a.join_units;
-  if (me >= shares) {
-    if (tid == 0 && join_blocks) a.joins[me].x = -1;
-    clear_empty();
-    return;
-  }
-  // shares differ by one position at most, the longer ones first
-  const uint32_t even = list / shares, longer = list - even * shares;
-  const uint32_t begin = me * even + min(me, longer);
-  const uint32_t end = begin + even + (me < longer ? 1 : 0);
-  if (begin >= (upto - mine) * units && begin < upto * units) {  // exactly one thread
-    uint32_t sum = upto - mine;
-    int b = b_lo;
-    while (true) {
-      const uint32_t here = positions(b);
-      if (begin < (sum + here) * units) break;
-      sum += here;
-      ++b;
-    }
-    first_request = b;
-    first_before = sum;
-  }
-  __syncthreads();
-
+  Share share;
   Cursor<TILE> load, work;
-  work.set_request(a, first_request);
-  {
-    const uint32_t at = begin - first_before * units;  // inside the request's units
-    const int hr = (int)(at / (work.tiles + 1));
-    work.t = at - hr * (work.tiles + 1);
-    work.h = hr / a.row_blocks;
-    work.rb = hr - work.h * a.row_blocks;
-    work.pos = begin;
-  }
-  bool some = true;                    // whether this share has a tile at all
-  if (work.t == work.tiles) {          // it begins with a unit's end: the first tile is the next unit's
-    some = begin + 1 < end;
-    if (some) {
-      --work.t;
-      --work.pos;
-      work.next(a);
-    }
-  }
-  if (!some) {
+  if (!find_share<TILE>(a, scratch, share) || !first_tile(a, share, work)) {
     if (tid == 0 && join_blocks) a.joins[me].x = -1;
-    clear_empty();
+    clear_empty(a);
     return;
   }
+  const uint32_t end = share.end;
   load = work;
 
   // ---- loads: lane r (of KW) looks up key r of the team's share of a tile
@@ -435,7 +260,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   // bandwidth and end far apart.  Whole ring against a third, D = 128: 8192
   // keys 171.5 and 165.6 us, 600 to 1000 keys 72.8 and 72.9, 200 to 600 keys
   // 72.3 and 74.5, so long starts at 10 tiles; D = 64, 8192 keys: 91.9 and 87.4.
-  const int depth = a.shallow && total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
+  const int depth = a.shallow && share.total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   int issued = 0;
@@ -459,7 +284,7 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
   }
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
-  clear_empty();
+  clear_empty(a);
   start_unit();
 
   int stage = 0, fill = depth;
@@ -699,10 +524,9 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     if (unit_t0 == 0 && tid == 0 && (a.join_units || !unit_done)) {
       // a unit that begins here and goes on ends in the share of its last tile
       const int hr = h * a.row_blocks + rb;
-      const uint32_t last = work.pos + (work.tiles - 1 - work.t), in_longer = longer * (even + 1);
-      const uint32_t share = last < in_longer ? last / (even + 1) : longer + (last - in_longer) / even;
+      const uint32_t last = share_of(share, work.pos + (work.tiles - 1 - work.t));
       a.joins[a.join_units ? (int64_t)b * units + hr : (int64_t)me] =
-          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)share);
+          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)last);
     }
     if (going) {
       work.next(a);
@@ -848,107 +672,6 @@ paged_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_cons
     }
 }
 
-// Joins the partials of a unit that was cut: slot 1 of its first share, slot 0
-// of the shares up to its last.  A group of D / 4 lanes takes one row, alone
-// or, where a unit has many partials, with `split` - 1 others that take every
-// split-th partial; each partial is read once, with a running maximum, and the
-// groups' results meet in shared memory.
-constexpr int kJoinThreads = 256;
-constexpr int kJoinBatch = 8;  // partials a group has in flight (4: 0.3 to 0.5 us more on calls of 12 to 50 us)
-
-template <bool BF16>
-__global__ void __launch_bounds__(kJoinThreads) paged_join_kernel(const PagedArgs a, int rows, int split) {
-  kf::griddep_wait();
-  kf::griddep_launch_dependents();
-  const int4 unit = a.joins[blockIdx.x];
-  if (unit.x < 0) return;
-  const int h = unit.y / a.row_blocks, rb = unit.y - h * a.row_blocks;
-  const int count = unit.w - unit.z + 1;
-  __shared__ float4 acc_s[kJoinThreads];
-  __shared__ float m_s[kJoinThreads / 4], l_s[kJoinThreads / 4];
-  const int lanes = a.D / 4, per_block = kJoinThreads / lanes / split;  // rows of a block
-  const int g = threadIdx.x / lanes, c = threadIdx.x % lanes;
-  const int part = g % split, r = blockIdx.y * per_block + g / split;
-  const bool mine = g < per_block * split && r < min(rows, a.G - rb * rows);
-  float m = -INFINITY, l = 0.f;
-  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (mine) {
-    for (int j0 = part; j0 < count; j0 += split * kJoinBatch) {
-      float lse[kJoinBatch];
-      float4 o[kJoinBatch];
-#pragma unroll
-      for (int x = 0; x < kJoinBatch; ++x) {
-        const int j = j0 + x * split;
-        lse[x] = -INFINITY;
-        o[x] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (j < count) {
-          const int64_t row = (((int64_t)unit.z + j) * 2 + (j == 0 ? 1 : 0)) * rows + r;
-          lse[x] = a.part_lse[row];
-          o[x] = *reinterpret_cast<const float4*>(a.part_o + row * a.D + c * 4);
-        }
-      }
-      float top = m;
-#pragma unroll
-      for (int x = 0; x < kJoinBatch; ++x) top = fmaxf(top, lse[x]);
-      const float mu = top == -INFINITY ? 0.f : top;
-      const float old = kf::ex2(m - mu);
-      l *= old;
-      acc.x *= old;
-      acc.y *= old;
-      acc.z *= old;
-      acc.w *= old;
-#pragma unroll
-      for (int x = 0; x < kJoinBatch; ++x) {
-        const float w = kf::ex2(lse[x] - mu);
-        l += w;
-        acc.x += w * o[x].x;
-        acc.y += w * o[x].y;
-        acc.z += w * o[x].z;
-        acc.w += w * o[x].w;
-      }
-      m = top;
-    }
-  }
-  if (split > 1) {
-    acc_s[threadIdx.x] = acc;
-    if (mine && c == 0) {
-      m_s[g] = m;
-      l_s[g] = l;
-    }
-    __syncthreads();
-    if (mine && part == 0) {
-      float top = m;
-      for (int i = 1; i < split; ++i) top = fmaxf(top, m_s[g + i]);
-      const float mu = top == -INFINITY ? 0.f : top;
-      const float old = kf::ex2(m - mu);
-      l *= old;
-      acc.x *= old;
-      acc.y *= old;
-      acc.z *= old;
-      acc.w *= old;
-      for (int i = 1; i < split; ++i) {
-        const float w = kf::ex2(m_s[g + i] - mu);
-        const float4 x = acc_s[threadIdx.x + i * lanes];
-        l += w * l_s[g + i];
-        acc.x += w * x.x;
-        acc.y += w * x.y;
-        acc.z += w * x.z;
-        acc.w += w * x.w;
-      }
-      m = top;
-    }
-  }
-  if (!mine || part != 0) return;
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int head = h * a.G + rb * rows + r;
-  *reinterpret_cast<uint2*>(a.o + ((int64_t)unit.x * a.Hq + head) * a.D + c * 4) =
-      make_uint2(kf::pack2<BF16>(acc.x * inv, acc.y * inv), kf::pack2<BF16>(acc.z * inv, acc.w * inv));
-  if (a.lse && c == 0) a.lse[(int64_t)unit.x * a.Hq + head] = l == 0.f ? -INFINITY : (m + log2f(l)) * kLn2;
-}
-
-// Query rows of a unit for G rows per KV head, and the variant that has them.
-int unit_rows(int64_t G) { return G <= 8 ? 8 : G <= 16 ? 16 : G <= 32 ? 32 : 64; }
-
 // KD of the variant for a head dim.
 int head_steps(int64_t D, bool wide) { return D <= 64 ? 4 : D <= 96 && !wide ? 6 : 8; }
 
@@ -962,10 +685,6 @@ int tile_keys_of(int rows) {
 }
 int tile_keys(int steps, int rows) {
   return steps == 4 ? tile_keys_of<4>(rows) : steps == 6 ? tile_keys_of<6>(rows) : tile_keys_of<8>(rows);
-}
-
-size_t workspace_need(int blocks, int rows, int64_t D) {
-  return 256 + (size_t)blocks * (16 + (size_t)2 * rows * 4 + (size_t)2 * rows * D * 4);
 }
 
 template <bool BF16, int KD, bool FULL, int NT, int RG>
@@ -1080,14 +799,9 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.Hkv = (int)Hkv;
   a.G = (int)(Hq / Hkv);
   a.D = (int)D;
-  a.row_blocks = (a.G + rows - 1) / rows;
-  const int64_t capacity = max_pages * page_size;
-  a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
-  a.max_pages = (uint32_t)max_pages;
   a.page_size = (uint32_t)page_size;
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
-  kf::division(page_size, &a.page_mul, &a.page_shift);
   // Boxes of 16 rows (32 where one panel or no swizzle holds a row) never cross
   // a page nor a team's keys; smaller ones where 16 does not divide the pages.
   const bool full = D == 64 || D == 128, odd = D % 16 != 0;
@@ -1118,31 +832,13 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
   a.scale_log2 = fmaxf(fabsf((float)args->scale) * kLog2e, FLT_TRUE_MIN);
   a.q_sign = args->scale < 0 ? 0x80008000u : 0u;
 
-  // One wave of blocks, or fewer when the tables cannot hold that many tiles.
-  // A unit of one tile is never cut, so nothing is left to join.
   const int steps = head_steps(D, wide);
-  const int64_t tile = tile_keys(steps, rows), most = (a.capacity + tile - 1) / tile;
-  const int64_t units = B * Hkv * a.row_blocks;
-  int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
-  if (units * (most + 1) > 0x7fffffffLL) return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
-  if (most == 1 && units < blocks) blocks = units;
-  if (units * (most + 1) < blocks) blocks = units * (most + 1);
-  a.part_o = nullptr;
-  a.part_lse = nullptr;
-  a.joins = nullptr;
-  a.join_units = false;
-  if (most > 1) {
-    const size_t need = workspace_need((int)blocks, rows, D);
-    if (!args->workspace || args->workspace_bytes < need)
-      return set_error(KF_ERR_WORKSPACE, "%s: workspace needs %zu bytes", what, need);
-    uintptr_t base = (reinterpret_cast<uintptr_t>(args->workspace) + 255) & ~uintptr_t(255);
-    a.joins = reinterpret_cast<int4*>(base);
-    a.part_o = reinterpret_cast<float*>(a.joins + blocks);
-    a.part_lse = a.part_o + (size_t)blocks * 2 * rows * D;
-    a.join_units = units < blocks;  // whichever list is shorter
-  }
+  int64_t blocks, most;
+  int rc = plan_work(what, a, max_pages, rows, tile_keys(steps, rows), args->workspace, args->workspace_bytes, &blocks,
+                     &most);
+  if (rc != KF_OK) return rc;
   CUtensorMap mk, mv;
-  int rc = kf::encode_tmap_pages(&mk, k_pages, cols, a.box, panels, a.width != 0);
+  rc = kf::encode_tmap_pages(&mk, k_pages, cols, a.box, panels, a.width != 0);
   if (rc != KF_OK) return rc;
   rc = kf::encode_tmap_pages(&mv, v_pages, cols, a.box, panels, a.width != 0);
   if (rc != KF_OK) return rc;
@@ -1164,14 +860,5 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
     rc = bf16 ? dispatch_rows<true, 8, false>(a, mk, mv, rows, (int)blocks, st)
               : dispatch_rows<false, 8, false>(a, mk, mv, rows, (int)blocks, st);
   if (rc != KF_OK || most == 1) return rc;
-  // Groups that share a row: as many as leave each about one batch of the
-  // partials that a unit has on average (2 where units outnumber the blocks).
-  const int groups = kJoinThreads / (int)(D / 4);
-  const int64_t partials = a.join_units ? blocks / units + 1 : 2;
-  int split = 1;
-  while (split * kJoinBatch < partials && split * 2 <= groups) split *= 2;
-  const int per_block = groups / split, row_count = a.G < rows ? a.G : rows;
-  const dim3 grid((unsigned)(a.join_units ? units : blocks), (unsigned)((row_count + per_block - 1) / per_block));
-  return bf16 ? kf::launch_dependent(paged_join_kernel<true>, grid, dim3(kJoinThreads), 0, st, what, a, rows, split)
-              : kf::launch_dependent(paged_join_kernel<false>, grid, dim3(kJoinThreads), 0, st, what, a, rows, split);
+  return launch_join(what, a, bf16, rows, blocks, st);
 }
