@@ -342,6 +342,106 @@ typedef struct kf_paged_release_args {
 int kf_paged_reserve(const kf_paged_reserve_args* args);
 int kf_paged_release(const kf_paged_release_args* args);
 
+/* ---- K7: rotary positions -------------------------------------------------
+ * No counterpart in the reference.  Column pairs of the first `rotated`
+ * columns of q [B, Hq, S, D] and k [B, Hkv, S, D] (k and k_out may be absent:
+ * ptr NULL) turn by position * frequency: pair i is column i with i + rotated
+ * / 2, or, interleaved, 2 i with 2 i + 1;
+ *   a' = (a cos t - b sin t) magnitude,  b' = (b cos t + a sin t) magnitude.
+ * The other columns are copied.  inverse != 0 turns by -t, which is the
+ * gradient.  positions: int32 or int64 (position_bits) by batch entry and
+ * token, with element strides; frequencies: rotated / 2 doubles, radians per
+ * position.  Any strides with a contiguous last dim; q_out may be q and k_out
+ * k, with the same strides. */
+typedef struct kf_rotary_args {
+  kf_tensor4    q, k, q_out, k_out;
+  const void*   positions;
+  int64_t       position_bits;
+  int64_t       position_strides[2];
+  const double* frequencies;
+  int64_t       rotated, interleaved, inverse;
+  double        magnitude;
+  int64_t       dtype;
+  void*         stream;
+} kf_rotary_args;
+int kf_rotary(const kf_rotary_args* args);
+
+/* ---- K8, K9: the paged cache in 8 bits -------------------------------------
+ * No counterpart in the reference.  Pools as in K5, with elements of one byte:
+ * k_pages and v_pages [pages, Hkv, page_size, D], contiguous last dim, rows on
+ * 16 bytes, strides in elements and positive.  format: KF_E4M3 (4 exponent and
+ * 3 fraction bits, no infinities) or KF_INT8.  k_scales and v_scales hold one
+ * byte for each `scale_block` rows (a power of two up to 128 that divides
+ * page_size) of a page and head, [pages, Hkv, page_size / scale_block] with
+ * strides for the first two and a contiguous last: 127 + the exponent of a
+ * power of two, or 255 for NaN.  An element is its code times that power.
+ *
+ * Storing gives a block the smallest power of two with which its rows' largest
+ * magnitude is at most 448 (e4m3) or rounds to at most 127 (int8), exponents
+ * lying within +-60, and rounds to nearest, ties to even.  A block with an
+ * infinity, a NaN or a magnitude beyond that gets scale 255, and its rows'
+ * codes are 0.  With more than one row to a scale, rows are written in order:
+ * a row that is not its block's first joins the rows before it, whose codes
+ * are rounded again if the scale grows (a scale never shrinks, and 255 stays);
+ * the block's first row begins it anew.  Rows behind the newest are left.
+ *
+ * kf_paged8_append stores new_k / new_v [N, Hkv, S, D], token t = n * S + s,
+ * at slot slots[t], skipping those outside the pool.  With more than one row
+ * to a scale, the tokens of one block follow one another in slots (as
+ * kf_paged_reserve gives them); two separate runs into one block leave either's
+ * scale.
+ *
+ * kf_paged8_read is the way back: k_out / v_out [N, Hkv, S, D], rounded once
+ * (and only where the type cannot hold code times power); rows whose slot is
+ * outside the pool are 0.
+ *
+ * kf_paged8_decode is kf_paged_decode over such a cache; dtype is that of q, o
+ * and the new rows, which are attended to as they are stored.  With more than
+ * one row to a scale the new rows take a launch of their own. */
+#define KF_E4M3 0
+#define KF_INT8 1
+typedef struct kf_paged8_cache {
+  kf_tensor4 k_pages, v_pages;
+  uint8_t*   k_scales;
+  uint8_t*   v_scales;
+  int64_t    k_scale_strides[2], v_scale_strides[2];
+  int64_t    scale_block;
+  int64_t    format;
+} kf_paged8_cache;
+typedef struct kf_paged8_append_args {
+  kf_paged8_cache cache;
+  kf_tensor4      new_k, new_v;
+  const int64_t*  slots;
+  int64_t         dtype;
+  void*           stream;
+} kf_paged8_append_args;
+typedef struct kf_paged8_read_args {
+  kf_paged8_cache cache;
+  kf_tensor4      k_out, v_out;
+  const int64_t*  slots;
+  int64_t         dtype;
+  void*           stream;
+} kf_paged8_read_args;
+typedef struct kf_paged8_decode_args {
+  kf_paged8_cache cache;
+  kf_tensor4      q, new_k, new_v;
+  const int64_t*  slots;
+  const int32_t*  block_table;
+  int64_t         max_pages, table_stride;
+  const int32_t*  lengths;
+  void*           o;
+  float*          lse;
+  int64_t         dtype;
+  double          scale;
+  void*           workspace;
+  uint64_t        workspace_bytes;  /* kf_paged_decode_workspace_bytes(...) */
+  int32_t*        status;
+  void*           stream;
+} kf_paged8_decode_args;
+int kf_paged8_append(const kf_paged8_append_args* args);
+int kf_paged8_read(const kf_paged8_read_args* args);
+int kf_paged8_decode(const kf_paged8_decode_args* args);
+
 /* ---- the process's status word -------------------------------------------
  * No counterpart in the reference.  *word is the address of an int32 of
  * `device`'s memory for the `status` arguments above: 0 until an expired wait

@@ -11,6 +11,8 @@ from . import _ext
 from .attention import attention
 from .cache import PreallocatedKVCache, append_kv_cache, decode_step
 from .paged import PagedKVCache, append_paged_kv, paged_attention, release_pages, reserve_pages
+from .paged8 import PagedKVCache8, append_paged_kv8, paged_attention8, read_paged_kv8
+from .rotary import apply_rotary, rotary_frequencies
 
 
 def triton_available() -> bool:
@@ -39,5 +41,11 @@ __all__ = [
     "append_paged_kv",
     "reserve_pages",
     "release_pages",
+    "PagedKVCache8",
+    "paged_attention8",
+    "append_paged_kv8",
+    "read_paged_kv8",
+    "apply_rotary",
+    "rotary_frequencies",
 ]
 __version__ = "1.0.0"

@@ -37,6 +37,9 @@ KF_ERR_WORKSPACE = 4
 KF_F16 = 0
 KF_BF16 = 1
 
+KF_E4M3 = 0
+KF_INT8 = 1
+
 
 class KFTensor4(ctypes.Structure):
     _fields_ = [
@@ -77,6 +80,10 @@ SIGNATURES = {
     "kf_paged_append": (_I, [_BYTES]),
     "kf_paged_reserve": (_I, [_BYTES]),
     "kf_paged_release": (_I, [_BYTES]),
+    "kf_rotary": (_I, [_BYTES]),
+    "kf_paged8_append": (_I, [_BYTES]),
+    "kf_paged8_read": (_I, [_BYTES]),
+    "kf_paged8_decode": (_I, [_BYTES]),
     "kf_device_status": (_I, [_I, ctypes.POINTER(_VP)]),
     "kf_selftest_bounded_wait": (_I, [_VP, _I64, _VP]),
     "kf_selftest_exp2_poly": (_I, [_VP, _VP, _I64, _VP]),
@@ -176,6 +183,11 @@ pack_paged_append = struct.Struct("=" + _PT4 * 4 + "QqQ").pack
 _TABLES = "QqQqqQqQqQQQ"  # a kf_page_tables
 pack_paged_reserve = struct.Struct("=" + _TABLES + "QQqqQ").pack
 pack_paged_release = struct.Struct("=" + _TABLES + "Q").pack
+_CACHE8 = _PT4 * 2 + "QQqqqqqq"  # a kf_paged8_cache
+pack_paged8_append = struct.Struct("=" + _CACHE8 + _PT4 * 2 + "QqQ").pack  # and of a read
+pack_paged8_decode = struct.Struct("=" + _CACHE8 + _PT4 + "152x" + _DECODE).pack
+pack_paged8_step = struct.Struct("=" + _CACHE8 + _PT4 * 3 + "Q" + _DECODE).pack
+pack_rotary = struct.Struct("=" + _PT4 * 4 + "QqqqQqqqdqQ").pack
 
 
 def ref(d: Optional[KFTensor4]):

@@ -1,0 +1,383 @@
+// K8: rows of K and V into 8-bit pools of pages, and back.
+//
+// Storing reads 2 bytes and writes 1 per element of K and V, reading back the
+// reverse, with a few operations between, so HBM bounds both.  A row (one
+// token, one head) belongs to a group of 2 to 16 lanes with 8 values each;
+// the largest magnitude goes round the group by shuffles, as 16-bit patterns,
+// two at a time.
+#include "paged8.cuh"
+
+namespace {
+
+constexpr int kThreads = 256;
+
+struct Rows8Args {
+  uint16_t* rows[2];       // K and V: the source of a store, the destination of a load
+  uint8_t* pages[2];
+  uint8_t* scales[2];
+  const int64_t* slots;
+  int64_t rs[2][3], ps[2][3], ss[2][2];
+  int64_t num_slots;
+  uint32_t T, S, heads;    // tokens in all, and per batch entry
+  uint32_t page_size, page_mul, page_shift;
+  int chunks;              // D / 8
+  int block_shift;         // log2 of the tokens of a scale
+};
+
+// Page and row of a slot; slots of a pool fit 31 bits unless it holds over 2^31 tokens.
+__device__ __forceinline__ int64_t page_of(const Rows8Args& a, int64_t slot, uint32_t& row) {
+  const int64_t page = a.num_slots <= 0x7fffffffLL ? (int64_t)(((uint64_t)(uint32_t)slot * a.page_mul) >> a.page_shift)
+                                                   : slot / a.page_size;
+  row = (uint32_t)(slot - page * a.page_size);
+  return page;
+}
+
+__device__ __forceinline__ uint16_t* row_at(const Rows8Args& a, int w, uint32_t t, uint32_t h) {
+  const uint32_t n = a.S == a.T ? 0 : t / a.S, s = t - n * a.S;
+  return a.rows[w] + n * a.rs[w][0] + h * a.rs[w][1] + s * a.rs[w][2];
+}
+
+// ---------------------------------------------------------------- a scale for each row
+template <bool INT8, bool BF16, int GROUP, int U>
+__global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
+  constexpr uint32_t ROWS = kThreads / GROUP;  // of a block, side by side
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  const int c = threadIdx.x % GROUP;
+  const uint32_t total = a.T * a.heads, first = blockIdx.x * (ROWS * U) + threadIdx.x / GROUP;
+  uint32_t token[U], head[U];
+  int64_t slot[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint32_t r = first + u * ROWS;
+    token[u] = r / a.heads;
+    head[u] = r - token[u] * a.heads;
+    slot[u] = r < total ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token[u]) : -1;
+    if (slot[u] >= a.num_slots) slot[u] = -1;  // no such slot: the token is not stored
+  }
+  uint4 val[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      val[u][w] = make_uint4(0, 0, 0, 0);
+      if (slot[u] >= 0 && c < a.chunks)
+        val[u][w] = __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, token[u], head[u])) + c);
+    }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint32_t row;
+    const int64_t page = page_of(a, slot[u] < 0 ? 0 : slot[u], row);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      uint32_t m = kf::magnitudes(val[u][w]);
+#pragma unroll
+      for (int off = 1; off < GROUP; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
+      const int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
+      const bool nan = e > kf::kMaxExponent;
+      uint2 codes = kf::encode8<INT8, BF16>(val[u][w], nan ? 0.f : kf::power2(-e));
+      if (nan) codes = make_uint2(0, 0);
+      if (slot[u] < 0) continue;
+      if (c < a.chunks)
+        *reinterpret_cast<uint2*>(a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * 8) = codes;
+      if (c == 0) a.scales[w][page * a.ss[w][0] + head[u] * a.ss[w][1] + row] = (uint8_t)kf::scale_byte(e);
+    }
+  }
+}
+
+// ---------------------------------------------------------------- a scale for several rows
+// The tokens of a call that go to one block one after another (a run) are
+// one warp's: their largest magnitude, with the block's scale if it has rows
+// before them, gives the scale; if it grows, those rows are rounded again.  A
+// warp looks after the runs that begin in a window of `block` tokens.
+template <bool INT8, bool BF16>
+__global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Args a) {
+  constexpr int GROUP = 16, SIDE = 32 / GROUP;
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  const int lane = threadIdx.x & 31, c = lane % GROUP, g = lane / GROUP;
+  const uint32_t warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
+  const uint32_t size = 1u << a.block_shift;
+  const uint32_t window = warp / (2 * a.heads), hw = warp - window * (2 * a.heads), h = hw >> 1;
+  const int w = hw & 1;
+  const uint64_t from = (uint64_t)window * size, until = min(from + size, (uint64_t)a.T);
+  auto slot_at = [&](uint64_t t) { return __ldcg(reinterpret_cast<const long long*>(a.slots) + t); };
+  auto follows = [&](int64_t before, int64_t s) { return before == s - 1 && before >> a.block_shift == s >> a.block_shift; };
+  for (uint64_t base = from; base < until; base += 32) {
+    const uint64_t t = base + lane;
+    const int64_t s = t < until ? slot_at(t) : -1, before = t > 0 && t < until ? slot_at(t - 1) : -2;
+    uint32_t leaders = __ballot_sync(0xffffffffu, s >= 0 && s < a.num_slots && !follows(before, s));
+    for (; leaders; leaders &= leaders - 1) {
+      const int who = __ffs(leaders) - 1;
+      const uint64_t t0 = base + who;
+      const int64_t s0 = __shfl_sync(0xffffffffu, (long long)s, who);
+      const uint32_t inside = (uint32_t)(s0 & (size - 1));
+      uint32_t n = 0;  // tokens of the run
+      for (uint32_t more = 32; more == 32 && n < size - inside;) {
+        const uint64_t i = n + lane;
+        const uint32_t in = __ballot_sync(0xffffffffu, i < size - inside && t0 + i < a.T && slot_at(t0 + i) == s0 + (int64_t)i);
+        more = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+        n += more;
+      }
+      uint32_t row;
+      const int64_t page = page_of(a, s0, row);
+      auto source = [&](uint32_t i) { return __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, (uint32_t)t0 + i, h)) + c); };
+      uint8_t* codes = a.pages[w] + page * a.ps[w][0] + h * a.ps[w][1] + (int64_t)row * a.ps[w][2] + c * 8;
+      uint8_t* scale = a.scales[w] + page * a.ss[w][0] + h * a.ss[w][1] + (row >> a.block_shift);
+      uint32_t m = 0;
+      if (c < a.chunks) {
+#pragma unroll 4
+        for (uint32_t i = g; i < n; i += SIDE) m = kf::max_magnitudes(m, kf::magnitudes(source(i)));
+      }
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
+      int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
+      bool nan = e > kf::kMaxExponent;
+      if (inside > 0) {
+        const uint32_t old = __ldcg(scale);
+        const int was = kf::scale_of_byte(old);
+        nan |= old == kf::kNanScale;
+        e = max(e, was);
+        if ((nan || e > was) && c < a.chunks) {
+          const float shift = nan ? 0.f : kf::power2(max(was - e, -126));
+          for (uint32_t i = g; i < inside; i += SIDE) {
+            uint2* at = reinterpret_cast<uint2*>(codes - (int64_t)(inside - i) * a.ps[w][2]);
+            const uint2 x = __ldcg(at);
+            float p[4], q[4];
+            kf::decode4<INT8>(x.x, p);
+            kf::decode4<INT8>(x.y, q);
+            *at = nan ? make_uint2(0, 0)
+                      : make_uint2(kf::encode4<INT8>(p[0] * shift, p[1] * shift, p[2] * shift, p[3] * shift),
+                                   kf::encode4<INT8>(q[0] * shift, q[1] * shift, q[2] * shift, q[3] * shift));
+          }
+        }
+      }
+      const float by = nan ? 0.f : kf::power2(-e);
+      if (c < a.chunks) {
+#pragma unroll 4
+        for (uint32_t i = g; i < n; i += SIDE) {
+          const uint2 x = kf::encode8<INT8, BF16>(source(i), by);
+          *reinterpret_cast<uint2*>(codes + (int64_t)i * a.ps[w][2]) = nan ? make_uint2(0, 0) : x;
+        }
+      }
+      __syncwarp();  // every lane has read the old scale
+      if (lane == 0) *scale = (uint8_t)(nan ? kf::kNanScale : kf::scale_byte(e));
+    }
+  }
+}
+
+// ---------------------------------------------------------------- reading back
+// A thread takes VEC / 8 chunks of a row of K and of V, for U rows.
+template <bool INT8, bool BF16, int VEC, int U>
+__global__ void __launch_bounds__(kThreads) read8_kernel(const Rows8Args a) {
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+  constexpr int W = VEC / 4;  // words of codes
+  const uint32_t per_row = a.chunks * 8 / VEC, total = a.T * a.heads;
+  const uint32_t index = blockIdx.x * kThreads + threadIdx.x, r0 = index / per_row, c = index - r0 * per_row;
+  const uint32_t step = gridDim.x * kThreads / per_row;  // rows apart, a thread's own
+  if (r0 >= step) return;
+  int64_t slot[U];
+  uint32_t token[U], head[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const uint64_t r = r0 + (uint64_t)u * step;
+    head[u] = r < total ? (uint32_t)r / a.T : 0;
+    token[u] = r < total ? (uint32_t)r - head[u] * a.T : 0;
+    slot[u] = r < total ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token[u]) : -2;
+    if (slot[u] >= a.num_slots || slot[u] < -1) slot[u] = slot[u] == -2 && r >= total ? -2 : -1;
+  }
+  uint32_t codes[U][2][W], scale[U][2];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    uint32_t row;
+    const int64_t page = page_of(a, slot[u] < 0 ? 0 : slot[u], row);
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      scale[u][w] = 127;
+#pragma unroll
+      for (int i = 0; i < W; ++i) codes[u][w][i] = 0;
+      if (slot[u] < 0) continue;
+      const uint8_t* p = a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * VEC;
+      if constexpr (VEC == 16) {
+        const uint4 x = __ldcg(reinterpret_cast<const uint4*>(p));
+        codes[u][w][0] = x.x, codes[u][w][1] = x.y, codes[u][w][2] = x.z, codes[u][w][3] = x.w;
+      } else {
+        const uint2 x = __ldcg(reinterpret_cast<const uint2*>(p));
+        codes[u][w][0] = x.x, codes[u][w][1] = x.y;
+      }
+      scale[u][w] = __ldcg(a.scales[w] + page * a.ss[w][0] + head[u] * a.ss[w][1] + (row >> a.block_shift));
+    }
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      if (slot[u] == -2) continue;
+      const float by = scale[u][w] == kf::kNanScale ? __uint_as_float(0x7fc00000u)
+                                                    : kf::power2(kf::scale_of_byte(scale[u][w]));
+      uint4* to = reinterpret_cast<uint4*>(row_at(a, w, token[u], head[u])) + c * (VEC / 8);
+#pragma unroll
+      for (int i = 0; i < W; i += 2) {
+        float p[4], q[4];
+        if (slot[u] < 0) {
+          to[i / 2] = make_uint4(0, 0, 0, 0);
+          continue;
+        }
+        kf::decode4<INT8>(codes[u][w][i], p);
+        kf::decode4<INT8>(codes[u][w][i + 1], q);
+        to[i / 2] = make_uint4(kf::pack2<BF16>(p[0] * by, p[1] * by), kf::pack2<BF16>(p[2] * by, p[3] * by),
+                               kf::pack2<BF16>(q[0] * by, q[1] * by), kf::pack2<BF16>(q[2] * by, q[3] * by));
+      }
+    }
+}
+
+bool rows16(const kf_tensor4& t) {
+  if (!kf::aligned16(t.ptr) || t.stride[3] != 1) return false;
+  for (int i = 0; i < 3; ++i)
+    if (t.size[i] > 1 && t.stride[i] % 8 != 0) return false;
+  return true;
+}
+
+// Arguments that a store and a load share: a cache, two tensors of rows, slots.
+int set_up(const char* what, const kf_paged8_cache& cache, const kf_tensor4& k, const kf_tensor4& v, const int64_t* slots,
+           int64_t dtype, Rows8Args* a) {
+  using kf::set_error;
+  if (dtype != KF_F16 && dtype != KF_BF16) return set_error(KF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  const int rc = kf::check_cache8(what, cache);
+  if (rc != KF_OK) return rc;
+  for (int i = 0; i < 4; ++i)
+    if (k.size[i] != v.size[i]) return set_error(KF_ERR_INVALID, "%s: the shapes of the K and V rows must match", what);
+  const int64_t N = k.size[0], H = k.size[1], S = k.size[2], D = k.size[3];
+  if (H != cache.k_pages.size[1] || D != cache.k_pages.size[3])
+    return set_error(KF_ERR_INVALID, "%s: heads and head_dim of the rows must match the pages", what);
+  if (N <= 0 || S <= 0) return set_error(KF_ERR_INVALID, "%s: dimensions must be non-zero", what);
+  if (N > 0x7fffffffLL || S > 0x7fffffffLL || N * S > 0x7fffffffLL || N * S * H > 0x0fffffffLL)
+    return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
+  if (!k.ptr || !v.ptr || !slots) return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (!rows16(k) || !rows16(v))
+    return set_error(KF_ERR_INVALID, "%s: K/V rows must be contiguous and 16-byte aligned", what);
+  a->rows[0] = static_cast<uint16_t*>(k.ptr);
+  a->rows[1] = static_cast<uint16_t*>(v.ptr);
+  a->pages[0] = static_cast<uint8_t*>(cache.k_pages.ptr);
+  a->pages[1] = static_cast<uint8_t*>(cache.v_pages.ptr);
+  a->scales[0] = cache.k_scales;
+  a->scales[1] = cache.v_scales;
+  a->slots = slots;
+  for (int i = 0; i < 3; ++i) {
+    a->rs[0][i] = k.stride[i];
+    a->rs[1][i] = v.stride[i];
+    a->ps[0][i] = cache.k_pages.stride[i];
+    a->ps[1][i] = cache.v_pages.stride[i];
+  }
+  for (int i = 0; i < 2; ++i) {
+    a->ss[0][i] = cache.k_scale_strides[i];
+    a->ss[1][i] = cache.v_scale_strides[i];
+  }
+  const int64_t page_size = cache.k_pages.size[2];
+  a->num_slots = cache.k_pages.size[0] * page_size;
+  a->T = (uint32_t)(N * S);
+  a->S = (uint32_t)S;
+  a->heads = (uint32_t)H;
+  a->page_size = (uint32_t)page_size;
+  kf::division(page_size, &a->page_mul, &a->page_shift);
+  a->chunks = (int)(D / 8);
+  a->block_shift = 0;
+  while (((int64_t)1 << a->block_shift) < cache.scale_block) ++a->block_shift;
+  return KF_OK;
+}
+
+template <bool INT8, bool BF16>
+int launch_append(const Rows8Args& a, cudaStream_t st) {
+  const char* what = "kf_paged8_append";
+  if (a.block_shift > 0) {
+    const uint64_t windows = ((uint64_t)a.T + (1u << a.block_shift) - 1) >> a.block_shift;
+    const uint64_t warps = windows * 2 * a.heads;
+    const unsigned blocks = (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32));
+    return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kThreads), 0, st, what, a);
+  }
+  const uint64_t rows = (uint64_t)a.T * a.heads;
+  auto go = [&](auto kern, int group, int u) {
+    const uint64_t per_block = (uint64_t)(kThreads / group) * u;
+    return kf::launch_dependent(kern, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(kThreads), 0, st, what, a);
+  };
+  // Two rows of K and V a thread in flight once that still leaves a block per SM.
+  const bool many = rows * 16 >= (uint64_t)kf::sm_count_current_device() * kThreads * 2;
+  if (a.chunks <= 2) return go(append8_kernel<INT8, BF16, 2, 1>, 2, 1);
+  if (a.chunks <= 4) return go(append8_kernel<INT8, BF16, 4, 1>, 4, 1);
+  if (a.chunks <= 8) return many ? go(append8_kernel<INT8, BF16, 8, 2>, 8, 2) : go(append8_kernel<INT8, BF16, 8, 1>, 8, 1);
+  return many ? go(append8_kernel<INT8, BF16, 16, 2>, 16, 2) : go(append8_kernel<INT8, BF16, 16, 1>, 16, 1);
+}
+
+template <bool INT8, bool BF16>
+int launch_read(const Rows8Args& a, cudaStream_t st) {
+  const int vec = a.chunks % 2 == 0 ? 16 : 8;
+  const uint32_t per_row = a.chunks * 8 / vec;
+  constexpr int U = 2;
+  const uint64_t rows = (uint64_t)a.T * a.heads, threads = (rows + U - 1) / U * per_row;
+  // whole rows in the grid's stride: kThreads * blocks divided by per_row, rounded down, covers them
+  const unsigned blocks = (unsigned)((threads + per_row + kThreads - 1) / kThreads);
+  return vec == 16 ? kf::launch_dependent(read8_kernel<INT8, BF16, 16, U>, dim3(blocks), dim3(kThreads), 0, st,
+                                          "kf_paged8_read", a)
+                   : kf::launch_dependent(read8_kernel<INT8, BF16, 8, U>, dim3(blocks), dim3(kThreads), 0, st,
+                                          "kf_paged8_read", a);
+}
+
+}  // namespace
+
+namespace kf {
+
+int check_cache8(const char* what, const kf_paged8_cache& c) {
+  const kf_tensor4 &k = c.k_pages, &v = c.v_pages;
+  if (c.format != KF_E4M3 && c.format != KF_INT8)
+    return set_error(KF_ERR_INVALID, "%s: pages must be e4m3 or int8", what);
+  for (int i = 0; i < 4; ++i)
+    if (k.size[i] != v.size[i]) return set_error(KF_ERR_INVALID, "%s: K/V page shapes must match", what);
+  const int64_t D = k.size[3], page_size = k.size[2], block = c.scale_block;
+  if (k.size[0] <= 0 || k.size[1] <= 0 || page_size <= 0)
+    return set_error(KF_ERR_INVALID, "%s: dimensions must be non-zero", what);
+  if (D < 16 || D > 128 || D % 8 != 0)
+    return set_error(KF_ERR_UNSUPPORTED, "%s: head_dim must be a multiple of 8 in [16, 128]", what);
+  if (page_size > (1 << 20) || k.size[0] > 0x7fffffffLL || k.size[1] > (1 << 16))
+    return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
+  if (block <= 0 || block > 128 || (block & (block - 1)) || page_size % block)
+    return set_error(KF_ERR_INVALID, "%s: the tokens of a scale must be a power of two up to 128 that divides page_size", what);
+  for (const kf_tensor4* t : {&k, &v}) {
+    bool good = aligned16(t->ptr) && t->stride[3] == 1;
+    for (int i = 0; i < 3; ++i)
+      if (t->size[i] > 1 && (t->stride[i] % 16 != 0 || t->stride[i] <= 0)) good = false;
+    if (!good) return set_error(KF_ERR_INVALID, "%s: pages need a contiguous last dim and 16-byte aligned rows", what);
+  }
+  if (!k.ptr || !v.ptr || !c.k_scales || !c.v_scales) return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  return KF_OK;
+}
+
+}  // namespace kf
+
+extern "C" int kf_paged8_append(const kf_paged8_append_args* args) {
+  const char* what = "kf_paged8_append";
+  if (!args) return kf::set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  Rows8Args a;
+  const int rc = set_up(what, args->cache, args->new_k, args->new_v, args->slots, args->dtype, &a);
+  if (rc != KF_OK) return rc;
+  kf::DeviceGuard guard(args->cache.k_pages.ptr);
+  if (guard.status()) return guard.status();
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
+  if (args->cache.format == KF_INT8)
+    return args->dtype == KF_BF16 ? launch_append<true, true>(a, st) : launch_append<true, false>(a, st);
+  return args->dtype == KF_BF16 ? launch_append<false, true>(a, st) : launch_append<false, false>(a, st);
+}
+
+extern "C" int kf_paged8_read(const kf_paged8_read_args* args) {
+  const char* what = "kf_paged8_read";
+  if (!args) return kf::set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  Rows8Args a;
+  const int rc = set_up(what, args->cache, args->k_out, args->v_out, args->slots, args->dtype, &a);
+  if (rc != KF_OK) return rc;
+  kf::DeviceGuard guard(args->cache.k_pages.ptr);
+  if (guard.status()) return guard.status();
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
+  if (args->cache.format == KF_INT8)
+    return args->dtype == KF_BF16 ? launch_read<true, true>(a, st) : launch_read<true, false>(a, st);
+  return args->dtype == KF_BF16 ? launch_read<false, true>(a, st) : launch_read<false, false>(a, st);
+}

@@ -1,0 +1,930 @@
+// K9: attention of one new token per request over an 8-bit paged K/V cache,
+// split over the cache's length and joined, with an optional fused append.
+//
+// With codes k^, v^ and the scales' exponents e, f of position j, and x_j =
+// scale q.k^_j 2^e_j in base 2:
+//   l = sum 2^x_j,  O = sum 2^(x_j + f_j) v^_j / l,  LSE = ln l.
+// Weights 2^(x_j + f_j - m) carry V's scale as a part of the exponent, with m
+// a running reference of x_j + f_j: whatever the scales, the key that adds
+// most to O has a weight at the top of fp16's range, and l is summed as
+// 2^(x_j + f_j - m) 2^-f_j in 32 bits (|f| <= 60 keeps it in range).  So codes
+// enter the products as they are, exact in fp16, and K's scale is one factor
+// of a score.
+//
+// Every K/V row is read once for G query rows, 2 D bytes for 4 G D flops, so
+// HBM bounds it up to about 16 rows per KV head; at half the bytes of a 16-bit
+// cache, the latency of a step and the conversions are the next bound.
+//
+// The split over blocks, teams and rings is paged_decode.cu's (see there and
+// paged_split.cuh).  What differs, for a team of warps:
+// - A step takes 64 keys of rows up to 64 bytes, else 32: the bytes in flight
+//   and the cost of a step stay those of 16-bit rows.
+// - K is loaded by ldmatrix as pairs of bytes: a lane gets columns 4 c .. 4 c +
+//   3 of a key, which after conversion are the columns that a lane holds for k
+//   = 2 c, 2 c + 1 and 2 c + 8, 2 c + 9, so Q is loaded in that order.  V comes
+//   through the 8-bit transposing ldmatrix: a lane gets keys 4 c .. 4 c + 3 of
+//   a column, and rows of K are taken in the order that makes P^T match.
+// - Q of bf16 is brought to fp16 by a power of two per row: exact for elements
+//   down to 2^-30 of the row's largest, off by 2^-39 of it below.
+// - Scales are read by the lane that looks a key's page up, a step after its
+//   page, and kept as (2^e, f) beside the ring.
+#include <float.h>
+
+#include "paged8.cuh"
+#include "paged_split.cuh"
+
+namespace {
+
+struct Paged8Args : PagedWork {
+  const uint16_t* q;
+  uint8_t* k;              // written only by the fused append
+  uint8_t* v;
+  uint8_t* ks_;            // scales
+  uint8_t* vs_;
+  const uint16_t* nk;      // null: no fused append
+  const uint16_t* nv;
+  const int64_t* slots;    // of the new rows; < 0: this request has none
+  int64_t qs[2], ks[3], vs[3], nks[2], nvs[2];
+  int64_t kss[2], vss[2];  // strides of the scales
+  int block_shift;         // log2 of the tokens of a scale
+  int box;                 // rows of a TMA box
+  int pitch;               // bytes from row to row of a tile
+  int width;               // 16-byte chunks that the swizzle permutes (8, 4 or 2), or 0
+  bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
+  bool q_bf16;
+  float scale_log2;        // scale log2(e)
+};
+
+// Variants: KD = 16-column chunks of the head dim (4, 6 or 8); FULL: D is KD *
+// 16; NT = 8-row tiles of query rows per warp; RG = warps of a team.
+template <int KD, int NT, int RG>
+struct Cfg8 {
+  static constexpr int KW = KD == 4 ? 64 : 32;               // keys a team takes of a tile
+  static constexpr int TEAMS = kWarps / RG;
+  static constexpr int TILE = TEAMS * KW;
+  static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
+  static constexpr int PITCH = KD == 6 ? 112 : KD * 16;      // largest of a row
+  static constexpr int STAGE = KW * PITCH * 2;               // bytes: K rows, then V rows
+  static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
+  static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;
+  static constexpr int HANDED = KD * 4 * 32;                 // floats of a warp's O^T of one row tile
+  static constexpr int SCALES = TEAMS * STAGES * KW * 8;     // bytes
+  static constexpr int SMEM =
+      1024 + TEAMS * STAGES * STAGE + SCALES + (TEAMS > 1 ? 2 * HANDED + kWarps * NT * 32 : 0) * 4;
+};
+
+// Offset of 16-byte chunk c of row r of a tile: rows of 2, 4 or 8 chunks lie
+// dense with their chunks swizzled as TMA does it, so that the 8 rows an
+// ldmatrix reads lie on different banks; rows of an odd number of chunks need
+// no swizzle.  Six chunks are padded to seven.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c, int pitch, int width) {
+  if (width == 0) return (uint32_t)(r * pitch + c * 16);
+  const int x = width == 8 ? r : width == 4 ? r >> 1 : r >> 2;
+  return (uint32_t)(r * pitch + (((c ^ x) & (width - 1)) << 4));
+}
+
+// x4 over two 16 x 16 matrices of bytes, transposed: lane l gets of each
+// column l / 4 (then l / 4 + 8) rows 4 (l % 4) .. + 3.
+__device__ __forceinline__ void ldmatrix_trans_b8(uint32_t (&r)[4], uint32_t saddr) {
+  asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(saddr));
+}
+
+template <bool INT8, int KD, bool FULL, int NT, int RG>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                     const Paged8Args a) {
+  using C = Cfg8<KD, NT, RG>;
+  constexpr int KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
+  constexpr int H = KW / 16;           // 16-key parts of a step
+  constexpr int LOOKS = KW / 32;       // keys that a lane looks up
+  constexpr int PAIRS = KD / 2;        // pairs of chunks
+  // Weights lie between 2^BELOW and 2^LIMIT at the row's largest x + f, the
+  // top of fp16's range: its 11 bits hold down to 2^-25 of the largest, and
+  // what is lost below is at most 2^-36 of it.
+  constexpr float BELOW = 11.f, LIMIT = 15.f;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = smem_raw + (-kf::smem_u32(smem_raw) & 1023u);
+  __shared__ ShareScratch scratch;
+  __shared__ __align__(8) uint64_t full[C::TEAMS][STAGES];
+  __shared__ uint32_t seen_s[C::TEAMS][STAGES][LOOKS];  // visible keys of each stage
+  __shared__ uint32_t nan_s[C::TEAMS][STAGES][LOOKS];   // keys whose V has the scale NaN
+  __shared__ int abort_any;
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int team = warp / RG, rg = warp % RG;
+  const int units = a.Hkv * a.row_blocks;  // per request
+  uint8_t* ring = smem + team * STAGES * C::STAGE;
+  float2* scales = reinterpret_cast<float2*>(smem + C::TEAMS * STAGES * C::STAGE) + team * STAGES * KW;  // (2^e, f)
+  float* handed = reinterpret_cast<float*>(smem + C::TEAMS * STAGES * C::STAGE + C::SCALES);  // [2][KD][lane][4]
+  float* ml = handed + 2 * C::HANDED;  // [warp][NT][4 lanes][2 rows](m, l, sum of the cut weights, -)
+
+  if (tid == 0) {
+    for (int i = 0; i < C::TEAMS * STAGES; ++i) kf::mbar_init(&full[0][0] + i, 1);
+    kf::fence_barrier_init();
+    abort_any = 0;
+    kf::tma_prefetch_desc(&map_k);
+    kf::tma_prefetch_desc(&map_v);
+  }
+  // The chain lengths -> table -> K/V starts cold: hints while the previous
+  // kernel still runs.
+  {
+    const uint32_t line = blockIdx.x * kThreads + tid;  // of 32 entries
+    if (line * 32 < (uint32_t)a.B) prefetch_l2(a.lengths + line * 32);
+    const uint32_t lines_per_row = (a.max_pages + 31) / 32, b = line / lines_per_row;
+    if (b < (uint32_t)a.B) prefetch_l2(a.table + b * a.table_stride + (line - b * lines_per_row) * 32);
+    const uint32_t request = line / a.Hq;
+    if (request < (uint32_t)a.B)
+      kf::prefetch_l2_bulk(a.q + request * a.qs[0] + (line - request * a.Hq) * a.qs[1], a.D * 2);
+  }
+  const int pitch = FULL ? KD * 16 : a.pitch, width = FULL ? KD : a.width;
+  const int chunks = FULL ? KD : (a.D + 15) / 16;
+  const int v_bytes = KW * pitch;      // where V's rows begin
+  // Offsets of a lane's ldmatrix rows, by pair of chunks.  Row i of the first
+  // (second) 8 x 8 part of K is key 4 (i / 2) + i % 2 (+ 2); a missing second
+  // chunk repeats the first.  (Rows 16 h later lie 16 h pitch on: the swizzle
+  // repeats after 8 rows.)
+  uint32_t k_off[PAIRS], v_off[PAIRS];
+#pragma unroll
+  for (int x = 0; x < PAIRS; ++x) {
+    const int i = lane & 7, c = min(2 * x + (lane >> 4), chunks - 1);
+    k_off[x] = chunk_at(4 * (i >> 1) + (i & 1) + ((lane >> 3) & 1) * 2, c, pitch, width);
+    v_off[x] = chunk_at(lane & 15, c, pitch, width);
+  }
+  kf::griddep_wait();
+  kf::griddep_launch_dependents();
+
+  const uint32_t me = blockIdx.x;
+  const bool join_blocks = a.joins && !a.join_units;
+  Share share;
+  Cursor<TILE> load, work;
+  if (!find_share<TILE>(a, scratch, share) || !first_tile(a, share, work)) {
+    if (tid == 0 && join_blocks) a.joins[me].x = -1;
+    clear_empty(a);
+    return;
+  }
+  const uint32_t end = share.end;
+  load = work;
+
+  // ---- loads: a lane looks up keys lane (and lane + 32) of the team's share of a tile
+  struct Place {
+    uint32_t page[LOOKS], row[LOOKS];
+    int h;
+  };
+  auto look_up = [&]() {
+    Place p;
+    p.h = load.h;
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      const uint32_t key = load.t * TILE + team * KW + i * 32 + lane;
+      const uint32_t pg = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
+      p.row[i] = key - pg * a.page_size;
+      p.page[i] = key < load.keys ? (uint32_t)a.table[load.b * a.table_stride + pg] : 0xffffffffu;
+    }
+    return p;
+  };
+  struct Scale {
+    uint32_t k[LOOKS], v[LOOKS];       // bytes; 256: no such key
+  };
+  auto issue = [&](int stage, const Place& p, Scale& s) {
+    uint32_t seen[LOOKS], boxes = 0;
+    bool starts[LOOKS];
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      const bool valid = p.page[i] < a.num_pages;
+      seen[i] = __ballot_sync(0xffffffffu, valid);
+      starts[i] = valid && ((i * 32 + lane) & (a.box - 1)) == 0;
+      boxes += __popc(__ballot_sync(0xffffffffu, starts[i]));
+    }
+    uint64_t* bar = &full[team][stage];
+    if (lane == 0) {
+#pragma unroll
+      for (int i = 0; i < LOOKS; ++i) seen_s[team][stage][i] = seen[i];
+      kf::mbar_arrive_expect_tx(bar, boxes * (uint32_t)(a.box * pitch * 2));
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      if (starts[i]) {
+        uint8_t* st = ring + stage * C::STAGE + (i * 32 + lane) * pitch;
+        kf::tma_load_5d(st, &map_k, bar, 0, p.row[i], 0, p.h, p.page[i]);
+        kf::tma_load_5d(st + v_bytes, &map_v, bar, 0, p.row[i], 0, p.h, p.page[i]);
+      }
+      s.k[i] = s.v[i] = 256;
+      if (p.page[i] < a.num_pages) {
+        const uint32_t r = p.row[i] >> a.block_shift;
+        s.k[i] = __ldcg(a.ks_ + p.page[i] * a.kss[0] + p.h * a.kss[1] + r);
+        s.v[i] = __ldcg(a.vs_ + p.page[i] * a.vss[0] + p.h * a.vss[1] + r);
+      }
+    }
+  };
+  // the scales of a tile that was issued a step before, to where its readers find them
+  auto keep = [&](int stage, const Scale& s) {
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      const float k = s.k[i] == kf::kNanScale ? NAN : kf::power2(kf::scale_of_byte(s.k[i]));
+      const float f = s.v[i] >= kf::kNanScale ? 0.f : (float)kf::scale_of_byte(s.v[i]);
+      scales[stage * KW + i * 32 + lane] = make_float2(k, f);
+      const uint32_t nan = __ballot_sync(0xffffffffu, s.v[i] == kf::kNanScale);
+      if (lane == 0) nan_s[team][stage][i] = nan;
+    }
+  };
+
+  // ---- state of the unit being worked on
+  uint32_t qb[NT][KD][2];              // Q^T as B fragments
+  // rows 2 (lane % 4) + {0, 1} of each row tile: the factor of a product, the
+  // reference m of the weights 2^(x + f - m), the sums of 2^(x - m) exact and
+  // of the weights as cut to fp16, and m as it enters the exponent (0 for -inf)
+  float factor[NT][2], m_run[NT][2], l_run[NT][2], l_held[NT][2], mu[NT][2];
+  float ot[NT][KD][4];                 // O^T
+  bool v_nan = false;
+  // The loads of the unit's Q, issued early.  start_unit() follows where the
+  // unit begins.
+  auto load_q = [&]() {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const int row = work.rb * C::ROWS + rg * NT * 8 + nt * 8 + (lane >> 2);
+      const uint16_t* src = a.q + work.b * a.qs[0] + (int64_t)(work.h * a.G + row) * a.qs[1] + 4 * (lane & 3);
+#pragma unroll
+      for (int x = 0; x < KD; ++x) {
+        qb[nt][x][0] = qb[nt][x][1] = 0u;
+        if (row < a.G && x * 16 + 4 * (lane & 3) < a.D)
+          asm volatile("ld.global.v2.b32 {%0, %1}, [%2];" : "=r"(qb[nt][x][0]), "=r"(qb[nt][x][1]) : "l"(src + x * 16));
+      }
+    }
+  };
+  auto start_unit = [&]() {
+    v_nan = false;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float back = 1.f;                // of row lane / 4: what its factor makes up for
+      if (a.q_bf16) {
+        uint32_t m = 0;
+#pragma unroll
+        for (int x = 0; x < KD; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) m = kf::max_magnitudes(m, qb[nt][x][e] & 0x7fff7fffu);
+        m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, 1));
+        m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, 2));
+        // largest element to [2^14, 2^15), as far as a power of two in 32 bits does it
+        const int up = 14 - max((int)(max(m & 0xffffu, m >> 16) >> 7) - 127, -100);
+        const float by = kf::power2(up);
+        back = kf::power2(-up);
+#pragma unroll
+        for (int x = 0; x < KD; ++x)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 y = kf::unpack2<true>(qb[nt][x][e]);
+            qb[nt][x][e] = kf::pack2<false>(y.x * by, y.y * by);
+          }
+      }
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        factor[nt][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * (lane & 3) + 4 * j);
+        m_run[nt][j] = -INFINITY;
+        l_run[nt][j] = l_held[nt][j] = mu[nt][j] = 0.f;
+      }
+#pragma unroll
+      for (int x = 0; x < KD; ++x) ot[nt][x][0] = ot[nt][x][1] = ot[nt][x][2] = ot[nt][x][3] = 0.f;
+    }
+  };
+
+  load_q();
+  // Tiles loaded ahead of the one in use (see paged_decode.cu).
+  const int depth = a.shallow && share.total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
+  // The first warp of a team loads.  To begin with it looks up the pages of the
+  // whole ring at once, then always one step ahead of their use.
+  bool more = rg == 0;                 // whether the load cursor stands on a tile that is not loaded yet
+  int issued = 0, late = -1;           // `late`: stage whose scales are on their way
+  Place ahead;
+  Scale coming;
+  if (rg == 0) {
+    Place first[STAGES - 1];
+    Scale got[STAGES - 1];
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (more && s < depth) {
+        first[s] = look_up();
+        issued = s + 1;
+        more = load.more(end);
+        if (more) load.next(a);
+      }
+    }
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < issued) issue(s, first[s], got[s]);
+    if (more) ahead = look_up();
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < issued) keep(s, got[s]);
+  }
+  uint32_t unit_t0 = work.t;           // first tile of the unit in this share
+  if (tid == 0 && join_blocks) a.joins[me].x = -1;
+  clear_empty(a);
+  start_unit();
+
+  int stage = 0, fill = depth;
+  uint32_t parity = 0;
+  bool alive = true;                   // false once a wait of this block has expired
+  for (bool going = true; going;) {
+    // scales that were asked for a step ago; their stage's last readers left it before it was issued
+    if (rg == 0 && late >= 0) keep(late, coming);
+    late = -1;
+    bool landed = kf::mbar_try_wait(&full[team][stage], parity);
+    if (!landed) landed = alive && !*(volatile int*)&abort_any && kf::mbar_wait(&full[team][stage], parity, a.status);
+    // One outcome for the team: no lane reaches a collective instruction alone.
+    // The barrier also says that the team has left stage i - 1.
+    __syncwarp();
+    alive = team_and<RG>(team, alive && landed);
+    if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
+    uint32_t seen[LOOKS], any = 0, all = 0xffffffffu;
+    auto sees = [&](uint32_t key) { return ((seen[LOOKS == 1 || key < 32 ? 0 : LOOKS - 1] >> (key & 31)) & 1) != 0; };
+#pragma unroll
+    for (int i = 0; i < LOOKS; ++i) {
+      seen[i] = alive ? seen_s[team][stage][i] : 0u;
+      any |= seen[i];
+      all &= seen[i];
+    }
+    if (rg == 0 && alive && more) {
+      issue(fill, ahead, coming);
+      late = fill;
+      ++issued;
+      more = load.more(end);
+      if (more) {
+        load.next(a);
+        ahead = look_up();
+      }
+    }
+
+    uint8_t* kt = ring + stage * C::STAGE;
+    uint8_t* vt = kt + v_bytes;
+    const uint32_t key0 = work.t * TILE + team * KW;
+    if (any != 0 && (all != 0xffffffffu || (a.nk && key0 + KW >= work.keys))) {
+      // The end of a request or pages without a table entry.  Rows that nobody
+      // sees hold anything: their scores are replaced below, their V rows must
+      // be zero (a code can be NaN).  A new row takes its place here and goes
+      // to its page, in 8 bits.
+#pragma unroll
+      for (int x = rg; x < KW / 4; x += RG) {
+        const int r = 4 * x + (lane >> 3);
+        clear16(kf::smem_u32(vt) + r * pitch + (lane & 7) * 16, (lane & 7) * 16 < pitch && !sees(r));
+      }
+      const uint32_t r = work.keys - 1 - key0;  // the newest position, unless the table is too short for it
+      if (a.nk && r < (uint32_t)KW && sees(r) && work.whole && a.slots[work.b] >= 0 && rg == 0) {
+        const int c = lane & 15;       // 8 columns of K (lanes 0 to 15) or V
+        const bool is_v = lane >= 16;
+        const uint32_t pg = (uint32_t)(((uint64_t)(key0 + r) * a.page_mul) >> a.page_shift);
+        const int64_t page = a.table[work.b * a.table_stride + pg], row = key0 + r - pg * a.page_size;
+        uint4 x = make_uint4(0, 0, 0, 0);
+        if (c < a.D / 8)
+          x = __ldcg(reinterpret_cast<const uint4*>(is_v ? a.nv + work.b * a.nvs[0] + work.h * a.nvs[1]
+                                                         : a.nk + work.b * a.nks[0] + work.h * a.nks[1]) + c);
+        uint32_t m = kf::magnitudes(x);
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
+        const int e = kf::scale_exponent<INT8>(a.q_bf16 ? kf::largest<true>(m) : kf::largest<false>(m));
+        const bool nan = e > kf::kMaxExponent;
+        const float by = nan ? 0.f : kf::power2(-e);
+        uint2 codes = a.q_bf16 ? kf::encode8<INT8, true>(x, by) : kf::encode8<INT8, false>(x, by);
+        if (nan) codes = make_uint2(0, 0);
+        if (c < a.D / 8) {
+          *reinterpret_cast<uint2*>((is_v ? vt : kt) + chunk_at((int)r, c >> 1, pitch, width) + (c & 1) * 8) = codes;
+          if (work.rb == 0)
+            *reinterpret_cast<uint2*>(is_v ? a.v + page * a.vs[0] + work.h * a.vs[1] + row * a.vs[2] + c * 8
+                                           : a.k + page * a.ks[0] + work.h * a.ks[1] + row * a.ks[2] + c * 8) = codes;
+        }
+        if (c == 0) {
+          float* at = reinterpret_cast<float*>(scales + stage * KW + r) + (is_v ? 1 : 0);
+          *at = is_v ? (nan ? 0.f : (float)e) : (nan ? NAN : kf::power2(e));
+          if (work.rb == 0)
+            (is_v ? a.vs_ + page * a.vss[0] + work.h * a.vss[1] : a.ks_ + page * a.kss[0] + work.h * a.kss[1])[row] =
+                (uint8_t)kf::scale_byte(e);
+        }
+        // what the slot's byte said before does not count, what the new row says does
+        const uint32_t v_is_nan = __shfl_sync(0xffffffffu, (uint32_t)nan, 16);
+        if (lane == 0) {
+          uint32_t& word = nan_s[team][stage][r >> 5];
+          word = (word & ~(1u << (r & 31))) | (v_is_nan << (r & 31));
+        }
+      }
+      kf::fence_proxy_async_smem();    // before a later load into this stage
+      __syncwarp();                    // (the vote of a team of one warp orders no memory)
+      team_and<RG>(team, true);
+    }
+    if (any != 0) {
+#pragma unroll
+      for (int i = 0; i < LOOKS; ++i) v_nan |= nan_s[team][stage][i] != 0;
+      const uint32_t sk = kf::smem_u32(kt), sv = kf::smem_u32(vt);
+      // S^T (keys x rows)
+      float cc[H][NT][4];
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) cc[h][nt][0] = cc[h][nt][1] = cc[h][nt][2] = cc[h][nt][3] = 0.f;
+#pragma unroll
+      for (int x = 0; x < PAIRS; ++x) {
+        if (!FULL && 2 * x >= chunks) continue;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          uint32_t w[4], f[2][4];
+          kf::ldmatrix_x4(w, sk + k_off[x] + h * 16 * pitch);
+          kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
+          kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
+          kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
+          kf::decode4<INT8>(w[3], f[1][1], f[1][3]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) kf::mma_16816<false>(cc[h][nt], f[0], qb[nt][2 * x][0], qb[nt][2 * x][1]);
+          if (FULL || 2 * x + 1 < chunks) {
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+              kf::mma_16816<false>(cc[h][nt], f[1], qb[nt][2 * x + 1][0], qb[nt][2 * x + 1][1]);
+          }
+        }
+      }
+      // Scores with V's exponent: keys 16 h + 4 (g / 2) + g % 2 (+ 2 for the
+      // second pair of a fragment), g = lane / 4, of rows 2 (lane % 4) + {0, 1}.
+      const int g = lane >> 2, own_key = 4 * (g >> 1) + (g & 1);
+      float less[H][2];                // 2^-f
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const int key = h * 16 + own_key + 2 * y;
+          const float2 s = scales[stage * KW + key];
+          less[h][y] = __int_as_float((127 << 23) - (__float2int_rn(s.y) << 23));
+          const bool hidden = all != 0xffffffffu && !((seen[h >> 1] >> ((h & 1) * 16 + own_key + 2 * y)) & 1);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              float& v = cc[h][nt][2 * y + j];
+              v = hidden ? -INFINITY : fmaf(v * s.x, factor[nt][j], s.y);
+            }
+        }
+      // The reference of a row follows its maximum only when a score passes it
+      // by LIMIT.
+      bool raise = false;
+      float top[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          top[nt][j] = fmaxf(cc[0][nt][j], cc[0][nt][2 + j]);
+#pragma unroll
+          for (int h = 1; h < H; ++h) top[nt][j] = kf::fmax3(top[nt][j], cc[h][nt][j], cc[h][nt][2 + j]);
+          raise |= top[nt][j] - m_run[nt][j] > LIMIT;
+        }
+      if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            float t = top[nt][j];
+#pragma unroll
+            for (int off = 4; off < 32; off <<= 1) t = fmaxf(t, __shfl_xor_sync(0xffffffffu, t, off));
+            const float m_new = fmaxf(m_run[nt][j], t - BELOW);
+            mu[nt][j] = m_new == -INFINITY ? 0.f : m_new;
+            const float old = kf::ex2(m_run[nt][j] - mu[nt][j]);
+            m_run[nt][j] = m_new;
+            l_run[nt][j] *= old;
+            l_held[nt][j] *= old;
+#pragma unroll
+            for (int dm = 0; dm < KD; ++dm) {
+              ot[nt][dm][j] *= old;
+              ot[nt][dm][2 + j] *= old;
+            }
+          }
+      }
+      // Weights, cut to fp16's 11 bits: O is divided by the sum of the cut ones,
+      // so that only the differences of what is cut off count (half of 2^-10 of
+      // a weight at most, no more than rounding would leave).  They are cut in
+      // 32 bits: a key whose V is small next to the others' (a row of zeros,
+      // say) has a weight that fp16 loses, and counts in the sum all the same.
+      // The LSE has the sum of the whole ones.
+      uint32_t pb[H][NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float sum[2] = {0.f, 0.f}, held[2] = {0.f, 0.f};  // of the step: fewer roundings against a large l
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            float p[2];
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              const float w = kf::ex2(cc[h][nt][2 * y + j] - mu[nt][j]);
+              sum[j] = fmaf(w, less[h][y], sum[j]);
+              p[j] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);
+              held[j] = fmaf(p[j], less[h][y], held[j]);
+            }
+            pb[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(p[0], p[1]));
+          }
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          l_run[nt][j] += sum[j];
+          l_held[nt][j] += held[j];
+        }
+      }
+      // O^T (head dim x rows) += V^T P^T.  The products of a step are summed
+      // from zero and then added, as an MMA cuts each of its products off where
+      // its accumulator's digits end.
+#pragma unroll
+      for (int x = 0; x < PAIRS; ++x) {
+        if (!FULL && 2 * x >= chunks) continue;
+        float step[2][NT][4];
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) step[e][nt][0] = step[e][nt][1] = step[e][nt][2] = step[e][nt][3] = 0.f;
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+          uint32_t w[4], f[2][4];
+          ldmatrix_trans_b8(w, sv + v_off[x] + h * 16 * pitch);
+          kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
+          kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
+          kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
+          kf::decode4<INT8>(w[3], f[1][1], f[1][3]);
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            if (FULL || 2 * x + e < chunks) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) kf::mma_16816<false>(step[e][nt], f[e], pb[h][nt][0], pb[h][nt][1]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) ot[nt][2 * x + e][i] += step[e][nt][i];
+      }
+    }
+    if (++stage == STAGES) {
+      stage = 0;
+      parity ^= 1;
+    }
+    if (++fill == STAGES) fill = 0;
+
+    const bool unit_done = work.unit_ends();
+    going = work.more(end);
+    if (!unit_done && going) {
+      ++work.t;
+      ++work.pos;
+      continue;
+    }
+    // ---- join the teams and write the unit's rows (or its partial)
+    const int b = work.b, h = work.h, rb = work.rb;
+    if (unit_t0 == 0 && tid == 0 && (a.join_units || !unit_done)) {
+      // a unit that begins here and goes on ends in the share of its last tile
+      const int hr = h * a.row_blocks + rb;
+      const uint32_t last = share_of(share, work.pos + (work.tiles - 1 - work.t));
+      a.joins[a.join_units ? (int64_t)b * units + hr : (int64_t)me] =
+          unit_done ? make_int4(-1, 0, 0, 0) : make_int4(b, hr, (int)me, (int)last);
+    }
+    if (going) {
+      work.next(a);
+      load_q();  // of the next unit: it arrives during what follows
+    }
+    const bool direct = unit_t0 == 0 && unit_done;
+    const int64_t slot = (int64_t)me * 2 + (unit_t0 > 0 ? 0 : 1);  // 0: began in an earlier share, 1: begins here
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int off = 4; off < 32; off <<= 1) {
+          l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], off);
+          l_held[nt][j] += __shfl_xor_sync(0xffffffffu, l_held[nt][j], off);
+        }
+        if (v_nan) l_held[nt][j] = NAN;             // O, not the LSE
+        if (!alive) l_run[nt][j] = l_held[nt][j] = m_run[nt][j] = NAN;  // a lost load shows in the result
+      }
+    // Each warp scales its O^T to the rows' common reference and sum; then the
+    // upper half of the teams hand theirs over, lane by lane as they hold it,
+    // and the lower half add, until team 0 has the sum.
+    if constexpr (C::TEAMS > 1) {
+      if (lane < 4) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            *reinterpret_cast<float4*>(ml + (((warp * NT + nt) * 4 + lane) * 2 + j) * 4) =
+                make_float4(m_run[nt][j], l_run[nt][j], l_held[nt][j], 0.f);
+      }
+      __syncthreads();
+    }
+    float lse2[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float by[2];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float most = m_run[nt][j], sum = l_run[nt][j], held = l_held[nt][j], own = 1.f;
+        if constexpr (C::TEAMS > 1) {
+          float4 x[C::TEAMS];
+#pragma unroll
+          for (int t = 0; t < C::TEAMS; ++t) {
+            x[t] = *reinterpret_cast<const float4*>(ml + ((((t * RG + rg) * NT + nt) * 4 + (lane & 3)) * 2 + j) * 4);
+            most = fmaxf(most, x[t].x);
+          }
+          const float ref = most == -INFINITY ? 0.f : most;
+          sum = held = 0.f;
+#pragma unroll
+          for (int t = 0; t < C::TEAMS; ++t) {
+            const float w = kf::ex2(x[t].x - ref);
+            sum += w * x[t].y;
+            held += w * x[t].z;
+          }
+          own = kf::ex2(m_run[nt][j] - ref);
+        }
+        by[j] = held == 0.f ? 0.f : own * reciprocal(held);
+        if (team == 0) lse2[nt][j] = sum == 0.f ? -INFINITY : most + log2f(sum);
+      }
+#pragma unroll
+      for (int dm = 0; dm < KD; ++dm) {
+        ot[nt][dm][0] *= by[0];
+        ot[nt][dm][1] *= by[1];
+        ot[nt][dm][2] *= by[0];
+        ot[nt][dm][3] *= by[1];
+      }
+    }
+    const int valid_rows = min(C::ROWS, a.G - rb * C::ROWS);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      // handed[0]: to team 0, handed[1]: to team 1 and then from it.  Team t's
+      // writes follow its reads of that buffer; the next unit's first barrier
+      // keeps its writes behind team 0's last reads.
+#pragma unroll
+      for (int step = C::TEAMS / 2; step >= 1; step /= 2) {
+        if (RG == 1 && nt > 0 && step == 2) __syncthreads();  // team 0 has read the row tile before
+        if (RG == 2 && nt > 0) __syncthreads();
+        if (team >= step && team < 2 * step) {
+          float* to = handed + (RG == 2 ? rg : step == 2 ? team - 2 : 1) * C::HANDED;
+#pragma unroll
+          for (int dm = 0; dm < KD; ++dm)
+            *reinterpret_cast<float4*>(to + (dm * 32 + lane) * 4) =
+                make_float4(ot[nt][dm][0], ot[nt][dm][1], ot[nt][dm][2], ot[nt][dm][3]);
+        }
+        __syncthreads();
+        if (team < step) {
+          const float* from = handed + (RG == 2 ? rg : step == 2 ? team : 1) * C::HANDED;
+#pragma unroll
+          for (int dm = 0; dm < KD; ++dm) {
+            const float4 x = *reinterpret_cast<const float4*>(from + (dm * 32 + lane) * 4);
+            ot[nt][dm][0] += x.x;
+            ot[nt][dm][1] += x.y;
+            ot[nt][dm][2] += x.z;
+            ot[nt][dm][3] += x.w;
+          }
+        }
+      }
+      if (team != 0) continue;
+      // rows of the unit: 8-row tile rg * NT + nt; O^T holds columns dm * 16 +
+      // lane / 4 (+ 8) of rows 2 (lane % 4) + {0, 1}
+      const int row0 = (rg * NT + nt) * 8;
+      if (direct) {
+        // 8 x 8 blocks transposed: row lane / 4, columns 2 (lane % 4) + {0, 1}
+        const int r = row0 + (lane >> 2), head = h * a.G + rb * C::ROWS + r;
+        uint16_t* out = a.o + ((int64_t)b * a.Hq + head) * a.D + 2 * (lane & 3);
+#pragma unroll
+        for (int dm = 0; dm < KD; ++dm)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float lo = ot[nt][dm][2 * e], hi = ot[nt][dm][2 * e + 1];
+            const uint32_t x = kf::movmatrix_trans(a.q_bf16 ? kf::pack2<true>(lo, hi) : kf::pack2<false>(lo, hi));
+            if (r < valid_rows && dm * 16 + e * 8 < a.D) *reinterpret_cast<uint32_t*>(out + dm * 16 + e * 8) = x;
+          }
+        if (a.lse && lane < 4) {
+#pragma unroll
+          for (int j = 0; j < 2; ++j)
+            if (row0 + 2 * lane + j < valid_rows)
+              a.lse[(int64_t)b * a.Hq + h * a.G + rb * C::ROWS + row0 + 2 * lane + j] = lse2[nt][j] * kLn2;
+        }
+      } else {
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int r = row0 + 2 * (lane & 3) + j;
+          if (r >= valid_rows) continue;
+          float* out = a.part_o + (slot * C::ROWS + r) * a.D + (lane >> 2);
+#pragma unroll
+          for (int dm = 0; dm < KD; ++dm)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+              if (dm * 16 + e * 8 < a.D) out[dm * 16 + e * 8] = ot[nt][dm][2 * e + j];
+          if (lane < 4) a.part_lse[slot * C::ROWS + r] = lse2[nt][j];
+        }
+      }
+    }
+    if (going) {
+      start_unit();
+      unit_t0 = 0;
+    }
+  }
+  // after a failed wait, let the loads still in flight land (bounded) before leaving
+  if (!alive && rg == 0 && lane == 0)
+    for (int s = 0; s < STAGES; ++s) {
+      const int used = issued / STAGES + (s < issued % STAGES ? 1 : 0);
+      if (used > 0) kf::mbar_wait(&full[team][s], (uint32_t)(used - 1) & 1, nullptr, 100000000ull);
+    }
+}
+
+// How the rows of a pool lie in a tile, and the variant that takes them.
+struct Layout {
+  int steps, pitch, width, box, cols;  // cols: of a TMA box, in pairs of bytes
+  bool full;
+};
+
+Layout layout_of(int64_t D, int64_t page_size) {
+  Layout l;
+  const int chunks = (int)((D + 15) / 16);
+  l.box = 64;                          // rows that never cross a page
+  while (page_size % l.box) l.box /= 2;
+  // A box begins on 128 bytes of shared memory.  Where boxes of few rows and
+  // short rows would not, rows are 128 bytes apart.
+  const int pitch = chunks == 6 ? 112 : chunks * 16;
+  if (chunks != 8 && pitch * l.box % 128 == 0) {
+    l.pitch = pitch;
+    l.width = chunks == 2 || chunks == 4 ? chunks : 0;
+  } else {
+    l.pitch = 128;
+    l.width = 8;
+  }
+  l.steps = l.pitch == 128 ? 8 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : 8;
+  if (l.steps != 4 && l.box > 32) l.box = 32;
+  l.cols = l.pitch / 2;
+  l.full = D == 128 || (D == 64 && l.pitch == 64);
+  return l;
+}
+
+template <int KD>
+int tile_keys_of(int rows) {
+  return rows == 8    ? Cfg8<KD, 1, 1>::TILE
+         : rows == 16 ? Cfg8<KD, 2, 1>::TILE
+         : rows == 32 ? Cfg8<KD, 2, 2>::TILE
+                      : Cfg8<KD, 2, 4>::TILE;
+}
+int tile_keys(int steps, int rows) {
+  return steps == 4 ? tile_keys_of<4>(rows) : steps == 6 ? tile_keys_of<6>(rows) : tile_keys_of<8>(rows);
+}
+
+template <bool INT8, int KD, bool FULL, int NT, int RG>
+int launch_variant(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
+  using C = Cfg8<KD, NT, RG>;
+  static_assert(C::STAGES >= 2, "the ring needs two stages");
+  static_assert(C::SMEM <= 112 * 1024, "two blocks per SM");
+  auto kern = paged8_decode_kernel<INT8, KD, FULL, NT, RG>;
+  if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
+    (void)cudaGetLastError();
+    return kf::set_error(KF_ERR_CUDA, "kf_paged8_decode: cannot reserve %d bytes of shared memory", C::SMEM);
+  }
+  return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged8_decode", mk, mv, a);
+}
+
+template <bool INT8, int KD, bool FULL>
+int dispatch_rows(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
+                  cudaStream_t st) {
+  switch (rows) {  // unit_rows()'s
+    case 8: return launch_variant<INT8, KD, FULL, 1, 1>(a, mk, mv, blocks, st);
+    case 16: return launch_variant<INT8, KD, FULL, 2, 1>(a, mk, mv, blocks, st);
+    case 32: return launch_variant<INT8, KD, FULL, 2, 2>(a, mk, mv, blocks, st);
+    default: return launch_variant<INT8, KD, FULL, 2, 4>(a, mk, mv, blocks, st);
+  }
+}
+
+template <bool INT8>
+int dispatch(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int rows, int blocks,
+             cudaStream_t st) {
+  if (l.steps == 4)
+    return l.full ? dispatch_rows<INT8, 4, true>(a, mk, mv, rows, blocks, st)
+                  : dispatch_rows<INT8, 4, false>(a, mk, mv, rows, blocks, st);
+  if (l.steps == 6) return dispatch_rows<INT8, 6, false>(a, mk, mv, rows, blocks, st);
+  return l.full ? dispatch_rows<INT8, 8, true>(a, mk, mv, rows, blocks, st)
+                : dispatch_rows<INT8, 8, false>(a, mk, mv, rows, blocks, st);
+}
+
+bool rows16(const kf_tensor4& t) {
+  if (!kf::aligned16(t.ptr) || t.stride[3] != 1) return false;
+  for (int i = 0; i < 2; ++i)
+    if (t.size[i] > 1 && t.stride[i] % 8 != 0) return false;
+  return true;
+}
+
+}  // namespace
+
+extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
+  using kf::set_error;
+  const char* what = "kf_paged8_decode";
+  if (!args) return set_error(KF_ERR_INVALID, "%s: null arguments", what);
+  const kf_tensor4 &q = args->q, &new_k = args->new_k, &new_v = args->new_v;
+  const kf_paged8_cache& cache = args->cache;
+  const kf_tensor4 &k_pages = cache.k_pages, &v_pages = cache.v_pages;
+  if (args->dtype != KF_F16 && args->dtype != KF_BF16)
+    return set_error(KF_ERR_INVALID, "%s: dtype must be fp16 or bf16", what);
+  int rc = kf::check_cache8(what, cache);
+  if (rc != KF_OK) return rc;
+  const int64_t B = q.size[0], Hq = q.size[1], D = q.size[3], max_pages = args->max_pages;
+  const int64_t pages = k_pages.size[0], Hkv = k_pages.size[1], page_size = k_pages.size[2];
+  if (B <= 0 || Hq <= 0 || max_pages <= 0) return set_error(KF_ERR_INVALID, "%s: dimensions must be non-zero", what);
+  if (q.size[2] != 1) return set_error(KF_ERR_INVALID, "%s: Q must hold one token per request", what);
+  if (k_pages.size[3] != D) return set_error(KF_ERR_INVALID, "%s: Q/K/V head dimensions must match", what);
+  if (Hq % Hkv != 0)
+    return set_error(KF_ERR_INVALID, "%s: num_query_heads must be divisible by num_kv_heads", what);
+  if (max_pages > 0x7fffffffLL || B > (1 << 20) || Hq > (1 << 16))
+    return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
+  if (!rows16(q) || !kf::aligned16(args->o))
+    return set_error(KF_ERR_INVALID, "%s: tensors need a contiguous last dim and 16-byte aligned rows", what);
+  if (!q.ptr || !args->o || !args->block_table || !args->lengths)
+    return set_error(KF_ERR_INVALID, "%s: null data pointer", what);
+  if (!isfinite((float)args->scale * kLog2e))
+    return set_error(KF_ERR_INVALID, "%s: scale must be finite in single precision", what);
+  const bool fused = new_k.ptr || new_v.ptr || args->slots;
+  if (fused) {
+    if (!new_k.ptr || !new_v.ptr || !args->slots)
+      return set_error(KF_ERR_INVALID, "%s: new_k, new_v and slots go together", what);
+    for (int i = 0; i < 4; ++i)
+      if (new_v.size[i] != new_k.size[i])
+        return set_error(KF_ERR_INVALID, "%s: new K and V shapes must match", what);
+    if (new_k.size[0] != B || new_k.size[1] != Hkv || new_k.size[2] != 1 || new_k.size[3] != D)
+      return set_error(KF_ERR_INVALID, "%s: new K/V must be [B, Hkv, 1, D]", what);
+    if (!rows16(new_k) || !rows16(new_v))
+      return set_error(KF_ERR_INVALID, "%s: new K/V rows must be 16-byte aligned", what);
+  }
+  kf::DeviceGuard guard(q.ptr);
+  if (guard.status()) return guard.status();
+
+  const int rows = unit_rows(Hq / Hkv);
+  const Layout l = layout_of(D, page_size);
+  Paged8Args a;
+  a.q = static_cast<const uint16_t*>(q.ptr);
+  a.k = static_cast<uint8_t*>(k_pages.ptr);
+  a.v = static_cast<uint8_t*>(v_pages.ptr);
+  a.ks_ = cache.k_scales;
+  a.vs_ = cache.v_scales;
+  a.block_shift = 0;
+  while (((int64_t)1 << a.block_shift) < cache.scale_block) ++a.block_shift;
+  // Blocks of several tokens: a new row may change how the rows before it are
+  // held, which other units of this launch may be reading; so it is stored first.
+  const bool inside = fused && a.block_shift == 0;
+  a.nk = inside ? static_cast<const uint16_t*>(new_k.ptr) : nullptr;
+  a.nv = inside ? static_cast<const uint16_t*>(new_v.ptr) : nullptr;
+  a.slots = args->slots;
+  a.o = static_cast<uint16_t*>(args->o);
+  a.lse = args->lse;
+  a.table = args->block_table;
+  a.lengths = args->lengths;
+  for (int i = 0; i < 2; ++i) {
+    a.qs[i] = q.stride[i];
+    a.nks[i] = inside ? new_k.stride[i] : 0;
+    a.nvs[i] = inside ? new_v.stride[i] : 0;
+    a.kss[i] = cache.k_scale_strides[i];
+    a.vss[i] = cache.v_scale_strides[i];
+  }
+  for (int i = 0; i < 3; ++i) {
+    a.ks[i] = k_pages.stride[i];
+    a.vs[i] = v_pages.stride[i];
+  }
+  a.table_stride = args->table_stride;
+  a.B = (int)B;
+  a.Hq = (int)Hq;
+  a.Hkv = (int)Hkv;
+  a.G = (int)(Hq / Hkv);
+  a.D = (int)D;
+  a.page_size = (uint32_t)page_size;
+  a.num_pages = (uint32_t)pages;
+  a.status = args->status;
+  a.box = l.box;
+  a.pitch = l.pitch;
+  a.width = l.width;
+  a.shallow = l.full;
+  a.q_bf16 = args->dtype == KF_BF16;
+  a.scale_log2 = (float)args->scale * kLog2e;
+
+  int64_t blocks, most;
+  rc = plan_work(what, a, max_pages, rows, tile_keys(l.steps, rows), args->workspace, args->workspace_bytes, &blocks, &most);
+  if (rc != KF_OK) return rc;
+  CUtensorMap mk, mv;
+  for (int w = 0; w < 2; ++w) {
+    kf_tensor4 pairs = w ? v_pages : k_pages;  // as pairs of bytes
+    pairs.size[3] /= 2;
+    for (int i = 0; i < 3; ++i) pairs.stride[i] /= 2;
+    rc = kf::encode_tmap_pages(w ? &mv : &mk, &pairs, l.cols, l.box, 1, l.width != 0);
+    if (rc != KF_OK) return rc;
+  }
+  if (fused && !inside) {
+    kf_paged8_append_args store;
+    store.cache = cache;
+    store.new_k = new_k;
+    store.new_v = new_v;
+    store.slots = args->slots;
+    store.dtype = args->dtype;
+    store.stream = args->stream;
+    rc = kf_paged8_append(&store);
+    if (rc != KF_OK) return rc;
+  }
+  cudaStream_t st = static_cast<cudaStream_t>(args->stream);
+  rc = cache.format == KF_INT8 ? dispatch<true>(a, mk, mv, l, rows, (int)blocks, st)
+                               : dispatch<false>(a, mk, mv, l, rows, (int)blocks, st);
+  if (rc != KF_OK || most == 1) return rc;
+  return launch_join(what, a, a.q_bf16, rows, blocks, st);
+}

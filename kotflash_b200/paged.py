@@ -437,14 +437,18 @@ class PagedKVCache:
     def __init__(self, num_pages: int, page_size: int, kv_heads: int, head_dim: int, max_requests: int,
                  max_pages: int, *, layers: int = 1, device: Union[torch.device, str],
                  dtype: torch.dtype) -> None:
+        self._set_up(num_pages, page_size, kv_heads, head_dim, max_requests, max_pages, layers, device)
+        self.k = torch.empty((layers, num_pages, kv_heads, page_size, head_dim), device=device, dtype=dtype)
+        self.v = torch.empty_like(self.k)
+
+    def _set_up(self, num_pages, page_size, kv_heads, head_dim, max_requests, max_pages, layers, device) -> None:
+        """Everything but the pools."""
         dims = {"num_pages": num_pages, "page_size": page_size, "kv_heads": kv_heads, "head_dim": head_dim,
                 "max_requests": max_requests, "max_pages": max_pages, "layers": layers}
         for name, value in dims.items():
             if isinstance(value, bool) or not isinstance(value, int) or value <= 0:
                 raise ValueError(f"{name} must be a positive integer")
         self.page_size = page_size
-        self.k = torch.empty((layers, num_pages, kv_heads, page_size, head_dim), device=device, dtype=dtype)
-        self.v = torch.empty_like(self.k)
         self.block_table = torch.full((max_requests, max_pages), -1, device=device, dtype=torch.int32)
         self.lengths = torch.zeros(max_requests, device=device, dtype=torch.int32)
         # the stack gives out page 0 first
