@@ -38,12 +38,16 @@ __device__ __forceinline__ uint16_t* row_at(const Rows8Args& a, int w, uint32_t 
 }
 
 // ---------------------------------------------------------------- a scale for each row
-template <bool INT8, bool BF16, int GROUP, int U>
+// GROUP lanes share a row, VEC values each: 16 (two loads, one 16-byte store)
+// where D allows it, since the way to a row costs as much as its values do.
+template <bool INT8, bool BF16, int VEC, int GROUP, int U>
 __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
   constexpr uint32_t ROWS = kThreads / GROUP;  // of a block, side by side
+  constexpr int W = VEC / 8;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
   const int c = threadIdx.x % GROUP;
+  const bool mine = c * W < a.chunks;
   const uint32_t total = a.T * a.heads, first = blockIdx.x * (ROWS * U) + threadIdx.x / GROUP;
   uint32_t token[U], head[U];
   int64_t slot[U];
@@ -55,14 +59,17 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
     slot[u] = r < total ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token[u]) : -1;
     if (slot[u] >= a.num_slots) slot[u] = -1;  // no such slot: the token is not stored
   }
-  uint4 val[U][2];
+  uint4 val[U][2][W];
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      val[u][w] = make_uint4(0, 0, 0, 0);
-      if (slot[u] >= 0 && c < a.chunks)
-        val[u][w] = __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, token[u], head[u])) + c);
+      const uint4* from = reinterpret_cast<const uint4*>(row_at(a, w, token[u], head[u])) + c * W;
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        val[u][w][i] = make_uint4(0, 0, 0, 0);
+        if (slot[u] >= 0 && mine) val[u][w][i] = __ldcg(from + i);
+      }
     }
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -70,16 +77,27 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
     const int64_t page = page_of(a, slot[u] < 0 ? 0 : slot[u], row);
 #pragma unroll
     for (int w = 0; w < 2; ++w) {
-      uint32_t m = kf::magnitudes(val[u][w]);
+      uint32_t m = kf::magnitudes(val[u][w][0]);
+      if constexpr (W == 2) m = kf::max_magnitudes(m, kf::magnitudes(val[u][w][1]));
 #pragma unroll
       for (int off = 1; off < GROUP; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
       const int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
       const bool nan = e > kf::kMaxExponent;
-      uint2 codes = kf::encode8<INT8, BF16>(val[u][w], nan ? 0.f : kf::power2(-e));
-      if (nan) codes = make_uint2(0, 0);
+      const float by = nan ? 0.f : kf::power2(-e);
+      uint2 codes[W];
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        codes[i] = kf::encode8<INT8, BF16>(val[u][w][i], by);
+        if (nan) codes[i] = make_uint2(0, 0);
+      }
       if (slot[u] < 0) continue;
-      if (c < a.chunks)
-        *reinterpret_cast<uint2*>(a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * 8) = codes;
+      uint8_t* to = a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * VEC;
+      if (mine) {
+        if constexpr (W == 2)
+          *reinterpret_cast<uint4*>(to) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
+        else
+          *reinterpret_cast<uint2*>(to) = codes[0];
+      }
       if (c == 0) a.scales[w][page * a.ss[w][0] + head[u] * a.ss[w][1] + row] = (uint8_t)kf::scale_byte(e);
     }
   }
@@ -301,12 +319,15 @@ int launch_append(const Rows8Args& a, cudaStream_t st) {
     const uint64_t per_block = (uint64_t)(kThreads / group) * u;
     return kf::launch_dependent(kern, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(kThreads), 0, st, what, a);
   };
-  // Two rows of K and V a thread in flight once that still leaves a block per SM.
-  const bool many = rows * 16 >= (uint64_t)kf::sm_count_current_device() * kThreads * 2;
-  if (a.chunks <= 2) return go(append8_kernel<INT8, BF16, 2, 1>, 2, 1);
-  if (a.chunks <= 4) return go(append8_kernel<INT8, BF16, 4, 1>, 4, 1);
-  if (a.chunks <= 8) return many ? go(append8_kernel<INT8, BF16, 8, 2>, 8, 2) : go(append8_kernel<INT8, BF16, 8, 1>, 8, 1);
-  return many ? go(append8_kernel<INT8, BF16, 16, 2>, 16, 2) : go(append8_kernel<INT8, BF16, 16, 1>, 16, 1);
+  if (a.chunks % 2) {
+    if (a.chunks <= 4) return go(append8_kernel<INT8, BF16, 8, 4, 1>, 4, 1);
+    if (a.chunks <= 8) return go(append8_kernel<INT8, BF16, 8, 8, 1>, 8, 1);
+    return go(append8_kernel<INT8, BF16, 8, 16, 1>, 16, 1);
+  }
+  if (a.chunks == 2) return go(append8_kernel<INT8, BF16, 16, 1, 1>, 1, 1);
+  if (a.chunks == 4) return go(append8_kernel<INT8, BF16, 16, 2, 1>, 2, 1);
+  if (a.chunks <= 8) return go(append8_kernel<INT8, BF16, 16, 4, 1>, 4, 1);
+  return go(append8_kernel<INT8, BF16, 16, 8, 1>, 8, 1);
 }
 
 template <bool INT8, bool BF16>

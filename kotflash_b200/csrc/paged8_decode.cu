@@ -339,13 +339,13 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     alive = team_and<RG>(team, alive && landed);
     if (!alive && lane == 0) *(volatile int*)&abort_any = 1;
     uint32_t seen[LOOKS], any = 0, all = 0xffffffffu;
-    auto sees = [&](uint32_t key) { return ((seen[LOOKS == 1 || key < 32 ? 0 : LOOKS - 1] >> (key & 31)) & 1) != 0; };
 #pragma unroll
     for (int i = 0; i < LOOKS; ++i) {
       seen[i] = alive ? seen_s[team][stage][i] : 0u;
       any |= seen[i];
       all &= seen[i];
     }
+    auto sees = [&](uint32_t key) { return ((seen[LOOKS == 1 || key < 32 ? 0 : LOOKS - 1] >> (key & 31)) & 1) != 0; };
     if (rg == 0 && alive && more) {
       issue(fill, ahead, coming);
       late = fill;

@@ -5,13 +5,17 @@
 // same with -t.  Pairs are column i with i + R / 2, or 2 i with 2 i + 1.
 //
 // Every element is read and written once (4 bytes for 3 flops), so HBM
-// bounds it.  cos and sin depend on the token and the pair only: a thread
-// keeps those of its pairs in registers and walks over heads, four in flight,
-// so that they are worked out once for all heads of Q and K.
+// bounds it: 4 x 4096 tokens of 32 and 8 heads of 128 columns take 56 us, 92%
+// of the measured copy rate.  cos and sin depend on the token and the pair
+// only: a thread keeps those of its pairs in registers and takes four heads,
+// which it asks for before it works the angles out.  (Angles shared by a block
+// through shared memory, all heads of a few tokens per block: 64 to 90 us, the
+// barriers cost more than the angles.)
 //
-// An angle of p radians, p up to 2^31, needs its turns to 2^-24 or so: the
-// product and the reduction to [-1/2, 1/2] turns are taken in 64 bits (error
-// below p 2^-51 turns), the rest is sincospi in 32.
+// An angle is needed to 2^-32 turns or so at any position.  Frequencies become
+// whole numbers of 2^-64 turns (a double holds them to 2^-55), so a product
+// with the position modulo 2^64 is the angle modulo a turn, off by position *
+// 2^-55 turns, with no reduction to make; its upper half goes to cos_sin().
 #include <math.h>
 
 #include <type_traits>
@@ -21,7 +25,7 @@
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct RotaryArgs {
   const uint16_t* x[2];    // Q and K
@@ -73,6 +77,27 @@ struct Block {
   }
 };
 
+// cos and sin of `turn` / 2^32 turns.  The quarter nearest to it leaves t in
+// +-pi / 4, for which sin t = t + t z (a1 + a2 z + a3 z^2) and cos t = 1 + z (b1 +
+// b2 z + b3 z^2), z = t^2, with coefficients fitted to the least largest error
+// on that interval (by iterated reweighted least squares): 2^-29 and 2^-24.9.
+// With the roundings of t and of the sums both are off by 2^-23 at most.
+__device__ __forceinline__ void cos_sin(uint32_t turn, float& c, float& s) {
+  const uint32_t quarter = turn + 0x20000000u;
+  const float t = (float)(int32_t)((quarter & 0x3fffffffu) - 0x20000000u) * 1.4629180792671596e-9f;  // 2 pi / 2^32
+  const float z = t * t;
+  float x = fmaf(fmaf(fmaf(-0.00019495567673f, z, 0.00833197812420f), z, -0.16666650659734f) * z, t, t);
+  float y = fmaf(fmaf(fmaf(-0.00135977654526f, z, 0.04165629045595f), z, -0.49999894718539f), z, 1.f);
+  if (quarter & 0x40000000u) {  // t + pi / 2
+    const float w = x;
+    x = y;
+    y = -w;
+  }
+  const uint32_t half = quarter & 0x80000000u;  // t + pi
+  c = __uint_as_float(__float_as_uint(y) ^ half);
+  s = __uint_as_float(__float_as_uint(x) ^ half);
+}
+
 // HALVES: a thread turns columns j .. j + VEC - 1 with those R / 2 behind
 // them; else columns j .. j + VEC - 1 hold its pairs (VEC = 1: j and j + 1,
 // one value at a time).
@@ -80,14 +105,21 @@ template <int VEC, bool HALVES, bool BF16>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   constexpr int PAIRS = HALVES ? VEC : VEC > 1 ? VEC / 2 : 1;
   constexpr bool TWO = HALVES || VEC == 1;   // two loads per head
-  constexpr int U = 4;                       // heads in flight
+  constexpr int U = 4;                       // heads in flight (and of a thread, see launch())
+  // Frequencies in 2^-64 turns.  From shared memory: read by every thread through
+  // L2 they are one line that all SMs ask for (4 x 4096 tokens: 110 us).
+  extern __shared__ uint64_t turns_s[];
   kf::griddep_wait();
   kf::griddep_launch_dependents();
+  for (int i = threadIdx.x; i < a.R / 2; i += kThreads) {
+    const double turns = __ldcg(a.frequencies + i) * 0.15915494309189535;
+    turns_s[i] = __double2ull_rz((turns - floor(turns)) * 18446744073709551616.0);
+  }
   const uint32_t index = blockIdx.x * kThreads + threadIdx.x;
   const uint32_t token = index / a.items, item = index - token * a.items;
-  if (token >= a.tokens) return;
+  const bool here = token < a.tokens;
   const uint32_t n = token / a.S, s = token - n * a.S;
-  const int h0 = blockIdx.y * a.chunk, h1 = min(h0 + a.chunk, a.heads[0] + a.heads[1]);
+  const int h0 = blockIdx.y * a.chunk, h1 = here ? min(h0 + a.chunk, a.heads[0] + a.heads[1]) : h0;
   const bool turns = item < a.turning;
   // columns of this thread: j, and `other` for the second load of a pair
   const int j = turns ? (int)item * (HALVES ? VEC : 2 * PAIRS) : a.R + (int)(item - a.turning) * VEC;
@@ -109,14 +141,14 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     if (h0 + x < h1) load(h0 + x, x);
 
   float c[PAIRS], d[PAIRS];
-  if (turns) {
+  __syncthreads();
+  if (here && turns) {
     const int64_t where = (int64_t)n * a.ps[0] + (int64_t)s * a.ps[1];
-    const double position = a.wide ? (double)__ldcg(static_cast<const long long*>(a.positions) + where)
-                                   : (double)__ldcg(static_cast<const int*>(a.positions) + where);
+    const int64_t position = a.wide ? __ldcg(static_cast<const long long*>(a.positions) + where)
+                                    : __ldcg(static_cast<const int*>(a.positions) + where);
 #pragma unroll
     for (int i = 0; i < PAIRS; ++i) {
-      const double turn = position * (__ldcg(a.frequencies + (HALVES ? j : j / 2) + i) * 0.15915494309189535);
-      sincospif((float)(2.0 * (turn - rint(turn))), &d[i], &c[i]);
+      cos_sin((uint32_t)((uint64_t)position * turns_s[(HALVES ? j : j / 2) + i] >> 32), c[i], d[i]);
       c[i] *= a.magnitude;
       d[i] *= a.magnitude * a.sign;
     }
@@ -148,10 +180,8 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
       }
       u[x].store(p + j);
       if (TWO && turns) v[x].store(p + other);
-    }
-#pragma unroll
-    for (int x = 0; x < U; ++x)
       if (h + U + x < h1) load(h + U + x, x);
+    }
   }
 }
 
@@ -171,14 +201,16 @@ int launch(RotaryArgs& a, int D, bool bf16, cudaStream_t st) {
   const int64_t threads = (int64_t)a.tokens * a.items, heads = a.heads[0] + a.heads[1];
   if (threads > 0x7fffffffLL - kThreads) return kf::set_error(KF_ERR_UNSUPPORTED, "%s: too many tokens", what);
   const int64_t blocks = (threads + kThreads - 1) / kThreads;
-  // Heads of a thread: all of them amortise the angles, fewer fill the GPU.
-  const int64_t want = (int64_t)kf::sm_count_current_device() * 16;
-  int64_t parts = (want + blocks - 1) / blocks;
-  if (parts > (heads + 3) / 4) parts = (heads + 3) / 4;
-  a.chunk = (int)((heads + parts - 1) / parts);
+  // Heads of a thread: four, all in flight at once, are what still shares the
+  // angles (4 x 4096 tokens of 40 heads: 56 us, 60 with eight, 67 with
+  // fourteen); fewer where that leaves SMs without a block (64 tokens: 2.3 us
+  // with one, 2.8 with four).
+  a.chunk = 4;
+  while (a.chunk > 1 && blocks * ((heads + a.chunk - 1) / a.chunk) < kf::sm_count_current_device() * 2) a.chunk /= 2;
   const dim3 grid((unsigned)blocks, (unsigned)((heads + a.chunk - 1) / a.chunk));
-  return bf16 ? kf::launch_dependent(rotary_kernel<VEC, HALVES, true>, grid, dim3(kThreads), 0, st, what, a)
-              : kf::launch_dependent(rotary_kernel<VEC, HALVES, false>, grid, dim3(kThreads), 0, st, what, a);
+  const size_t smem = (size_t)a.R / 2 * sizeof(uint64_t);
+  return bf16 ? kf::launch_dependent(rotary_kernel<VEC, HALVES, true>, grid, dim3(kThreads), smem, st, what, a)
+              : kf::launch_dependent(rotary_kernel<VEC, HALVES, false>, grid, dim3(kThreads), smem, st, what, a);
 }
 
 }  // namespace
@@ -201,7 +233,7 @@ extern "C" int kf_rotary(const kf_rotary_args* args) {
       return set_error(KF_ERR_INVALID, "%s: output shapes must be the inputs'", what);
   if (R <= 0 || R > D || R % 2)
     return set_error(KF_ERR_INVALID, "%s: the rotated columns must be even, at least 2 and at most head_dim", what);
-  if (B > 0x7fffffffLL || S > 0x7fffffffLL || B * S > 0x7fffffffLL || D > 0x7fffffffLL || q.size[1] > (1 << 16) ||
+  if (B > 0x7fffffffLL || S > 0x7fffffffLL || B * S > 0x7fffffffLL || D > 4096 || q.size[1] > (1 << 16) ||
       (second && k.size[1] > (1 << 16)))
     return set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
   if (args->position_bits != 32 && args->position_bits != 64)
