@@ -2,14 +2,16 @@
 //
 // Storing reads 2 bytes and writes 1 per element of K and V, reading back the
 // reverse, with a few operations between, so HBM bounds both.  A row (one
-// token, one head) belongs to a group of 2 to 16 lanes with 8 values each;
-// the largest magnitude goes round the group by shuffles, as 16-bit patterns,
-// two at a time.
+// token, one head) belongs to a group of 1 to 8 lanes with two pieces of 8
+// values each; the largest magnitude goes round the group by shuffles, as
+// 16-bit patterns, two at a time.
+#include <type_traits>
+
 #include "paged8.cuh"
 
 namespace {
 
-constexpr int kThreads = 256;
+constexpr int kThreads = 128;
 
 struct Rows8Args {
   uint16_t* rows[2];       // K and V: the source of a store, the destination of a load
@@ -38,68 +40,47 @@ __device__ __forceinline__ uint16_t* row_at(const Rows8Args& a, int w, uint32_t 
 }
 
 // ---------------------------------------------------------------- a scale for each row
-// GROUP lanes share a row, VEC values each: 16 (two loads, one 16-byte store)
-// where D allows it, since the way to a row costs as much as its values do.
-template <bool INT8, bool BF16, int VEC, int GROUP, int U>
+// GROUP lanes share a row; lane c takes its 8-column pieces c and c + GROUP,
+// so that every access of a warp covers whole sectors (16384 tokens 17.1 us;
+// with pieces 2 c and 2 c + 1 and one 16-byte store 17.9).  One row of K and of V
+// a thread: with two, fewer threads fit (18.9).
+template <bool INT8, bool BF16, int GROUP>
 __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
-  constexpr uint32_t ROWS = kThreads / GROUP;  // of a block, side by side
-  constexpr int W = VEC / 8;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
   const int c = threadIdx.x % GROUP;
-  const bool mine = c * W < a.chunks;
-  const uint32_t total = a.T * a.heads, first = blockIdx.x * (ROWS * U) + threadIdx.x / GROUP;
-  uint32_t token[U], head[U];
-  int64_t slot[U];
+  const uint32_t r = blockIdx.x * (kThreads / GROUP) + threadIdx.x / GROUP;
+  const uint32_t token = r / a.heads, head = r - token * a.heads;
+  int64_t slot = r < a.T * a.heads ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token) : -1;
+  if (slot >= a.num_slots) slot = -1;  // no such slot: the token is not stored
+  uint4 val[2][2];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint32_t r = first + u * ROWS;
-    token[u] = r / a.heads;
-    head[u] = r - token[u] * a.heads;
-    slot[u] = r < total ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token[u]) : -1;
-    if (slot[u] >= a.num_slots) slot[u] = -1;  // no such slot: the token is not stored
+  for (int w = 0; w < 2; ++w) {
+    const uint4* from = reinterpret_cast<const uint4*>(row_at(a, w, token, head)) + c;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      val[w][i] = make_uint4(0, 0, 0, 0);
+      if (slot >= 0 && c + i * GROUP < a.chunks) val[w][i] = __ldcg(from + i * GROUP);
+    }
   }
-  uint4 val[U][2][W];
+  uint32_t row;
+  const int64_t page = page_of(a, slot < 0 ? 0 : slot, row);
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int w = 0; w < 2; ++w) {
+    uint32_t m = kf::max_magnitudes(kf::magnitudes(val[w][0]), kf::magnitudes(val[w][1]));
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      const uint4* from = reinterpret_cast<const uint4*>(row_at(a, w, token[u], head[u])) + c * W;
+    for (int off = 1; off < GROUP; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
+    const int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
+    const bool nan = e > kf::kMaxExponent;
+    const float by = nan ? 0.f : kf::power2(-e);
+    uint8_t* to = a.pages[w] + page * a.ps[w][0] + head * a.ps[w][1] + row * a.ps[w][2] + c * 8;
 #pragma unroll
-      for (int i = 0; i < W; ++i) {
-        val[u][w][i] = make_uint4(0, 0, 0, 0);
-        if (slot[u] >= 0 && mine) val[u][w][i] = __ldcg(from + i);
-      }
+    for (int i = 0; i < 2; ++i) {
+      const uint2 codes = kf::encode8<INT8, BF16>(val[w][i], by);
+      if (slot >= 0 && c + i * GROUP < a.chunks)
+        *reinterpret_cast<uint2*>(to + i * GROUP * 8) = nan ? make_uint2(0, 0) : codes;
     }
-#pragma unroll
-  for (int u = 0; u < U; ++u) {
-    uint32_t row;
-    const int64_t page = page_of(a, slot[u] < 0 ? 0 : slot[u], row);
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      uint32_t m = kf::magnitudes(val[u][w][0]);
-      if constexpr (W == 2) m = kf::max_magnitudes(m, kf::magnitudes(val[u][w][1]));
-#pragma unroll
-      for (int off = 1; off < GROUP; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
-      const int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
-      const bool nan = e > kf::kMaxExponent;
-      const float by = nan ? 0.f : kf::power2(-e);
-      uint2 codes[W];
-#pragma unroll
-      for (int i = 0; i < W; ++i) {
-        codes[i] = kf::encode8<INT8, BF16>(val[u][w][i], by);
-        if (nan) codes[i] = make_uint2(0, 0);
-      }
-      if (slot[u] < 0) continue;
-      uint8_t* to = a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * VEC;
-      if (mine) {
-        if constexpr (W == 2)
-          *reinterpret_cast<uint4*>(to) = make_uint4(codes[0].x, codes[0].y, codes[1].x, codes[1].y);
-        else
-          *reinterpret_cast<uint2*>(to) = codes[0];
-      }
-      if (c == 0) a.scales[w][page * a.ss[w][0] + head[u] * a.ss[w][1] + row] = (uint8_t)kf::scale_byte(e);
-    }
+    if (slot >= 0 && c == 0) a.scales[w][page * a.ss[w][0] + head * a.ss[w][1] + row] = (uint8_t)kf::scale_byte(e);
   }
 }
 
@@ -107,10 +88,15 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 // The tokens of a call that go to one block one after another (a run) are
 // one warp's: their largest magnitude, with the block's scale if it has rows
 // before them, gives the scale; if it grows, those rows are rounded again.  A
-// warp looks after the runs that begin in a window of `block` tokens.
+// warp looks after the runs that begin in a window of `block` tokens.  Three
+// trips to memory bound it (slots, rows with the old scale, stores), so slots
+// are read once and, of blocks up to 16 tokens, rows too and kept.  (With
+// slots and rows read twice 4096 tokens took 13.7 us.)
+constexpr int kKept = 16;  // rows of a run that a warp keeps
+
 template <bool INT8, bool BF16>
 __global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Args a) {
-  constexpr int GROUP = 16, SIDE = 32 / GROUP;
+  constexpr int GROUP = 8, SIDE = 32 / GROUP;  // lanes of a row, rows side by side
   kf::griddep_wait();
   kf::griddep_launch_dependents();
   const int lane = threadIdx.x & 31, c = lane % GROUP, g = lane / GROUP;
@@ -119,65 +105,94 @@ __global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Arg
   const uint32_t window = warp / (2 * a.heads), hw = warp - window * (2 * a.heads), h = hw >> 1;
   const int w = hw & 1;
   const uint64_t from = (uint64_t)window * size, until = min(from + size, (uint64_t)a.T);
-  auto slot_at = [&](uint64_t t) { return __ldcg(reinterpret_cast<const long long*>(a.slots) + t); };
-  auto follows = [&](int64_t before, int64_t s) { return before == s - 1 && before >> a.block_shift == s >> a.block_shift; };
+  auto slot_at = [&](uint64_t t) { return t < a.T ? __ldcg(reinterpret_cast<const long long*>(a.slots) + t) : -1; };
+  // Windows of up to 16 tokens see with 32 slots where their runs end.
   for (uint64_t base = from; base < until; base += 32) {
-    const uint64_t t = base + lane;
-    const int64_t s = t < until ? slot_at(t) : -1, before = t > 0 && t < until ? slot_at(t - 1) : -2;
-    uint32_t leaders = __ballot_sync(0xffffffffu, s >= 0 && s < a.num_slots && !follows(before, s));
+    const int64_t s = slot_at(base + lane);
+    int64_t before = __shfl_up_sync(0xffffffffu, (long long)s, 1);
+    if (lane == 0) before = base > 0 ? slot_at(base - 1) : -2;
+    const bool follows = before == s - 1 && before >> a.block_shift == s >> a.block_shift;
+    const uint32_t runs_on = __ballot_sync(0xffffffffu, follows);
+    uint32_t leaders = __ballot_sync(0xffffffffu, base + lane < until && s >= 0 && s < a.num_slots && !follows);
     for (; leaders; leaders &= leaders - 1) {
       const int who = __ffs(leaders) - 1;
       const uint64_t t0 = base + who;
       const int64_t s0 = __shfl_sync(0xffffffffu, (long long)s, who);
       const uint32_t inside = (uint32_t)(s0 & (size - 1));
-      uint32_t n = 0;  // tokens of the run
-      for (uint32_t more = 32; more == 32 && n < size - inside;) {
-        const uint64_t i = n + lane;
-        const uint32_t in = __ballot_sync(0xffffffffu, i < size - inside && t0 + i < a.T && slot_at(t0 + i) == s0 + (int64_t)i);
-        more = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-        n += more;
+      uint32_t n = who == 31 ? 1 : __ffs(~(runs_on >> (who + 1)));  // tokens of the run in these slots
+      if (who + n == 32) {                       // and behind them
+        for (uint32_t more = 32; more == 32 && n < size - inside;) {
+          const uint32_t i = n + lane;
+          const uint32_t in = __ballot_sync(0xffffffffu, i < size - inside && slot_at(t0 + i) == s0 + (int64_t)i);
+          more = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+          n += more;
+        }
       }
       uint32_t row;
       const int64_t page = page_of(a, s0, row);
-      auto source = [&](uint32_t i) { return __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, (uint32_t)t0 + i, h)) + c); };
       uint8_t* codes = a.pages[w] + page * a.ps[w][0] + h * a.ps[w][1] + (int64_t)row * a.ps[w][2] + c * 8;
       uint8_t* scale = a.scales[w] + page * a.ss[w][0] + h * a.ss[w][1] + (row >> a.block_shift);
+      const uint32_t old = inside > 0 ? __ldcg(scale) : 0;
+      auto source = [&](uint32_t i, int x) {
+        return i < n && c + x * GROUP < a.chunks
+                   ? __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, (uint32_t)t0 + i, h)) + c + x * GROUP)
+                   : make_uint4(0, 0, 0, 0);
+      };
+      uint4 kept[kKept / SIDE][2];
       uint32_t m = 0;
-      if (c < a.chunks) {
+#pragma unroll
+      for (int k = 0; k < kKept / SIDE; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) kept[k][x] = source(k * SIDE + g, x);
+#pragma unroll
+      for (int k = 0; k < kKept / SIDE; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) m = kf::max_magnitudes(m, kf::magnitudes(kept[k][x]));
 #pragma unroll 4
-        for (uint32_t i = g; i < n; i += SIDE) m = kf::max_magnitudes(m, kf::magnitudes(source(i)));
-      }
+      for (uint32_t i = kKept + g; i < n; i += SIDE)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) m = kf::max_magnitudes(m, kf::magnitudes(source(i, x)));
+      // (lanes may have left the loop apart from one another)
+      __syncwarp();
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
       int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
       bool nan = e > kf::kMaxExponent;
       if (inside > 0) {
-        const uint32_t old = __ldcg(scale);
         const int was = kf::scale_of_byte(old);
         nan |= old == kf::kNanScale;
         e = max(e, was);
-        if ((nan || e > was) && c < a.chunks) {
-          const float shift = nan ? 0.f : kf::power2(max(was - e, -126));
-          for (uint32_t i = g; i < inside; i += SIDE) {
-            uint2* at = reinterpret_cast<uint2*>(codes - (int64_t)(inside - i) * a.ps[w][2]);
-            const uint2 x = __ldcg(at);
-            float p[4], q[4];
-            kf::decode4<INT8>(x.x, p);
-            kf::decode4<INT8>(x.y, q);
-            *at = nan ? make_uint2(0, 0)
-                      : make_uint2(kf::encode4<INT8>(p[0] * shift, p[1] * shift, p[2] * shift, p[3] * shift),
-                                   kf::encode4<INT8>(q[0] * shift, q[1] * shift, q[2] * shift, q[3] * shift));
-          }
+        if (nan || e > was) {
+          const float shift = nan ? 0.f : kf::power2(was - e);
+          for (uint32_t i = g; i < inside; i += SIDE)
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+              if (c + x * GROUP >= a.chunks) continue;
+              uint2* at = reinterpret_cast<uint2*>(codes - (int64_t)(inside - i) * a.ps[w][2] + x * GROUP * 8);
+              const uint2 y = __ldcg(at);
+              float p[4], q[4];
+              kf::decode4<INT8>(y.x, p);
+              kf::decode4<INT8>(y.y, q);
+              *at = nan ? make_uint2(0, 0)
+                        : make_uint2(kf::encode4<INT8>(p[0] * shift, p[1] * shift, p[2] * shift, p[3] * shift),
+                                     kf::encode4<INT8>(q[0] * shift, q[1] * shift, q[2] * shift, q[3] * shift));
+            }
         }
       }
       const float by = nan ? 0.f : kf::power2(-e);
-      if (c < a.chunks) {
+      auto put = [&](uint32_t i, int x, uint4 value) {
+        const uint2 y = kf::encode8<INT8, BF16>(value, by);
+        if (i < n && c + x * GROUP < a.chunks)
+          *reinterpret_cast<uint2*>(codes + (int64_t)i * a.ps[w][2] + x * GROUP * 8) = nan ? make_uint2(0, 0) : y;
+      };
+#pragma unroll
+      for (int k = 0; k < kKept / SIDE; ++k)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) put(k * SIDE + g, x, kept[k][x]);
 #pragma unroll 4
-        for (uint32_t i = g; i < n; i += SIDE) {
-          const uint2 x = kf::encode8<INT8, BF16>(source(i), by);
-          *reinterpret_cast<uint2*>(codes + (int64_t)i * a.ps[w][2]) = nan ? make_uint2(0, 0) : x;
-        }
-      }
+      for (uint32_t i = kKept + g; i < n; i += SIDE)
+#pragma unroll
+        for (int x = 0; x < 2; ++x) put(i, x, source(i, x));
       __syncwarp();  // every lane has read the old scale
       if (lane == 0) *scale = (uint8_t)(nan ? kf::kNanScale : kf::scale_byte(e));
     }
@@ -185,69 +200,48 @@ __global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Arg
 }
 
 // ---------------------------------------------------------------- reading back
-// A thread takes VEC / 8 chunks of a row of K and of V, for U rows.
-template <bool INT8, bool BF16, int VEC, int U>
+// As append8_kernel, with the tokens of a head side by side: they are
+// neighbours in the page and in the output (16384 tokens 15.7 us; with 16 codes
+// and two stores a lane, which cover half of each sector, 22.1).
+template <bool INT8, bool BF16, int GROUP>
 __global__ void __launch_bounds__(kThreads) read8_kernel(const Rows8Args a) {
   kf::griddep_wait();
   kf::griddep_launch_dependents();
-  constexpr int W = VEC / 4;  // words of codes
-  const uint32_t per_row = a.chunks * 8 / VEC, total = a.T * a.heads;
-  const uint32_t index = blockIdx.x * kThreads + threadIdx.x, r0 = index / per_row, c = index - r0 * per_row;
-  const uint32_t step = gridDim.x * kThreads / per_row;  // rows apart, a thread's own
-  if (r0 >= step) return;
-  int64_t slot[U];
-  uint32_t token[U], head[U];
+  const int c = threadIdx.x % GROUP;
+  const uint32_t r = blockIdx.x * (kThreads / GROUP) + threadIdx.x / GROUP;
+  if (r >= a.T * a.heads) return;
+  const uint32_t head = r / a.T, token = r - head * a.T;
+  int64_t slot = __ldcg(reinterpret_cast<const long long*>(a.slots) + token);
+  if (slot >= a.num_slots) slot = -1;
+  uint32_t row;
+  const int64_t page = page_of(a, slot < 0 ? 0 : slot, row);
+  uint2 codes[2][2];
+  uint32_t scale[2];
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    const uint64_t r = r0 + (uint64_t)u * step;
-    head[u] = r < total ? (uint32_t)r / a.T : 0;
-    token[u] = r < total ? (uint32_t)r - head[u] * a.T : 0;
-    slot[u] = r < total ? __ldcg(reinterpret_cast<const long long*>(a.slots) + token[u]) : -2;
-    if (slot[u] >= a.num_slots || slot[u] < -1) slot[u] = slot[u] == -2 && r >= total ? -2 : -1;
-  }
-  uint32_t codes[U][2][W], scale[U][2];
+  for (int w = 0; w < 2; ++w) {
+    const uint8_t* from = a.pages[w] + page * a.ps[w][0] + head * a.ps[w][1] + row * a.ps[w][2] + c * 8;
+    scale[w] = 127;
 #pragma unroll
-  for (int u = 0; u < U; ++u) {
-    uint32_t row;
-    const int64_t page = page_of(a, slot[u] < 0 ? 0 : slot[u], row);
-#pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      scale[u][w] = 127;
-#pragma unroll
-      for (int i = 0; i < W; ++i) codes[u][w][i] = 0;
-      if (slot[u] < 0) continue;
-      const uint8_t* p = a.pages[w] + page * a.ps[w][0] + head[u] * a.ps[w][1] + row * a.ps[w][2] + c * VEC;
-      if constexpr (VEC == 16) {
-        const uint4 x = __ldcg(reinterpret_cast<const uint4*>(p));
-        codes[u][w][0] = x.x, codes[u][w][1] = x.y, codes[u][w][2] = x.z, codes[u][w][3] = x.w;
-      } else {
-        const uint2 x = __ldcg(reinterpret_cast<const uint2*>(p));
-        codes[u][w][0] = x.x, codes[u][w][1] = x.y;
-      }
-      scale[u][w] = __ldcg(a.scales[w] + page * a.ss[w][0] + head[u] * a.ss[w][1] + (row >> a.block_shift));
+    for (int i = 0; i < 2; ++i) {
+      codes[w][i] = make_uint2(0, 0);  // rows without a slot read as 0
+      if (slot >= 0 && c + i * GROUP < a.chunks) codes[w][i] = __ldcg(reinterpret_cast<const uint2*>(from + i * GROUP * 8));
     }
+    if (slot >= 0) scale[w] = __ldcg(a.scales[w] + page * a.ss[w][0] + head * a.ss[w][1] + (row >> a.block_shift));
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u)
+  for (int w = 0; w < 2; ++w) {
+    const float by = scale[w] == kf::kNanScale ? __uint_as_float(0x7fc00000u) : kf::power2(kf::scale_of_byte(scale[w]));
+    uint4* to = reinterpret_cast<uint4*>(row_at(a, w, token, head)) + c;
 #pragma unroll
-    for (int w = 0; w < 2; ++w) {
-      if (slot[u] == -2) continue;
-      const float by = scale[u][w] == kf::kNanScale ? __uint_as_float(0x7fc00000u)
-                                                    : kf::power2(kf::scale_of_byte(scale[u][w]));
-      uint4* to = reinterpret_cast<uint4*>(row_at(a, w, token[u], head[u])) + c * (VEC / 8);
-#pragma unroll
-      for (int i = 0; i < W; i += 2) {
-        float p[4], q[4];
-        if (slot[u] < 0) {
-          to[i / 2] = make_uint4(0, 0, 0, 0);
-          continue;
-        }
-        kf::decode4<INT8>(codes[u][w][i], p);
-        kf::decode4<INT8>(codes[u][w][i + 1], q);
-        to[i / 2] = make_uint4(kf::pack2<BF16>(p[0] * by, p[1] * by), kf::pack2<BF16>(p[2] * by, p[3] * by),
-                               kf::pack2<BF16>(q[0] * by, q[1] * by), kf::pack2<BF16>(q[2] * by, q[3] * by));
-      }
+    for (int i = 0; i < 2; ++i) {
+      float p[4], q[4];
+      kf::decode4<INT8>(codes[w][i].x, p);
+      kf::decode4<INT8>(codes[w][i].y, q);
+      if (c + i * GROUP < a.chunks)
+        to[i * GROUP] = make_uint4(kf::pack2<BF16>(p[0] * by, p[1] * by), kf::pack2<BF16>(p[2] * by, p[3] * by),
+                                   kf::pack2<BF16>(q[0] * by, q[1] * by), kf::pack2<BF16>(q[2] * by, q[3] * by));
     }
+  }
 }
 
 bool rows16(const kf_tensor4& t) {
@@ -305,6 +299,24 @@ int set_up(const char* what, const kf_paged8_cache& cache, const kf_tensor4& k, 
   return KF_OK;
 }
 
+template <int N>
+using Number = std::integral_constant<int, N>;
+
+// Launches kernel(lanes of a row) over all rows.
+template <typename Kernel>
+int launch_rows(const char* what, const Rows8Args& a, cudaStream_t st, Kernel kernel) {
+  const uint64_t rows = (uint64_t)a.T * a.heads;
+  auto go = [&](auto group) {
+    const uint64_t per_block = kThreads / group;
+    return kf::launch_dependent(kernel(group), dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(kThreads), 0, st,
+                                what, a);
+  };
+  if (a.chunks <= 2) return go(Number<1>());
+  if (a.chunks <= 4) return go(Number<2>());
+  if (a.chunks <= 8) return go(Number<4>());
+  return go(Number<8>());
+}
+
 template <bool INT8, bool BF16>
 int launch_append(const Rows8Args& a, cudaStream_t st) {
   const char* what = "kf_paged8_append";
@@ -314,34 +326,12 @@ int launch_append(const Rows8Args& a, cudaStream_t st) {
     const unsigned blocks = (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32));
     return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kThreads), 0, st, what, a);
   }
-  const uint64_t rows = (uint64_t)a.T * a.heads;
-  auto go = [&](auto kern, int group, int u) {
-    const uint64_t per_block = (uint64_t)(kThreads / group) * u;
-    return kf::launch_dependent(kern, dim3((unsigned)((rows + per_block - 1) / per_block)), dim3(kThreads), 0, st, what, a);
-  };
-  if (a.chunks % 2) {
-    if (a.chunks <= 4) return go(append8_kernel<INT8, BF16, 8, 4, 1>, 4, 1);
-    if (a.chunks <= 8) return go(append8_kernel<INT8, BF16, 8, 8, 1>, 8, 1);
-    return go(append8_kernel<INT8, BF16, 8, 16, 1>, 16, 1);
-  }
-  if (a.chunks == 2) return go(append8_kernel<INT8, BF16, 16, 1, 1>, 1, 1);
-  if (a.chunks == 4) return go(append8_kernel<INT8, BF16, 16, 2, 1>, 2, 1);
-  if (a.chunks <= 8) return go(append8_kernel<INT8, BF16, 16, 4, 1>, 4, 1);
-  return go(append8_kernel<INT8, BF16, 16, 8, 1>, 8, 1);
+  return launch_rows(what, a, st, [](auto group) { return append8_kernel<INT8, BF16, group>; });
 }
 
 template <bool INT8, bool BF16>
 int launch_read(const Rows8Args& a, cudaStream_t st) {
-  const int vec = a.chunks % 2 == 0 ? 16 : 8;
-  const uint32_t per_row = a.chunks * 8 / vec;
-  constexpr int U = 2;
-  const uint64_t rows = (uint64_t)a.T * a.heads, threads = (rows + U - 1) / U * per_row;
-  // whole rows in the grid's stride: kThreads * blocks divided by per_row, rounded down, covers them
-  const unsigned blocks = (unsigned)((threads + per_row + kThreads - 1) / kThreads);
-  return vec == 16 ? kf::launch_dependent(read8_kernel<INT8, BF16, 16, U>, dim3(blocks), dim3(kThreads), 0, st,
-                                          "kf_paged8_read", a)
-                   : kf::launch_dependent(read8_kernel<INT8, BF16, 8, U>, dim3(blocks), dim3(kThreads), 0, st,
-                                          "kf_paged8_read", a);
+  return launch_rows("kf_paged8_read", a, st, [](auto group) { return read8_kernel<INT8, BF16, group>; });
 }
 
 }  // namespace
