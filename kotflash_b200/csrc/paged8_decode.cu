@@ -47,9 +47,9 @@ struct Paged8Args : PagedWork {
   int64_t qs[2], ks[3], vs[3], nks[2], nvs[2];
   int64_t kss[2], vss[2];  // strides of the scales
   int block_shift;         // log2 of the tokens of a scale
-  int box;                 // rows of a TMA box
-  int pitch;               // bytes from row to row of a tile
-  int width;               // 16-byte chunks that the swizzle permutes (8, 4 or 2), or 0
+  int box;                 // keys of a TMA box
+  int pitch;               // bytes from key to key of a tile
+  bool swizzle;
   bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
   bool q_bf16;
   float scale_log2;        // scale log2(e)
@@ -59,29 +59,44 @@ struct Paged8Args : PagedWork {
 // 16; NT = 8-row tiles of query rows per warp; RG = warps of a team.
 template <int KD, int NT, int RG>
 struct Cfg8 {
-  static constexpr int KW = KD == 4 ? 64 : 32;               // keys a team takes of a tile
+  static constexpr int KW = KD <= 6 ? 64 : 32;               // keys a team takes of a tile
   static constexpr int TEAMS = kWarps / RG;
   static constexpr int TILE = TEAMS * KW;
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
-  static constexpr int PITCH = KD == 6 ? 112 : KD * 16;      // largest of a row
-  static constexpr int STAGE = KW * PITCH * 2;               // bytes: K rows, then V rows
+  static constexpr int STAGE = KW * KD * 16 * 2;             // bytes: K rows, then V rows
   static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
   static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;
   static constexpr int HANDED = KD * 4 * 32;                 // floats of a warp's O^T of one row tile
   static constexpr int SCALES = TEAMS * STAGES * KW * 8;     // bytes
+  // All of it is dynamic, with the ring, which wants to begin on 1024 bytes, in front.
+  struct Tail {
+    uint64_t full[TEAMS][STAGES];
+    uint32_t seen[TEAMS][STAGES][KW / 32];                   // visible keys of each stage
+    uint32_t nan[TEAMS][STAGES][KW / 32];                    // keys whose V has the scale NaN
+    ShareScratch scratch;
+    int abort_any;
+  };
   static constexpr int SMEM =
-      1024 + TEAMS * STAGES * STAGE + SCALES + (TEAMS > 1 ? 2 * HANDED + kWarps * NT * 32 : 0) * 4;
+      TEAMS * STAGES * STAGE + SCALES + (TEAMS > 1 ? 2 * HANDED + kWarps * NT * 32 : 0) * 4 + (int)sizeof(Tail);
 };
 
-// Offset of 16-byte chunk c of row r of a tile: rows of 2, 4 or 8 chunks lie
-// dense with their chunks swizzled as TMA does it, so that the 8 rows an
-// ldmatrix reads lie on different banks; rows of an odd number of chunks need
-// no swizzle.  Six chunks are padded to seven.
-__device__ __forceinline__ uint32_t chunk_at(int r, int c, int pitch, int width) {
-  if (width == 0) return (uint32_t)(r * pitch + c * 16);
-  const int x = width == 8 ? r : width == 4 ? r >> 1 : r >> 2;
-  return (uint32_t)(r * pitch + (((c ^ x) & (width - 1)) << 4));
+// Offset of 16-byte chunk c of key r of a tile.  A tile holds keys as a page
+// does, one behind the other, brought as lines of 128 bytes whatever a row's
+// length: a TMA load of rows takes a cycle for each row and each sector of 32
+// bytes that it touches, which rows of 64 to 96 bytes pay more for than for
+// HBM (32 requests of 8192 keys, loads alone: D = 64 49 us, D = 72 67, D = 96 70).
+// Where a row's chunks are even in number the lines are swizzled; where they
+// are odd, keys lie on different banks as they are.
+__device__ __forceinline__ uint32_t chunk_at(int r, int c, int pitch, bool swizzle) {
+  const uint32_t at = (uint32_t)(r * pitch + c * 16);
+  return swizzle ? at ^ ((at >> 3) & 0x70u) : at;
 }
+
+// The key of a 16-key part that stands in place x of a product.  V's fragments
+// hold keys 4 c .. 4 c + 3 of a lane, so K's two 8 x 8 parts take places {0, 1,
+// 4, 5, ..} and {2, 3, 6, 7, ..}; with this order of keys both those and eight
+// places in a row lie on different banks (six chunks apart, on pairs of them).
+__device__ __forceinline__ int key_of(int x) { return x ^ ((x >> 2) & 2); }
 
 // x4 over two 16 x 16 matrices of bytes, transposed: lane l gets of each
 // column l / 4 (then l / 4 + 8) rows 4 (l % 4) .. + 3.
@@ -89,6 +104,14 @@ __device__ __forceinline__ void ldmatrix_trans_b8(uint32_t (&r)[4], uint32_t sad
   asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
                : "r"(saddr));
+}
+
+// A scale, and the rest of its line of 128 bytes to L2: the other heads of the
+// page, which other blocks ask for at about the same time.
+__device__ __forceinline__ uint32_t load_scale(const uint8_t* p) {
+  uint32_t x;
+  asm volatile("ld.global.L2::128B.u8 %0, [%1];" : "=r"(x) : "l"(p));
+  return x;
 }
 
 template <bool INT8, int KD, bool FULL, int NT, int RG>
@@ -104,13 +127,12 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   // top of fp16's range: its 11 bits hold down to 2^-25 of the largest, and
   // what is lost below is at most 2^-36 of it.
   constexpr float BELOW = 11.f, LIMIT = 15.f;
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = smem_raw + (-kf::smem_u32(smem_raw) & 1023u);
-  __shared__ ShareScratch scratch;
-  __shared__ __align__(8) uint64_t full[C::TEAMS][STAGES];
-  __shared__ uint32_t seen_s[C::TEAMS][STAGES][LOOKS];  // visible keys of each stage
-  __shared__ uint32_t nan_s[C::TEAMS][STAGES][LOOKS];   // keys whose V has the scale NaN
-  __shared__ int abort_any;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  typename C::Tail& tail = *reinterpret_cast<typename C::Tail*>(smem + C::SMEM - sizeof(typename C::Tail));
+  auto& full = tail.full;
+  auto& seen_s = tail.seen;
+  auto& nan_s = tail.nan;
+  int& abort_any = tail.abort_any;
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int team = warp / RG, rg = warp % RG;
@@ -138,20 +160,25 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (request < (uint32_t)a.B)
       kf::prefetch_l2_bulk(a.q + request * a.qs[0] + (line - request * a.Hq) * a.qs[1], a.D * 2);
   }
-  const int pitch = FULL ? KD * 16 : a.pitch, width = FULL ? KD : a.width;
+  const int pitch = FULL ? KD * 16 : a.pitch;
+  const bool swizzle = FULL || a.swizzle;
   const int chunks = FULL ? KD : (a.D + 15) / 16;
-  const int v_bytes = KW * pitch;      // where V's rows begin
-  // Offsets of a lane's ldmatrix rows, by pair of chunks.  Row i of the first
-  // (second) 8 x 8 part of K is key 4 (i / 2) + i % 2 (+ 2); a missing second
-  // chunk repeats the first.  (Rows 16 h later lie 16 h pitch on: the swizzle
-  // repeats after 8 rows.)
+  const int v_bytes = (KW * pitch + 1023) & ~1023;  // where V's rows begin
+  // Offsets of a lane's ldmatrix rows, by pair of chunks; a missing second
+  // chunk repeats the first.  Keys 16 h later lie 16 h pitch on, and in lines of
+  // four keys every other 16 are swizzled the other way about.
   uint32_t k_off[PAIRS], v_off[PAIRS];
 #pragma unroll
   for (int x = 0; x < PAIRS; ++x) {
     const int i = lane & 7, c = min(2 * x + (lane >> 4), chunks - 1);
-    k_off[x] = chunk_at(4 * (i >> 1) + (i & 1) + ((lane >> 3) & 1) * 2, c, pitch, width);
-    v_off[x] = chunk_at(lane & 15, c, pitch, width);
+    k_off[x] = chunk_at(key_of(4 * (i >> 1) + (i & 1) + ((lane >> 3) & 1) * 2), c, pitch, swizzle);
+    v_off[x] = chunk_at(key_of(lane & 15), c, pitch, swizzle);
   }
+  const uint32_t flip = !FULL && swizzle && pitch == 32 ? 64u : 0u;
+  auto part = [&](uint32_t off, int h) { return (off ^ ((h & 1) ? flip : 0u)) + h * 16 * pitch; };
+  // Half a chunk at the end of a row: what lies behind it can be a code of NaN,
+  // which Q's zeros do not silence.
+  const uint32_t edge = !FULL && (a.D & 8) && (lane & 3) >= 2 ? 0u : 0xffffffffu;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
@@ -159,7 +186,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const bool join_blocks = a.joins && !a.join_units;
   Share share;
   Cursor<TILE> load, work;
-  if (!find_share<TILE>(a, scratch, share) || !first_tile(a, share, work)) {
+  if (!find_share<TILE>(a, tail.scratch, share) || !first_tile(a, share, work)) {
     if (tid == 0 && join_blocks) a.joins[me].x = -1;
     clear_empty(a);
     return;
@@ -172,6 +199,9 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint32_t page[LOOKS], row[LOOKS];
     int h;
   };
+  // K/V rows pass through L2 once and leave it to the scales' lines (32 requests
+  // of 8192 keys 91.2 -> 88.8 us)
+  const uint64_t once = kf::l2_evict_first();
   auto look_up = [&]() {
     Place p;
     p.h = load.h;
@@ -208,14 +238,15 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     for (int i = 0; i < LOOKS; ++i) {
       if (starts[i]) {
         uint8_t* st = ring + stage * C::STAGE + (i * 32 + lane) * pitch;
-        kf::tma_load_5d(st, &map_k, bar, 0, p.row[i], 0, p.h, p.page[i]);
-        kf::tma_load_5d(st + v_bytes, &map_v, bar, 0, p.row[i], 0, p.h, p.page[i]);
+        const int line = (int)(((uint64_t)p.row[i] * pitch) >> 7);
+        kf::tma_load_5d_once(st, &map_k, bar, 0, line, 0, p.h, p.page[i], once);
+        kf::tma_load_5d_once(st + v_bytes, &map_v, bar, 0, line, 0, p.h, p.page[i], once);
       }
       s.k[i] = s.v[i] = 256;
       if (p.page[i] < a.num_pages) {
         const uint32_t r = p.row[i] >> a.block_shift;
-        s.k[i] = __ldcg(a.ks_ + p.page[i] * a.kss[0] + p.h * a.kss[1] + r);
-        s.v[i] = __ldcg(a.vs_ + p.page[i] * a.vss[0] + p.h * a.vss[1] + r);
+        s.k[i] = load_scale(a.ks_ + p.page[i] * a.kss[0] + p.h * a.kss[1] + r);
+        s.v[i] = load_scale(a.vs_ + p.page[i] * a.vss[0] + p.h * a.vss[1] + r);
       }
     }
   };
@@ -368,7 +399,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
       for (int x = rg; x < KW / 4; x += RG) {
         const int r = 4 * x + (lane >> 3);
-        clear16(kf::smem_u32(vt) + r * pitch + (lane & 7) * 16, (lane & 7) * 16 < pitch && !sees(r));
+        clear16(kf::smem_u32(vt) + chunk_at(r, lane & 7, pitch, swizzle), (lane & 7) * 16 < pitch && !sees(r));
       }
       const uint32_t r = work.keys - 1 - key0;  // the newest position, unless the table is too short for it
       if (a.nk && r < (uint32_t)KW && sees(r) && work.whole && a.slots[work.b] >= 0 && rg == 0) {
@@ -389,7 +420,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         uint2 codes = a.q_bf16 ? kf::encode8<INT8, true>(x, by) : kf::encode8<INT8, false>(x, by);
         if (nan) codes = make_uint2(0, 0);
         if (c < a.D / 8) {
-          *reinterpret_cast<uint2*>((is_v ? vt : kt) + chunk_at((int)r, c >> 1, pitch, width) + (c & 1) * 8) = codes;
+          *reinterpret_cast<uint2*>((is_v ? vt : kt) + chunk_at((int)r, c >> 1, pitch, swizzle) + (c & 1) * 8) = codes;
           if (work.rb == 0)
             *reinterpret_cast<uint2*>(is_v ? a.v + page * a.vs[0] + work.h * a.vs[1] + row * a.vs[2] + c * 8
                                            : a.k + page * a.ks[0] + work.h * a.ks[1] + row * a.ks[2] + c * 8) = codes;
@@ -428,7 +459,11 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t w[4], f[2][4];
-          kf::ldmatrix_x4(w, sk + k_off[x] + h * 16 * pitch);
+          kf::ldmatrix_x4(w, sk + part(k_off[x], h));
+          if constexpr (!FULL) {
+            if (2 * x + 1 == chunks) w[0] &= edge, w[1] &= edge;
+            if (2 * x + 2 == chunks) w[2] &= edge, w[3] &= edge;
+          }
           kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
           kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
           kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
@@ -442,26 +477,36 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
           }
         }
       }
-      // Scores with V's exponent: keys 16 h + 4 (g / 2) + g % 2 (+ 2 for the
+      // Scores with V's exponent: places 16 h + 4 (g / 2) + g % 2 (+ 2 for the
       // second pair of a fragment), g = lane / 4, of rows 2 (lane % 4) + {0, 1}.
-      const int g = lane >> 2, own_key = 4 * (g >> 1) + (g & 1);
+      const int g = lane >> 2;
+      const int own_key[2] = {key_of(4 * (g >> 1) + (g & 1)), key_of(4 * (g >> 1) + (g & 1) + 2)};
       float less[H][2];                // 2^-f
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
-          const int key = h * 16 + own_key + 2 * y;
+          const int key = h * 16 + own_key[y];
           const float2 s = scales[stage * KW + key];
-          less[h][y] = __int_as_float((127 << 23) - (__float2int_rn(s.y) << 23));
-          const bool hidden = all != 0xffffffffu && !((seen[h >> 1] >> ((h & 1) * 16 + own_key + 2 * y)) & 1);
+          less[h][y] = kf::ex2(-s.y);
+          const uint64_t sx = kf::f2(s.x, s.x), sy = kf::f2(s.y, s.y);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              float& v = cc[h][nt][2 * y + j];
-              v = hidden ? -INFINITY : fmaf(v * s.x, factor[nt][j], s.y);
-            }
+          for (int nt = 0; nt < NT; ++nt) {
+            uint64_t v = kf::f2(cc[h][nt][2 * y], cc[h][nt][2 * y + 1]);
+            v = kf::mul2(v, sx);
+            kf::f2_split(kf::fma2(v, kf::f2(factor[nt][0], factor[nt][1]), sy), cc[h][nt][2 * y], cc[h][nt][2 * y + 1]);
+          }
         }
+      if (all != 0xffffffffu) {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            if (!((seen[h >> 1] >> ((h & 1) * 16 + own_key[y])) & 1)) {
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) cc[h][nt][2 * y] = cc[h][nt][2 * y + 1] = -INFINITY;
+            }
+      }
       // The reference of a row follows its maximum only when a score passes it
       // by LIMIT.
       bool raise = false;
@@ -505,21 +550,27 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       uint32_t pb[H][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float sum[2] = {0.f, 0.f}, held[2] = {0.f, 0.f};  // of the step: fewer roundings against a large l
+        uint64_t sum2 = 0, held2 = 0;  // of the step: fewer roundings against a large l
+        const uint64_t mu2 = kf::f2(mu[nt][0], mu[nt][1]);
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float p[2];
+            float p[2], w[2];
+            kf::f2_split(kf::sub2(kf::f2(cc[h][nt][2 * y], cc[h][nt][2 * y + 1]), mu2), w[0], w[1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-              const float w = kf::ex2(cc[h][nt][2 * y + j] - mu[nt][j]);
-              sum[j] = fmaf(w, less[h][y], sum[j]);
-              p[j] = __uint_as_float(__float_as_uint(w) & 0xffffe000u);
-              held[j] = fmaf(p[j], less[h][y], held[j]);
+              w[j] = kf::ex2(w[j]);
+              p[j] = __uint_as_float(__float_as_uint(w[j]) & 0xffffe000u);
             }
+            const uint64_t le = kf::f2(less[h][y], less[h][y]);
+            sum2 = kf::fma2(kf::f2(w[0], w[1]), le, sum2);
+            held2 = kf::fma2(kf::f2(p[0], p[1]), le, held2);
             pb[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(p[0], p[1]));
           }
+        float sum[2], held[2];
+        kf::f2_split(sum2, sum[0], sum[1]);
+        kf::f2_split(held2, held[0], held[1]);
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           l_run[nt][j] += sum[j];
@@ -540,7 +591,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t w[4], f[2][4];
-          ldmatrix_trans_b8(w, sv + v_off[x] + h * 16 * pitch);
+          ldmatrix_trans_b8(w, sv + part(v_off[x], h));
           kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
           kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
           kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
@@ -557,7 +608,9 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) ot[nt][2 * x + e][i] += step[e][nt][i];
+            for (int i = 0; i < 4; i += 2)
+              kf::f2_split(kf::add2(kf::f2(ot[nt][2 * x + e][i], ot[nt][2 * x + e][i + 1]), kf::f2(step[e][nt][i], step[e][nt][i + 1])),
+                           ot[nt][2 * x + e][i], ot[nt][2 * x + e][i + 1]);
       }
     }
     if (++stage == STAGES) {
@@ -731,29 +784,27 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 
 // How the rows of a pool lie in a tile, and the variant that takes them.
 struct Layout {
-  int steps, pitch, width, box, cols;  // cols: of a TMA box, in pairs of bytes
-  bool full;
+  int steps, pitch, box;
+  bool lines;    // pages are brought as lines of 128 bytes
+  bool swizzle, full;
 };
 
-Layout layout_of(int64_t D, int64_t page_size) {
+Layout layout_of(int64_t D, const kf_tensor4& k, const kf_tensor4& v) {
   Layout l;
+  const int64_t page_size = k.size[2];
   const int chunks = (int)((D + 15) / 16);
-  l.box = 64;                          // rows that never cross a page
+  l.box = 64;                          // keys that never cross a page
   while (page_size % l.box) l.box /= 2;
-  // A box begins on 128 bytes of shared memory.  Where boxes of few rows and
-  // short rows would not, rows are 128 bytes apart.
-  const int pitch = chunks == 6 ? 112 : chunks * 16;
-  if (chunks != 8 && pitch * l.box % 128 == 0) {
-    l.pitch = pitch;
-    l.width = chunks == 2 || chunks == 4 ? chunks : 0;
-  } else {
-    l.pitch = 128;
-    l.width = 8;
-  }
-  l.steps = l.pitch == 128 ? 8 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : 8;
-  if (l.steps != 4 && l.box > 32) l.box = 32;
-  l.cols = l.pitch / 2;
-  l.full = D == 128 || (D == 64 && l.pitch == 64);
+  l.pitch = chunks * 16;
+  // Pages as lines: rows of whole chunks without a gap, a box of them full
+  // lines.  Else each row is a line of its own (rows of 128 bytes always are).
+  l.lines = chunks < 8 && l.pitch * l.box % 128 == 0 &&
+            (page_size == 1 || (k.stride[2] == l.pitch && v.stride[2] == l.pitch));
+  if (!l.lines) l.pitch = 128;
+  l.steps = !l.lines ? 8 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : 8;
+  if (l.steps == 8 && l.box > 32) l.box = 32;
+  l.swizzle = !l.lines || chunks == 2 || chunks == 4;
+  l.full = D == 128 || (D == 64 && l.lines);
   return l;
 }
 
@@ -854,7 +905,7 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   if (guard.status()) return guard.status();
 
   const int rows = unit_rows(Hq / Hkv);
-  const Layout l = layout_of(D, page_size);
+  const Layout l = layout_of(D, k_pages, v_pages);
   Paged8Args a;
   a.q = static_cast<const uint16_t*>(q.ptr);
   a.k = static_cast<uint8_t*>(k_pages.ptr);
@@ -895,7 +946,7 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   a.status = args->status;
   a.box = l.box;
   a.pitch = l.pitch;
-  a.width = l.width;
+  a.swizzle = l.swizzle;
   a.shallow = l.full;
   a.q_bf16 = args->dtype == KF_BF16;
   a.scale_log2 = (float)args->scale * kLog2e;
@@ -905,10 +956,14 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   if (rc != KF_OK) return rc;
   CUtensorMap mk, mv;
   for (int w = 0; w < 2; ++w) {
-    kf_tensor4 pairs = w ? v_pages : k_pages;  // as pairs of bytes
-    pairs.size[3] /= 2;
+    kf_tensor4 pairs = w ? v_pages : k_pages;  // of bytes
     for (int i = 0; i < 3; ++i) pairs.stride[i] /= 2;
-    rc = kf::encode_tmap_pages(w ? &mv : &mk, &pairs, l.cols, l.box, 1, l.width != 0);
+    pairs.size[3] = l.lines ? 64 : D / 2;
+    if (l.lines) {
+      pairs.size[2] = page_size * l.pitch / 128;
+      pairs.stride[2] = 64;
+    }
+    rc = kf::encode_tmap_pages(w ? &mv : &mk, &pairs, 64, l.lines ? l.box * l.pitch / 128 : l.box, 1, l.swizzle);
     if (rc != KF_OK) return rc;
   }
   if (fused && !inside) {
