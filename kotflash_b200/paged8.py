@@ -84,24 +84,22 @@ def _check_rows(what: str, rows, dtype=None) -> None:
             raise ValueError(f"{what}: expected 4-D tensors")
 
 
-def _cache(k_pages, v_pages, k_scales, v_scales):
-    """The fields of a kf_paged8_cache."""
-    page_size, blocks = k_pages.shape[2], k_scales.shape[2]
-    (k0, k1, _), (v0, v1, _) = k_scales.stride(), v_scales.stride()
-    return (k_pages.data_ptr(), *k_pages.shape, *k_pages.stride(), v_pages.data_ptr(), *v_pages.shape, *v_pages.stride(),
-            k_scales.data_ptr(), v_scales.data_ptr(), k0, k1, v0, v1, page_size // blocks, _FORMATS[k_pages.dtype])
-
-
-def _cache_good(index, k_pages, v_pages, k_scales, v_scales) -> bool:
-    pages, hkv, page_size, _ = ks = k_pages.shape
-    ss = k_scales.shape
-    return (
-        index >= 0 and k_pages.get_device() == index and v_pages.get_device() == index and k_scales.get_device() == index
-        and v_scales.get_device() == index and _is_sm100(index) and k_pages.dtype in _FORMATS
-        and v_pages.dtype is k_pages.dtype and k_scales.dtype is _SCALES and v_scales.dtype is _SCALES
-        and v_pages.shape == ks and len(ss) == 3 and ss[0] == pages and ss[1] == hkv and ss[2] > 0
-        and page_size % ss[2] == 0 and v_scales.shape == ss
-        and (ss[2] == 1 or (k_scales.stride(2) == 1 and v_scales.stride(2) == 1)))
+def _cache(index, k_pages, v_pages, k_scales, v_scales):
+    """The fields of a kf_paged8_cache on device ``index``, or None where
+    ``_check_cache`` or ``_check_device`` would complain."""
+    pages, hkv, page_size, d = ks = k_pages.shape
+    n, h, blocks = ss = k_scales.shape
+    (k0, k1, k2), (v0, v1, v2) = k_scales.stride(), v_scales.stride()
+    dtype = k_pages.dtype
+    if (index < 0 or k_pages.get_device() != index or v_pages.get_device() != index or k_scales.get_device() != index
+            or v_scales.get_device() != index or not _is_sm100(index) or dtype not in _FORMATS
+            or v_pages.dtype is not dtype or k_scales.dtype is not _SCALES or v_scales.dtype is not _SCALES
+            or v_pages.shape != ks or n != pages or h != hkv or blocks == 0 or page_size % blocks
+            or v_scales.shape != ss or (blocks > 1 and (k2 != 1 or v2 != 1))):
+        return None
+    return (k_pages.data_ptr(), pages, hkv, page_size, d, *k_pages.stride(), v_pages.data_ptr(), pages, hkv, page_size, d,
+            *v_pages.stride(), k_scales.data_ptr(), v_scales.data_ptr(), k0, k1, v0, v1, page_size // blocks,
+            _FORMATS[dtype])
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
@@ -140,8 +138,9 @@ def append_paged_kv8(
     try:
         index = k_pages.get_device()
         ns = new_k.shape
+        cache = _cache(index, k_pages, v_pages, k_scales, v_scales)
         good = (
-            _cache_good(index, k_pages, v_pages, k_scales, v_scales) and new_k.dtype in _DTYPES
+            cache is not None and new_k.dtype in _DTYPES
             and new_v.dtype is new_k.dtype and new_k.get_device() == index and new_v.get_device() == index
             and slots.get_device() == index and slots.dtype is _INT64 and len(ns) == 4 and new_v.dim() == 4
             and slots.shape == (ns[0] * ns[2],) and slots.is_contiguous()
@@ -154,7 +153,7 @@ def append_paged_kv8(
         _check_slots(what, slots, new_k.shape[0] * new_k.shape[2], "one slot for each new K/V row")
         _check_inference(what, new_k, new_v)
         _check_device(what, k_pages, v_pages, k_scales, v_scales, new_k, new_v, slots)
-        index, ns = k_pages.get_device(), new_k.shape
+        raise RuntimeError(f"{what}: invalid arguments")
     if new_v.shape != ns:
         raise ValueError(f"{what}: new K/V shapes must match")
     if ns[1] != k_pages.shape[1] or ns[3] != k_pages.shape[3]:
@@ -163,8 +162,7 @@ def append_paged_kv8(
         return
     new_k, new_v = _aligned(new_k), _aligned(new_v)
     rc = _ext.load().kf_paged8_append(_pack_append(
-        *_cache(k_pages, v_pages, k_scales, v_scales), new_k.data_ptr(), *ns, *new_k.stride(), new_v.data_ptr(), *ns,
-        *new_v.stride(), slots.data_ptr(), _DTYPES[new_k.dtype], _raw_stream(index)))
+        *cache, new_k.data_ptr(), *ns, *new_k.stride(), new_v.data_ptr(), *ns, *new_v.stride(), slots.data_ptr(), _DTYPES[new_k.dtype], _raw_stream(index)))
     if rc:
         _ext.check(rc, "kf_paged8_append")
 
@@ -188,7 +186,8 @@ def read_paged_kv8(
         raise TypeError(f"{what} supports float16 and bfloat16, got {dtype}")
     try:
         index = k_pages.get_device()
-        good = (_cache_good(index, k_pages, v_pages, k_scales, v_scales) and slots.get_device() == index
+        cache = _cache(index, k_pages, v_pages, k_scales, v_scales)
+        good = (cache is not None and slots.get_device() == index
                 and slots.dtype is _INT64 and slots.dim() == 1 and slots.is_contiguous())
     except (AttributeError, TypeError, ValueError, RuntimeError):
         good = False
@@ -196,16 +195,16 @@ def read_paged_kv8(
         _check_cache(what, k_pages, v_pages, k_scales, v_scales)
         _check_slots(what, slots, slots.numel() if isinstance(slots, torch.Tensor) else 0, "[tokens]")
         _check_device(what, k_pages, v_pages, k_scales, v_scales, slots)
-        index = k_pages.get_device()
+        raise RuntimeError(f"{what}: invalid arguments")
     _, hkv, _, d = k_pages.shape
     tokens = slots.shape[0]
     k = slots.new_empty((1, hkv, tokens, d), dtype=dtype)
     v = torch.empty_like(k)
     if tokens == 0:
         return k, v
+    rows = (1, hkv, tokens, d, hkv * tokens * d, tokens * d, d, 1)
     rc = _ext.load().kf_paged8_read(_pack_append(
-        *_cache(k_pages, v_pages, k_scales, v_scales), k.data_ptr(), *k.shape, *k.stride(), v.data_ptr(), *v.shape,
-        *v.stride(), slots.data_ptr(), _DTYPES[dtype], _raw_stream(index)))
+        *cache, k.data_ptr(), *rows, v.data_ptr(), *rows, slots.data_ptr(), _DTYPES[dtype], _raw_stream(index)))
     if rc:
         _ext.check(rc, "kf_paged8_read")
     return k, v
@@ -272,13 +271,14 @@ def paged_attention8(
     try:
         index = q.get_device()
         dtype = q.dtype
-        b, hq, _, d = q.shape
+        b, hq, _, d = qs = q.shape
+        cache = _cache(index, k_pages, v_pages, k_scales, v_scales)
         hkv = k_pages.shape[1]
         requests, max_pages = block_table.shape
         row_stride, column_stride = block_table.stride()
         grad = torch.is_grad_enabled()
         good = (
-            _cache_good(index, k_pages, v_pages, k_scales, v_scales) and block_table.get_device() == index
+            cache is not None and block_table.get_device() == index
             and lengths.get_device() == index and dtype in _DTYPES and block_table.dtype is _INT32
             and lengths.dtype is _INT32 and lengths.dim() == 1 and lengths.numel() == b and requests == b
             and column_stride == 1 and lengths.is_contiguous() and b > 0 and hq > 0 and hkv > 0 and hq % hkv == 0
@@ -293,10 +293,7 @@ def paged_attention8(
         good = False
     if not good:
         _check_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, new_k, new_v, slots)
-        # a table of one column may have any stride
-        index, dtype = q.get_device(), q.dtype
-        b, hq, _, d = q.shape
-        hkv, max_pages, row_stride = k_pages.shape[1], block_table.shape[1], block_table.stride(0)
+        # all is well: a table of one column may have any stride
     if scale is None:
         scale = 1.0 / math.sqrt(d) if d else 1.0
     out = torch.empty_like(q, memory_format=_CONTIGUOUS)
@@ -307,13 +304,12 @@ def paged_attention8(
         lse_ptr = lse.data_ptr()
     else:
         lse_ptr = 0
-    cache = _cache(k_pages, v_pages, k_scales, v_scales)
     rest = (block_table.data_ptr(), max_pages, row_stride, lengths.data_ptr(), out.data_ptr(), lse_ptr, _DTYPES[dtype], scale,
             workspace.data_ptr(), elements * 2, _status_ptr(index), _raw_stream(index))
     if new_k is None:
-        args = _pack_decode(*cache, q.data_ptr(), *q.shape, *q.stride(), *rest)
+        args = _pack_decode(*cache, q.data_ptr(), *qs, *q.stride(), *rest)
     else:
-        args = _pack_step(*cache, q.data_ptr(), *q.shape, *q.stride(), new_k.data_ptr(), *new_k.shape, *new_k.stride(),
+        args = _pack_step(*cache, q.data_ptr(), *qs, *q.stride(), new_k.data_ptr(), *new_k.shape, *new_k.stride(),
                           new_v.data_ptr(), *new_v.shape, *new_v.stride(), slots.data_ptr(), *rest)
     rc = _ext.load().kf_paged8_decode(args)
     if rc:

@@ -19,7 +19,10 @@ from . import _ext
 
 _DTYPES = {torch.float16: _ext.KF_F16, torch.bfloat16: _ext.KF_BF16}
 _POSITION_BITS = {torch.int32: 32, torch.int64: 64}
+_FLOAT64 = torch.float64
+_CONTIGUOUS = torch.contiguous_format
 _NONE = (0,) * 9
+_pack, _is_sm100 = _ext.pack_rotary, _ext.is_sm100
 
 
 def rotary_frequencies(
@@ -111,23 +114,32 @@ def _check(q, k, positions, frequencies) -> None:
 
 def _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse):
     """(q', k') as new contiguous tensors; either of q and k may be None."""
-    tensors = [t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous() for t in (q, k)]
-    outs = [None if t is None else torch.empty_like(t, memory_format=torch.contiguous_format) for t in tensors]
-    pairs = [(t, o) for t, o in zip(tensors, outs) if t is not None and t.numel()]
-    if not pairs:
-        return outs
-    ins = [(t.data_ptr(), *t.shape, *t.stride()) for t, _ in pairs]
-    to = [(o.data_ptr(), *o.shape, *o.stride()) for _, o in pairs]
-    if len(pairs) == 1:
-        ins.append(_NONE)
-        to.append(_NONE)
-    first = pairs[0][0]
-    index = first.get_device()
-    by_batch, by_token = positions.stride() if positions.ndim == 2 else (0, positions.stride(0))
-    rc = _ext.load().kf_rotary(_ext.pack_rotary(
-        *ins[0], *ins[1], *to[0], *to[1], positions.data_ptr(), _POSITION_BITS[positions.dtype], by_batch, by_token,
-        frequencies.data_ptr(), 2 * frequencies.shape[0], interleaved, inverse, magnitude, _DTYPES[first.dtype],
-        _ext.raw_stream(index)))
+    if q is not None and q.stride(3) != 1:
+        q = q.contiguous()
+    if k is not None and k.stride(3) != 1:
+        k = k.contiguous()
+    q_out = None if q is None else torch.empty_like(q, memory_format=_CONTIGUOUS)
+    k_out = None if k is None else torch.empty_like(k, memory_format=_CONTIGUOUS)
+    outs = q_out, k_out
+    if q is None or q.numel() == 0:  # the first of the two has something to rotate
+        q, q_out, k, k_out = k, k_out, None, None
+        if q is None or q.numel() == 0:
+            return outs
+    qs = q.shape
+    index = q.get_device()
+    second = _NONE
+    second_out = _NONE
+    if k is not None and k.numel():
+        ks = k.shape
+        _, h, s, d = ks
+        second = (k.data_ptr(), *ks, *k.stride())
+        second_out = (k_out.data_ptr(), *ks, h * s * d, s * d, d, 1)
+    _, h, s, d = qs
+    by_batch, by_token = positions.stride() if positions.dim() == 2 else (0, positions.stride(0))
+    rc = _ext.load().kf_rotary(_pack(
+        q.data_ptr(), *qs, *q.stride(), *second, q_out.data_ptr(), *qs, h * s * d, s * d, d, 1, *second_out,
+        positions.data_ptr(), _POSITION_BITS[positions.dtype], by_batch, by_token, frequencies.data_ptr(),
+        2 * frequencies.numel(), interleaved, inverse, magnitude, _DTYPES[q.dtype], _ext.raw_stream(index)))
     if rc:
         _ext.check(rc, "kf_rotary")
     return outs
@@ -139,17 +151,21 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, frequencies)
         ctx.set_materialize_grads(False)
         ctx.how = interleaved, magnitude, inverse
-        return tuple(_rotate(q, k, positions, frequencies, interleaved, magnitude, inverse))
+        return _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse)
 
     @staticmethod
     def backward(ctx, dq, dk):
         positions, frequencies = ctx.saved_tensors
         interleaved, magnitude, inverse = ctx.how
-        dq, dk = (g if need else None for g, need in zip((dq, dk), ctx.needs_input_grad))
-        grads = [None, None]
+        need_q, need_k = ctx.needs_input_grad[:2]
+        if not need_q:
+            dq = None
+        if not need_k:
+            dk = None
         if dq is not None or dk is not None:
-            grads = _Rotary.apply(dq, dk, positions, frequencies, interleaved, magnitude, not inverse)
-        return (*grads, None, None, None, None, None)
+            back = _Rotary.apply if torch.is_grad_enabled() else _rotate  # a gradient of the gradient
+            dq, dk = back(dq, dk, positions, frequencies, interleaved, magnitude, not inverse)
+        return dq, dk, None, None, None, None, None
 
 
 def apply_rotary(
@@ -171,12 +187,27 @@ def apply_rotary(
     rounded once.  Any strides; new contiguous tensors are returned, ``(q',
     k')``, or q' alone where k is None.  Differentiable in q and k.
     """
-    _check(q, k, positions, frequencies)
+    try:  # what a valid call of q and k pays for; _check() finds out what to say
+        index = q.get_device()
+        b, _, s, d = q.shape
+        kb, _, ks, kd = k.shape
+        ps = positions.shape
+        good = (
+            index >= 0 and k.get_device() == index and positions.get_device() == index
+            and frequencies.get_device() == index and _is_sm100(index) and q.dtype in _DTYPES and k.dtype is q.dtype
+            and kb == b and ks == s and kd == d and positions.dtype in _POSITION_BITS and (ps == (b, s) or ps == (s,))
+            and frequencies.dtype is _FLOAT64 and frequencies.dim() == 1 and 0 < 2 * frequencies.numel() <= d
+            and frequencies.is_contiguous() and not frequencies.requires_grad)
+    except (AttributeError, TypeError, ValueError, RuntimeError):
+        good = False
+    if not good:
+        _check(q, k, positions, frequencies)
     magnitude = float(magnitude)
     if not math.isfinite(magnitude):
         raise ValueError("magnitude must be finite")
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        outs = _Rotary.apply(q, k, positions, frequencies, bool(interleaved), magnitude, False)
+    interleaved = bool(interleaved)
+    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
+        outs = _Rotary.apply(q, k, positions, frequencies, interleaved, magnitude, False)
     else:
-        outs = _rotate(q, k, positions, frequencies, bool(interleaved), magnitude, False)
-    return outs[0] if k is None else (outs[0], outs[1])
+        outs = _rotate(q, k, positions, frequencies, interleaved, magnitude, False)
+    return outs[0] if k is None else outs
