@@ -110,6 +110,31 @@ int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows,
   return KF_OK;
 }
 
+int encode_tmap_lines(CUtensorMap* map, const PageLines& t, int box, bool swizzle) {
+  EncodeTiledFn fn = get_encode_fn();
+  if (!fn) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
+  if (!aligned16(t.base)) return set_error(KF_ERR_INVALID, "TMA base pointer not 16-byte aligned");
+  cuuint64_t dims[5] = {(cuuint64_t)t.bytes / 2, (cuuint64_t)t.lines, (cuuint64_t)t.planes, (cuuint64_t)t.heads,
+                        (cuuint64_t)t.pages};
+  cuuint64_t strides[4] = {(cuuint64_t)t.line_stride, (cuuint64_t)t.plane_stride, (cuuint64_t)t.head_stride,
+                           (cuuint64_t)t.page_stride};
+  for (int i = 0; i < 4; ++i) {
+    if (dims[i + 1] == 1) {
+      strides[i] = 128;  // a size-1 dimension may carry any stride; give it a legal one
+    } else if (strides[i] % 16 != 0 || strides[i] == 0) {
+      return set_error(KF_ERR_INVALID, "TMA stride %llu bytes is not a positive multiple of 16",
+                       (unsigned long long)strides[i]);
+    }
+  }
+  cuuint32_t boxes[5] = {64, (cuuint32_t)box, (cuuint32_t)t.planes, 1, 1};
+  cuuint32_t estr[5] = {1, 1, 1, 1, 1};
+  CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, t.base, dims, strides, boxes, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_NONE,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled (lines) failed (%d)", (int)r);
+  return KF_OK;
+}
+
 int encode_tmap_2d_f32(CUtensorMap* map, void* ptr, int64_t rows, int64_t cols, int box_cols,
                        int box_rows) {
   EncodeTiledFn fn = get_encode_fn();

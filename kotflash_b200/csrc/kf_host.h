@@ -34,6 +34,20 @@ int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box
 // read as zero.
 int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows, int panels, bool swizzle);
 
+// A pool of pages of bytes as lines of at most 128: sizes and strides in bytes.
+struct PageLines {
+  void* base;
+  int64_t bytes;                   // of a line
+  int64_t lines, line_stride;      // of a page and head
+  int64_t planes, plane_stride;    // pools of the same shape and strides
+  int64_t heads, head_stride, pages, page_stride;
+};
+
+// Encode a 5-D tiled TMA descriptor over it with coordinates (pair of bytes,
+// line, plane, head, page) and boxes of 128 bytes x `box` lines x all planes;
+// 128-byte swizzle or none; what lies outside reads as zero.
+int encode_tmap_lines(CUtensorMap* map, const PageLines& t, int box, bool swizzle);
+
 // Encode a 2-D tiled TMA descriptor over a row-major fp32 matrix
 // [rows][cols] (cols contiguous) with a (box_cols x box_rows) box and 128-byte
 // swizzle (box_cols * 4 must be <= 128).

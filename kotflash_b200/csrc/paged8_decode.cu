@@ -17,8 +17,12 @@
 //
 // The split over blocks, teams and rings is paged_decode.cu's (see there and
 // paged_split.cuh).  What differs, for a team of warps:
-// - A step takes 64 keys of rows up to 64 bytes, else 32: the bytes in flight
-//   and the cost of a step stay those of 16-bit rows.
+// - A step takes 32 keys of the longest rows, 64 or 128 of shorter ones: half of
+//   a microsecond of a step does not depend on its keys (32 requests of 8192
+//   keys, D = 64: 69 us with 32 a step, 56 with 64).
+// - One TMA load brings a box of keys of both K and V where the two pools have
+//   the same strides: the pair is a dimension of the tensor map, as long as the
+//   distance of the pools.  (A load takes a lane about 66 cycles to issue.)
 // - K is loaded by ldmatrix as pairs of bytes: a lane gets columns 4 c .. 4 c +
 //   3 of a key, which after conversion are the columns that a lane holds for k
 //   = 2 c, 2 c + 1 and 2 c + 8, 2 c + 9, so Q is loaded in that order.  V comes
@@ -48,24 +52,30 @@ struct Paged8Args : PagedWork {
   int64_t kss[2], vss[2];  // strides of the scales
   int block_shift;         // log2 of the tokens of a scale
   int box;                 // keys of a TMA box
-  int pitch;               // bytes from key to key of a tile
-  bool swizzle;
-  bool shallow;            // long units are loaded a third of the ring ahead instead of all of it
+  int group;               // keys whose K rows and then V rows lie together in a tile: 16 or more, box or more
+  int k_plane, v_plane;    // 0 and 1, or 1 and 0: which of the two lies first
+  bool paired;             // one load brings both
   bool q_bf16;
   float scale_log2;        // scale log2(e)
 };
 
-// Variants: KD = 16-column chunks of the head dim (4, 6 or 8); FULL: D is KD *
-// 16; NT = 8-row tiles of query rows per warp; RG = warps of a team.
+// Variants: KD = 16-column chunks of the head dim; LINES: pages are brought as
+// lines of 128 bytes, keys lie KD * 16 bytes apart (otherwise KD is 8, each row
+// has a line and the chunks are counted at run time); NT = 8-row tiles of query
+// rows per warp; RG = warps of a team.
 template <int KD, int NT, int RG>
 struct Cfg8 {
-  static constexpr int KW = KD <= 6 ? 64 : 32;               // keys a team takes of a tile
+  static constexpr int KW = KD <= 3 ? 128 : KD <= 6 ? 64 : 32;  // keys a team takes of a tile
   static constexpr int TEAMS = kWarps / RG;
   static constexpr int TILE = TEAMS * KW;
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
-  static constexpr int STAGE = KW * KD * 16 * 2;             // bytes: K rows, then V rows
-  static constexpr int STAGES = 98304 / (TEAMS * STAGE);     // 96 KB of ring per block, two blocks per SM
+  static constexpr int PITCH = KD * 16;                      // bytes from key to key
+  static constexpr int STAGE = KW * PITCH * 2;               // K and V rows
+  static constexpr int FIT = 98304 / (TEAMS * STAGE);        // 96 KB of ring per block, two blocks per SM
+  static constexpr int MOST = KD == 1 ? 4 : 8;
+  static constexpr int STAGES = FIT < MOST ? FIT : MOST;
   static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;
+  static constexpr bool SWIZZLE = KD == 2 || KD == 4 || KD == 8;
   static constexpr int HANDED = KD * 4 * 32;                 // floats of a warp's O^T of one row tile
   static constexpr int SCALES = TEAMS * STAGES * KW * 8;     // bytes
   // All of it is dynamic, with the ring, which wants to begin on 1024 bytes, in front.
@@ -80,22 +90,21 @@ struct Cfg8 {
       TEAMS * STAGES * STAGE + SCALES + (TEAMS > 1 ? 2 * HANDED + kWarps * NT * 32 : 0) * 4 + (int)sizeof(Tail);
 };
 
-// Offset of 16-byte chunk c of key r of a tile.  A tile holds keys as a page
-// does, one behind the other, brought as lines of 128 bytes whatever a row's
-// length: a TMA load of rows takes a cycle for each row and each sector of 32
-// bytes that it touches, which rows of 64 to 96 bytes pay more for than for
-// HBM (32 requests of 8192 keys, loads alone: D = 64 49 us, D = 72 67, D = 96 70).
-// Where a row's chunks are even in number the lines are swizzled; where they
-// are odd, keys lie on different banks as they are.
-__device__ __forceinline__ uint32_t chunk_at(int r, int c, int pitch, bool swizzle) {
-  const uint32_t at = (uint32_t)(r * pitch + c * 16);
-  return swizzle ? at ^ ((at >> 3) & 0x70u) : at;
+// A tile holds keys as a page does, one behind the other, brought as lines of
+// 128 bytes whatever a row's length: a TMA load of rows takes a cycle for each
+// row and each sector of 32 bytes that it touches, which rows of 64 to 96 bytes
+// pay more for than for HBM.  Where a row's chunks of 16 bytes are even in
+// number the lines are swizzled; where they are odd, keys lie on different
+// banks as they are (and six chunks apart, on pairs of them).
+template <bool SWIZZLE>
+__device__ __forceinline__ uint32_t swizzled(uint32_t at) {
+  return SWIZZLE ? at ^ ((at >> 3) & 0x70u) : at;
 }
 
 // The key of a 16-key part that stands in place x of a product.  V's fragments
 // hold keys 4 c .. 4 c + 3 of a lane, so K's two 8 x 8 parts take places {0, 1,
 // 4, 5, ..} and {2, 3, 6, 7, ..}; with this order of keys both those and eight
-// places in a row lie on different banks (six chunks apart, on pairs of them).
+// places in a row lie on different banks.
 __device__ __forceinline__ int key_of(int x) { return x ^ ((x >> 2) & 2); }
 
 // x4 over two 16 x 16 matrices of bytes, transposed: lane l gets of each
@@ -114,7 +123,7 @@ __device__ __forceinline__ uint32_t load_scale(const uint8_t* p) {
   return x;
 }
 
-template <bool INT8, int KD, bool FULL, int NT, int RG>
+template <bool INT8, int KD, bool LINES, int NT, int RG>
 __global__ void __launch_bounds__(kThreads, kBlocksPerSm)
 paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const Paged8Args a) {
@@ -122,7 +131,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   constexpr int KW = C::KW, STAGES = C::STAGES, TILE = C::TILE;
   constexpr int H = KW / 16;           // 16-key parts of a step
   constexpr int LOOKS = KW / 32;       // keys that a lane looks up
-  constexpr int PAIRS = KD / 2;        // pairs of chunks
+  constexpr int PAIRS = (KD + 1) / 2;  // pairs of chunks
   // Weights lie between 2^BELOW and 2^LIMIT at the row's largest x + f, the
   // top of fp16's range: its 11 bits hold down to 2^-25 of the largest, and
   // what is lost below is at most 2^-36 of it.
@@ -160,25 +169,35 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (request < (uint32_t)a.B)
       kf::prefetch_l2_bulk(a.q + request * a.qs[0] + (line - request * a.Hq) * a.qs[1], a.D * 2);
   }
-  const int pitch = FULL ? KD * 16 : a.pitch;
-  const bool swizzle = FULL || a.swizzle;
-  const int chunks = FULL ? KD : (a.D + 15) / 16;
-  const int v_bytes = (KW * pitch + 1023) & ~1023;  // where V's rows begin
+  constexpr int PITCH = C::PITCH;
+  const int chunks = LINES ? KD : (a.D + 15) / 16;
+  // Where key r's chunk c lies in a stage: groups of keys, K rows and then V
+  // rows (or V rows first) of each.
+  const uint32_t k_base = (uint32_t)(a.k_plane * a.group * PITCH), v_base = (uint32_t)(a.v_plane * a.group * PITCH);
+  auto place = [&](int r, int c, uint32_t base) {
+    const int inside = r & (a.group - 1);
+    return swizzled<C::SWIZZLE>(base + (uint32_t)((2 * r - inside) * PITCH + c * 16));
+  };
   // Offsets of a lane's ldmatrix rows, by pair of chunks; a missing second
-  // chunk repeats the first.  Keys 16 h later lie 16 h pitch on, and in lines of
-  // four keys every other 16 are swizzled the other way about.
+  // chunk repeats the first.
   uint32_t k_off[PAIRS], v_off[PAIRS];
 #pragma unroll
   for (int x = 0; x < PAIRS; ++x) {
     const int i = lane & 7, c = min(2 * x + (lane >> 4), chunks - 1);
-    k_off[x] = chunk_at(key_of(4 * (i >> 1) + (i & 1) + ((lane >> 3) & 1) * 2), c, pitch, swizzle);
-    v_off[x] = chunk_at(key_of(lane & 15), c, pitch, swizzle);
+    k_off[x] = place(key_of(4 * (i >> 1) + (i & 1) + ((lane >> 3) & 1) * 2), c, k_base);
+    v_off[x] = place(key_of(lane & 15), c, v_base);
   }
-  const uint32_t flip = !FULL && swizzle && pitch == 32 ? 64u : 0u;
-  auto part = [&](uint32_t off, int h) { return (off ^ ((h & 1) ? flip : 0u)) + h * 16 * pitch; };
+  // From a 16-key part to the next, the one after and the fourth; in lines of
+  // four keys a step of 512 bytes swizzles the other way about.
+  const uint32_t step1 = (a.group > 16 ? 16 : 32) * PITCH, step2 = (a.group > 32 ? 32 : 64) * PITCH,
+                 step4 = (a.group > 64 ? 64 : 128) * PITCH;
+  const uint32_t flip = C::SWIZZLE && PITCH == 32 && a.group > 16 ? 64u : 0u;
+  auto part = [&](uint32_t off, int h) {
+    return (PITCH == 32 && (h & 1) ? off ^ flip : off) + (h & 1 ? step1 : 0) + (h & 2 ? step2 : 0) + (h & 4 ? step4 : 0);
+  };
   // Half a chunk at the end of a row: what lies behind it can be a code of NaN,
   // which Q's zeros do not silence.
-  const uint32_t edge = !FULL && (a.D & 8) && (lane & 3) >= 2 ? 0u : 0xffffffffu;
+  const uint32_t edge = (a.D & 8) && (lane & 3) >= 2 ? 0u : 0xffffffffu;
   kf::griddep_wait();
   kf::griddep_launch_dependents();
 
@@ -231,16 +250,21 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < LOOKS; ++i) seen_s[team][stage][i] = seen[i];
-      kf::mbar_arrive_expect_tx(bar, boxes * (uint32_t)(a.box * pitch * 2));
+      kf::mbar_arrive_expect_tx(bar, boxes * (uint32_t)(a.box * PITCH * 2));
     }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < LOOKS; ++i) {
       if (starts[i]) {
-        uint8_t* st = ring + stage * C::STAGE + (i * 32 + lane) * pitch;
-        const int line = (int)(((uint64_t)p.row[i] * pitch) >> 7);
-        kf::tma_load_5d_once(st, &map_k, bar, 0, line, 0, p.h, p.page[i], once);
-        kf::tma_load_5d_once(st + v_bytes, &map_v, bar, 0, line, 0, p.h, p.page[i], once);
+        const int r = i * 32 + lane, inside = r & (a.group - 1);
+        uint8_t* st = ring + stage * C::STAGE + (2 * r - inside) * PITCH;
+        const int line = LINES ? (int)(p.row[i] * (uint32_t)KD >> 3) : (int)p.row[i];
+        if (a.paired) {
+          kf::tma_load_5d_once(st, &map_k, bar, 0, line, 0, p.h, p.page[i], once);
+        } else {
+          kf::tma_load_5d_once(st + k_base, &map_k, bar, 0, line, 0, p.h, p.page[i], once);
+          kf::tma_load_5d_once(st + v_base, &map_v, bar, 0, line, 0, p.h, p.page[i], once);
+        }
       }
       s.k[i] = s.v[i] = 256;
       if (p.page[i] < a.num_pages) {
@@ -261,6 +285,9 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       if (lane == 0) nan_s[team][stage][i] = nan;
     }
   };
+
+  // (an index within KD for what odd numbers of chunks do not use)
+  constexpr auto last = [](int x) { return x < KD ? x : KD - 1; };
 
   // ---- state of the unit being worked on
   uint32_t qb[NT][KD][2];              // Q^T as B fragments
@@ -322,8 +349,12 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   };
 
   load_q();
-  // Tiles loaded ahead of the one in use (see paged_decode.cu).
-  const int depth = a.shallow && share.total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
+  // Tiles loaded ahead of the one in use: all of the ring where units are short
+  // and drain it at each end, and where shares are long (32 requests of 8192
+  // keys 86.8 us, 89.1 with a third of it); else a third, since whoever comes
+  // first in a short call would take the others' bandwidth (8 requests of 4200
+  // keys 19.6 us, 20.3 with all of it).
+  const int depth = share.even < 32 && share.total >= 10u * a.B ? C::SHALLOW : STAGES - 1;
   // The first warp of a team loads.  To begin with it looks up the pages of the
   // whole ring at once, then always one step ahead of their use.
   bool more = rg == 0;                 // whether the load cursor stands on a tile that is not loaded yet
@@ -376,7 +407,12 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       any |= seen[i];
       all &= seen[i];
     }
-    auto sees = [&](uint32_t key) { return ((seen[LOOKS == 1 || key < 32 ? 0 : LOOKS - 1] >> (key & 31)) & 1) != 0; };
+    auto sees = [&](uint32_t key) {
+      uint32_t word = seen[0];
+#pragma unroll
+      for (int i = 1; i < LOOKS; ++i) word = key >> 5 == i ? seen[i] : word;
+      return ((word >> (key & 31)) & 1) != 0;
+    };
     if (rg == 0 && alive && more) {
       issue(fill, ahead, coming);
       late = fill;
@@ -388,8 +424,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       }
     }
 
-    uint8_t* kt = ring + stage * C::STAGE;
-    uint8_t* vt = kt + v_bytes;
+    uint8_t* tile = ring + stage * C::STAGE;
     const uint32_t key0 = work.t * TILE + team * KW;
     if (any != 0 && (all != 0xffffffffu || (a.nk && key0 + KW >= work.keys))) {
       // The end of a request or pages without a table entry.  Rows that nobody
@@ -399,7 +434,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
       for (int x = rg; x < KW / 4; x += RG) {
         const int r = 4 * x + (lane >> 3);
-        clear16(kf::smem_u32(vt) + chunk_at(r, lane & 7, pitch, swizzle), (lane & 7) * 16 < pitch && !sees(r));
+        clear16(kf::smem_u32(tile) + place(r, lane & 7, v_base), (lane & 7) * 16 < PITCH && !sees(r));
       }
       const uint32_t r = work.keys - 1 - key0;  // the newest position, unless the table is too short for it
       if (a.nk && r < (uint32_t)KW && sees(r) && work.whole && a.slots[work.b] >= 0 && rg == 0) {
@@ -420,7 +455,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         uint2 codes = a.q_bf16 ? kf::encode8<INT8, true>(x, by) : kf::encode8<INT8, false>(x, by);
         if (nan) codes = make_uint2(0, 0);
         if (c < a.D / 8) {
-          *reinterpret_cast<uint2*>((is_v ? vt : kt) + chunk_at((int)r, c >> 1, pitch, swizzle) + (c & 1) * 8) = codes;
+          *reinterpret_cast<uint2*>(tile + place((int)r, c >> 1, is_v ? v_base : k_base) + (c & 1) * 8) = codes;
           if (work.rb == 0)
             *reinterpret_cast<uint2*>(is_v ? a.v + page * a.vs[0] + work.h * a.vs[1] + row * a.vs[2] + c * 8
                                            : a.k + page * a.ks[0] + work.h * a.ks[1] + row * a.ks[2] + c * 8) = codes;
@@ -446,7 +481,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (any != 0) {
 #pragma unroll
       for (int i = 0; i < LOOKS; ++i) v_nan |= nan_s[team][stage][i] != 0;
-      const uint32_t sk = kf::smem_u32(kt), sv = kf::smem_u32(vt);
+      const uint32_t st = kf::smem_u32(tile);
       // S^T (keys x rows)
       float cc[H][NT][4];
 #pragma unroll
@@ -455,25 +490,23 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int nt = 0; nt < NT; ++nt) cc[h][nt][0] = cc[h][nt][1] = cc[h][nt][2] = cc[h][nt][3] = 0.f;
 #pragma unroll
       for (int x = 0; x < PAIRS; ++x) {
-        if (!FULL && 2 * x >= chunks) continue;
+        if (!LINES && 2 * x >= chunks) continue;
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t w[4], f[2][4];
-          kf::ldmatrix_x4(w, sk + part(k_off[x], h));
-          if constexpr (!FULL) {
-            if (2 * x + 1 == chunks) w[0] &= edge, w[1] &= edge;
-            if (2 * x + 2 == chunks) w[2] &= edge, w[3] &= edge;
-          }
+          kf::ldmatrix_x4(w, st + part(k_off[x], h));
+          if (2 * x + 1 == chunks) w[0] &= edge, w[1] &= edge;
+          if (2 * x + 2 == chunks) w[2] &= edge, w[3] &= edge;
           kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
           kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
           kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
           kf::decode4<INT8>(w[3], f[1][1], f[1][3]);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) kf::mma_16816<false>(cc[h][nt], f[0], qb[nt][2 * x][0], qb[nt][2 * x][1]);
-          if (FULL || 2 * x + 1 < chunks) {
+          if (2 * x + 1 < chunks) {
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-              kf::mma_16816<false>(cc[h][nt], f[1], qb[nt][2 * x + 1][0], qb[nt][2 * x + 1][1]);
+              kf::mma_16816<false>(cc[h][nt], f[1], qb[nt][last(2 * x + 1)][0], qb[nt][last(2 * x + 1)][1]);
           }
         }
       }
@@ -582,7 +615,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       // its accumulator's digits end.
 #pragma unroll
       for (int x = 0; x < PAIRS; ++x) {
-        if (!FULL && 2 * x >= chunks) continue;
+        if (!LINES && 2 * x >= chunks) continue;
         float step[2][NT][4];
 #pragma unroll
         for (int e = 0; e < 2; ++e)
@@ -591,14 +624,14 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
         for (int h = 0; h < H; ++h) {
           uint32_t w[4], f[2][4];
-          ldmatrix_trans_b8(w, sv + part(v_off[x], h));
+          ldmatrix_trans_b8(w, st + part(v_off[x], h));
           kf::decode4<INT8>(w[0], f[0][0], f[0][2]);
           kf::decode4<INT8>(w[1], f[0][1], f[0][3]);
           kf::decode4<INT8>(w[2], f[1][0], f[1][2]);
           kf::decode4<INT8>(w[3], f[1][1], f[1][3]);
 #pragma unroll
           for (int e = 0; e < 2; ++e)
-            if (FULL || 2 * x + e < chunks) {
+            if (2 * x + e < chunks) {
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) kf::mma_16816<false>(step[e][nt], f[e], pb[h][nt][0], pb[h][nt][1]);
             }
@@ -608,9 +641,10 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int i = 0; i < 4; i += 2)
-              kf::f2_split(kf::add2(kf::f2(ot[nt][2 * x + e][i], ot[nt][2 * x + e][i + 1]), kf::f2(step[e][nt][i], step[e][nt][i + 1])),
-                           ot[nt][2 * x + e][i], ot[nt][2 * x + e][i + 1]);
+            for (int i = 0; i < 4 && 2 * x + e < KD; i += 2)
+              kf::f2_split(kf::add2(kf::f2(ot[nt][last(2 * x + e)][i], ot[nt][last(2 * x + e)][i + 1]),
+                                    kf::f2(step[e][nt][i], step[e][nt][i + 1])),
+                           ot[nt][last(2 * x + e)][i], ot[nt][last(2 * x + e)][i + 1]);
       }
     }
     if (++stage == STAGES) {
@@ -784,27 +818,21 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 
 // How the rows of a pool lie in a tile, and the variant that takes them.
 struct Layout {
-  int steps, pitch, box;
+  int steps, box;
   bool lines;    // pages are brought as lines of 128 bytes
-  bool swizzle, full;
 };
 
 Layout layout_of(int64_t D, const kf_tensor4& k, const kf_tensor4& v) {
   Layout l;
   const int64_t page_size = k.size[2];
-  const int chunks = (int)((D + 15) / 16);
-  l.box = 64;                          // keys that never cross a page
+  const int chunks = (int)((D + 15) / 16), pitch = chunks * 16, keys = chunks <= 3 ? 128 : chunks <= 6 ? 64 : 32;
+  l.box = keys;                        // keys that never cross a page
   while (page_size % l.box) l.box /= 2;
-  l.pitch = chunks * 16;
   // Pages as lines: rows of whole chunks without a gap, a box of them full
-  // lines.  Else each row is a line of its own (rows of 128 bytes always are).
-  l.lines = chunks < 8 && l.pitch * l.box % 128 == 0 &&
-            (page_size == 1 || (k.stride[2] == l.pitch && v.stride[2] == l.pitch));
-  if (!l.lines) l.pitch = 128;
-  l.steps = !l.lines ? 8 : chunks <= 4 ? 4 : chunks <= 6 ? 6 : 8;
-  if (l.steps == 8 && l.box > 32) l.box = 32;
-  l.swizzle = !l.lines || chunks == 2 || chunks == 4;
-  l.full = D == 128 || (D == 64 && l.lines);
+  // lines.  Else each row is a line of its own.
+  l.lines = pitch * l.box % 128 == 0 && (page_size == 1 || (k.stride[2] == pitch && v.stride[2] == pitch));
+  l.steps = l.lines ? chunks : 8;
+  if (!l.lines && l.box > 32) l.box = 32;
   return l;
 }
 
@@ -816,15 +844,16 @@ int tile_keys_of(int rows) {
                       : Cfg8<KD, 2, 4>::TILE;
 }
 int tile_keys(int steps, int rows) {
-  return steps == 4 ? tile_keys_of<4>(rows) : steps == 6 ? tile_keys_of<6>(rows) : tile_keys_of<8>(rows);
+  return steps <= 3 ? tile_keys_of<3>(rows) : steps <= 6 ? tile_keys_of<6>(rows) : tile_keys_of<8>(rows);
 }
 
-template <bool INT8, int KD, bool FULL, int NT, int RG>
+template <bool INT8, int KD, bool LINES, int NT, int RG>
 int launch_variant(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, cudaStream_t st) {
   using C = Cfg8<KD, NT, RG>;
   static_assert(C::STAGES >= 2, "the ring needs two stages");
+  static_assert(C::STAGE % 1024 == 0, "stages begin where a swizzle does");
   static_assert(C::SMEM <= 112 * 1024, "two blocks per SM");
-  auto kern = paged8_decode_kernel<INT8, KD, FULL, NT, RG>;
+  auto kern = paged8_decode_kernel<INT8, KD, LINES, NT, RG>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
     (void)cudaGetLastError();
     return kf::set_error(KF_ERR_CUDA, "kf_paged8_decode: cannot reserve %d bytes of shared memory", C::SMEM);
@@ -832,26 +861,31 @@ int launch_variant(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap
   return kf::launch_dependent(kern, dim3((unsigned)blocks), dim3(kThreads), C::SMEM, st, "kf_paged8_decode", mk, mv, a);
 }
 
-template <bool INT8, int KD, bool FULL>
+template <bool INT8, int KD, bool LINES>
 int dispatch_rows(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, int rows, int blocks,
                   cudaStream_t st) {
   switch (rows) {  // unit_rows()'s
-    case 8: return launch_variant<INT8, KD, FULL, 1, 1>(a, mk, mv, blocks, st);
-    case 16: return launch_variant<INT8, KD, FULL, 2, 1>(a, mk, mv, blocks, st);
-    case 32: return launch_variant<INT8, KD, FULL, 2, 2>(a, mk, mv, blocks, st);
-    default: return launch_variant<INT8, KD, FULL, 2, 4>(a, mk, mv, blocks, st);
+    case 8: return launch_variant<INT8, KD, LINES, 1, 1>(a, mk, mv, blocks, st);
+    case 16: return launch_variant<INT8, KD, LINES, 2, 1>(a, mk, mv, blocks, st);
+    case 32: return launch_variant<INT8, KD, LINES, 2, 2>(a, mk, mv, blocks, st);
+    default: return launch_variant<INT8, KD, LINES, 2, 4>(a, mk, mv, blocks, st);
   }
 }
 
 template <bool INT8>
 int dispatch(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap& mv, const Layout& l, int rows, int blocks,
              cudaStream_t st) {
-  if (l.steps == 4)
-    return l.full ? dispatch_rows<INT8, 4, true>(a, mk, mv, rows, blocks, st)
-                  : dispatch_rows<INT8, 4, false>(a, mk, mv, rows, blocks, st);
-  if (l.steps == 6) return dispatch_rows<INT8, 6, false>(a, mk, mv, rows, blocks, st);
-  return l.full ? dispatch_rows<INT8, 8, true>(a, mk, mv, rows, blocks, st)
-                : dispatch_rows<INT8, 8, false>(a, mk, mv, rows, blocks, st);
+  if (!l.lines) return dispatch_rows<INT8, 8, false>(a, mk, mv, rows, blocks, st);
+  switch (l.steps) {
+    case 1: return dispatch_rows<INT8, 1, true>(a, mk, mv, rows, blocks, st);
+    case 2: return dispatch_rows<INT8, 2, true>(a, mk, mv, rows, blocks, st);
+    case 3: return dispatch_rows<INT8, 3, true>(a, mk, mv, rows, blocks, st);
+    case 4: return dispatch_rows<INT8, 4, true>(a, mk, mv, rows, blocks, st);
+    case 5: return dispatch_rows<INT8, 5, true>(a, mk, mv, rows, blocks, st);
+    case 6: return dispatch_rows<INT8, 6, true>(a, mk, mv, rows, blocks, st);
+    case 7: return dispatch_rows<INT8, 7, true>(a, mk, mv, rows, blocks, st);
+    default: return dispatch_rows<INT8, 8, true>(a, mk, mv, rows, blocks, st);
+  }
 }
 
 bool rows16(const kf_tensor4& t) {
@@ -945,27 +979,40 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   a.num_pages = (uint32_t)pages;
   a.status = args->status;
   a.box = l.box;
-  a.pitch = l.pitch;
-  a.swizzle = l.swizzle;
-  a.shallow = l.full;
+  a.group = l.box < 16 ? 16 : l.box;
   a.q_bf16 = args->dtype == KF_BF16;
   a.scale_log2 = (float)args->scale * kLog2e;
 
   int64_t blocks, most;
   rc = plan_work(what, a, max_pages, rows, tile_keys(l.steps, rows), args->workspace, args->workspace_bytes, &blocks, &most);
   if (rc != KF_OK) return rc;
+  // K and V as two planes of one tensor, where that describes both and a box
+  // is a whole group.
+  const int64_t apart = static_cast<const uint8_t*>(v_pages.ptr) - static_cast<const uint8_t*>(k_pages.ptr);
+  a.paired = l.box >= 16 && apart != 0 && (apart > 0 ? apart : -apart) < ((int64_t)1 << 39);
+  for (int i = 0; i < 3; ++i) a.paired = a.paired && (k_pages.size[i] == 1 || k_pages.stride[i] == v_pages.stride[i]);
+  a.k_plane = a.paired && apart < 0 ? 1 : 0;
+  a.v_plane = 1 - a.k_plane;
+  const int pitch = l.steps * 16, lines = l.lines ? l.box * pitch / 128 : l.box;
+  const bool swizzle = l.steps == 2 || l.steps == 4 || l.steps == 8;
   CUtensorMap mk, mv;
-  for (int w = 0; w < 2; ++w) {
-    kf_tensor4 pairs = w ? v_pages : k_pages;  // of bytes
-    for (int i = 0; i < 3; ++i) pairs.stride[i] /= 2;
-    pairs.size[3] = l.lines ? 64 : D / 2;
-    if (l.lines) {
-      pairs.size[2] = page_size * l.pitch / 128;
-      pairs.stride[2] = 64;
-    }
-    rc = kf::encode_tmap_pages(w ? &mv : &mk, &pairs, 64, l.lines ? l.box * l.pitch / 128 : l.box, 1, l.swizzle);
+  for (int w = 0; w < (a.paired ? 1 : 2); ++w) {
+    const kf_tensor4& pool = a.paired ? (apart > 0 ? k_pages : v_pages) : w ? v_pages : k_pages;
+    kf::PageLines t;
+    t.base = pool.ptr;
+    t.bytes = l.lines ? 128 : D;
+    t.lines = l.lines ? page_size * pitch / 128 : page_size;
+    t.line_stride = l.lines ? 128 : pool.stride[2];
+    t.planes = a.paired ? 2 : 1;
+    t.plane_stride = apart > 0 ? apart : -apart;
+    t.heads = Hkv;
+    t.head_stride = pool.stride[1];
+    t.pages = pages;
+    t.page_stride = pool.stride[0];
+    rc = kf::encode_tmap_lines(w ? &mv : &mk, t, lines, swizzle);
     if (rc != KF_OK) return rc;
   }
+  if (a.paired) mv = mk;
   if (fused && !inside) {
     kf_paged8_append_args store;
     store.cache = cache;
