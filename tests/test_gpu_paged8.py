@@ -440,6 +440,36 @@ def test_pools_with_any_strides():
     assert torch.equal(both[:, 0].contiguous().view(torch.uint8), cache[2].view(torch.uint8))
 
 
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 32), (72, 16), (32, 64), (16, 128), (96, 8)])
+def test_k_and_v_however_they_lie_to_one_another(d, page):
+    """K before V, V before K, both in one buffer, side by side in every page, one
+    pool as both, with different strides: the same values, so the same results."""
+    lens, hkv = [300, 41, 900], 2
+    cache, kv, vv, table, lengths = _requests(lens, page, hkv, d, "e4m3", 75)
+    kp, vp, ks, vs = cache
+    n, pitch = kp.shape[0], kp.stride(2)
+    q = _rand((3, 6, 1, d), BF16, 76)
+    want, want_lse = paged_attention8(q, *cache, table, lengths, return_lse=True)
+
+    def blank(*shape):
+        return torch.full((*shape, pitch), 0x7f, device="cuda", dtype=torch.uint8).view(kp.dtype)[..., :d]
+
+    both = blank(2, n, hkv, page)
+    for first, second in ((0, 1), (1, 0)):
+        k, v = both[first], both[second]
+        k.copy_(kp), v.copy_(vp)
+        out, lse = paged_attention8(q, k, v, ks, vs, table, lengths, return_lse=True)
+        assert torch.equal(out, want) and torch.equal(lse, want_lse)
+    side = blank(n, 2, hkv, page)
+    k, v = side[:, 1], side[:, 0]
+    k.copy_(kp), v.copy_(vp)
+    assert torch.equal(paged_attention8(q, k, v, ks, vs, table, lengths), want)
+    wide = blank(n, hkv + 1, page)[:, 1:]                     # V with other strides than K
+    wide.copy_(vp)
+    assert torch.equal(paged_attention8(q, kp, wide, ks, vs, table, lengths), want)
+    _check(paged_attention8(q, kp, kp, ks, ks, table, lengths), None, q, kv, kv, table, lengths, d ** -0.5, "one pool")
+
+
 # ---------------------------------------------------------------- the append on the way
 
 @pytest.mark.parametrize("hq,hkv,d,dtype,held,page,block", [
