@@ -434,12 +434,13 @@ typedef struct kf_paged8_decode_args {
   int64_t         dtype;
   double          scale;
   void*           workspace;
-  uint64_t        workspace_bytes;  /* kf_paged_decode_workspace_bytes(...) */
+  uint64_t        workspace_bytes;  /* kf_paged8_decode_workspace_bytes(...) */
   int32_t*        status;
   void*           stream;
 } kf_paged8_decode_args;
 int kf_paged8_append(const kf_paged8_append_args* args);
 int kf_paged8_read(const kf_paged8_read_args* args);
+size_t kf_paged8_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int sm_count);
 int kf_paged8_decode(const kf_paged8_decode_args* args);
 
 /* ---- the process's status word -------------------------------------------

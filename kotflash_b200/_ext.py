@@ -83,6 +83,7 @@ SIGNATURES = {
     "kf_rotary": (_I, [_BYTES]),
     "kf_paged8_append": (_I, [_BYTES]),
     "kf_paged8_read": (_I, [_BYTES]),
+    "kf_paged8_decode_workspace_bytes": (_SZ, [_I64, _I64, _I64, _I]),
     "kf_paged8_decode": (_I, [_BYTES]),
     "kf_device_status": (_I, [_I, ctypes.POINTER(_VP)]),
     "kf_selftest_bounded_wait": (_I, [_VP, _I64, _VP]),

@@ -59,6 +59,14 @@ struct Paged8Args : PagedWork {
   float scale_log2;        // scale log2(e)
 };
 
+// Blocks per SM.  Three where registers allow it without a spill and the
+// conversions and the latency of a step, not HBM, set the pace (D = 64: 32
+// requests of 8192 keys 54.1 -> 48.5 us, two of 100000 with 32 heads 42.3 ->
+// 39.1); two for longer rows, where three ask for more than HBM gives and end far
+// apart (D = 128: 86.8 -> 115), and shorter ones, whose 128 keys a step want
+// the registers (D = 32: 42 -> 52).
+constexpr int blocks_per_sm(int steps, int rows) { return steps == 4 && rows == 8 ? 3 : 2; }
+
 // Variants: KD = 16-column chunks of the head dim; LINES: pages are brought as
 // lines of 128 bytes, keys lie KD * 16 bytes apart (otherwise KD is 8, each row
 // has a line and the chunks are counted at run time); NT = 8-row tiles of query
@@ -71,7 +79,8 @@ struct Cfg8 {
   static constexpr int ROWS = NT * 8 * RG;                   // query rows of a unit
   static constexpr int PITCH = KD * 16;                      // bytes from key to key
   static constexpr int STAGE = KW * PITCH * 2;               // K and V rows
-  static constexpr int FIT = 98304 / (TEAMS * STAGE);        // 96 KB of ring per block, two blocks per SM
+  static constexpr int BLOCKS = blocks_per_sm(KD, ROWS);
+  static constexpr int FIT = 196608 / BLOCKS / (TEAMS * STAGE);  // of 192 KB of ring per SM
   static constexpr int MOST = KD == 1 ? 4 : 8;
   static constexpr int STAGES = FIT < MOST ? FIT : MOST;
   static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;
@@ -124,7 +133,7 @@ __device__ __forceinline__ uint32_t load_scale(const uint8_t* p) {
 }
 
 template <bool INT8, int KD, bool LINES, int NT, int RG>
-__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+__global__ void __launch_bounds__(kThreads, (Cfg8<KD, NT, RG>::BLOCKS))
 paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                      const Paged8Args a) {
   using C = Cfg8<KD, NT, RG>;
@@ -852,7 +861,8 @@ int launch_variant(const Paged8Args& a, const CUtensorMap& mk, const CUtensorMap
   using C = Cfg8<KD, NT, RG>;
   static_assert(C::STAGES >= 2, "the ring needs two stages");
   static_assert(C::STAGE % 1024 == 0, "stages begin where a swizzle does");
-  static_assert(C::SMEM <= 112 * 1024, "two blocks per SM");
+  // an SM has 228 KB, of which each block takes 1 KB besides its own
+  static_assert(C::SMEM <= (228 / C::BLOCKS - 1) * 1024, "the blocks of an SM");
   auto kern = paged8_decode_kernel<INT8, KD, LINES, NT, RG>;
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess) {
     (void)cudaGetLastError();
@@ -896,6 +906,12 @@ bool rows16(const kf_tensor4& t) {
 }
 
 }  // namespace
+
+extern "C" size_t kf_paged8_decode_workspace_bytes(int64_t Hq, int64_t Hkv, int64_t D, int sm_count) {
+  if (Hq <= 0 || Hkv <= 0 || D <= 0 || sm_count <= 0) return 0;
+  const int rows = unit_rows(Hq / Hkv), steps = (int)((D + 15) / 16);
+  return workspace_need(sm_count * blocks_per_sm(steps, rows), rows, D);
+}
 
 extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   using kf::set_error;
@@ -984,7 +1000,8 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   a.scale_log2 = (float)args->scale * kLog2e;
 
   int64_t blocks, most;
-  rc = plan_work(what, a, max_pages, rows, tile_keys(l.steps, rows), args->workspace, args->workspace_bytes, &blocks, &most);
+  rc = plan_work(what, a, max_pages, rows, tile_keys(l.steps, rows), blocks_per_sm(l.steps, rows), args->workspace,
+                 args->workspace_bytes, &blocks, &most);
   if (rc != KF_OK) return rc;
   // K and V as two planes of one tensor, where that describes both and a box
   // is a whole group.

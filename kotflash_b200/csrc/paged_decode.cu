@@ -834,8 +834,8 @@ extern "C" int kf_paged_decode(const kf_paged_decode_args* args) {
 
   const int steps = head_steps(D, wide);
   int64_t blocks, most;
-  int rc = plan_work(what, a, max_pages, rows, tile_keys(steps, rows), args->workspace, args->workspace_bytes, &blocks,
-                     &most);
+  int rc = plan_work(what, a, max_pages, rows, tile_keys(steps, rows), kBlocksPerSm, args->workspace,
+                     args->workspace_bytes, &blocks, &most);
   if (rc != KF_OK) return rc;
   CUtensorMap mk, mv;
   rc = kf::encode_tmap_pages(&mk, k_pages, cols, a.box, panels, a.width != 0);

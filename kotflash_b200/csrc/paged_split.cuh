@@ -324,8 +324,8 @@ inline size_t workspace_need(int blocks, int rows, int64_t D) {
 // tile, `rows`: query rows of a unit.  One wave of blocks, or fewer when the
 // tables cannot hold that many tiles.  A unit of one tile is never cut, so
 // nothing is left to join (*most == 1).
-inline int plan_work(const char* what, PagedWork& a, int64_t max_pages, int rows, int64_t tile, void* workspace,
-                     uint64_t workspace_bytes, int64_t* blocks_out, int64_t* most_out) {
+inline int plan_work(const char* what, PagedWork& a, int64_t max_pages, int rows, int64_t tile, int blocks_per_sm,
+                     void* workspace, uint64_t workspace_bytes, int64_t* blocks_out, int64_t* most_out) {
   a.row_blocks = (a.G + rows - 1) / rows;
   const int64_t capacity = max_pages * a.page_size;
   a.capacity = (uint32_t)(capacity < 0x7fffffffLL ? capacity : 0x7fffffffLL);
@@ -333,7 +333,7 @@ inline int plan_work(const char* what, PagedWork& a, int64_t max_pages, int rows
   kf::division(a.page_size, &a.page_mul, &a.page_shift);
   const int64_t most = (a.capacity + tile - 1) / tile;
   const int64_t units = (int64_t)a.B * a.Hkv * a.row_blocks;
-  int64_t blocks = (int64_t)kf::sm_count_current_device() * kBlocksPerSm;
+  int64_t blocks = (int64_t)kf::sm_count_current_device() * blocks_per_sm;
   if (units * (most + 1) > 0x7fffffffLL) return kf::set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
   if (most == 1 && units < blocks) blocks = units;
   if (units * (most + 1) < blocks) blocks = units * (most + 1);

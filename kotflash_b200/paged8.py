@@ -28,13 +28,13 @@ implementation.  Inference only.  The reference has neither pages nor 8 bits.
 from __future__ import annotations
 
 import math
+from functools import lru_cache
 from typing import Optional, Tuple, Union
 
 import torch
 
 from . import _ext
-from .paged import (PagedKVCache, _check_device, _check_inference, _check_int32, _check_slots, _check_table,
-                    _workspace_elements)
+from .paged import PagedKVCache, _check_device, _check_inference, _check_int32, _check_slots, _check_table
 
 _DTYPES = {torch.float16: _ext.KF_F16, torch.bfloat16: _ext.KF_BF16}
 _FORMATS = {torch.float8_e4m3fn: _ext.KF_E4M3, torch.int8: _ext.KF_INT8}
@@ -231,6 +231,12 @@ def _check_attention(q, k_pages, v_pages, k_scales, v_scales, block_table, lengt
         raise ValueError("num_query_heads must be divisible by num_kv_heads (GQA/MQA)")
     _check_inference(what, q, *rows)
     _check_device(what, q, k_pages, v_pages, k_scales, v_scales, block_table, lengths, *rows, *((slots,) if rows else ()))
+
+
+@lru_cache(maxsize=256)
+def _workspace_elements(hq: int, hkv: int, d: int, device_index: int) -> int:
+    """Workspace of kf_paged8_decode in 16-bit elements."""
+    return _ext.load().kf_paged8_decode_workspace_bytes(hq, hkv, d, _ext.sm_count(device_index)) // 2 + 8
 
 
 def paged_attention8(
