@@ -151,7 +151,11 @@ class _Rotary(torch.autograd.Function):
         ctx.save_for_backward(positions, frequencies)
         ctx.set_materialize_grads(False)
         ctx.how = interleaved, magnitude, inverse
-        return _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse)
+        outs = _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse)
+        constant = [out for out, need in zip(outs, ctx.needs_input_grad) if out is not None and not need]
+        if constant:
+            ctx.mark_non_differentiable(*constant)
+        return outs
 
     @staticmethod
     def backward(ctx, dq, dk):

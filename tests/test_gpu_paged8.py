@@ -576,6 +576,30 @@ def test_serving_with_rotary_positions(held, block, dtype):
     del graph
 
 
+def test_pools_past_4_gb():
+    """Pages, rows and scales whose offsets need more than 32 bits: stored, read
+    and attended to at both ends of a pool of 5 GB, as in a small one."""
+    hkv, page, d, far = 8, 64, 128, 81000
+    slots_at = lambda first: torch.arange(100, device="cuda") + first * page  # noqa: E731
+    k, v, q = (_rand((1, 100, h, d), BF16, 96 + i).transpose(1, 2) for i, h in enumerate((hkv, hkv, 16)))
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device="cuda")
+    lengths = torch.tensor([100], dtype=torch.int32, device="cuda")
+    outs = []
+    for pages, first in ((2, 0), (far + 2, far)):
+        pools = [torch.empty(pages, hkv, page, d, device="cuda", dtype=torch.uint8).view(torch.float8_e4m3fn) for _ in range(2)]
+        scales = [torch.empty(pages, hkv, page, device="cuda", dtype=torch.uint8).view(torch.float8_e8m0fnu) for _ in range(2)]
+        cache = (*pools, *scales)
+        append_paged_kv8(*cache, k, v, slots_at(first))
+        back = read_paged_kv8(*cache, slots_at(first), dtype=BF16)
+        new = [x[:, :, 50:51].contiguous() for x in (k, v)]
+        out = paged_attention8(q[:, :, :1].contiguous(), *cache, table + first, lengths, new_k=new[0], new_v=new[1],
+                               slots=slots_at(first)[99:], return_lse=True)
+        outs.append((*back, *out, *read_paged_kv8(*cache, slots_at(first)[99:], dtype=BF16)))
+        del pools, scales, cache
+    for x, y in zip(*outs):
+        assert torch.equal(x, y)
+
+
 def test_two_streams_at_once():
     """Two calls in flight with workspaces of their own."""
     cache, kv, vv, table, lengths = _requests([9000, 8000], 16, 2, 128, "e4m3", 91)

@@ -133,6 +133,7 @@ def test_gradients_of_one_of_two_and_expanded_ones():
     positions = torch.arange(11, device="cuda")
     q, k = _rand((1, 2, 11, 64), BF16, 1), _rand((1, 1, 11, 64), BF16, 2).requires_grad_(True)
     oq, ok = apply_rotary(q, k, positions, freqs)
+    assert ok.requires_grad and not oq.requires_grad
     (dk,) = torch.autograd.grad(ok.sum(), (k,))       # a gradient of stride 0
     _check(dk, torch.ones_like(k), positions, freqs, False, 1.0, -1.0)
     q.requires_grad_(True)
