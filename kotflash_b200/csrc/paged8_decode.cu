@@ -369,10 +369,9 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   bool more = rg == 0;                 // whether the load cursor stands on a tile that is not loaded yet
   int issued = 0, late = -1;           // `late`: stage whose scales are on their way
   Place ahead;
-  Scale coming;
+  Scale coming, got[STAGES - 1];
   if (rg == 0) {
     Place first[STAGES - 1];
-    Scale got[STAGES - 1];
 #pragma unroll
     for (int s = 0; s < STAGES - 1; ++s) {
       if (more && s < depth) {
@@ -386,14 +385,16 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     for (int s = 0; s < STAGES - 1; ++s)
       if (s < issued) issue(s, first[s], got[s]);
     if (more) ahead = look_up();
-#pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s)
-      if (s < issued) keep(s, got[s]);
   }
   uint32_t unit_t0 = work.t;           // first tile of the unit in this share
   if (tid == 0 && join_blocks) a.joins[me].x = -1;
   clear_empty(a);
   start_unit();
+  if (rg == 0) {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s)
+      if (s < issued) keep(s, got[s]);
+  }
 
   int stage = 0, fill = depth;
   uint32_t parity = 0;

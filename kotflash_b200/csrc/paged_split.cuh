@@ -50,9 +50,9 @@ struct Cursor {
   uint32_t t, tiles, keys, pos;
   bool whole;  // the table holds all of the request's positions
 
-  __device__ __forceinline__ void set_request(const PagedWork& a, int request) {
+  __device__ __forceinline__ void set_request(const PagedWork& a, int request) { set_request(a, request, a.lengths[request]); }
+  __device__ __forceinline__ void set_request(const PagedWork& a, int request, int32_t length) {
     b = request;
-    const int32_t length = a.lengths[b];
     whole = length <= 0 || (uint32_t)length <= a.capacity;
     keys = length <= 0 ? 0u : min((uint32_t)length, a.capacity);
     tiles = (keys + TILE - 1) / TILE;
@@ -82,11 +82,13 @@ struct Cursor {
 struct Share {
   uint32_t begin, end, even, longer, total, before;
   int first;
+  int32_t length;                      // of request `first`
 };
 struct ShareScratch {  // shared memory
   uint32_t warp_tiles[kWarps];
   int first;
   uint32_t before;
+  int32_t length;
 };
 
 // By a prefix sum over the requests' lengths (fewer than 2^31 positions, see
@@ -136,17 +138,19 @@ __device__ __forceinline__ bool find_share(const PagedWork& a, ShareScratch& scr
     }
     scratch.first = b;
     scratch.before = sum;
+    scratch.length = a.lengths[b];
   }
   __syncthreads();
   s.first = scratch.first;
   s.before = scratch.before;
+  s.length = scratch.length;
   return true;
 }
 
 // The first tile of a share; false where it holds only the end of a unit.
 template <int TILE>
 __device__ __forceinline__ bool first_tile(const PagedWork& a, const Share& s, Cursor<TILE>& work) {
-  work.set_request(a, s.first);
+  work.set_request(a, s.first, s.length);
   const uint32_t at = s.begin - s.before * (a.Hkv * a.row_blocks);  // inside the request's units
   const int hr = (int)(at / (work.tiles + 1));
   work.t = at - hr * (work.tiles + 1);
