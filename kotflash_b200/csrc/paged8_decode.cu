@@ -128,7 +128,7 @@ __device__ __forceinline__ void ldmatrix_trans_b8(uint32_t (&r)[4], uint32_t sad
 // page, which other blocks ask for at about the same time.
 __device__ __forceinline__ uint32_t load_scale(const uint8_t* p) {
   uint32_t x;
-  asm volatile("ld.global.L2::128B.u8 %0, [%1];" : "=r"(x) : "l"(p));
+  asm volatile("ld.global.cg.L2::128B.u8 %0, [%1];" : "=r"(x) : "l"(p));
   return x;
 }
 
@@ -222,7 +222,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   const uint32_t end = share.end;
   load = work;
 
-  // ---- loads: a lane looks up keys lane (and lane + 32) of the team's share of a tile
+  // ---- loads: a lane looks up keys lane, lane + 32, .. of the team's share of a tile
   struct Place {
     uint32_t page[LOOKS], row[LOOKS];
     int h;
