@@ -100,4 +100,18 @@ KF_DEVI uint2 encode8(uint4 w, float by) {
 // Checks what every entry point asks of a cache (before any launch).
 int check_cache8(const char* what, const kf_paged8_cache& c);
 
+// One launch of the attention kernel; args is a Paged8Args of paged8_decode.cuh.
+struct Paged8Launch {
+  const void* args;
+  const CUtensorMap *map_k, *map_v;
+  int steps;                       // 16-byte chunks of a row
+  bool lines;                      // pages are brought as lines
+  int rows, blocks;
+  cudaStream_t stream;
+};
+int paged8_launch_e4m3_f16(const Paged8Launch& l);
+int paged8_launch_e4m3_bf16(const Paged8Launch& l);
+int paged8_launch_int8_f16(const Paged8Launch& l);
+int paged8_launch_int8_bf16(const Paged8Launch& l);
+
 }  // namespace kf

@@ -215,7 +215,8 @@ def _check(out, lse, q, kv, vv, table, lengths, scale, name):
     itself, that is by 2^-11 and 2^-11 more or less; O is divided by the sum of
     the cut ones, so the first part cancels and the second moves O by 2^-11 max
     |v - O| <= 2^-10 max |v|; or, of a small one, by 2^-36 of the largest
-    weight, of n.  Products and weights are summed 16 at a time in fp32 over n
+    weight, of n.  For fp16 queries what is cut off is a second part, off by
+    2^-11 of its 2^-10: 2^-21 of a weight, 2^-20 of max |v|.  Products and weights are summed 16 at a time in fp32 over n
     keys, plus a handful of joins; the output is rounded once (u)."""
     eo, el, sizes = oracle.attention(q, kv, vv, table, lengths, scale)
     o = out.double().cpu()
@@ -229,7 +230,8 @@ def _check(out, lse, q, kv, vv, table, lengths, scale, name):
         dx = prod * (d + 4) * 2.0 ** -23 + 60 * 2.0 ** -23 + 2.0 ** -22
         summed = (n / 16 + 64) * 2.0 ** -23
         err = (o[b] - eo[b]).abs()
-        bound = UNIT[q.dtype] * eo[b].abs() + vmax * (2.0 ** -10 + 2 * dx + summed + n * 2.0 ** -35) + 2.0 ** -24
+        held = 2.0 ** -10 if q.dtype == BF16 else 2.0 ** -20
+        bound = UNIT[q.dtype] * eo[b].abs() + vmax * (held + 2 * dx + summed + n * 2.0 ** -35) + 2.0 ** -24
         assert (err <= bound).all(), f"{name}: request {b} (n={n}) off by {err.max():.3e}, bound {bound.min():.3e}"
         if lse is not None:
             assert lse.shape == q.shape[:3] and lse.dtype == torch.float32
