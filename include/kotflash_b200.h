@@ -350,8 +350,8 @@ int kf_paged_release(const kf_paged_release_args* args);
  *   a' = (a cos t - b sin t) magnitude,  b' = (b cos t + a sin t) magnitude.
  * The other columns are copied.  inverse != 0 turns by -t, which is the
  * gradient.  positions: int32 or int64 (position_bits) by batch entry and
- * token, with element strides; frequencies: rotated / 2 doubles, radians per
- * position.  Any strides with a contiguous last dim; q_out may be q and k_out
+ * token, with element strides; frequencies: rotated / 2 finite doubles, radians
+ * per position.  Any strides with a contiguous last dim; q_out may be q and k_out
  * k, with the same strides. */
 typedef struct kf_rotary_args {
   kf_tensor4    q, k, q_out, k_out;
@@ -386,7 +386,8 @@ int kf_rotary(const kf_rotary_args* args);
  * the block's first row begins it anew.  Rows behind the newest are left.
  *
  * kf_paged8_append stores new_k / new_v [N, Hkv, S, D], token t = n * S + s,
- * at slot slots[t], skipping those outside the pool.  With more than one row
+ * at slot slots[t], skipping those outside the pool.  No two tokens share a
+ * slot (codes of one and the scale of the other may stay).  With more than one row
  * to a scale, the tokens of one block follow one another in slots (as
  * kf_paged_reserve gives them); two separate runs into one block leave either's
  * scale.

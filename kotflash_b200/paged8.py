@@ -123,7 +123,7 @@ def append_paged_kv8(
     new_k and new_v are [N, Hkv, S, D] with any strides; token t = n * S + s
     goes to slot slots[t] (int64 [N * S]), row slots[t] % page_size of page
     slots[t] // page_size.  Tokens whose slot is outside the pool (-1) are
-    skipped; N or S may be 0.  k_scales and v_scales are [pages, Hkv, page_size
+    skipped; no two tokens share a slot; N or S may be 0.  k_scales and v_scales are [pages, Hkv, page_size
     / block], block a power of two up to 128.
 
     With more than one token to a scale, a row that is not the first of its

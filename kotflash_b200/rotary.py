@@ -184,7 +184,7 @@ def apply_rotary(
     """Rotate q [B, Hq, S, D] and k [B, Hkv, S, D] (or None) by their positions.
 
     positions is int32 or int64, [B, S] or, for all batch entries, [S];
-    frequencies float64 [R / 2] on the same device, radians per position.  The
+    frequencies float64 [R / 2] on the same device, finite, radians per position.  The
     first R columns turn in pairs, column i with i + R / 2 or, interleaved,
     2i with 2i + 1; the columns behind them pass.  Rotated columns are
     multiplied by magnitude.  Angles are worked out in 64 bits, the rest in 32,

@@ -602,6 +602,28 @@ def test_pools_past_4_gb():
         assert torch.equal(x, y)
 
 
+@pytest.mark.skipif(not torch.cuda.is_available() or torch.cuda.device_count() < 2, reason="needs two CUDA devices")
+def test_calls_follow_their_tensors_device():
+    """Everything on cuda:1 while cuda:0 is current: the results of cuda:0."""
+    results = []
+    for index in (0, 1):
+        dev = torch.device("cuda", index)
+        with torch.cuda.device(index):
+            g = torch.Generator(device=dev).manual_seed(1)
+            q, k, v = (torch.randn(1, h, 40, 64, device=dev, generator=g).bfloat16() for h in (4, 2, 2))
+            cache = PagedKVCache8(8, 16, 2, 64, 1, 4, device=dev)
+            freqs, _ = rotary_frequencies(64, device=dev)
+            torch.cuda.synchronize(dev)
+        with torch.cuda.device(0):
+            q, k = apply_rotary(q, k, torch.arange(40, device=dev), freqs)
+            slots, _ = cache.reserve(torch.tensor([40], dtype=torch.int32, device=dev), num_tokens=40)
+            cache.append(k, v, slots)
+            out, lse = cache.attend(q[:, :, :1].contiguous(), return_lse=True)
+            results.append([x.cpu() for x in (out, lse, *cache.read(slots, dtype=torch.float16))])
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
 def test_two_streams_at_once():
     """Two calls in flight with workspaces of their own."""
     cache, kv, vv, table, lengths = _requests([9000, 8000], 16, 2, 128, "e4m3", 91)
