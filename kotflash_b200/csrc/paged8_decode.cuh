@@ -147,7 +147,6 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   // top of fp16's range: its 11 bits hold down to 2^-25 of the largest, and
   // what is lost below is at most 2^-36 of it.
   constexpr float BELOW = 11.f, LIMIT = 15.f;
-  constexpr bool TWO = !BF16;          // weights are held in two parts
   extern __shared__ __align__(1024) uint8_t smem[];
   typename C::Tail& tail = *reinterpret_cast<typename C::Tail*>(smem + C::SMEM - sizeof(typename C::Tail));
   auto& full = tail.full;
@@ -161,7 +160,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   uint8_t* ring = smem + team * STAGES * C::STAGE;
   float2* scales = reinterpret_cast<float2*>(smem + C::TEAMS * STAGES * C::STAGE) + team * STAGES * KW;  // (2^e, f)
   float* handed = reinterpret_cast<float*>(smem + C::TEAMS * STAGES * C::STAGE + C::SCALES);  // [2][KD][lane][4]
-  float* ml = handed + 2 * C::HANDED;  // [warp][NT][4 lanes][2 rows](m, l, sum of the cut weights, -)
+  float* ml = handed + 2 * C::HANDED;  // [warp][NT][4 lanes][2 rows](m, l, NaN if V has one, -)
 
   if (tid == 0) {
     for (int i = 0; i < C::TEAMS * STAGES; ++i) kf::mbar_init(&full[0][0] + i, 1);
@@ -304,9 +303,9 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   // ---- state of the unit being worked on
   uint32_t qb[NT][KD][2];              // Q^T as B fragments
   // rows 2 (lane % 4) + {0, 1} of each row tile: the factor of a product, the
-  // reference m of the weights 2^(x + f - m), the sums of 2^(x - m) exact and
-  // of the weights as cut to fp16, and m as it enters the exponent (0 for -inf)
-  float factor[NT][2], m_run[NT][2], l_run[NT][2], l_held[NT][2], mu[NT][2];
+  // reference m of the weights 2^(x + f - m), the sum of 2^(x - m), and m as it
+  // enters the exponent (0 for -inf)
+  float factor[NT][2], m_run[NT][2], l_run[NT][2], mu[NT][2];
   float ot[NT][KD][4];                 // O^T
   bool v_nan = false;
   // The loads of the unit's Q, issued early.  start_unit() follows where the
@@ -353,7 +352,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       for (int j = 0; j < 2; ++j) {
         factor[nt][j] = a.scale_log2 * __shfl_sync(0xffffffffu, back, 8 * (lane & 3) + 4 * j);
         m_run[nt][j] = -INFINITY;
-        l_run[nt][j] = l_held[nt][j] = mu[nt][j] = 0.f;
+        l_run[nt][j] = mu[nt][j] = 0.f;
       }
 #pragma unroll
       for (int x = 0; x < KD; ++x) ot[nt][x][0] = ot[nt][x][1] = ot[nt][x][2] = ot[nt][x][3] = 0.f;
@@ -579,7 +578,6 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float old = kf::ex2(m_run[nt][j] - mu[nt][j]);
             m_run[nt][j] = m_new;
             l_run[nt][j] *= old;
-            l_held[nt][j] *= old;
 #pragma unroll
             for (int dm = 0; dm < KD; ++dm) {
               ot[nt][dm][j] *= old;
@@ -587,18 +585,16 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             }
           }
       }
-      // Weights, cut to fp16's 11 bits.  For bf16 outputs that is all: O is
-      // divided by the sum of the cut ones, so that only the differences of what
-      // is cut off count (half of 2^-10 of a weight at most).  For fp16 outputs,
-      // whose own rounding is no larger, what is cut off makes a second product
-      // (one product: 1.5 times the error against 64 bits).  They are cut in 32
-      // bits: a key whose V is small next to the others' (a row of zeros, say)
-      // has a weight that fp16 loses, and counts in the sum all the same.  The
-      // LSE has the sum of the whole ones.
-      uint32_t pb[H][NT][2], pl[TWO ? H : 1][NT][2];
+      // Weights in two parts of fp16, 11 bits each: cut, and what was cut off.
+      // One part alone is off by 2^-11: 1.5 times the error of an fp16 O, an
+      // eighth of a bf16 O's rounding (64 ragged requests in bf16 86.5 us instead
+      // of 88.7, 16 query rows per KV head 105 instead of 117).  They are cut in
+      // 32 bits: a key whose V is small next to the others' (a row of zeros, say)
+      // has a weight that fp16 loses, and counts in the sum all the same.
+      uint32_t pb[H][NT][2], pl[H][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        uint64_t sum2 = 0, held2 = 0;  // of the step: fewer roundings against a large l
+        uint64_t sum2 = 0;             // of the step: fewer roundings against a large l
         const uint64_t mu2 = kf::f2(mu[nt][0], mu[nt][1]);
 #pragma unroll
         for (int h = 0; h < H; ++h)
@@ -611,22 +607,14 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
               w[j] = kf::ex2(w[j]);
               p[j] = __uint_as_float(__float_as_uint(w[j]) & 0xffffe000u);
             }
-            const uint64_t le = kf::f2(less[h][y], less[h][y]);
-            sum2 = kf::fma2(kf::f2(w[0], w[1]), le, sum2);
-            if constexpr (TWO)
-              pl[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(w[0] - p[0], w[1] - p[1]));
-            else
-              held2 = kf::fma2(kf::f2(p[0], p[1]), le, held2);
+            sum2 = kf::fma2(kf::f2(w[0], w[1]), kf::f2(less[h][y], less[h][y]), sum2);
+            pl[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(w[0] - p[0], w[1] - p[1]));
             pb[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(p[0], p[1]));
           }
-        float sum[2], held[2];
+        float sum[2];
         kf::f2_split(sum2, sum[0], sum[1]);
-        kf::f2_split(held2, held[0], held[1]);
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          l_run[nt][j] += sum[j];
-          l_held[nt][j] += held[j];
-        }
+        l_run[nt][0] += sum[0];
+        l_run[nt][1] += sum[1];
       }
       // O^T (head dim x rows) += V^T P^T.  The products of a step are summed
       // from zero and then added, as an MMA cuts each of its products off where
@@ -653,7 +641,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
               for (int nt = 0; nt < NT; ++nt) {
                 kf::mma_16816<false>(step[e][nt], f[e], pb[h][nt][0], pb[h][nt][1]);
-                if constexpr (TWO) kf::mma_16816<false>(step[e][nt], f[e], pl[h][nt][0], pl[h][nt][1]);
+                kf::mma_16816<false>(step[e][nt], f[e], pl[h][nt][0], pl[h][nt][1]);
               }
             }
         }
@@ -701,14 +689,10 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
-        for (int off = 4; off < 32; off <<= 1) {
-          l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], off);
-          l_held[nt][j] += __shfl_xor_sync(0xffffffffu, l_held[nt][j], off);
-        }
-        if (TWO) l_held[nt][j] = l_run[nt][j];
-        if (v_nan) l_held[nt][j] = NAN;             // O, not the LSE
-        if (!alive) l_run[nt][j] = l_held[nt][j] = m_run[nt][j] = NAN;  // a lost load shows in the result
+        for (int off = 4; off < 32; off <<= 1) l_run[nt][j] += __shfl_xor_sync(0xffffffffu, l_run[nt][j], off);
+        if (!alive) l_run[nt][j] = m_run[nt][j] = NAN;  // a lost load shows in the result
       }
+    const float spoiled = v_nan ? NAN : 0.f;        // O, not the LSE
     // Each warp scales its O^T to the rows' common reference and sum; then the
     // upper half of the teams hand theirs over, lane by lane as they hold it,
     // and the lower half add, until team 0 has the sum.
@@ -719,7 +703,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 #pragma unroll
           for (int j = 0; j < 2; ++j)
             *reinterpret_cast<float4*>(ml + (((warp * NT + nt) * 4 + lane) * 2 + j) * 4) =
-                make_float4(m_run[nt][j], l_run[nt][j], l_held[nt][j], 0.f);
+                make_float4(m_run[nt][j], l_run[nt][j], spoiled, 0.f);
       }
       __syncthreads();
     }
@@ -729,7 +713,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       float by[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float most = m_run[nt][j], sum = l_run[nt][j], held = l_held[nt][j], own = 1.f;
+        float most = m_run[nt][j], sum = l_run[nt][j], held = spoiled, own = 1.f;
         if constexpr (C::TEAMS > 1) {
           float4 x[C::TEAMS];
 #pragma unroll
@@ -738,16 +722,16 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             most = fmaxf(most, x[t].x);
           }
           const float ref = most == -INFINITY ? 0.f : most;
-          sum = held = 0.f;
+          sum = 0.f;
 #pragma unroll
           for (int t = 0; t < C::TEAMS; ++t) {
             const float w = kf::ex2(x[t].x - ref);
             sum += w * x[t].y;
-            held += w * x[t].z;
+            held += x[t].z;
           }
           own = kf::ex2(m_run[nt][j] - ref);
         }
-        by[j] = held == 0.f ? 0.f : own * reciprocal(held);
+        by[j] = sum + held == 0.f ? 0.f : own * reciprocal(sum + held);
         if (team == 0) lse2[nt][j] = sum == 0.f ? -INFINITY : most + log2f(sum);
       }
 #pragma unroll
