@@ -6,10 +6,13 @@
 //   l = sum 2^x_j,  O = sum 2^(x_j + f_j) v^_j / l,  LSE = ln l.
 // Weights 2^(x_j + f_j - m) carry V's scale as a part of the exponent, with m
 // a running reference of x_j + f_j: whatever the scales, the key that adds
-// most to O has a weight at the top of fp16's range, and l is summed as
-// 2^(x_j + f_j - m) 2^-f_j in 32 bits (|f| <= 60 keeps it in range).  So codes
-// enter the products as they are, exact in fp16, and K's scale is one factor
-// of a score.
+// most to O has a weight at the top of fp16's range.  So codes enter the
+// products as they are, exact in fp16, and K's scale is one factor of a score.
+// l is summed in 32 bits, as 2^(x_j - m) from an exponential of its own: a key
+// with a small V can lie far below m and weigh more than all others.  The key
+// at the reference has x - m >= 11 - 60 and no key x - m > 15 + 60, so l lies
+// between 2^-49 and 2^75 times the number of keys, and what is lost below
+// 2^-126 is less than 2^-77 of it per key.
 //
 // Every K/V row is read once for G query rows, 2 D bytes for 4 G D flops, so
 // HBM bounds it up to about 16 rows per KV head; at half the bytes of a 16-bit
@@ -526,14 +529,14 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       // second pair of a fragment), g = lane / 4, of rows 2 (lane % 4) + {0, 1}.
       const int g = lane >> 2;
       const int own_key[2] = {key_of(4 * (g >> 1) + (g & 1)), key_of(4 * (g >> 1) + (g & 1) + 2)};
-      float less[H][2];                // 2^-f
+      float own_f[H][2];
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int y = 0; y < 2; ++y) {
           const int key = h * 16 + own_key[y];
           const float2 s = scales[stage * KW + key];
-          less[h][y] = kf::ex2(-s.y);
+          own_f[h][y] = s.y;
           const uint64_t sx = kf::f2(s.x, s.x), sy = kf::f2(s.y, s.y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
@@ -576,8 +579,10 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
             const float m_new = fmaxf(m_run[nt][j], t - BELOW);
             mu[nt][j] = m_new == -INFINITY ? 0.f : m_new;
             const float old = kf::ex2(m_run[nt][j] - mu[nt][j]);
+            // (in two halves: where m leaps, `old` can be 0 and a sum of keys with small values not)
+            const float half = kf::ex2(0.5f * (m_run[nt][j] - mu[nt][j]));
             m_run[nt][j] = m_new;
-            l_run[nt][j] *= old;
+            l_run[nt][j] = l_run[nt][j] * half * half;
 #pragma unroll
             for (int dm = 0; dm < KD; ++dm) {
               ot[nt][dm][j] *= old;
@@ -588,9 +593,7 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       // Weights in two parts of fp16, 11 bits each: cut, and what was cut off.
       // One part alone is off by 2^-11: 1.5 times the error of an fp16 O, an
       // eighth of a bf16 O's rounding (64 ragged requests in bf16 86.5 us instead
-      // of 88.7, 16 query rows per KV head 105 instead of 117).  They are cut in
-      // 32 bits: a key whose V is small next to the others' (a row of zeros, say)
-      // has a weight that fp16 loses, and counts in the sum all the same.
+      // of 88.7, 16 query rows per KV head 105 instead of 117).
       uint32_t pb[H][NT][2], pl[H][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
@@ -600,14 +603,16 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
         for (int h = 0; h < H; ++h)
 #pragma unroll
           for (int y = 0; y < 2; ++y) {
-            float p[2], w[2];
-            kf::f2_split(kf::sub2(kf::f2(cc[h][nt][2 * y], cc[h][nt][2 * y + 1]), mu2), w[0], w[1]);
+            float p[2], w[2], x[2];
+            const uint64_t over = kf::sub2(kf::f2(cc[h][nt][2 * y], cc[h][nt][2 * y + 1]), mu2);
+            kf::f2_split(over, w[0], w[1]);
+            kf::f2_split(kf::sub2(over, kf::f2(own_f[h][y], own_f[h][y])), x[0], x[1]);
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
               w[j] = kf::ex2(w[j]);
               p[j] = __uint_as_float(__float_as_uint(w[j]) & 0xffffe000u);
             }
-            sum2 = kf::fma2(kf::f2(w[0], w[1]), kf::f2(less[h][y], less[h][y]), sum2);
+            sum2 = kf::add2(sum2, kf::f2(kf::ex2(x[0]), kf::ex2(x[1])));
             pl[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(w[0] - p[0], w[1] - p[1]));
             pb[h][nt][y] = kf::movmatrix_trans(kf::pack2<false>(p[0], p[1]));
           }
@@ -713,26 +718,27 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
       float by[2];
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float most = m_run[nt][j], sum = l_run[nt][j], held = spoiled, own = 1.f;
+        float ref = m_run[nt][j], sum = l_run[nt][j], held = spoiled, own = 1.f;
         if constexpr (C::TEAMS > 1) {
+          // By the teams' sums: a reference of their m can lie past all of l.
           float4 x[C::TEAMS];
+          ref = -INFINITY;
 #pragma unroll
           for (int t = 0; t < C::TEAMS; ++t) {
             x[t] = *reinterpret_cast<const float4*>(ml + ((((t * RG + rg) * NT + nt) * 4 + (lane & 3)) * 2 + j) * 4);
-            most = fmaxf(most, x[t].x);
+            ref = fmaxf(ref, x[t].x + __log2f(x[t].y));
           }
-          const float ref = most == -INFINITY ? 0.f : most;
+          ref = ref == -INFINITY ? 0.f : ceilf(ref);
           sum = 0.f;
 #pragma unroll
           for (int t = 0; t < C::TEAMS; ++t) {
-            const float w = kf::ex2(x[t].x - ref);
-            sum += w * x[t].y;
+            sum += kf::ex2(x[t].x - ref) * x[t].y;
             held += x[t].z;
           }
           own = kf::ex2(m_run[nt][j] - ref);
         }
         by[j] = sum + held == 0.f ? 0.f : own * reciprocal(sum + held);
-        if (team == 0) lse2[nt][j] = sum == 0.f ? -INFINITY : most + log2f(sum);
+        if (team == 0) lse2[nt][j] = sum == 0.f ? -INFINITY : ref + log2f(sum);
       }
 #pragma unroll
       for (int dm = 0; dm < KD; ++dm) {

@@ -54,3 +54,35 @@ def test_outputs_are_a_32_bit_evaluation_rounded_once(held, dtype, hq, d, n):
     bound = 2.0 ** -17 * v.abs().max().item()
     assert over <= bound, f"{over:.3e} past half a step, bound {bound:.3e}"
     assert (lse.double() - torch.log(w.sum(-1))[..., None]).abs().max().item() <= 2.0 ** -17 + 8 * 2.0 ** -22
+
+
+@pytest.mark.parametrize("held", ["e4m3", "int8"])
+@pytest.mark.parametrize("n,d,hq", [(64, 128, 1), (64, 128, 40), (500, 64, 2), (2000, 32, 24), (131072, 64, 1), (131072, 64, 16), (30000, 104, 64)])
+@pytest.mark.parametrize("lead", [-20, 7, 18, 30])
+def test_keys_without_a_value_beside_one_of_the_largest(held, n, d, hq, lead):
+    """The scales' whole range: one key whose V has the largest exponent, 60,
+    all others zeros, which have the smallest, wherever the one stands.  Scores
+    are exact but for their scaling, 2^-22 of at most 30, and enter a weight by
+    a base-2 exponential (2^-22): 2^-17 of a weight or less; sums of n equal
+    ones as in any batch."""
+    page, top = 16, {"e4m3": 448.0, "int8": 127.0}[held]
+    pages = -(-n // page)
+    table = torch.randperm(pages, generator=torch.Generator().manual_seed(n)).to(torch.int32).cuda()[None]
+    q = torch.zeros(1, hq, 1, d, device="cuda", dtype=BF16)
+    q[..., 0] = 1
+    lengths = torch.tensor([n], dtype=torch.int32, device="cuda")
+    others = (n - 1) * 2.0 ** -lead
+    bound = 2.0 ** -17 + (n / 16 + 64) * 2.0 ** -23
+    for where in (0, 31, n // 2, n - 1):
+        at, row = int(table[0, where // page]), where % page
+        k, v = (torch.zeros(pages, page, d, device="cuda") for _ in range(2))
+        ke, ve = torch.zeros(pages, page, device="cuda"), torch.full((pages, page), -60.0, device="cuda")
+        k[at, row, 0], v[at, row], ve[at, row] = lead, top, 60
+        (kp, ks), (vp, vs) = _pool(k, ke, held), _pool(v, ve, held)
+        out, lse = paged_attention8(q, kp, vp, ks, vs, table, lengths, scale=math.log(2), return_lse=True)
+        want = top * 2.0 ** 60 / (1 + others)
+        err = (out.double() / want - 1).abs().max().item()
+        assert err <= 2.0 ** -8 + 2 * bound, f"key {where}: off by {err:.3e} of the value"
+        want = lead * math.log(2) + math.log1p(others)
+        err = (lse.double() - want).abs().max().item()
+        assert err <= bound + abs(want) * 2.0 ** -22, f"key {where}: LSE off by {err:.3e}"
