@@ -14,6 +14,7 @@ import math
 from typing import Optional, Tuple, Union
 
 import torch
+from torch.autograd.forward_ad import unpack_dual
 
 from . import _ext
 
@@ -146,30 +147,53 @@ def _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse):
 
 
 class _Rotary(torch.autograd.Function):
+    """The rotation, linear in q and k: tangents are rotated as q and k are,
+    gradients back.  Neither of the two is a constant where one has a tangent."""
+
     @staticmethod
-    def forward(ctx, q, k, positions, frequencies, interleaved, magnitude, inverse):
+    def forward(ctx, q, k, positions, frequencies, interleaved, magnitude, inverse, tangents):
         ctx.save_for_backward(positions, frequencies)
+        ctx.save_for_forward(positions, frequencies)
         ctx.set_materialize_grads(False)
         ctx.how = interleaved, magnitude, inverse
         outs = _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse)
-        constant = [out for out, need in zip(outs, ctx.needs_input_grad) if out is not None and not need]
+        constant = [] if tangents else [out for out, need in zip(outs, ctx.needs_input_grad) if out is not None and not need]
         if constant:
             ctx.mark_non_differentiable(*constant)
         return outs
 
     @staticmethod
     def backward(ctx, dq, dk):
-        positions, frequencies = ctx.saved_tensors
-        interleaved, magnitude, inverse = ctx.how
+        inverse = ctx.how[2]
         need_q, need_k = ctx.needs_input_grad[:2]
-        if not need_q:
-            dq = None
-        if not need_k:
-            dk = None
-        if dq is not None or dk is not None:
-            back = _Rotary.apply if torch.is_grad_enabled() else _rotate  # a gradient of the gradient
-            dq, dk = back(dq, dk, positions, frequencies, interleaved, magnitude, not inverse)
-        return dq, dk, None, None, None, None, None
+        dq, dk = _turned(ctx, dq if need_q else None, dk if need_k else None, not inverse)
+        return dq, dk, None, None, None, None, None, None
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        return _turned(ctx, tq, tk, ctx.how[2])
+
+
+def _turned(ctx, x, y, inverse):
+    """A gradient's or tangent's rotation, differentiable as the call itself is."""
+    if x is None and y is None:
+        return None, None
+    positions, frequencies = ctx.saved_tensors
+    interleaved, magnitude, _ = ctx.how
+    return _differentiable(x, y, positions, frequencies, interleaved, magnitude, inverse)
+
+
+def _differentiable(q, k, positions, frequencies, interleaved, magnitude, inverse):
+    """_rotate(), through autograd where q or k has a gradient or a tangent."""
+    q_tangent = q is not None and unpack_dual(q)[1] is not None
+    k_tangent = k is not None and unpack_dual(k)[1] is not None
+    if q_tangent != k_tangent and q is not None and k is not None:  # one call would give the other a tangent
+        return (_differentiable(q, None, positions, frequencies, interleaved, magnitude, inverse)[0],
+                _differentiable(None, k, positions, frequencies, interleaved, magnitude, inverse)[1])
+    tangents = q_tangent or k_tangent
+    if tangents or (((q is not None and q.requires_grad) or (k is not None and k.requires_grad)) and torch.is_grad_enabled()):
+        return _Rotary.apply(q, k, positions, frequencies, interleaved, magnitude, inverse, tangents)
+    return _rotate(q, k, positions, frequencies, interleaved, magnitude, inverse)
 
 
 def apply_rotary(
@@ -189,7 +213,8 @@ def apply_rotary(
     2i with 2i + 1; the columns behind them pass.  Rotated columns are
     multiplied by magnitude.  Angles are worked out in 64 bits, the rest in 32,
     rounded once.  Any strides; new contiguous tensors are returned, ``(q',
-    k')``, or q' alone where k is None.  Differentiable in q and k.
+    k')``, or q' alone where k is None.  Differentiable in q and k, backwards and,
+    with ``torch.autograd.forward_ad``, forwards.
     """
     try:  # what a valid call of q and k pays for; _check() finds out what to say
         index = q.get_device()
@@ -210,8 +235,5 @@ def apply_rotary(
     if not math.isfinite(magnitude):
         raise ValueError("magnitude must be finite")
     interleaved = bool(interleaved)
-    if (q.requires_grad or (k is not None and k.requires_grad)) and torch.is_grad_enabled():
-        outs = _Rotary.apply(q, k, positions, frequencies, interleaved, magnitude, False)
-    else:
-        outs = _rotate(q, k, positions, frequencies, interleaved, magnitude, False)
+    outs = _differentiable(q, k, positions, frequencies, interleaved, magnitude, False)
     return outs[0] if k is None else outs
