@@ -380,17 +380,16 @@ int kf_rotary(const kf_rotary_args* args);
  * magnitude is at most 448 (e4m3) or rounds to at most 127 (int8), exponents
  * lying within +-60, and rounds to nearest, ties to even.  A block with an
  * infinity, a NaN or a magnitude beyond that gets scale 255, and its rows'
- * codes are 0.  With more than one row to a scale, rows are written in order:
- * a row that is not its block's first joins the rows before it, whose codes
- * are rounded again if the scale grows (a scale never shrinks, and 255 stays);
- * the block's first row begins it anew.  Rows behind the newest are left.
+ * codes are 0.  With more than one row to a scale, a call's rows of one block
+ * share its scale, wherever their tokens stand; if the block's first row is not
+ * among them they join the rows before the first of them, whose codes are
+ * rounded again if the scale grows (a scale never shrinks, and 255 stays); the
+ * block's first row begins it anew.  Rows behind the first written one that the
+ * call does not write keep their codes and take the new scale.
  *
  * kf_paged8_append stores new_k / new_v [N, Hkv, S, D], token t = n * S + s,
  * at slot slots[t], skipping those outside the pool.  No two tokens share a
- * slot (codes of one and the scale of the other may stay).  With more than one row
- * to a scale, the tokens of one block follow one another in slots (as
- * kf_paged_reserve gives them); two separate runs into one block leave either's
- * scale.
+ * slot (codes of one and the scale of the other may stay).
  *
  * kf_paged8_read is the way back: k_out / v_out [N, Hkv, S, D], rounded once
  * (and only where the type cannot hold code times power); rows whose slot is

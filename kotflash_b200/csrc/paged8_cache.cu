@@ -85,65 +85,139 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 }
 
 // ---------------------------------------------------------------- a scale for several rows
-// The tokens of a call that go to one block one after another (a run) are
-// one warp's: their largest magnitude, with the block's scale if it has rows
-// before them, gives the scale; if it grows, those rows are rounded again.  A
-// warp looks after the runs that begin in a window of `block` tokens.  Three
-// trips to memory bound it (slots, rows with the old scale, stores), so slots
-// are read once and, of blocks up to 16 tokens, rows too and kept.  (With
-// slots and rows read twice 4096 tokens took 13.7 us.)
-constexpr int kKept = 16;  // rows of a run that a warp keeps
+// The tokens of a call that go to one block of rows determine its scale
+// together: by their largest magnitude and, if the block has rows before the
+// first of them, by its scale; if that grows, the rows before are rounded
+// again.  Tokens that follow one another into a block are a run.  A warp
+// takes one head of K or V of the runs that begin in a window of `block`
+// tokens, the warps of a thread block those of one window.
+//
+// Three trips to memory bound it (slots, rows with the old scale, stores), so
+// slots are read once and, of blocks up to 16 tokens, rows too and kept.  (With
+// slots and rows read twice 4096 tokens took 13.7 us.)  A run that does not
+// fill its block may have others beside it: the warps look through all slots
+// for them, once for up to 32 runs, and the first of several runs takes all of
+// them, in loops that read slots and rows again.  (That look costs 4096 tokens
+// 2.5 us, 9.3 without it.)
+constexpr int kKept = 16;        // rows of a run that a warp keeps
+constexpr int kWindowWarps = 4;  // of a thread block
+constexpr int kLook = 16;        // slots that a thread has in flight when it looks through them
+
+// The runs of `partial` that have tokens of their block before and behind
+// them, as far as this thread's slots say.  (Not inlined: it would take the
+// registers that let seven thread blocks share an SM.)
+__device__ __noinline__ uint2 look_through(const int64_t* slots, uint32_t T, int64_t num_slots, int shift, const uint32_t* run_block,
+                                           const uint32_t* run_end, uint64_t base, uint32_t partial) {
+  uint32_t earlier = 0, later = 0;
+  for (uint32_t at = threadIdx.x; at < T; at += kLook * blockDim.x) {
+    uint32_t block[kLook];
+#pragma unroll
+    for (int x = 0; x < kLook; ++x) {
+      const uint32_t t = at + x * blockDim.x;
+      const int64_t s = t < T ? __ldcg(reinterpret_cast<const long long*>(slots) + t) : -1;
+      block[x] = s >= 0 && s < num_slots ? (uint32_t)(s >> shift) : 0xffffffffu;
+    }
+    for (uint32_t left = partial; left; left &= left - 1) {
+      const int i = __ffs(left) - 1;
+      const uint32_t own = run_block[i], begin = (uint32_t)base + i, end = run_end[i];
+#pragma unroll
+      for (int x = 0; x < kLook; ++x) {
+        const uint32_t t = at + x * blockDim.x;
+        if (block[x] == own && t < begin) earlier |= 1u << i;
+        if (block[x] == own && t >= end) later |= 1u << i;
+      }
+    }
+  }
+  return make_uint2(earlier, later);
+}
 
 template <bool INT8, bool BF16>
-__global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Args a) {
+__global__ void __launch_bounds__(kWindowWarps * 32, 7) append8_blocks_kernel(const Rows8Args a) {
   constexpr int GROUP = 8, SIDE = 32 / GROUP;  // lanes of a row, rows side by side
   kf::griddep_wait();
   kf::griddep_launch_dependents();
   const int lane = threadIdx.x & 31, c = lane % GROUP, g = lane / GROUP;
-  const uint32_t warp = blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5);
   const uint32_t size = 1u << a.block_shift;
-  const uint32_t window = warp / (2 * a.heads), hw = warp - window * (2 * a.heads), h = hw >> 1;
+  const uint32_t parts = (2 * a.heads + kWindowWarps - 1) / kWindowWarps;  // thread blocks of a window
+  const uint32_t windows = gridDim.x / parts;
+  const uint32_t turn = blockIdx.x / parts, hw = (blockIdx.x - turn * parts) * kWindowWarps + (threadIdx.x >> 5);
+  const uint32_t window = turn == 0 ? windows - 1 : turn - 1;  // the last run is seldom a whole block: it comes first
+  const bool active = hw < 2 * a.heads;  // a warp without a head helps to look through the slots
+  const uint32_t h = hw >> 1;
   const int w = hw & 1;
   const uint64_t from = (uint64_t)window * size, until = min(from + size, (uint64_t)a.T);
   auto slot_at = [&](uint64_t t) { return t < a.T ? __ldcg(reinterpret_cast<const long long*>(a.slots) + t) : -1; };
-  // Windows of up to 16 tokens see with 32 slots where their runs end.
+  // Blocks by their number in the pool (which memory holds fewer than 2^32 - 1 of, see the host's check).
+  auto block_of = [&](int64_t s) { return s >= 0 && s < a.num_slots ? (uint32_t)(s >> a.block_shift) : 0xffffffffu; };
+  __shared__ uint32_t run_block[32];     // of the runs of these 32 slots, by the lane of their first
+  __shared__ uint32_t run_end[32], earlier_s, later_s;
+  // Windows of up to 16 tokens see with 32 slots where their runs end.  What
+  // the loop branches on is alike in all warps.
   for (uint64_t base = from; base < until; base += 32) {
     const int64_t s = slot_at(base + lane);
     int64_t before = __shfl_up_sync(0xffffffffu, (long long)s, 1);
     if (lane == 0) before = base > 0 ? slot_at(base - 1) : -2;
     const bool follows = before == s - 1 && before >> a.block_shift == s >> a.block_shift;
     const uint32_t runs_on = __ballot_sync(0xffffffffu, follows);
-    uint32_t leaders = __ballot_sync(0xffffffffu, base + lane < until && s >= 0 && s < a.num_slots && !follows);
+    const bool leads = base + lane < until && s >= 0 && s < a.num_slots && !follows;
+    // Tokens of the run that this lane leads: in these slots ...
+    uint32_t tokens = lane == 31 ? 1 : __ffs(~(runs_on >> (lane + 1)));
+    const uint32_t goes_on = __ballot_sync(0xffffffffu, leads && lane + tokens == 32);
+    if (goes_on) {                             // ... and, of one, behind them
+      const int who = __ffs(goes_on) - 1;
+      const int64_t s0 = __shfl_sync(0xffffffffu, (long long)s, who);
+      const uint32_t room = size - (uint32_t)(s0 & (size - 1));
+      uint32_t n = 32 - who;
+      for (uint32_t more = 32; more == 32 && n < room;) {
+        const uint32_t i = n + lane;
+        const uint32_t in = __ballot_sync(0xffffffffu, i < room && slot_at(base + who + i) == s0 + (int64_t)i);
+        more = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
+        n += more;
+      }
+      if (lane == who) tokens = n;
+    }
+    uint32_t leaders = __ballot_sync(0xffffffffu, leads), several = 0;
+    const uint32_t partial = __ballot_sync(0xffffffffu, leads && tokens < size);
+    if (partial) {
+      __syncthreads();                         // the masks of the slots before have been read
+      if (threadIdx.x < 32) {
+        run_block[lane] = block_of(s);
+        run_end[lane] = (uint32_t)base + lane + tokens;
+        if (lane == 0) earlier_s = later_s = 0;
+      }
+      __syncthreads();
+      const uint2 found = look_through(a.slots, a.T, a.num_slots, a.block_shift, run_block, run_end, base, partial);
+      const uint32_t earlier = found.x, later = found.y;
+      if (earlier) atomicOr(&earlier_s, earlier);
+      if (later) atomicOr(&later_s, later);
+      __syncthreads();
+      leaders &= ~earlier_s;                   // taken with the first of them
+      several = later_s;
+    }
+    if (!active) continue;
     for (; leaders; leaders &= leaders - 1) {
       const int who = __ffs(leaders) - 1;
-      const uint64_t t0 = base + who;
+      const uint32_t t0 = (uint32_t)base + who, n = __shfl_sync(0xffffffffu, tokens, who);
       const int64_t s0 = __shfl_sync(0xffffffffu, (long long)s, who);
       const uint32_t inside = (uint32_t)(s0 & (size - 1));
-      uint32_t n = who == 31 ? 1 : __ffs(~(runs_on >> (who + 1)));  // tokens of the run in these slots
-      if (who + n == 32) {                       // and behind them
-        for (uint32_t more = 32; more == 32 && n < size - inside;) {
-          const uint32_t i = n + lane;
-          const uint32_t in = __ballot_sync(0xffffffffu, i < size - inside && slot_at(t0 + i) == s0 + (int64_t)i);
-          more = in == 0xffffffffu ? 32 : __ffs(~in) - 1;
-          n += more;
-        }
-      }
+      const bool with_others = (several >> who) & 1;
       uint32_t row;
       const int64_t page = page_of(a, s0, row);
-      uint8_t* codes = a.pages[w] + page * a.ps[w][0] + h * a.ps[w][1] + (int64_t)row * a.ps[w][2] + c * 8;
+      // the block's first row
+      uint8_t* codes = a.pages[w] + page * a.ps[w][0] + h * a.ps[w][1] + (int64_t)(row - inside) * a.ps[w][2];
       uint8_t* scale = a.scales[w] + page * a.ss[w][0] + h * a.ss[w][1] + (row >> a.block_shift);
       const uint32_t old = inside > 0 ? __ldcg(scale) : 0;
       auto source = [&](uint32_t i, int x) {
         return i < n && c + x * GROUP < a.chunks
-                   ? __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, (uint32_t)t0 + i, h)) + c + x * GROUP)
+                   ? __ldcg(reinterpret_cast<const uint4*>(row_at(a, w, t0 + i, h)) + c + x * GROUP)
                    : make_uint4(0, 0, 0, 0);
       };
       uint4 kept[kKept / SIDE][2];
-      uint32_t m = 0;
 #pragma unroll
       for (int k = 0; k < kKept / SIDE; ++k)
 #pragma unroll
         for (int x = 0; x < 2; ++x) kept[k][x] = source(k * SIDE + g, x);
+      uint32_t m = 0, first = inside;
 #pragma unroll
       for (int k = 0; k < kKept / SIDE; ++k)
 #pragma unroll
@@ -152,23 +226,40 @@ __global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Arg
       for (uint32_t i = kKept + g; i < n; i += SIDE)
 #pragma unroll
         for (int x = 0; x < 2; ++x) m = kf::max_magnitudes(m, kf::magnitudes(source(i, x)));
+      // act(row of the block, piece of a token's row) for the tokens of the block behind the first run
+      auto others = [&](auto act) {
+        for (uint64_t at = (uint64_t)t0 + n; at < a.T; at += 32) {
+          const int64_t mine = slot_at(at + lane);
+          uint32_t in = __ballot_sync(0xffffffffu, mine >> a.block_shift == s0 >> a.block_shift);
+          for (; in; in &= in - 1) {
+            const uint32_t to = (uint32_t)__shfl_sync(0xffffffffu, (long long)mine, __ffs(in) - 1) & (size - 1);
+            const uint16_t* src = row_at(a, w, (uint32_t)at + __ffs(in) - 1, h);
+            act(to, lane < a.chunks ? __ldcg(reinterpret_cast<const uint4*>(src) + lane) : make_uint4(0, 0, 0, 0));
+          }
+        }
+      };
+      if (with_others)
+        others([&](uint32_t to, uint4 value) {
+          first = min(first, to);
+          m = kf::max_magnitudes(m, kf::magnitudes(value));
+        });
       // (lanes may have left the loop apart from one another)
       __syncwarp();
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) m = kf::max_magnitudes(m, __shfl_xor_sync(0xffffffffu, m, off));
       int e = kf::scale_exponent<INT8>(kf::largest<BF16>(m));
       bool nan = e > kf::kMaxExponent;
-      if (inside > 0) {
+      if (first > 0) {
         const int was = kf::scale_of_byte(old);
         nan |= old == kf::kNanScale;
         e = max(e, was);
         if (nan || e > was) {
           const float shift = nan ? 0.f : kf::power2(was - e);
-          for (uint32_t i = g; i < inside; i += SIDE)
+          for (uint32_t i = g; i < first; i += SIDE)
 #pragma unroll
             for (int x = 0; x < 2; ++x) {
               if (c + x * GROUP >= a.chunks) continue;
-              uint2* at = reinterpret_cast<uint2*>(codes - (int64_t)(inside - i) * a.ps[w][2] + x * GROUP * 8);
+              uint2* at = reinterpret_cast<uint2*>(codes + (int64_t)i * a.ps[w][2] + (c + x * GROUP) * 8);
               const uint2 y = __ldcg(at);
               float p[4], q[4];
               kf::decode4<INT8>(y.x, p);
@@ -180,20 +271,22 @@ __global__ void __launch_bounds__(kThreads) append8_blocks_kernel(const Rows8Arg
         }
       }
       const float by = nan ? 0.f : kf::power2(-e);
-      auto put = [&](uint32_t i, int x, uint4 value) {
+      auto put = [&](uint32_t to, int piece, uint4 value) {
         const uint2 y = kf::encode8<INT8, BF16>(value, by);
-        if (i < n && c + x * GROUP < a.chunks)
-          *reinterpret_cast<uint2*>(codes + (int64_t)i * a.ps[w][2] + x * GROUP * 8) = nan ? make_uint2(0, 0) : y;
+        if (piece < a.chunks)
+          *reinterpret_cast<uint2*>(codes + (int64_t)to * a.ps[w][2] + piece * 8) = nan ? make_uint2(0, 0) : y;
       };
 #pragma unroll
       for (int k = 0; k < kKept / SIDE; ++k)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) put(k * SIDE + g, x, kept[k][x]);
+        for (int x = 0; x < 2; ++x)
+          if (k * SIDE + g < n) put(inside + k * SIDE + g, c + x * GROUP, kept[k][x]);
 #pragma unroll 4
       for (uint32_t i = kKept + g; i < n; i += SIDE)
 #pragma unroll
-        for (int x = 0; x < 2; ++x) put(i, x, source(i, x));
+        for (int x = 0; x < 2; ++x) put(inside + i, c + x * GROUP, source(i, x));
       __syncwarp();  // every lane has read the old scale
+      if (with_others) others([&](uint32_t to, uint4 value) { put(to, lane, value); });
       if (lane == 0) *scale = (uint8_t)(nan ? kf::kNanScale : kf::scale_byte(e));
     }
   }
@@ -322,9 +415,8 @@ int launch_append(const Rows8Args& a, cudaStream_t st) {
   const char* what = "kf_paged8_append";
   if (a.block_shift > 0) {
     const uint64_t windows = ((uint64_t)a.T + (1u << a.block_shift) - 1) >> a.block_shift;
-    const uint64_t warps = windows * 2 * a.heads;
-    const unsigned blocks = (unsigned)((warps + kThreads / 32 - 1) / (kThreads / 32));
-    return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kThreads), 0, st, what, a);
+    const unsigned blocks = (unsigned)(windows * ((2 * a.heads + kWindowWarps - 1) / kWindowWarps));
+    return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kWindowWarps * 32), 0, st, what, a);
   }
   return launch_rows(what, a, st, [](auto group) { return append8_kernel<INT8, BF16, group>; });
 }
@@ -371,6 +463,8 @@ extern "C" int kf_paged8_append(const kf_paged8_append_args* args) {
   Rows8Args a;
   const int rc = set_up(what, args->cache, args->new_k, args->new_v, args->slots, args->dtype, &a);
   if (rc != KF_OK) return rc;
+  if (a.block_shift > 0 && (a.num_slots >> a.block_shift) >= 0xffffffffLL)  // (twice what memory holds)
+    return kf::set_error(KF_ERR_UNSUPPORTED, "%s: tensors too large", what);
   kf::DeviceGuard guard(args->cache.k_pages.ptr);
   if (guard.status()) return guard.status();
   cudaStream_t st = static_cast<cudaStream_t>(args->stream);

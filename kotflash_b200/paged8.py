@@ -126,13 +126,13 @@ def append_paged_kv8(
     skipped; no two tokens share a slot; N or S may be 0.  k_scales and v_scales are [pages, Hkv, page_size
     / block], block a power of two up to 128.
 
-    With more than one token to a scale, a row that is not the first of its
-    block joins the rows before it there: if the scale has to grow for it,
-    their codes are rounded again (a scale never shrinks while its block
-    lasts).  The first row of a block begins it anew, and rows behind the
-    newest are left as they are.  The tokens of one block must follow one
-    another in slots, as ``reserve_pages`` gives them; of two separate runs
-    into one block either may determine its scale.
+    With more than one token to a scale, a call's rows of one block share its
+    scale, wherever their tokens stand in slots.  If the block's first row is
+    not among them, they join the rows before the first of them: if the scale
+    has to grow, those rows' codes are rounded again (a scale never shrinks
+    while its block lasts).  The first row of a block begins it anew.  Rows
+    behind the first written one that the call does not write keep their codes
+    and take the new scale: write them before they are read.
     """
     what = "append_paged_kv8"
     try:
