@@ -16,8 +16,11 @@ What a row stands for.  A block's scale is the smallest power of two with which
 its largest magnitude is at most 448 (e4m3) or rounds to at most 127 (int8),
 within 2^-60 and 2^60; codes are rounded to nearest, ties to even.  So an
 element is off by at most 2^-4 of itself or 2^-10 of the scale, whichever is
-larger (e4m3), or by half of the scale (int8: 2^-7 of its block's largest).
-Blocks with an infinity, a NaN or a magnitude that no scale holds stand for NaN
+larger (e4m3), or by half of the scale (int8; above the smallest scale that is
+less than 1 / 127.5 of its block's largest).  With several tokens to a scale,
+rows stored before it grew were rounded again each time: they are off by less
+than 2^-4 of the element and 2^-9 of the scale together (e4m3), or by less than
+the scale (int8).  Blocks with an infinity, a NaN or a magnitude that no scale holds stand for NaN
 as a whole.  What the codes stand for is exact in bf16 and, within its range,
 in fp16.
 
