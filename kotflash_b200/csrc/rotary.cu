@@ -5,7 +5,7 @@
 // same with -t.  Pairs are column i with i + R / 2, or 2 i with 2 i + 1.
 //
 // Every element is read and written once (4 bytes for 3 flops), so HBM
-// bounds it: 4 x 4096 tokens of 32 and 8 heads of 128 columns take 56 us, 92%
+// bounds it: 4 x 4096 tokens of 32 and 8 heads of 128 columns take 53.4 us, 96%
 // of the measured copy rate.  cos and sin depend on the token and the pair
 // only: a thread keeps those of its pairs in registers and takes four heads,
 // which it asks for before it works the angles out.  (Angles shared by a block
@@ -26,6 +26,7 @@
 namespace {
 
 constexpr int kThreads = 128;
+constexpr int kHeads = 4;  // of a thread, at most
 
 struct RotaryArgs {
   const uint16_t* x[2];    // Q and K
@@ -105,7 +106,6 @@ template <int VEC, bool HALVES, bool BF16>
 __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
   constexpr int PAIRS = HALVES ? VEC : VEC > 1 ? VEC / 2 : 1;
   constexpr bool TWO = HALVES || VEC == 1;   // two loads per head
-  constexpr int U = 4;                       // heads in flight (and of a thread, see launch())
   // Frequencies in 2^-64 turns.  From shared memory: read by every thread through
   // L2 they are one line that all SMs ask for (4 x 4096 tokens: 110 us).
   extern __shared__ uint64_t turns_s[];
@@ -129,15 +129,15 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
     const int which = h >= a.heads[0];
     return (int64_t)n * st[which][0] + (int64_t)(h - (which ? a.heads[0] : 0)) * st[which][1] + (int64_t)s * st[which][2];
   };
-  Block<VEC> u[U], v[U];
+  Block<VEC> u[kHeads], v[kHeads];
   auto load = [&](int h, int x) {
     const uint16_t* p = a.x[h >= a.heads[0]] + at(a.xs, h);
     u[x].load(p + j);
     if (TWO && turns) v[x].load(p + other);
   };
-  // the first heads' values travel while the angles are worked out
+  // the heads' values travel while the angles are worked out
 #pragma unroll
-  for (int x = 0; x < U; ++x)
+  for (int x = 0; x < kHeads; ++x)
     if (h0 + x < h1) load(h0 + x, x);
 
   float c[PAIRS], d[PAIRS];
@@ -153,35 +153,32 @@ __global__ void __launch_bounds__(kThreads) rotary_kernel(const RotaryArgs a) {
       d[i] *= a.magnitude * a.sign;
     }
   }
-  for (int h = h0; h < h1; h += U) {
 #pragma unroll
-    for (int x = 0; x < U; ++x) {
-      if (h + x >= h1) continue;
-      uint16_t* p = a.y[h + x >= a.heads[0]] + at(a.ys, h + x);
-      if (turns) {
-        if constexpr (HALVES && VEC > 1) {
+  for (int x = 0; x < kHeads; ++x) {
+    if (h0 + x >= h1) continue;
+    uint16_t* p = a.y[h0 + x >= a.heads[0]] + at(a.ys, h0 + x);
+    if (turns) {
+      if constexpr (HALVES && VEC > 1) {
 #pragma unroll
-          for (int i = 0; i < VEC / 2; ++i) {
-            const float2 r = kf::unpack2<BF16>(u[x].w[i]), q = kf::unpack2<BF16>(v[x].w[i]);
-            u[x].w[i] = kf::pack2<BF16>(r.x * c[2 * i] - q.x * d[2 * i], r.y * c[2 * i + 1] - q.y * d[2 * i + 1]);
-            v[x].w[i] = kf::pack2<BF16>(q.x * c[2 * i] + r.x * d[2 * i], q.y * c[2 * i + 1] + r.y * d[2 * i + 1]);
-          }
-        } else if constexpr (!HALVES && VEC > 1) {
-#pragma unroll
-          for (int i = 0; i < PAIRS; ++i) {
-            const float2 r = kf::unpack2<BF16>(u[x].w[i]);
-            u[x].w[i] = kf::pack2<BF16>(r.x * c[i] - r.y * d[i], r.y * c[i] + r.x * d[i]);
-          }
-        } else {
-          const float r = kf::unpack2<BF16>(u[x].w[0]).x, q = kf::unpack2<BF16>(v[x].w[0]).x;
-          u[x].w[0] = kf::pack2<BF16>(r * c[0] - q * d[0], 0.f);
-          v[x].w[0] = kf::pack2<BF16>(q * c[0] + r * d[0], 0.f);
+        for (int i = 0; i < VEC / 2; ++i) {
+          const float2 r = kf::unpack2<BF16>(u[x].w[i]), q = kf::unpack2<BF16>(v[x].w[i]);
+          u[x].w[i] = kf::pack2<BF16>(r.x * c[2 * i] - q.x * d[2 * i], r.y * c[2 * i + 1] - q.y * d[2 * i + 1]);
+          v[x].w[i] = kf::pack2<BF16>(q.x * c[2 * i] + r.x * d[2 * i], q.y * c[2 * i + 1] + r.y * d[2 * i + 1]);
         }
+      } else if constexpr (!HALVES && VEC > 1) {
+#pragma unroll
+        for (int i = 0; i < PAIRS; ++i) {
+          const float2 r = kf::unpack2<BF16>(u[x].w[i]);
+          u[x].w[i] = kf::pack2<BF16>(r.x * c[i] - r.y * d[i], r.y * c[i] + r.x * d[i]);
+        }
+      } else {
+        const float r = kf::unpack2<BF16>(u[x].w[0]).x, q = kf::unpack2<BF16>(v[x].w[0]).x;
+        u[x].w[0] = kf::pack2<BF16>(r * c[0] - q * d[0], 0.f);
+        v[x].w[0] = kf::pack2<BF16>(q * c[0] + r * d[0], 0.f);
       }
-      u[x].store(p + j);
-      if (TWO && turns) v[x].store(p + other);
-      if (h + U + x < h1) load(h + U + x, x);
     }
+    u[x].store(p + j);
+    if (TWO && turns) v[x].store(p + other);
   }
 }
 
@@ -202,10 +199,10 @@ int launch(RotaryArgs& a, int D, bool bf16, cudaStream_t st) {
   if (threads > 0x7fffffffLL - kThreads) return kf::set_error(KF_ERR_UNSUPPORTED, "%s: too many tokens", what);
   const int64_t blocks = (threads + kThreads - 1) / kThreads;
   // Heads of a thread: four, all in flight at once, are what still shares the
-  // angles (4 x 4096 tokens of 40 heads: 56 us, 60 with eight, 67 with
-  // fourteen); fewer where that leaves SMs without a block (64 tokens: 2.3 us
+  // angles (4 x 4096 tokens of 40 heads: 53.4 us; with more in turns of four, and
+  // the registers for the next turn, 60 for eight and 67 for fourteen); fewer where that leaves SMs without a block (64 tokens: 2.3 us
   // with one, 2.8 with four).
-  a.chunk = 4;
+  a.chunk = kHeads;
   while (a.chunk > 1 && blocks * ((heads + a.chunk - 1) / a.chunk) < kf::sm_count_current_device() * 2) a.chunk /= 2;
   const dim3 grid((unsigned)blocks, (unsigned)((heads + a.chunk - 1) / a.chunk));
   const size_t smem = (size_t)a.R / 2 * sizeof(uint64_t);
