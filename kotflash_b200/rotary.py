@@ -69,7 +69,7 @@ def rotary_frequencies(
     if scaling == "linear":
         f = f / factor
     elif scaling == "yarn":
-        if trained_length is None or trained_length <= 0:
+        if trained_length is None or not trained_length > 0:
             raise ValueError("yarn needs trained_length")
         if not 0 <= slow < fast:
             raise ValueError("slow must be at least 0 and below fast")
