@@ -13,7 +13,7 @@
 
 namespace kf {
 
-constexpr int kMaxExponent = 60;
+constexpr int kMaxExponent = 60;  // (the sums of paged8_decode.cuh and their reciprocals rely on it)
 constexpr int kNanScale = 255;
 
 // Exponent of the smallest power of two that holds magnitudes up to x >= 0:

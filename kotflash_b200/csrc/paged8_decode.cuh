@@ -86,7 +86,7 @@ struct Cfg8 {
   static constexpr int STAGE = KW * PITCH * 2;               // K and V rows
   static constexpr int BLOCKS = blocks_per_sm(KD, ROWS);
   static constexpr int FIT = 196608 / BLOCKS / (TEAMS * STAGE);  // of 192 KB of ring per SM
-  static constexpr int MOST = KD == 1 ? 4 : 8;
+  static constexpr int MOST = KD == 1 ? 4 : 8;                // (six of the shortest rows do not fit with their scales)
   static constexpr int STAGES = FIT < MOST ? FIT : MOST;
   static constexpr int SHALLOW = STAGES / 3 > 1 ? STAGES / 3 : 1;
   static constexpr bool SWIZZLE = KD == 2 || KD == 4 || KD == 8;
@@ -232,8 +232,10 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     uint32_t page[LOOKS], row[LOOKS];
     int h;
   };
-  // K/V rows pass through L2 once and leave it to the scales' lines (32 requests
-  // of 8192 keys 91.2 -> 88.8 us)
+  // K/V rows leave L2 first, to the scales' lines: 32 requests of 8192 keys
+  // 86.8 us, 94.4 without.  Where rows are read again it makes no difference (the
+  // same with 7168 of them in pages that all share 85.1 and 85.3; 8 requests of
+  // 32768 keys with 72 query rows per KV head, in two row blocks, 219 and 219).
   const uint64_t once = kf::l2_evict_first();
   auto look_up = [&]() {
     Place p;

@@ -195,8 +195,10 @@ __device__ __forceinline__ void clear16(uint32_t at, bool pred) {
                : "memory");
 }
 
-// 1 / x to one unit in the last place (x is a sum of weights, 1 or more
-// wherever a row sees anything finite).
+// 1 / x to one unit in the last place.  x is a sum of weights: wherever a row
+// sees anything finite 1 or more in a 16-bit cache, between 2^-49 and 2^75
+// times the number of keys over an 8-bit one (kf::kMaxExponent), so neither x
+// nor 1 / x is subnormal, which the instruction takes for 0.
 __device__ __forceinline__ float reciprocal(float x) {
   float y;
   asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));

@@ -12,10 +12,13 @@
 // through shared memory, all heads of a few tokens per block: 64 to 90 us, the
 // barriers cost more than the angles.)
 //
-// An angle is needed to 2^-32 turns or so at any position.  Frequencies become
-// whole numbers of 2^-64 turns (a double holds them to 2^-55), so a product
-// with the position modulo 2^64 is the angle modulo a turn, off by position *
-// 2^-55 turns, with no reduction to make; its upper half goes to cos_sin().
+// Frequencies become whole numbers of 2^-64 turns, so a product with the
+// position modulo 2^64 is the angle modulo a turn, with no reduction to make;
+// its upper half, 2^-32 turns, goes to cos_sin().  A double holds a frequency
+// in turns to 2^-52 of itself after its roundings, so an angle of A turns is
+// off by A 2^-52 turns besides: below the 2^-23 of cos_sin() up to 2^26 turns,
+// which is as far as the same product in doubles goes (a frequency of 1 at
+// position 2^28; at 2^31 it is off by 2^-21 radians).
 #include <math.h>
 
 #include <type_traits>

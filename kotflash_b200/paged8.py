@@ -74,7 +74,7 @@ def _check_cache(what: str, k_pages, v_pages, k_scales, v_scales) -> None:
         raise ValueError(f"{what}: the scales of a page and head must be contiguous")
 
 
-def _check_rows(what: str, rows, dtype=None) -> None:
+def _check_rows(what: str, rows) -> None:
     for t in rows:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{what}: queries and K/V rows must be torch.Tensor instances")
@@ -259,7 +259,8 @@ def paged_attention8(
 ) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
     """``paged_attention`` over an 8-bit paged KV cache.
 
-    q is [B, Hq, 1, D] in fp16 or bf16; k_pages and v_pages [pages, Hkv,
+    q is [B, Hq, 1, D] in fp16 or bf16, rows contiguous and on 16 bytes like
+    those of new_k and new_v; k_pages and v_pages [pages, Hkv,
     page_size, D] in float8_e4m3fn or int8, with any positive strides whose rows
     are contiguous and 16-byte aligned; k_scales and v_scales [pages, Hkv,
     page_size / block].  block_table, lengths, masking and results are those of

@@ -48,8 +48,10 @@ def rotary_frequencies(
       pair is divided by factor and the fastest stays;
     * "yarn": pairs that turn ``slow`` times or less within trained_length are
       divided by factor, those that turn ``fast`` times or more stay, those
-      between are blended by their turns; q and k grow by the magnitude
-      0.1 ln(factor) + 1.
+      between are blended in proportion to their turns, as published; q and k
+      grow by the magnitude 0.1 ln(factor) + 1.  (A model that was trained with
+      a blend by the pairs' index has other frequencies between the two: pass
+      those.)
 
     Returns ``(frequencies, magnitude)`` for ``apply_rotary``; magnitude is 1
     but for "yarn".
@@ -211,8 +213,9 @@ def apply_rotary(
     frequencies float64 [R / 2] on the same device, finite, radians per position.  The
     first R columns turn in pairs, column i with i + R / 2 or, interleaved,
     2i with 2i + 1; the columns behind them pass.  Rotated columns are
-    multiplied by magnitude.  Angles are worked out in 64 bits, the rest in 32,
-    rounded once.  Any strides; new contiguous tensors are returned, ``(q',
+    multiplied by magnitude.  Angles are worked out in 64 bits (exact to 32-bit
+    rounding up to 2^28 radians, as position * frequency in float64 is), the
+    rest in 32, rounded once.  Any strides; new contiguous tensors are returned, ``(q',
     k')``, or q' alone where k is None.  Differentiable in q and k, backwards and,
     with ``torch.autograd.forward_ad``, forwards.
     """
