@@ -24,6 +24,7 @@ struct Rows8Args {
   uint32_t page_size, page_mul, page_shift;
   int chunks;              // D / 8
   int block_shift;         // log2 of the tokens of a scale
+  uint32_t front;          // thread blocks that take the runs that do not fill their block (0: all take both)
 };
 
 // Page and row of a slot; slots of a pool fit 31 bits unless it holds over 2^31 tokens.
@@ -97,10 +98,15 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 // slots and rows read twice 4096 tokens took 13.7 us.)  A run that does not
 // fill its block may have others beside it: the warps look through all slots
 // for them, once for up to 32 runs, and the first of several runs takes all of
-// them, in loops that read slots and rows again.  (That look costs 4096 tokens
-// 2.5 us, 9.3 without it.)
+// them, in loops that read slots and rows again.  In long calls, where most
+// runs are whole blocks, thread blocks in front take those that are not, so
+// that the look overlaps the rest (4096 tokens in 11 runs 10.4 us, 11.6 with
+// all alike and 9.2 without a look; 16384 in 8 runs 28.5, 32 and 24.6).  Short
+// calls are mostly single tokens, which would wait for one another there (512
+// of them 25 us, 47).
 constexpr int kKept = 16;        // rows of a run that a warp keeps
 constexpr int kWindowWarps = 4;  // of a thread block
+constexpr uint32_t kLong = 2048;  // tokens of a call with thread blocks for runs that do not fill their block
 constexpr int kLook = 16;        // slots that a thread has in flight when it looks through them
 
 // The runs of `partial` that have tokens of their block before and behind
@@ -139,13 +145,13 @@ __global__ void __launch_bounds__(kWindowWarps * 32, 7) append8_blocks_kernel(co
   const int lane = threadIdx.x & 31, c = lane % GROUP, g = lane / GROUP;
   const uint32_t size = 1u << a.block_shift;
   const uint32_t parts = (2 * a.heads + kWindowWarps - 1) / kWindowWarps;  // thread blocks of a window
-  const uint32_t windows = gridDim.x / parts;
-  const uint32_t turn = blockIdx.x / parts, hw = (blockIdx.x - turn * parts) * kWindowWarps + (threadIdx.x >> 5);
-  const uint32_t window = turn == 0 ? windows - 1 : turn - 1;  // the last run is seldom a whole block: it comes first
+  const bool partly = blockIdx.x < a.front, wholly = !partly && a.front > 0;
+  const uint32_t at = blockIdx.x - (wholly ? a.front : 0), turn = at / parts, hw = (at - turn * parts) * kWindowWarps + (threadIdx.x >> 5);
   const bool active = hw < 2 * a.heads;  // a warp without a head helps to look through the slots
   const uint32_t h = hw >> 1;
   const int w = hw & 1;
-  const uint64_t from = (uint64_t)window * size, until = min(from + size, (uint64_t)a.T);
+  const uint32_t window = partly ? max(size, 32u) : size;
+  const uint64_t from = (uint64_t)turn * window, until = min(from + window, (uint64_t)a.T);
   auto slot_at = [&](uint64_t t) { return t < a.T ? __ldcg(reinterpret_cast<const long long*>(a.slots) + t) : -1; };
   // Blocks by their number in the pool (which memory holds fewer than 2^32 - 1 of, see the host's check).
   auto block_of = [&](int64_t s) { return s >= 0 && s < a.num_slots ? (uint32_t)(s >> a.block_shift) : 0xffffffffu; };
@@ -178,7 +184,9 @@ __global__ void __launch_bounds__(kWindowWarps * 32, 7) append8_blocks_kernel(co
     }
     uint32_t leaders = __ballot_sync(0xffffffffu, leads), several = 0;
     const uint32_t partial = __ballot_sync(0xffffffffu, leads && tokens < size);
-    if (partial) {
+    if (partly) leaders &= partial;
+    if (wholly) leaders &= ~partial;
+    if (partial && !wholly) {
       __syncthreads();                         // the masks of the slots before have been read
       if (threadIdx.x < 32) {
         run_block[lane] = block_of(s);
@@ -411,11 +419,13 @@ int launch_rows(const char* what, const Rows8Args& a, cudaStream_t st, Kernel ke
 }
 
 template <bool INT8, bool BF16>
-int launch_append(const Rows8Args& a, cudaStream_t st) {
+int launch_append(Rows8Args& a, cudaStream_t st) {
   const char* what = "kf_paged8_append";
   if (a.block_shift > 0) {
-    const uint64_t windows = ((uint64_t)a.T + (1u << a.block_shift) - 1) >> a.block_shift;
-    const unsigned blocks = (unsigned)(windows * ((2 * a.heads + kWindowWarps - 1) / kWindowWarps));
+    const uint64_t size = (uint64_t)1 << a.block_shift, parts = (2 * a.heads + kWindowWarps - 1) / kWindowWarps;
+    const uint64_t windows = (a.T + size - 1) / size, chunk = size < 32 ? 32 : size;
+    a.front = a.T >= kLong ? (unsigned)((a.T + chunk - 1) / chunk * parts) : 0;
+    const unsigned blocks = (unsigned)(a.front + windows * parts);
     return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kWindowWarps * 32), 0, st, what, a);
   }
   return launch_rows(what, a, st, [](auto group) { return append8_kernel<INT8, BF16, group>; });

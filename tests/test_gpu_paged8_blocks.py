@@ -101,3 +101,24 @@ def test_runs_of_one_block_far_apart(held):
         _store(codes, exps, rows.cpu(), slots, held)
         assert torch.equal(scales.cpu().view(torch.uint8), oracle.bytes_of(exps))
         assert torch.equal(pages.cpu().double(), codes)
+
+
+@pytest.mark.parametrize("held,dtype,page,block", [("e4m3", BF16, 32, 2), ("int8", F16, 48, 16), ("e4m3", F16, 64, 32), ("int8", BF16, 128, 128)])
+def test_long_calls(held, dtype, page, block):
+    """Calls long enough for thread blocks of their own for runs that do not fill
+    their block: whole blocks, parts of blocks, and parts of one block apart."""
+    heads, d, n = 3, 24, 3200 // page
+    every = [p * page + i for p in torch.randperm(n, generator=torch.Generator().manual_seed(page)).tolist() for i in range(page)]
+    cuts = [every[:700], every[705:1500], every[2011:], every[1507:2003]]  # some rows are not written
+    apart = [x for c in cuts for x in (c[5:], c[:5])]
+    g = torch.Generator(device="cuda").manual_seed(block)
+    for slots in (sum(cuts, []), sum(apart, []), sum(cuts, [])[::-1]):
+        assert len(slots) >= 2048
+        kc, ke, kp, ks = _pool(n, heads, page, d, block, held, 1)
+        vc, ve, vp, vs = _pool(n, heads, page, d, block, held, 2)
+        new = (torch.randn(2, 1, heads, len(slots), d, device="cuda", generator=g) * 3).to(dtype)
+        append_paged_kv8(kp, vp, ks, vs, new[0], new[1], torch.tensor(slots, device="cuda"))
+        for codes, exps, pages, scales, rows in ((kc, ke, kp, ks, new[0]), (vc, ve, vp, vs, new[1])):
+            _store(codes, exps, rows.cpu(), slots, held)
+            assert torch.equal(scales.cpu().view(torch.uint8), oracle.bytes_of(exps))
+            assert torch.equal(pages.cpu().double(), codes)
