@@ -24,7 +24,9 @@ struct Rows8Args {
   uint32_t page_size, page_mul, page_shift;
   int chunks;              // D / 8
   int block_shift;         // log2 of the tokens of a scale
-  uint32_t front;          // thread blocks that take the runs that do not fill their block (0: all take both)
+  // Blocks of several tokens: the tokens of a window, and thread blocks in front
+  // that take the runs that do not fill their block (0: all take both).
+  uint32_t window, front;
 };
 
 // Page and row of a slot; slots of a pool fit 31 bits unless it holds over 2^31 tokens.
@@ -90,8 +92,9 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 // together: by their largest magnitude and, if the block has rows before the
 // first of them, by its scale; if that grows, the rows before are rounded
 // again.  Tokens that follow one another into a block are a run.  A warp
-// takes one head of K or V of the runs that begin in a window of `block`
-// tokens, the warps of a thread block those of one window.
+// takes one head of K or V of the runs that begin in a window of tokens, one
+// after another, the warps of a thread block those of one window: `block`
+// tokens or, in short calls, as few as one wave of thread blocks allows.
 //
 // Three trips to memory bound it (slots, rows with the old scale, stores), so
 // slots are read once and, of blocks up to 16 tokens, rows too and kept.  (With
@@ -102,10 +105,10 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 // runs are whole blocks, thread blocks in front take those that are not, so
 // that the look overlaps the rest (4096 tokens in 11 runs 10.4 us, 11.6 with
 // all alike and 9.2 without a look; 16384 in 8 runs 28.5, 32 and 24.6).  Short
-// calls are mostly single tokens, which would wait for one another there (512
-// of them 25 us, 47).
+// calls are mostly single tokens: 64 of them take 4.4 us, 24 in windows of 16.
 constexpr int kKept = 16;        // rows of a run that a warp keeps
 constexpr int kWindowWarps = 4;  // of a thread block
+constexpr int kWindowsPerSm = 7;
 constexpr uint32_t kLong = 2048;  // tokens of a call with thread blocks for runs that do not fill their block
 constexpr int kLook = 16;        // slots that a thread has in flight when it looks through them
 
@@ -138,7 +141,7 @@ __device__ __noinline__ uint2 look_through(const int64_t* slots, uint32_t T, int
 }
 
 template <bool INT8, bool BF16>
-__global__ void __launch_bounds__(kWindowWarps * 32, 7) append8_blocks_kernel(const Rows8Args a) {
+__global__ void __launch_bounds__(kWindowWarps * 32, kWindowsPerSm) append8_blocks_kernel(const Rows8Args a) {
   constexpr int GROUP = 8, SIDE = 32 / GROUP;  // lanes of a row, rows side by side
   kf::griddep_wait();
   kf::griddep_launch_dependents();
@@ -150,7 +153,7 @@ __global__ void __launch_bounds__(kWindowWarps * 32, 7) append8_blocks_kernel(co
   const bool active = hw < 2 * a.heads;  // a warp without a head helps to look through the slots
   const uint32_t h = hw >> 1;
   const int w = hw & 1;
-  const uint32_t window = partly ? max(size, 32u) : size;
+  const uint32_t window = partly ? max(size, 32u) : a.window;
   const uint64_t from = (uint64_t)turn * window, until = min(from + window, (uint64_t)a.T);
   auto slot_at = [&](uint64_t t) { return t < a.T ? __ldcg(reinterpret_cast<const long long*>(a.slots) + t) : -1; };
   // Blocks by their number in the pool (which memory holds fewer than 2^32 - 1 of, see the host's check).
@@ -422,10 +425,15 @@ template <bool INT8, bool BF16>
 int launch_append(Rows8Args& a, cudaStream_t st) {
   const char* what = "kf_paged8_append";
   if (a.block_shift > 0) {
-    const uint64_t size = (uint64_t)1 << a.block_shift, parts = (2 * a.heads + kWindowWarps - 1) / kWindowWarps;
-    const uint64_t windows = (a.T + size - 1) / size, chunk = size < 32 ? 32 : size;
-    a.front = a.T >= kLong ? (unsigned)((a.T + chunk - 1) / chunk * parts) : 0;
-    const unsigned blocks = (unsigned)(a.front + windows * parts);
+    const uint32_t size = 1u << a.block_shift, parts = (2 * a.heads + kWindowWarps - 1) / kWindowWarps;
+    auto blocks_of = [&](uint32_t window) { return ((uint64_t)a.T + window - 1) / window * parts; };
+    a.window = size;
+    a.front = 0;
+    if (a.T >= kLong)
+      a.front = (uint32_t)blocks_of(size < 32 ? 32 : size);
+    else
+      while (a.window > 1 && blocks_of(a.window / 2) <= (uint64_t)kWindowsPerSm * kf::sm_count_current_device()) a.window /= 2;
+    const unsigned blocks = (unsigned)(a.front + blocks_of(a.window));
     return kf::launch_dependent(append8_blocks_kernel<INT8, BF16>, dim3(blocks), dim3(kWindowWarps * 32), 0, st, what, a);
   }
   return launch_rows(what, a, st, [](auto group) { return append8_kernel<INT8, BF16, group>; });
