@@ -22,7 +22,7 @@
 // paged_split.cuh).  What differs, for a team of warps:
 // - A step takes 32 keys of the longest rows, 64 or 128 of shorter ones: half of
 //   a microsecond of a step does not depend on its keys (32 requests of 8192
-//   keys, D = 64: 69 us with 32 a step, 56 with 64).
+//   keys, D = 64, with two blocks to an SM: 69 us with 32 a step, 56 with 64).
 // - One TMA load brings a box of keys of both K and V where the two pools have
 //   the same strides: the pair is a dimension of the tensor map, as long as the
 //   distance of the pools.  (A load takes a lane about 66 cycles to issue.)
@@ -66,10 +66,10 @@ struct Paged8Args : PagedWork {
 
 // Blocks per SM.  Three where registers allow it without a spill and the
 // conversions and the latency of a step, not HBM, set the pace (D = 64: 32
-// requests of 8192 keys 54.1 -> 48.5 us, two of 100000 with 32 heads 42.3 ->
-// 39.1); two for longer rows, where three ask for more than HBM gives and end far
-// apart (D = 128: 86.8 -> 115), and shorter ones, whose 128 keys a step want
-// the registers (D = 32: 42 -> 52).
+// requests of 8192 keys 57 -> 52 us, two of 100000 with 32 heads 45.6 -> 41.4);
+// two for longer rows, where three ask for more than HBM gives and end far
+// apart (D = 128: 86.5 -> 109), and shorter ones, whose 128 keys a step want
+// the registers (D = 32, with weights in one part: 42 -> 52).
 constexpr int blocks_per_sm(int steps, int rows) { return steps == 4 && rows == 8 ? 3 : 2; }
 
 // Variants: KD = 16-column chunks of the head dim; LINES: pages are brought as
