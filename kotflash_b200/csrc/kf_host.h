@@ -34,11 +34,11 @@ int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box
 // read as zero.
 int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows, int panels, bool swizzle);
 
-// A pool of pages of bytes as lines of at most 128: sizes and strides in bytes.
+// A pool of pages of bytes as lines of 128: strides in bytes.  A box is as wide
+// as a line: wider ones have TMA ask for memory off the box (paged8_decode.cuh).
 struct PageLines {
   void* base;
-  int64_t bytes;                   // of a line
-  int64_t lines, line_stride;      // of a page and head
+  int64_t lines;                   // of a page and head
   int64_t planes, plane_stride;    // pools of the same shape and strides
   int64_t heads, head_stride, pages, page_stride;
 };

@@ -469,6 +469,13 @@ KF_DEVI void cp_async16(void* smem_dst, const void* gmem_src, bool pred) {
                "l"(gmem_src), "r"(n)
                : "memory");
 }
+KF_DEVI void cp_async16(uint32_t smem_dst, const void* gmem_src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(smem_dst), "l"(gmem_src) : "memory");
+}
+// Arrives on `bar` for this thread once all its copies so far are there.
+KF_DEVI void cp_async_mbar_arrive(uint64_t* bar) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
 KF_DEVI void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 KF_DEVI void cp_async_wait() {

@@ -112,20 +112,18 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
   // K and V as two planes of one tensor, where that describes both and a box
   // is a whole group.
   const int64_t apart = static_cast<const uint8_t*>(v_pages.ptr) - static_cast<const uint8_t*>(k_pages.ptr);
-  a.paired = l.box >= 16 && apart != 0 && (apart > 0 ? apart : -apart) < ((int64_t)1 << 39);
+  a.paired = l.lines && l.box >= 16 && apart != 0 && (apart > 0 ? apart : -apart) < ((int64_t)1 << 39);
   for (int i = 0; i < 3; ++i) a.paired = a.paired && (k_pages.size[i] == 1 || k_pages.stride[i] == v_pages.stride[i]);
   a.k_plane = a.paired && apart < 0 ? 1 : 0;
   a.v_plane = 1 - a.k_plane;
-  const int pitch = l.steps * 16, lines = l.lines ? l.box * pitch / 128 : l.box;
+  const int pitch = l.steps * 16, lines = l.box * pitch / 128;
   const bool swizzle = l.steps == 2 || l.steps == 4 || l.steps == 8;
-  CUtensorMap mk, mv;
-  for (int w = 0; w < (a.paired ? 1 : 2); ++w) {
+  CUtensorMap mk = {}, mv = {};
+  for (int w = 0; w < (!l.lines ? 0 : a.paired ? 1 : 2); ++w) {
     const kf_tensor4& pool = a.paired ? (apart > 0 ? k_pages : v_pages) : w ? v_pages : k_pages;
     kf::PageLines t;
     t.base = pool.ptr;
-    t.bytes = l.lines ? 128 : D;
-    t.lines = l.lines ? page_size * pitch / 128 : page_size;
-    t.line_stride = l.lines ? 128 : pool.stride[2];
+    t.lines = page_size * pitch / 128;
     t.planes = a.paired ? 2 : 1;
     t.plane_stride = apart > 0 ? apart : -apart;
     t.heads = Hkv;

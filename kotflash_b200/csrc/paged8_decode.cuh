@@ -74,7 +74,8 @@ constexpr int blocks_per_sm(int steps, int rows) { return steps == 4 && rows == 
 
 // Variants: KD = 16-column chunks of the head dim; LINES: pages are brought as
 // lines of 128 bytes, keys lie KD * 16 bytes apart (otherwise KD is 8, each row
-// has a line and the chunks are counted at run time); NT = 8-row tiles of query
+// has a line of the tile, is brought by its lane as chunks of 16 bytes, and the
+// chunks are counted at run time); NT = 8-row tiles of query
 // rows per warp; RG = warps of a team.
 template <int KD, int NT, int RG>
 struct Cfg8 {
@@ -166,11 +167,13 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
   float* ml = handed + 2 * C::HANDED;  // [warp][NT][4 lanes][2 rows](m, l, NaN if V has one, -)
 
   if (tid == 0) {
-    for (int i = 0; i < C::TEAMS * STAGES; ++i) kf::mbar_init(&full[0][0] + i, 1);
+    for (int i = 0; i < C::TEAMS * STAGES; ++i) kf::mbar_init(&full[0][0] + i, LINES ? 1 : 32);
     kf::fence_barrier_init();
     abort_any = 0;
-    kf::tma_prefetch_desc(&map_k);
-    kf::tma_prefetch_desc(&map_v);
+    if constexpr (LINES) {
+      kf::tma_prefetch_desc(&map_k);
+      kf::tma_prefetch_desc(&map_v);
+    }
   }
   // The chain lengths -> table -> K/V starts cold: hints while the previous
   // kernel still runs.
@@ -266,15 +269,29 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     if (lane == 0) {
 #pragma unroll
       for (int i = 0; i < LOOKS; ++i) seen_s[team][stage][i] = seen[i];
-      kf::mbar_arrive_expect_tx(bar, boxes * (uint32_t)(a.box * PITCH * 2));
+      if constexpr (LINES) kf::mbar_arrive_expect_tx(bar, boxes * (uint32_t)(a.box * PITCH * 2));
     }
     __syncwarp();
+    if constexpr (!LINES) {
+      // A row's own chunks by its lane, with no byte besides.
+      if (p.page[0] < a.num_pages) {
+        const uint8_t* k = a.k + p.page[0] * a.ks[0] + p.h * a.ks[1] + p.row[0] * a.ks[2];
+        const uint8_t* v = a.v + p.page[0] * a.vs[0] + p.h * a.vs[1] + p.row[0] * a.vs[2];
+        const uint32_t st = kf::smem_u32(ring + stage * C::STAGE);
+#pragma unroll 2
+        for (int c = 0; c < chunks; ++c) {
+          kf::cp_async16(st + place(lane, c, k_base), k + c * 16);
+          kf::cp_async16(st + place(lane, c, v_base), v + c * 16);
+        }
+      }
+      kf::cp_async_mbar_arrive(bar);   // of each lane, once its copies are there
+    }
 #pragma unroll
     for (int i = 0; i < LOOKS; ++i) {
-      if (starts[i]) {
+      if (LINES && starts[i]) {
         const int r = i * 32 + lane, inside = r & (a.group - 1);
         uint8_t* st = ring + stage * C::STAGE + (2 * r - inside) * PITCH;
-        const int line = LINES ? (int)(p.row[i] * (uint32_t)KD >> 3) : (int)p.row[i];
+        const int line = (int)(p.row[i] * (uint32_t)KD >> 3);
         if (a.paired) {
           kf::tma_load_5d_once(st, &map_k, bar, 0, line, 0, p.h, p.page[i], once);
         } else {
@@ -830,7 +847,12 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
 }
 
-// How the rows of a pool lie in a tile, and the variant that takes them.
+// How the rows of a pool lie in a tile, and the variant that takes them.  Pages
+// whose boxes of keys are whole lines of 128 bytes come by TMA; other pages
+// (rows with gaps; sizes with few factors of two) row by row, by cp.async.  A TMA
+// box of such rows is wider than they are, and a load of two planes of such
+// boxes with its promotion to 256 bytes in L2 asks for blocks up to 20 KB off
+// the box, past the end of the pool's memory.
 struct Layout {
   int steps, box;
   bool lines;    // pages are brought as lines of 128 bytes
@@ -843,7 +865,7 @@ Layout layout_of(int64_t D, const kf_tensor4& k, const kf_tensor4& v) {
   l.box = keys;                        // keys that never cross a page
   while (page_size % l.box) l.box /= 2;
   // Pages as lines: rows of whole chunks without a gap, a box of them full
-  // lines.  Else each row is a line of its own.
+  // lines.
   l.lines = pitch * l.box % 128 == 0 && (page_size == 1 || (k.stride[2] == pitch && v.stride[2] == pitch));
   l.steps = l.lines ? chunks : 8;
   if (!l.lines && l.box > 32) l.box = 32;
