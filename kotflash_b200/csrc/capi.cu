@@ -115,7 +115,8 @@ int encode_tmap_lines(CUtensorMap* map, const PageLines& t, int box, bool swizzl
   if (!fn) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
   if (!aligned16(t.base)) return set_error(KF_ERR_INVALID, "TMA base pointer not 16-byte aligned");
   cuuint64_t dims[5] = {64, (cuuint64_t)t.lines, (cuuint64_t)t.planes, (cuuint64_t)t.heads, (cuuint64_t)t.pages};
-  cuuint64_t strides[4] = {128, (cuuint64_t)t.plane_stride, (cuuint64_t)t.head_stride, (cuuint64_t)t.page_stride};
+  cuuint64_t strides[4] = {(cuuint64_t)t.line_stride, (cuuint64_t)t.plane_stride, (cuuint64_t)t.head_stride,
+                           (cuuint64_t)t.page_stride};
   for (int i = 0; i < 4; ++i) {
     if (dims[i + 1] == 1) {
       strides[i] = 128;  // a size-1 dimension may carry any stride; give it a legal one

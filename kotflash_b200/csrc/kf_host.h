@@ -38,7 +38,7 @@ int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows,
 // as a line: wider ones have TMA ask for memory off the box (paged8_decode.cuh).
 struct PageLines {
   void* base;
-  int64_t lines;                   // of a page and head
+  int64_t lines, line_stride;      // of a page and head
   int64_t planes, plane_stride;    // pools of the same shape and strides
   int64_t heads, head_stride, pages, page_stride;
 };

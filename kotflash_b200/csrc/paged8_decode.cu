@@ -124,6 +124,7 @@ extern "C" int kf_paged8_decode(const kf_paged8_decode_args* args) {
     kf::PageLines t;
     t.base = pool.ptr;
     t.lines = page_size * pitch / 128;
+    t.line_stride = pitch == 128 ? pool.stride[2] : 128;
     t.planes = a.paired ? 2 : 1;
     t.plane_stride = apart > 0 ? apart : -apart;
     t.heads = Hkv;

@@ -74,8 +74,8 @@ constexpr int blocks_per_sm(int steps, int rows) { return steps == 4 && rows == 
 
 // Variants: KD = 16-column chunks of the head dim; LINES: pages are brought as
 // lines of 128 bytes, keys lie KD * 16 bytes apart (otherwise KD is 8, each row
-// has a line of the tile, is brought by its lane as chunks of 16 bytes, and the
-// chunks are counted at run time); NT = 8-row tiles of query
+// has a line of the tile, comes in chunks of 16 bytes, and the chunks are counted
+// at run time); NT = 8-row tiles of query
 // rows per warp; RG = warps of a team.
 template <int KD, int NT, int RG>
 struct Cfg8 {
@@ -273,15 +273,18 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
     }
     __syncwarp();
     if constexpr (!LINES) {
-      // A row's own chunks by its lane, with no byte besides.
-      if (p.page[0] < a.num_pages) {
-        const uint8_t* k = a.k + p.page[0] * a.ks[0] + p.h * a.ks[1] + p.row[0] * a.ks[2];
-        const uint8_t* v = a.v + p.page[0] * a.vs[0] + p.h * a.vs[1] + p.row[0] * a.vs[2];
-        const uint32_t st = kf::smem_u32(ring + stage * C::STAGE);
+      // The rows' own chunks, with no byte besides; neighbouring lanes take those
+      // of one row (a row per lane: half of each sector at a time).
+      const int64_t k_at = p.page[0] * a.ks[0] + p.h * a.ks[1] + p.row[0] * a.ks[2];
+      const int64_t v_at = p.page[0] * a.vs[0] + p.h * a.vs[1] + p.row[0] * a.vs[2];
+      const uint32_t st = kf::smem_u32(ring + stage * C::STAGE), per_row = (65536 + chunks - 1) / chunks;
 #pragma unroll 2
-        for (int c = 0; c < chunks; ++c) {
-          kf::cp_async16(st + place(lane, c, k_base), k + c * 16);
-          kf::cp_async16(st + place(lane, c, v_base), v + c * 16);
+      for (int i = 0; i < chunks; ++i) {
+        const uint32_t x = i * 32 + lane, r = x * per_row >> 16, c = x - r * chunks;  // of 32 chunks: exact
+        const int64_t k = __shfl_sync(0xffffffffu, (long long)k_at, r), v = __shfl_sync(0xffffffffu, (long long)v_at, r);
+        if ((seen[0] >> r) & 1) {
+          kf::cp_async16(st + place(r, c, k_base), a.k + k + c * 16);
+          kf::cp_async16(st + place(r, c, v_base), a.v + v + c * 16);
         }
       }
       kf::cp_async_mbar_arrive(bar);   // of each lane, once its copies are there
@@ -848,11 +851,11 @@ paged8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_con
 }
 
 // How the rows of a pool lie in a tile, and the variant that takes them.  Pages
-// whose boxes of keys are whole lines of 128 bytes come by TMA; other pages
-// (rows with gaps; sizes with few factors of two) row by row, by cp.async.  A TMA
-// box of such rows is wider than they are, and a load of two planes of such
-// boxes with its promotion to 256 bytes in L2 asks for blocks up to 20 KB off
-// the box, past the end of the pool's memory.
+// whose boxes of keys are whole lines of 128 bytes come by TMA, and rows of 128
+// bytes in any case; other pages (shorter rows with gaps, sizes with few factors
+// of two) by cp.async.  A TMA box of such rows is wider than they are, and a load of two
+// planes of such boxes with its promotion to 256 bytes in L2 asks for blocks up
+// to 20 KB off the box, past the end of the pool's memory.
 struct Layout {
   int steps, box;
   bool lines;    // pages are brought as lines of 128 bytes
@@ -864,9 +867,8 @@ Layout layout_of(int64_t D, const kf_tensor4& k, const kf_tensor4& v) {
   const int chunks = (int)((D + 15) / 16), pitch = chunks * 16, keys = chunks <= 3 ? 128 : chunks <= 6 ? 64 : 32;
   l.box = keys;                        // keys that never cross a page
   while (page_size % l.box) l.box /= 2;
-  // Pages as lines: rows of whole chunks without a gap, a box of them full
-  // lines.
-  l.lines = pitch * l.box % 128 == 0 && (page_size == 1 || (k.stride[2] == pitch && v.stride[2] == pitch));
+  l.lines = pitch * l.box % 128 == 0 &&
+            (pitch == 128 || page_size == 1 || (k.stride[2] == pitch && v.stride[2] == pitch));
   l.steps = l.lines ? chunks : 8;
   if (!l.lines && l.box > 32) l.box = 32;
   return l;
