@@ -49,6 +49,15 @@ static EncodeTiledFn get_encode_fn() {
   return fn;
 }
 
+// L2 promotion of a map whose boxes are `box` elements wide over rows of `row`.
+// Promoted to 256 bytes, a box that reaches past the rows asks for memory off
+// the box (columns 64 to 127 of 16 rows of 72: 146 sectors instead of 133; two
+// planes of narrow rows: up to 22 KB away, past the end of mapped memory once
+// in 1700 pools), to 128 bytes it does not.
+static CUtensorMapL2promotion promotion(cuuint64_t row, int box) {
+  return row % box == 0 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B;
+}
+
 int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box_rows) {
   EncodeTiledFn fn = get_encode_fn();
   if (!fn) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled entry point unavailable");
@@ -74,8 +83,8 @@ int encode_tmap_4d(CUtensorMap* map, const kf_tensor4* t, int box_inner, int box
   cuuint32_t box[4] = {(cuuint32_t)box_inner, (cuuint32_t)box_rows, 1, 1};
   cuuint32_t estr[4] = {1, 1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 4, t->ptr, dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, promotion(dims[0], box_inner),
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return KF_OK;
 }
@@ -104,8 +113,7 @@ int encode_tmap_pages(CUtensorMap* map, const kf_tensor4* t, int cols, int rows,
                                                : CU_TENSOR_MAP_SWIZZLE_32B;
   cuuint32_t estr[5] = {1, 1, 1, 1, 1};
   CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT16, 5, t->ptr, dims, strides, box, estr,
-                  CU_TENSOR_MAP_INTERLEAVE_NONE, mode,
-                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, mode, promotion(dims[0], cols), CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) return set_error(KF_ERR_CUDA, "cuTensorMapEncodeTiled (pages) failed (%d)", (int)r);
   return KF_OK;
 }
