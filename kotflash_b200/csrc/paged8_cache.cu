@@ -104,8 +104,11 @@ __global__ void __launch_bounds__(kThreads) append8_kernel(const Rows8Args a) {
 // them, in loops that read slots and rows again.  In long calls, where most
 // runs are whole blocks, thread blocks in front take those that are not, so
 // that the look overlaps the rest (4096 tokens in 11 runs 10.4 us, 11.6 with
-// all alike and 9.2 without a look; 16384 in 8 runs 28.5, 32 and 24.6).  Short
-// calls are mostly single tokens: 64 of them take 4.4 us, 24 in windows of 16.
+// all alike and 9.2 without a look; 16384 in 8 runs 28.5, 32 and 24.6; 1003 in
+// 3 runs 6.3, 6.1 and 5.1).  Single tokens would wait for one another there
+// (4096 of them 137 us, 82 with all alike), but calls of so many are rare; short
+// calls, which they are mostly, take small windows (64 of them 4.4 us, 24 in
+// windows of 16).
 constexpr int kKept = 16;        // rows of a run that a warp keeps
 constexpr int kWindowWarps = 4;  // of a thread block
 constexpr int kWindowsPerSm = 7;
